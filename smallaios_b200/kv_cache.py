@@ -20,16 +20,20 @@ DEFAULT_SEED = 0xDEADBEEFCAFE1234  # KVCacheConfig::default (kv_compression.rs:7
 
 
 class _DevArray:
-    """__cuda_array_interface__ wrapper so torch can view library memory."""
+    """__cuda_array_interface__ wrapper so torch can view library memory.
 
-    def __init__(self, ptr: int, shape, typestr: str):
+    torch keeps the wrapper, and so the memory's owner, as long as a tensor views it.
+    """
+
+    def __init__(self, ptr: int, shape, typestr: str, owner):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr, "data": (ptr, False),
                                          "version": 3, "strides": None}
 
 
-def _view(ptr: int, shape, typestr: str, device) -> torch.Tensor:
-    with torch.cuda.device(device):
-        return torch.as_tensor(_DevArray(ptr, shape, typestr), device=device)
+def _view(ptr: int, shape, typestr: str, owner) -> torch.Tensor:
+    with torch.cuda.device(owner.device):
+        return torch.as_tensor(_DevArray(ptr, shape, typestr, owner), device=owner.device)
 
 
 @dataclass
@@ -176,27 +180,27 @@ class GpuKvCache:
         _raise_op(rc, "kv_cache_append")
 
     def view(self, layer: int) -> LayerView:
+        """The layer's arrays.  The tensors keep the cache alive; ``close()`` ends them all the same."""
         v = _lib.KvLayerView()
         check(lib.sa_kv_cache_layer_view(self.handle, layer, ctypes.byref(v)))
         B, H, T, CB, D = v.batch, v.kv_heads, v.capacity, v.code_bytes, v.head_dim
-        dev = self.device
         return LayerView(
-            k_codes=_view(v.k_codes, (B, H, T, CB), "|u1", dev),
-            v_codes=_view(v.v_codes, (B, H, T // 16, CB // 4, 4, 4, 4), "|u1", dev),
-            k_meta=_view(v.k_meta, (B, H, T, 2), "<f4", dev),
-            v_meta=_view(v.v_meta, (B, H, T, 2), "<f4", dev),
-            signs=_view(v.signs, (H, D), "<f4", dev),
+            k_codes=_view(v.k_codes, (B, H, T, CB), "|u1", self),
+            v_codes=_view(v.v_codes, (B, H, T // 16, CB // 4, 4, 4, 4), "|u1", self),
+            k_meta=_view(v.k_meta, (B, H, T, 2), "<f4", self),
+            v_meta=_view(v.v_meta, (B, H, T, 2), "<f4", self),
+            signs=_view(v.signs, (H, D), "<f4", self),
             wht_scale=v.wht_scale, bits=v.bits, code_bytes=CB, capacity=T,
             **({} if not v.k_qjl_bits else dict(
-                k_qjl_bits=_view(v.k_qjl_bits, (B, H, T, D // 8), "|u1", dev),
-                v_qjl_bits=_view(v.v_qjl_bits, (B, H, T, D // 8), "|u1", dev),
-                k_qjl_mag=_view(v.k_qjl_mag, (B, H, T), "<f4", dev),
-                v_qjl_mag=_view(v.v_qjl_mag, (B, H, T), "<f4", dev))),
+                k_qjl_bits=_view(v.k_qjl_bits, (B, H, T, D // 8), "|u1", self),
+                v_qjl_bits=_view(v.v_qjl_bits, (B, H, T, D // 8), "|u1", self),
+                k_qjl_mag=_view(v.k_qjl_mag, (B, H, T), "<f4", self),
+                v_qjl_mag=_view(v.v_qjl_mag, (B, H, T), "<f4", self))),
             **({} if not v.lr_us else dict(
-                lr_vt=_view(v.lr_vt, (B, H, D), "<f4", dev),
-                lr_us=_view(v.lr_us, (B, H, T), "<f4", dev),
-                lr_kmeta=_view(v.lr_kmeta, (B, H, T, 2), "<f4", dev),
-                lr_vtr=_view(v.lr_vtr, (B, H, D), "<f4", dev))))
+                lr_vt=_view(v.lr_vt, (B, H, D), "<f4", self),
+                lr_us=_view(v.lr_us, (B, H, T), "<f4", self),
+                lr_kmeta=_view(v.lr_kmeta, (B, H, T, 2), "<f4", self),
+                lr_vtr=_view(v.lr_vtr, (B, H, D), "<f4", self))))
 
     def memory_bytes(self) -> tuple[int, int]:
         """(CompressedKVCache::memory_bytes of the rows written so far, summed over the batch,
