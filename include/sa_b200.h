@@ -212,7 +212,8 @@ int sa_kv_cache_get_config(const sa_kv_cache *cache, sa_kv_cache_config *config)
 int sa_kv_cache_memory_bytes(const sa_kv_cache *cache, uint64_t *reference_bytes, uint64_t *device_bytes);
 /* Device-side status of the kernels that used this cache: 0, or bit 0 set when
  * a bounded wait inside a kernel gave up (the kernel then stopped and its
- * output is not valid).  Synchronises with the device; `clear` resets it.
+ * output is not valid), bit 1 when sa_kv_cache_keep_drafts met a path entry
+ * outside the drafts.  Synchronises with the device; `clear` resets it.
  * The reference has no device-side waits; this reports the safety net that
  * replaces a hang. */
 int sa_kv_cache_device_status(sa_kv_cache *cache, int32_t *status, int32_t clear);
@@ -436,6 +437,91 @@ int sa_rotary_embedding(const void *x, void *y, int32_t dtype, int32_t layout, i
                         int32_t table_dtype, int64_t table_rows, int32_t table_cols, const void *position_ids,
                         int32_t position_dtype, int64_t position_count, int64_t start_position,
                         int32_t interleaved, int32_t rotary_dim, int32_t *device_status, sa_stream_t stream);
+
+/* ======================================================================
+ * Serving operators over the compressed cache: verification of a tree of
+ * drafted tokens, and attention over blocks that a cheap score selects.  The
+ * reference has neither; both read the cache through the same decode
+ * semantics as sa_gqa_attend.  Queries come already rotated to their
+ * positions (sa_qkv_project_append and sa_rotary_embedding do it).  A cache
+ * with a gather set (sa_kv_cache_set_gather) is SA_ERR_UNSUPPORTED here.
+ *
+ * Workspaces are the caller's: `workspace` (device, 256-byte aligned) holds
+ * at least what the matching *_workspace_bytes says; NULL is fine where that
+ * is 0.  Concurrent calls on one cache need one each.
+ * ====================================================================== */
+#define SA_MAX_DRAFT_NODES 64
+#define SA_BLOCK_TOKENS 64
+
+/* Attention of a tree of `nodes` (1..SA_MAX_DRAFT_NODES) drafted tokens per
+ * sequence.  The drafts' keys and values have been appended (sa_kv_append) at
+ * slots [p, p + nodes), p = the cache position, which has not moved; keys and
+ * queries are rotated to their depth in the tree, p + depth.
+ *
+ *   parents  int32 (batch, nodes), device: -1 = the node follows the prefix,
+ *            j in [0, i) = node i follows node j, anything else = slot i holds
+ *            no node (as do the slots that follow it)
+ *   query, attn_out  (batch, nodes, q_heads_local * head_dim) in dtype
+ *
+ * Node i attends to the prefix [0, p), to its ancestors and to itself.  Rows
+ * of slots without a node are zero. */
+int64_t sa_gqa_tree_workspace_bytes(const sa_kv_cache *cache, int32_t nodes, int32_t dtype);
+int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, const int32_t *parents,
+                       void *attn_out, int32_t dtype, int32_t batch, int32_t nodes, int64_t num_heads,
+                       int32_t has_scale, float scale, void *workspace, int64_t workspace_bytes,
+                       sa_stream_t stream);
+
+/* Keeps the accepted path of a verified tree: in every layer, row p + path[b][i]
+ * (codes, scale, zero point, QJL residual of K and V) moves to row p + i,
+ * i < n, as if all rows were read before any is written.  path: int32
+ * (batch, n), device, nodes in [0, drafted); drafted <= SA_MAX_DRAFT_NODES.
+ * An entry outside [0, drafted) leaves its destination as it was and sets bit 1
+ * of sa_kv_cache_device_status.  Does not advance the position: the caller
+ * advances it by n.  Not for low-rank K (its state follows writes in order). */
+int sa_kv_cache_keep_drafts(sa_kv_cache *cache, const int32_t *path, int32_t batch, int32_t n, int32_t drafted,
+                            sa_stream_t stream);
+
+/* Mean rotated key of blocks [block_begin, block_end) of SA_BLOCK_TOKENS tokens
+ * each, of every (batch row, KV head), from the codes.  means: bf16, unit
+ * u = b * kv_head_count + h at means + u * row_stride, block_begin first,
+ * head_dim values each.  In whole numbers, so that the result does not depend
+ * on an order of summation:
+ *   2^e > |scale|, |zero point| of the block's tokens (e >= -100; values at or
+ *   above 2^100 and NaN count as 0); S, Z = rint(. * 2^(15-e));
+ *   M_d = sum_t S_t c_td + Z_t;  m_d = M_d rounded (half up) to 8 bits under
+ *   the largest |M_d|'s exponent;  mean = m_d 2^(sh+e-21), sh the bits dropped.
+ * Not for low-rank K. */
+int sa_kv_block_means(sa_kv_cache *cache, int32_t layer, void *means, int64_t row_stride, int32_t block_begin,
+                      int32_t block_end, sa_stream_t stream);
+
+/* Blocks each query token attends to.  Query token s at position p + s scores
+ * the blocks before its own, block (p+s)/SA_BLOCK_TOKENS, as the largest dot
+ * product of a mean with its KV head's `group` query heads.  The queries go to
+ * a common 12-bit grid (rint(q 2^(12-e)), 2^e > every |q| of the group, e >=
+ * -100; values at or above 2^100 and NaN count as 0), are rotated exactly and
+ * rounded to 8 bits, so the scores are exact: ties, and only ties, go to the
+ * lower block.  The first sink_blocks blocks and the local_blocks (>= 1) last
+ * ones are always taken; max_blocks >= sink_blocks + local_blocks in all.
+ *
+ *   means      as sa_kv_block_means writes them from block 0; means_blocks of
+ *              them per unit, at least (p + seq_len - 1) / SA_BLOCK_TOKENS
+ *   block_ids  int32 (batch, seq_len, kv_head_count, max_blocks): ascending,
+ *              then -1 */
+int sa_gqa_select_blocks(sa_kv_cache *cache, int32_t layer, const void *query, int32_t dtype, int32_t batch,
+                         int32_t seq_len, int64_t num_heads, const void *means, int64_t row_stride,
+                         int64_t means_blocks, int32_t max_blocks, int32_t sink_blocks, int32_t local_blocks,
+                         int32_t *block_ids, sa_stream_t stream);
+
+/* Attention of query token s, at position p + s, over the cached tokens at or
+ * before its position of its listed blocks (block_ids as above; distinct ids;
+ * entries outside the cache's blocks count as -1; an empty list gives zeros).
+ * The query tokens' own keys and values have been appended; the position has
+ * not moved. */
+int64_t sa_gqa_sparse_workspace_bytes(const sa_kv_cache *cache, int32_t seq_len);
+int sa_gqa_sparse_attend(sa_kv_cache *cache, int32_t layer, const void *query, const int32_t *block_ids,
+                         int32_t max_blocks, void *attn_out, int32_t dtype, int32_t batch, int32_t seq_len,
+                         int64_t num_heads, int32_t has_scale, float scale, void *workspace,
+                         int64_t workspace_bytes, sa_stream_t stream);
 
 #ifdef __cplusplus
 }

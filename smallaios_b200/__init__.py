@@ -9,7 +9,8 @@ operator interface; all compute runs in the CUDA library.
 from .kv_cache import DEFAULT_SEED, GpuKvCache, LayerView, qjl_correction
 from .ops import (CapacityError, InternalError, InvalidAttribute, KvCacheDispatchCtx, OpError, PackedNBitsWeight,
                   ShapeMismatch, UnsupportedOp, dispatch_gpu_node, finalize_kv_cache, gqa_attend,
-                  group_query_attention, matmul_nbits, matmul_nbits_packed, qkv_project_append, rms_norm,
+                  gqa_select_blocks, gqa_sparse_attend, gqa_tree_attend, group_query_attention, kv_block_means,
+                  matmul_nbits, matmul_nbits_packed, qkv_project_append, rms_norm,
                   rotary_device_status, rotary_embedding, silu_mul, supports_op)
 from .layer import LayerWeights, decoder_layer_step, prefill_layer_step
 
@@ -18,5 +19,6 @@ __all__ = [
     "KvCacheDispatchCtx", "OpError", "ShapeMismatch", "UnsupportedOp", "dispatch_gpu_node", "finalize_kv_cache",
     "gqa_attend", "group_query_attention", "matmul_nbits", "matmul_nbits_packed", "PackedNBitsWeight",
     "qkv_project_append", "rms_norm", "silu_mul", "supports_op", "LayerWeights", "decoder_layer_step", "prefill_layer_step",
-    "qjl_correction", "rotary_embedding", "rotary_device_status",
+    "qjl_correction", "rotary_embedding", "rotary_device_status", "gqa_tree_attend", "kv_block_means",
+    "gqa_select_blocks", "gqa_sparse_attend",
 ]

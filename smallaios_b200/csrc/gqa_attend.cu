@@ -94,8 +94,41 @@ __device__ __forceinline__ void unrotate_store(float (&x)[EPL], int lane, int d,
     }
 }
 
+// Which cached tokens query token s sees.
+//   kCausal  tokens [0, pos0 + s]
+//   kTree    the prefix [0, pos0) and, of the drafts at pos0 .., the ancestors of node s and itself
+//   kBlocks  the tokens at or before pos0 + s of its listed 64-token blocks
+enum AttendMode { kCausal, kTree, kBlocks };
+
+// Weight of a partial result with maximum m and sum l against the maximum M of all.  A partial that
+// saw no token counts nothing; in the list and tree modes one whose sum is NaN spoils the row (the
+// causal mode, whose rows always see a token, keeps such rows at zero).
+template <int MODE>
+__device__ __forceinline__ float partial_weight(float m, float l, float M) {
+    if (MODE != kCausal && l != l) return l;
+    return m == -INFINITY ? 0.0f : exp2f(m - M);
+}
+
+// Whether a row's sum counts: rows that saw no token (or, in the causal mode, NaN) are zero.
+template <int MODE>
+__device__ __forceinline__ bool row_counts(float l) {
+    return MODE == kCausal ? l > 0.0f : !(l == 0.0f);
+}
+
+// Bit j: node j is node s or above it (tree_path); 0 when the slot holds no node.  Every thread
+// calls it; the walk is one thread's, through parents in shared memory.
+__device__ __forceinline__ uint64_t tree_row_mask(const int32_t *parents, int nodes, int s) {
+    __shared__ int s_par[kMaxDraftNodes];
+    __shared__ uint64_t s_mask;
+    for (int i = threadIdx.x; i < nodes; i += blockDim.x) s_par[i] = parents[i];
+    __syncthreads();
+    if (threadIdx.x == 0) s_mask = tree_path(s_par, s);
+    __syncthreads();
+    return s_mask;
+}
+
 // grid = (splits, heads, batch*seq_len), block = 32*kWarps.
-template <typename T, int EPL, int MAXG>
+template <typename T, int EPL, int MAXG, int MODE>
 __global__ void __launch_bounds__(32 * kWarps) attend_split_kernel(AttendArgs a, int n_splits, int tokens_per_split) {
     extern __shared__ float smem[];
     const int d = a.head_dim, G = a.group;
@@ -108,7 +141,17 @@ __global__ void __launch_bounds__(32 * kWarps) attend_split_kernel(AttendArgs a,
     const int split = blockIdx.x, h = blockIdx.y, row = blockIdx.z;
     const int b = row / a.seq_len, s = row % a.seq_len;
     const int64_t qpos = a.pos0 + s;
-    const int64_t total = qpos + 1;  // causal: keys [0, qpos]
+    int64_t total = qpos + 1;  // causal: keys [0, qpos]
+    uint64_t tree_mask = 0;
+    const int32_t *ids = nullptr;
+    if constexpr (MODE == kTree) {
+        tree_mask = tree_row_mask(a.parents + (int64_t)b * a.seq_len, a.seq_len, s);
+        total = tree_mask ? a.pos0 + a.seq_len : 0;  // a slot without a node sees nothing: zero output
+    }
+    if constexpr (MODE == kBlocks) {
+        ids = a.block_ids + ((int64_t)row * a.heads + h) * a.max_blocks;
+        total = (int64_t)a.max_blocks * kBlockTokens;  // counted along the list
+    }
     const float *sg = a.signs + (int64_t)h * d;
     const int qheads = a.heads * G;
 
@@ -154,7 +197,16 @@ __global__ void __launch_bounds__(32 * kWarps) attend_split_kernel(AttendArgs a,
     int64_t t_end = t_begin + tokens_per_split;
     if (t_end > total) t_end = total;
 
-    for (int64_t t = t_begin + warp; t < t_end; t += kWarps) {
+    for (int64_t ti = t_begin + warp; ti < t_end; ti += kWarps) {
+        int64_t t = ti;
+        if constexpr (MODE == kTree) {
+            if (t >= a.pos0 && !((tree_mask >> (t - a.pos0)) & 1)) continue;
+        }
+        if constexpr (MODE == kBlocks) {
+            const int id = ids[ti / kBlockTokens];
+            t = (int64_t)id * kBlockTokens + ti % kBlockTokens;
+            if (id < 0 || t > qpos) continue;
+        }
         const uint8_t *krow = kc + t * a.code_bytes;
         float ck[EPL], cv[EPL];
 #pragma unroll
@@ -205,7 +257,7 @@ __global__ void __launch_bounds__(32 * kWarps) attend_split_kernel(AttendArgs a,
         float L = 0.0f, Z = 0.0f, wts[kWarps];
         for (int w = 0; w < kWarps; w++) {
             const float mw = s_mlz[(w * MAXG + g) * 3];
-            wts[w] = (mw == -INFINITY) ? 0.0f : exp2f(mw - M);
+            wts[w] = partial_weight<MODE>(mw, s_mlz[(w * MAXG + g) * 3 + 1], M);
             L += wts[w] * s_mlz[(w * MAXG + g) * 3 + 1];
             Z += wts[w] * s_mlz[(w * MAXG + g) * 3 + 2];
         }
@@ -218,9 +270,10 @@ __global__ void __launch_bounds__(32 * kWarps) attend_split_kernel(AttendArgs a,
             x[r] = A;
         }
         if (n_splits == 1) {
-            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+            const bool counts = row_counts<MODE>(L);
+            const float inv = counts ? 1.0f / L : 0.0f;
 #pragma unroll
-            for (int r = 0; r < EPL; r++) x[r] = L > 0.0f ? (x[r] + Z) * inv : 0.0f;
+            for (int r = 0; r < EPL; r++) x[r] = counts ? (x[r] + Z) * inv : 0.0f;
             T *dst = static_cast<T *>(a.out) + ((int64_t)row * qheads + h * G + g) * d;
             unrotate_store<T, EPL>(x, lane, d, sg, a.wht_scale, dst);
         } else {
@@ -240,7 +293,7 @@ __global__ void __launch_bounds__(32 * kWarps) attend_split_kernel(AttendArgs a,
 
 // Merge split-K partials, normalise, inverse-rotate, store.
 // grid = (heads*group, batch*seq_len), block = 32.
-template <typename T, int EPL>
+template <typename T, int EPL, int MODE = kCausal>
 __global__ void __launch_bounds__(32) attend_combine_kernel(AttendArgs a, int n_splits) {
     const int lane = threadIdx.x;
     const int d = a.head_dim, G = a.group;
@@ -257,7 +310,7 @@ __global__ void __launch_bounds__(32) attend_combine_kernel(AttendArgs a, int n_
     for (int sp = 0; sp < n_splits; sp++) {
         const float *p = base + sp * sstride;
         const float ms = p[d];
-        const float w = (ms == -INFINITY) ? 0.0f : exp2f(ms - M);
+        const float w = partial_weight<MODE>(ms, p[d + 1], M);
         L += w * p[d + 1];
         Z += w * p[d + 2];
         if (active) {
@@ -265,9 +318,10 @@ __global__ void __launch_bounds__(32) attend_combine_kernel(AttendArgs a, int n_
             for (int r = 0; r < EPL; r++) x[r] += w * p[lane * EPL + r];
         }
     }
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const bool counts = row_counts<MODE>(L);
+    const float inv = counts ? 1.0f / L : 0.0f;
 #pragma unroll
-    for (int r = 0; r < EPL; r++) x[r] = L > 0.0f ? (x[r] + Z) * inv : 0.0f;
+    for (int r = 0; r < EPL; r++) x[r] = counts ? (x[r] + Z) * inv : 0.0f;
     const int qheads = a.heads * G;
     T *dst = static_cast<T *>(a.out) + ((int64_t)row * qheads + h * G + g) * d;
     unrotate_store<T, EPL>(x, lane, d, a.signs + (int64_t)h * d, a.wht_scale, dst);
@@ -278,10 +332,10 @@ size_t split_smem_bytes(int d) {
     return sizeof(float) * ((size_t)MAXG * d + MAXG + (size_t)kWarps * MAXG * d + (size_t)kWarps * MAXG * 3);
 }
 
-template <typename T, int EPL, int MAXG>
+template <typename T, int EPL, int MAXG, int MODE>
 int launch_generic(const AttendArgs &a, int n_splits, int tps, cudaStream_t stream) {
     const size_t smem = split_smem_bytes<MAXG>(a.head_dim);
-    auto kern = attend_split_kernel<T, EPL, MAXG>;
+    auto kern = attend_split_kernel<T, EPL, MAXG, MODE>;
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return check_cuda(e, "gqa_attend smem attribute");
@@ -297,30 +351,37 @@ int launch_generic(const AttendArgs &a, int n_splits, int tps, cudaStream_t stre
     count_launch();
     int rc = check_cuda(cudaGetLastError(), "gqa_attend split launch");
     if (rc != SA_OK || n_splits == 1) return rc;
-    attend_combine_kernel<T, EPL><<<dim3(a.heads * a.group, (unsigned)rows), 32, 0, stream>>>(a, n_splits);
+    attend_combine_kernel<T, EPL, MODE><<<dim3(a.heads * a.group, (unsigned)rows), 32, 0, stream>>>(a, n_splits);
     count_launch();
     return check_cuda(cudaGetLastError(), "gqa_attend combine launch");
 }
 
-template <typename T, int EPL>
+template <typename T, int EPL, int MODE>
 int launch_by_group(const AttendArgs &a, int n_splits, int tps, cudaStream_t stream) {
-    if (a.group <= 1) return launch_generic<T, EPL, 1>(a, n_splits, tps, stream);
-    if (a.group <= 2) return launch_generic<T, EPL, 2>(a, n_splits, tps, stream);
-    if (a.group <= 4) return launch_generic<T, EPL, 4>(a, n_splits, tps, stream);
-    if (a.group <= 8) return launch_generic<T, EPL, 8>(a, n_splits, tps, stream);
+    if (a.group <= 1) return launch_generic<T, EPL, 1, MODE>(a, n_splits, tps, stream);
+    if (a.group <= 2) return launch_generic<T, EPL, 2, MODE>(a, n_splits, tps, stream);
+    if (a.group <= 4) return launch_generic<T, EPL, 4, MODE>(a, n_splits, tps, stream);
+    if (a.group <= 8) return launch_generic<T, EPL, 8, MODE>(a, n_splits, tps, stream);
     return set_error(SA_ERR_UNSUPPORTED, "gqa_attend: group size %d > 8 not supported", a.group);
+}
+
+template <typename T, int MODE>
+int launch_by_dim_mode(const AttendArgs &a, int n_splits, int tps, cudaStream_t stream) {
+    switch (a.head_dim) {
+        case 16:
+        case 32: return launch_by_group<T, 1, MODE>(a, n_splits, tps, stream);
+        case 64: return launch_by_group<T, 2, MODE>(a, n_splits, tps, stream);
+        case 128: return launch_by_group<T, 4, MODE>(a, n_splits, tps, stream);
+        case 256: return launch_by_group<T, 8, MODE>(a, n_splits, tps, stream);
+        default: return set_error(SA_ERR_UNSUPPORTED, "gqa_attend: head_dim %d not supported", a.head_dim);
+    }
 }
 
 template <typename T>
 int launch_by_dim(const AttendArgs &a, int n_splits, int tps, cudaStream_t stream) {
-    switch (a.head_dim) {
-        case 16:
-        case 32: return launch_by_group<T, 1>(a, n_splits, tps, stream);
-        case 64: return launch_by_group<T, 2>(a, n_splits, tps, stream);
-        case 128: return launch_by_group<T, 4>(a, n_splits, tps, stream);
-        case 256: return launch_by_group<T, 8>(a, n_splits, tps, stream);
-        default: return set_error(SA_ERR_UNSUPPORTED, "gqa_attend: head_dim %d not supported", a.head_dim);
-    }
+    if (a.parents) return launch_by_dim_mode<T, kTree>(a, n_splits, tps, stream);
+    if (a.block_ids) return launch_by_dim_mode<T, kBlocks>(a, n_splits, tps, stream);
+    return launch_by_dim_mode<T, kCausal>(a, n_splits, tps, stream);
 }
 
 }  // namespace
@@ -393,7 +454,7 @@ int launch_gather_scatter(const AttendArgs &a, cudaStream_t stream) {
 }
 
 int launch_gqa_attend_generic(const AttendArgs &a, cudaStream_t stream) {
-    const int64_t total = a.pos0 + a.seq_len;
+    const int64_t total = a.block_ids ? (int64_t)a.max_blocks * kBlockTokens : a.pos0 + a.seq_len;
     int n_splits, tps;
     choose_splits(a, total, &n_splits, &tps);
     switch (a.dtype) {

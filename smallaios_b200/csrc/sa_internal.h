@@ -20,8 +20,23 @@ __host__ __device__ __forceinline__ int64_t v_byte_offset(int64_t t, int j, int 
     const int k = 4 * j + (int)(t & 3);
     return (t >> 4) * (int64_t)(16 * cb) + (k >> 4) * 64 + ((t >> 2) & 3) * 16 + (k & 15);
 }
+constexpr int kBlockTokens = SA_BLOCK_TOKENS;        // tokens of a block of the block-sparse attention
+constexpr int kMaxDraftNodes = SA_MAX_DRAFT_NODES;  // drafted nodes per sequence: one bit each of a 64-bit mask
 constexpr int kMaxSplits = 64;       // split-K partitions per (row, kv head)
 constexpr int kMaxGather = 8;        // ranks of one node in the head-sharded mode
+
+// Bits of node s and of the nodes above it in a draft tree (parents: -1 = follows the prefix, else an
+// earlier node); 0 when the slot, or one above it, holds no node (-2, or no earlier node).
+__host__ __device__ __forceinline__ uint64_t tree_path(const int *parents, int s) {
+    uint64_t mask = 0;
+    for (int n = s; n >= 0;) {
+        mask |= 1ull << n;
+        const int up = parents[n];
+        if (up < -1 || up >= n) return 0;
+        n = up;
+    }
+    return mask;
+}
 
 // Head-sharded output: the attention output of this rank's query heads goes
 // to every buffer p[0..n) (this GPU's and its peers', mapped into this
@@ -132,8 +147,53 @@ struct AttendArgs {
     // low-rank K: V^T rotated like q' (nullptr: off).  With it, k_meta holds {0, U*S[t]} and the
     // zero-point term's sum(q') becomes q'.lr_vtr, so scores are U*S[t] * (q . V^T).
     const float *lr_vtr;
+    // draft tree (nullptr: off): [batch][seq_len] parents, the query tokens are the tree's nodes
+    const int32_t *parents;
+    // block lists (nullptr: off): [batch][seq_len][heads][max_blocks] ascending block ids, -1 = none
+    const int32_t *block_ids;
+    int max_blocks;
 };
 
+// Moves drafted rows of every layer (sa_kv_cache_keep_drafts).
+struct KeepArgs {
+    uint8_t *k_codes, *v_codes;
+    float *k_meta, *v_meta;
+    uint8_t *k_qjl_bits, *v_qjl_bits;  // nullptr: not stored
+    float *k_qjl_mag, *v_qjl_mag;
+    const int32_t *path;  // [batch][n]
+    int layers, batch, heads, head_dim, code_bytes, capacity;
+    int n, drafted;
+    int64_t pos0;
+    int *dev_status;
+};
+
+// Block means of one layer (sa_kv_block_means).
+struct MeansArgs {
+    const uint8_t *k_codes;
+    const float *k_meta;
+    void *means;         // bf16, block `first` of unit u at u * row_stride
+    int64_t row_stride;  // elements between units (batch row, KV head)
+    int units, head_dim, bits, code_bytes, capacity;
+    int first, blocks;
+};
+
+// Block selection (sa_gqa_select_blocks).
+struct SelectArgs {
+    const void *query;
+    int dtype;
+    int batch, seq_len, heads, group, head_dim;
+    int64_t pos0;
+    const float *signs;
+    const void *means;  // bf16
+    int64_t row_stride;
+    int max_blocks, sink, local;
+    int32_t *block_ids;
+};
+
+int launch_keep_drafts(const KeepArgs &a, cudaStream_t stream);
+int launch_block_means(const MeansArgs &a, cudaStream_t stream);
+int launch_select_blocks(const SelectArgs &a, cudaStream_t stream);
+int launch_gqa_attend_generic(const AttendArgs &a, cudaStream_t stream);
 int launch_kv_append(const AppendArgs &a, cudaStream_t stream);
 int launch_lowrank_append(const AppendArgs &a, cudaStream_t stream);
 int launch_gqa_attend(const AttendArgs &a, cudaStream_t stream);

@@ -72,9 +72,6 @@ static void make_signs(uint64_t seed, int dim, float *out) {
     }
 }
 
-int launch_gqa_attend_generic(const AttendArgs &a, cudaStream_t stream);
-
-
 }  // namespace sa
 
 using namespace sa;

@@ -179,6 +179,24 @@ class GpuKvCache:
                               rows, int(do_rotary), int(rotary_interleaved), _stream_handle(stream, self.device))
         _raise_op(rc, "kv_cache_append")
 
+    def keep_drafts(self, path: torch.Tensor, *, drafted: int, stream=None) -> None:
+        """Move the accepted drafts of a verified tree to the front, in every layer (sa_kv_cache_keep_drafts).
+
+        ``path`` int32 (B, n) on the device: node path[b][i] of the ``drafted`` appended ones becomes token
+        position + i.  The position is not advanced (``advance_position(n)`` does).  An entry outside
+        [0, drafted) moves nothing and sets bit 1 of ``device_status``.
+        """
+        from .ops import ShapeMismatch, UnsupportedOp, _cuda, _raise_op, _stream_handle
+
+        _cuda(path, "path")
+        if path.dtype != torch.int32:
+            raise UnsupportedOp("keep_drafts: path must be int32")
+        if path.dim() != 2:
+            raise ShapeMismatch("keep_drafts: path must be (batch, n)")
+        rc = lib.sa_kv_cache_keep_drafts(self.handle, path.data_ptr(), path.shape[0], path.shape[1], int(drafted),
+                                         _stream_handle(stream, self.device))
+        _raise_op(rc, "keep_drafts")
+
     def view(self, layer: int) -> LayerView:
         """The layer's arrays.  The tensors keep the cache alive; ``close()`` ends them all the same."""
         v = _lib.KvLayerView()
@@ -267,7 +285,8 @@ class GpuKvCache:
 
     def device_status(self, clear: bool = False) -> int:
         """Device-side status bits of the kernels that used this cache: 0, or bit 0 when a bounded
-        wait inside a kernel gave up (that call's output is not valid).  Synchronises."""
+        wait inside a kernel gave up (that call's output is not valid), bit 1 when ``keep_drafts`` met
+        a node outside the drafts.  Synchronises."""
         st = ctypes.c_int32()
         check(lib.sa_kv_cache_device_status(self.handle, ctypes.byref(st), int(bool(clear))))
         return st.value

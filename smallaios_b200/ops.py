@@ -172,6 +172,147 @@ def gqa_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, *, num_heads:
     return out
 
 
+# ---- serving operators: draft trees and block-sparse attention ------------------
+def _rotated_query(op: str, query, cache: GpuKvCache, out):
+    """Checks of (B, S, Hq_local*D) query tokens already rotated to their positions; returns out."""
+    _cuda(query, "query")
+    cfg = cache.config
+    if query.dim() != 3:
+        raise ShapeMismatch(f"{op}: query must be rank-3")
+    if query.shape[2] != cfg.num_heads // cfg.num_kv_heads * cfg.kv_head_count * cfg.head_dim:
+        raise ShapeMismatch(f"{op}: hidden size does not match the cache's heads/head_dim")
+    if out is None:
+        return torch.empty_like(query)
+    _cuda(out, "out")
+    if out.shape != query.shape or out.dtype != query.dtype:
+        raise ShapeMismatch(f"{op}: out must have query's shape and dtype")
+    return out
+
+
+def _int32(op: str, t, shape: tuple, what: str):
+    _cuda(t, what)
+    if t.dtype != torch.int32:
+        raise UnsupportedOp(f"{op}: {what} must be int32")
+    if t.shape != shape:
+        raise ShapeMismatch(f"{op}: {what} must be {shape}, got {tuple(t.shape)}")
+
+
+def _workspace(workspace, nbytes: int, device):
+    """``workspace``, or a buffer of the stream-ordered allocator where the call needs one."""
+    if workspace is None and nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _cuda(workspace, "workspace")
+
+
+def gqa_tree_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, parents: torch.Tensor, *, num_heads: int,
+                    scale: float | None = None, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens over the cache (sa_gqa_tree_attend).
+
+    ``query`` (B, N, Hq*D), N <= 64 drafts rotated to position + depth, whose keys and values have been
+    appended at the cache position (not advanced).  ``parents`` int32 (B, N) on the device: -1 a node that
+    follows the prefix, j < i a node that follows node j, anything else no node (zero output, as for the
+    nodes below it).  Each node sees the prefix, its ancestors and itself.  ``workspace``: uint8, at least
+    ``sa_gqa_tree_workspace_bytes``; allocated when not given.
+    """
+    out = _rotated_query("gqa_tree_attend", query, cache, out)
+    b, n, _ = query.shape
+    _int32("gqa_tree_attend", parents, (b, n), "parents")
+    code = _dtype_code(query)
+    workspace = _workspace(workspace, lib.sa_gqa_tree_workspace_bytes(cache.handle, n, code), query.device)
+    rc = lib.sa_gqa_tree_attend(cache.handle, layer, query.data_ptr(), parents.data_ptr(), out.data_ptr(), code, b, n,
+                                int(num_heads), int(scale is not None), float(scale or 0.0),
+                                None if workspace is None else workspace.data_ptr(),
+                                0 if workspace is None else workspace.numel(), _stream_handle(stream, query.device))
+    _raise_op(rc, "gqa_tree_attend")
+    return out
+
+
+def _means_rows(op: str, means, cache: GpuKvCache):
+    """(blocks, row stride) of bf16 block means (B, H, blocks, D), which may be a slice of blocks."""
+    cfg = cache.config
+    if not isinstance(means, torch.Tensor) or not means.is_cuda:
+        raise TypeError("means must be a CUDA tensor")
+    if means.dtype != torch.bfloat16:
+        raise UnsupportedOp(f"{op}: means must be bfloat16")
+    b, h, d = cfg.batch, cfg.kv_head_count, cfg.head_dim
+    if means.dim() != 4 or means.shape[:2] != (b, h) or means.shape[3] != d:
+        raise ShapeMismatch(f"{op}: means must be ({b}, {h}, blocks, {d}), got {tuple(means.shape)}")
+    blocks = means.shape[2]
+    row = means.stride(1) if h > 1 else means.stride(0) if b > 1 else blocks * d
+    if means.stride(3) != 1 or (blocks > 1 and means.stride(2) != d) or (h > 1 and b > 1 and
+                                                                         means.stride(0) != h * row):
+        raise ValueError("means must be contiguous, or a slice of blocks of a contiguous tensor")
+    return blocks, row
+
+
+def kv_block_means(cache: GpuKvCache, layer: int, block_begin: int, block_end: int, *,
+                   out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Mean rotated keys of blocks of 64 cached tokens, bf16 (B, H, blocks, D) (sa_kv_block_means).
+
+    A serving loop keeps one tensor of all blocks per layer and updates the ones that filled up:
+    ``kv_block_means(cache, layer, i, j, out=means[:, :, i:j])``.
+    """
+    cfg = cache.config
+    n = max(int(block_end) - int(block_begin), 0)
+    if out is None:
+        out = torch.empty(cfg.batch, cfg.kv_head_count, n, cfg.head_dim, dtype=torch.bfloat16, device=cache.device)
+    blocks, row = _means_rows("kv_block_means", out, cache)
+    if blocks != n:
+        raise ShapeMismatch(f"kv_block_means: out holds {blocks} blocks, not {n}")
+    rc = lib.sa_kv_block_means(cache.handle, layer, out.data_ptr(), row, int(block_begin), int(block_end),
+                               _stream_handle(stream, cache.device))
+    _raise_op(rc, "kv_block_means")
+    return out
+
+
+def gqa_select_blocks(query: torch.Tensor, cache: GpuKvCache, layer: int, means: torch.Tensor, *, num_heads: int,
+                      max_blocks: int, sink_blocks: int = 1, local_blocks: int = 1,
+                      out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Blocks of 64 tokens each query token attends to: int32 (B, S, H, max_blocks), ascending, then -1.
+
+    ``query`` (B, S, Hq*D) rotated to positions p + s; ``means`` as kv_block_means writes them, from block 0
+    up to the query's own block at least.  The first ``sink_blocks`` and the last ``local_blocks`` blocks, and
+    of the others those with the largest exact scores, ties to the lower block (sa_gqa_select_blocks).
+    """
+    _rotated_query("gqa_select_blocks", query, cache, query)
+    b, s, _ = query.shape
+    blocks, row = _means_rows("gqa_select_blocks", means, cache)
+    shape = (b, s, cache.config.kv_head_count, max(int(max_blocks), 0))
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=query.device)
+    else:
+        _int32("gqa_select_blocks", out, shape, "out")
+    rc = lib.sa_gqa_select_blocks(cache.handle, layer, query.data_ptr(), _dtype_code(query), b, s, int(num_heads),
+                                  means.data_ptr(), row, blocks, int(max_blocks), int(sink_blocks), int(local_blocks),
+                                  out.data_ptr(), _stream_handle(stream, query.device))
+    _raise_op(rc, "gqa_select_blocks")
+    return out
+
+
+def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_ids: torch.Tensor, *, num_heads: int,
+                      scale: float | None = None, out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention over the listed blocks of 64 cached tokens (sa_gqa_sparse_attend).
+
+    ``query`` (B, S, Hq*D) rotated to positions p + s, own keys and values appended (position not advanced);
+    ``block_ids`` int32 (B, S, H, max_blocks), distinct ids, -1 = none (gqa_select_blocks).  Tokens after the
+    query's own position are masked; a query without blocks gives zeros.
+    """
+    out = _rotated_query("gqa_sparse_attend", query, cache, out)
+    b, s, _ = query.shape
+    if not isinstance(block_ids, torch.Tensor) or block_ids.dim() != 4:
+        raise ShapeMismatch("gqa_sparse_attend: block_ids must be rank-4")
+    _int32("gqa_sparse_attend", block_ids, (b, s, cache.config.kv_head_count, block_ids.shape[3]), "block_ids")
+    workspace = _workspace(workspace, lib.sa_gqa_sparse_workspace_bytes(cache.handle, s), query.device)
+    rc = lib.sa_gqa_sparse_attend(cache.handle, layer, query.data_ptr(), block_ids.data_ptr(), block_ids.shape[3],
+                                  out.data_ptr(), _dtype_code(query), b, s, int(num_heads), int(scale is not None),
+                                  float(scale or 0.0), None if workspace is None else workspace.data_ptr(),
+                                  0 if workspace is None else workspace.numel(), _stream_handle(stream, query.device))
+    _raise_op(rc, "gqa_sparse_attend")
+    return out
+
+
 def matmul_nbits(a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor | None = None,
                  bias: torch.Tensor | None = None, *, K: int, N: int, bits: int = 4, block_size: int = 32,
                  out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
