@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(320) decode_prep8_kernel(AttendArgs a, AppendA
         for (int r = 0; r < EPL; r++) x[r] *= sg[lane * EPL + r];
         warp_wht_butterfly<EPL>(x, lane, D);
         float mabs = 0.0f;
-        const float *vtr = a.lr_vtr ? a.lr_vtr + bh * D : nullptr;
+        const float *vtr = a.lr_vtr ? a.lr_vtr + kv_unit(a, (int)bh) * D : nullptr;
 #pragma unroll
         for (int r = 0; r < EPL; r++) {
             x[r] *= a.wht_scale;
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(320) decode_prep8_kernel(AttendArgs a, AppendA
 }
 
 // ---- decode: stream-K warp ranges over eight heads -------------------------------
-template <typename T, int BITS, int D>
+template <typename T, int BITS, int D, bool LIST>
 __global__ void __launch_bounds__(kNW8 * 32, 1)
     decode8_stream_kernel(AttendArgs a, int ncu, int F, int W, const uint32_t *__restrict__ qfrag,
                           const float *__restrict__ qscal) {
@@ -186,13 +186,22 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
     if (w >= W) return;
     const int f0 = (int)((int64_t)w * F / W), f1 = (int)((int64_t)(w + 1) * F / W);
     const int total = (int)a.pos0 + 1;
+    const BlockList list(a);
 
     unsigned pend = 0;
     bool failed = false;
     auto issue = [&](int s, int uu, int c, int kind) {
         constexpr uint32_t kCodeBytes = CT * KB, kMetaBytes = CT * 8;
-        const int64_t row = (int64_t)uu * a.capacity + c * CT;
+        int64_t row = (int64_t)uu * a.capacity + c * CT;
         uint64_t *bar = mybar + s;
+        if constexpr (LIST) {
+            if (list.tokens<CT>(uu, c) == 0) {  // no block here, or none of its tokens seen: an empty phase
+                if (lane == 0) mbar_arrive(bar);
+                pend |= 1u << (2 * s + kind);
+                return;
+            }
+            row = list.row<CT>(uu, c);
+        }
         if (lane == 0) mbar_expect_tx(bar, kCodeBytes + (kind == 0 ? 2 * kMetaBytes : kMetaBytes));
         if (lane < 3 - kind) {
             const void *src;
@@ -230,7 +239,7 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
     int u = f0 / ncu, ubase = u * ncu, fs = f0;
     int ns = min(2, min(f1, ubase + ncu) - fs);
     {
-        const bool new0 = fs - ubase == ncu - 1, new1 = ns > 1 && fs - ubase + 1 == ncu - 1;
+        const bool new0 = LIST || fs - ubase == ncu - 1, new1 = ns > 1 && (LIST || fs - ubase + 1 == ncu - 1);
         if (!new0) issue(0, u, fs - ubase, 0);
         if (ns < 2) issue_empty(1, 0);
         else if (!new1) issue(1, u, fs - ubase + 1, 0);
@@ -270,7 +279,12 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
             nsn = min(2, min(f1, ubn + ncu) - fn);
         }
         const int c0 = fs - ubase;
-        const int n_w = min(total - c0 * CT, ns * CT);
+        const int n_w = min(total - c0 * CT, ns * CT);       // tokens in the sub-segment
+        int n_c[2] = {0, 0};                                 // with a block list: tokens seen of each chunk
+        if constexpr (LIST) {
+            n_c[0] = list.tokens<CT>(u, c0);
+            if (ns > 1) n_c[1] = list.tokens<CT>(u, c0 + 1);
+        }
 
         // ---------------- phase 1: scores of the eight heads ----------------
         float rma = -INFINITY, rmb = -INFINITY, vmax = 0.0f;  // max score of heads q, q + 4; max vscale
@@ -344,7 +358,7 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
                             const float db = fmaf((float)acc[1][2 * hf], 65536.0f,
                                                   (float)(acc[1][2 * hf + 1] * 256 + acc[2][2 * hf + 1]));
                             const float2 km = *reinterpret_cast<const float2 *>(kms + 2 * row);
-                            const bool in = tl < n_w;
+                            const bool in = LIST ? row < n_c[cc] : tl < n_w;
                             const float sa_ = in ? fmaf(km.x * c1a, da, km.y * c2a) : -INFINITY;
                             const float sb_ = in ? fmaf(km.x * c1b, db, km.y * c2b) : -INFINITY;
                             vmax = fmaxf(vmax, in ? vms[2 * row] : 0.0f);
@@ -370,12 +384,13 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
         // new references of heads ph and 4 + ph (lane ph holds the maxima of heads ph and ph + 4)
         float Rq[2];
         {
+            if constexpr (LIST) vmax = fmaxf(vmax, kVScaleMin);
             const float lv = __log2f(vmax);
             const float mx[2] = {__shfl_sync(0xffffffffu, rma, ph), __shfl_sync(0xffffffffu, rmb, ph)};
 #pragma unroll
             for (int hh = 0; hh < 2; hh++) {
                 const float Rp = fmaxf(Rr[hh], mx[hh] + lv);
-                Rq[hh] = Rp - kLog2UMax;
+                Rq[hh] = LIST && Rp == -INFINITY ? 0.0f : Rp - kLog2UMax;  // chunks that show no token: R stays -inf
                 const float fac = (Rr[hh] == -INFINITY) ? 0.0f : exp2f(Rr[hh] - Rp);
                 Rr[hh] = Rp;
                 Lr[hh] *= fac;
@@ -410,7 +425,8 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
                             const float4 m01 = *reinterpret_cast<const float4 *>(vms + 2 * tc);
                             const float4 m23 = *reinterpret_cast<const float4 *>(vms + 2 * tc + 4);
                             const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
-                            const float vs[4] = {m01.x, m01.z, m23.x, m23.z}, vz[4] = {m01.y, m01.w, m23.y, m23.w};
+                            float vs[4] = {m01.x, m01.z, m23.x, m23.z}, vz[4] = {m01.y, m01.w, m23.y, m23.w};
+                            if constexpr (LIST) mask_unseen(n_c[cc] < CT, sv, vs, vz);
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const float ee = ex2_approx(sv[e] - Rq[hh]);
@@ -537,7 +553,7 @@ template <int BITS, int D>
 DecodeGrid8 decode8_grid(const AttendArgs &a) {
     using GG = G8Geo<BITS, D>;
     DecodeGrid8 g;
-    const int64_t total = a.pos0 + 1;
+    const int64_t total = a.block_ids ? (int64_t)a.max_blocks * kBlockTokens : a.pos0 + 1;
     g.ncu = (int)((total + GG::CT - 1) / GG::CT);
     g.F = a.batch * a.heads * g.ncu;
     g.W = min(a.sm_count * kNW8, g.F);
@@ -545,7 +561,7 @@ DecodeGrid8 decode8_grid(const AttendArgs &a) {
     return g;
 }
 
-template <typename T, int BITS, int D>
+template <typename T, int BITS, int D, bool LIST>
 int launch8_shape(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream) {
     using GG = G8Geo<BITS, D>;
     uint32_t *qfrag = a.qprep;
@@ -570,7 +586,7 @@ int launch8_shape(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream
     count_launch();
     if (rc != SA_OK) return rc;
 
-    auto kern = decode8_stream_kernel<T, BITS, D>;
+    auto kern = decode8_stream_kernel<T, BITS, D, LIST>;
     const size_t smem = GG::SMEM;
     static int configured[64];
     int dev = 0;
@@ -601,12 +617,17 @@ int launch8_shape(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream
     return rc;
 }
 
+template <typename T, bool LIST>
+int launch8_format(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream) {
+    if (a.bits == 4 && a.head_dim == 128) return launch8_shape<T, 4, 128, LIST>(a, ap, stream);
+    if (a.bits == 8 && a.head_dim == 128) return launch8_shape<T, 8, 128, LIST>(a, ap, stream);
+    if (a.bits == 4 && a.head_dim == 64) return launch8_shape<T, 4, 64, LIST>(a, ap, stream);
+    return launch8_shape<T, 8, 64, LIST>(a, ap, stream);
+}
+
 template <typename T>
 int launch8_dtype(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream) {
-    if (a.bits == 4 && a.head_dim == 128) return launch8_shape<T, 4, 128>(a, ap, stream);
-    if (a.bits == 8 && a.head_dim == 128) return launch8_shape<T, 8, 128>(a, ap, stream);
-    if (a.bits == 4 && a.head_dim == 64) return launch8_shape<T, 4, 64>(a, ap, stream);
-    return launch8_shape<T, 8, 64>(a, ap, stream);
+    return a.block_ids ? launch8_format<T, true>(a, ap, stream) : launch8_format<T, false>(a, ap, stream);
 }
 
 }  // namespace

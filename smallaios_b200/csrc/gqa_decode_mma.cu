@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(192) decode_prep_kernel(AttendArgs a, AppendAr
     for (int r = 0; r < EPL; r++) x[r] *= sg[lane * EPL + r];
     warp_wht_butterfly<EPL>(x, lane, D);
     float sum = 0.0f, mabs = 0.0f;
-    const float *vtr = a.lr_vtr ? a.lr_vtr + bh * D : nullptr;
+    const float *vtr = a.lr_vtr ? a.lr_vtr + kv_unit(a, (int)bh) * D : nullptr;
 #pragma unroll
     for (int r = 0; r < EPL; r++) {
         x[r] *= a.wht_scale;
@@ -184,7 +184,7 @@ struct WGeo {
     static constexpr int SMEM = kNW * 2 * SLOT + kNW * SCW * 4 + kNW * 12 * kTileW * 4 + 256;
 };
 
-template <typename T, int BITS, int D>
+template <typename T, int BITS, int D, bool LIST>
 __global__ void __launch_bounds__(kNW * 32, 2)
     decode_stream_kernel(AttendArgs a, int ncu, int F, int W, const uint32_t *__restrict__ qfrag,
                          const float *__restrict__ qscal) {
@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
     if (w >= W) return;
     const int f0 = (int)((int64_t)w * F / W), f1 = (int)((int64_t)(w + 1) * F / W);
     const int total = (int)a.pos0 + 1;
+    const BlockList list(a);
 
     // Copies of a chunk, one per lane: K chunk = codes (lane 0), K meta
     // (lane 1), V meta (lane 2); V chunk = codes (lane 0), V meta (lane 1).
@@ -230,8 +231,16 @@ __global__ void __launch_bounds__(kNW * 32, 2)
     // finite and masked by their -inf scores.
     auto issue = [&](int s, int uu, int c, int kind) {
         constexpr uint32_t kCodeBytes = CT * KB, kMetaBytes = CT * 8;
-        const int64_t row = (int64_t)uu * a.capacity + c * CT;  // first token of the chunk
+        int64_t row = (int64_t)uu * a.capacity + c * CT;  // first token of the chunk
         uint64_t *bar = mybar + s;
+        if constexpr (LIST) {
+            if (list.tokens<CT>(uu, c) == 0) {  // no block here, or none of its tokens seen: an empty phase
+                if (lane == 0) mbar_arrive(bar);
+                pend |= 1u << (2 * s + kind);
+                return;
+            }
+            row = list.row<CT>(uu, c);
+        }
         if (lane == 0) mbar_expect_tx(bar, kCodeBytes + (kind == 0 ? 2 * kMetaBytes : kMetaBytes));
         if (lane < 3 - kind) {
             const void *src;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
         // The first K chunks; one that holds the newest token (appended by
         // the prep kernel) is fetched after waiting for that kernel, the
         // older ones before.
-        const bool new0 = fs - ubase == ncu - 1, new1 = ns > 1 && fs - ubase + 1 == ncu - 1;
+        const bool new0 = LIST || fs - ubase == ncu - 1, new1 = ns > 1 && (LIST || fs - ubase + 1 == ncu - 1);
         if (!new0) issue(0, u, fs - ubase, 0);
         if (ns < 2) issue_empty(1, 0);
         else if (!new1) issue(1, u, fs - ubase + 1, 0);
@@ -308,6 +317,11 @@ __global__ void __launch_bounds__(kNW * 32, 2)
         }
         const int c0 = fs - ubase;                           // first chunk within the unit
         const int n_w = min(total - c0 * CT, ns * CT);       // tokens in the sub-segment
+        int n_c[2] = {0, 0};                                 // with a block list: tokens seen of each chunk
+        if constexpr (LIST) {
+            n_c[0] = list.tokens<CT>(u, c0);
+            if (ns > 1) n_c[1] = list.tokens<CT>(u, c0 + 1);
+        }
 
         // ---------------- phase 1: scores ----------------
         float rmax = -INFINITY, vmax = 0.0f;  // max score of head q, max vscale
@@ -376,7 +390,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
                             const float dot = fmaf((float)acc[0][2 * hf], 65536.0f,
                                                    (float)(acc[0][2 * hf + 1] * 256 + acc[1][2 * hf]));
                             const float2 km = *reinterpret_cast<const float2 *>(kms + 2 * row);
-                            const bool in = tl < n_w;
+                            const bool in = LIST ? row < n_c[cc] : tl < n_w;
                             const float s = in ? fmaf(km.x * c1, dot, km.y * c2) : -INFINITY;
                             vmax = fmaxf(vmax, in ? vms[2 * row] : 0.0f);
                             if (my_head) {
@@ -397,10 +411,12 @@ __global__ void __launch_bounds__(kNW * 32, 2)
             rmax = fmaxf(rmax, __shfl_xor_sync(0xffffffffu, rmax, m));
             vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, m));
         }
+        if constexpr (LIST) vmax = fmaxf(vmax, kVScaleMin);
         // new reference of head ph (lane ph holds head ph's max; u = 2^(s - R) * vscale <= 1)
         // and the factor that moves earlier sums to it
         const float Rp = fmaxf(Rr, __shfl_sync(0xffffffffu, rmax, ph) + __log2f(vmax));
-        const float Rq = Rp - kLog2UMax;  // sums and digits are kept in units of 1 / kUMax
+        // sums and digits are kept in units of 1 / kUMax; chunks that show no token leave R at -inf
+        const float Rq = LIST && Rp == -INFINITY ? 0.0f : Rp - kLog2UMax;
         const float fac = (Rr == -INFINITY) ? 0.0f : exp2f(Rr - Rp);
         Rr = Rp;
         Lr *= fac;
@@ -432,7 +448,8 @@ __global__ void __launch_bounds__(kNW * 32, 2)
                         const float4 m01 = *reinterpret_cast<const float4 *>(vms + 2 * tc);
                         const float4 m23 = *reinterpret_cast<const float4 *>(vms + 2 * tc + 4);
                         const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
-                        const float vs[4] = {m01.x, m01.z, m23.x, m23.z}, vz[4] = {m01.y, m01.w, m23.y, m23.w};
+                        float vs[4] = {m01.x, m01.z, m23.x, m23.z}, vz[4] = {m01.y, m01.w, m23.y, m23.w};
+                        if constexpr (LIST) mask_unseen(n_c[cc] < CT, sv, vs, vz);
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float ee = ex2_approx(sv[e] - Rq);  // kUMax * 2^(s - R)
@@ -567,7 +584,7 @@ template <int BITS, int D>
 DecodeGrid decode_grid(const AttendArgs &a) {
     using GG = WGeo<BITS, D>;
     DecodeGrid g;
-    const int64_t total = a.pos0 + 1;
+    const int64_t total = a.block_ids ? (int64_t)a.max_blocks * kBlockTokens : a.pos0 + 1;
     g.ncu = (int)((total + GG::CT - 1) / GG::CT);
     g.F = a.batch * a.heads * g.ncu;  // fits int: decode_fast_eligible bounds it
     g.W = min(2 * a.sm_count * kNW, g.F);
@@ -575,7 +592,7 @@ DecodeGrid decode_grid(const AttendArgs &a) {
     return g;
 }
 
-template <typename T, int BITS, int D>
+template <typename T, int BITS, int D, bool LIST>
 int launch_shape(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream) {
     uint32_t *qfrag = a.qprep;
     float *qscal = reinterpret_cast<float *>(a.qprep + (size_t)a.batch * a.heads * 32 * 16);
@@ -602,7 +619,7 @@ int launch_shape(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream)
     if (rc != SA_OK) return rc;
 
     using GG = WGeo<BITS, D>;
-    auto kern = decode_stream_kernel<T, BITS, D>;
+    auto kern = decode_stream_kernel<T, BITS, D, LIST>;
     const size_t smem = GG::SMEM;
     static int configured[64];
     int dev = 0;
@@ -632,12 +649,17 @@ int launch_shape(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream)
     return rc;
 }
 
+template <typename T, bool LIST>
+int launch_format(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream) {
+    if (a.bits == 4 && a.head_dim == 128) return launch_shape<T, 4, 128, LIST>(a, ap, stream);
+    if (a.bits == 8 && a.head_dim == 128) return launch_shape<T, 8, 128, LIST>(a, ap, stream);
+    if (a.bits == 4 && a.head_dim == 64) return launch_shape<T, 4, 64, LIST>(a, ap, stream);
+    return launch_shape<T, 8, 64, LIST>(a, ap, stream);
+}
+
 template <typename T>
 int launch_dtype(const AttendArgs &a, const AppendArgs *ap, cudaStream_t stream) {
-    if (a.bits == 4 && a.head_dim == 128) return launch_shape<T, 4, 128>(a, ap, stream);
-    if (a.bits == 8 && a.head_dim == 128) return launch_shape<T, 8, 128>(a, ap, stream);
-    if (a.bits == 4 && a.head_dim == 64) return launch_shape<T, 4, 64>(a, ap, stream);
-    return launch_shape<T, 8, 64>(a, ap, stream);
+    return a.block_ids ? launch_format<T, true>(a, ap, stream) : launch_format<T, false>(a, ap, stream);
 }
 
 }  // namespace
@@ -659,7 +681,8 @@ bool decode_fast_eligible(const AttendArgs &a) {
     if ((a.bits != 4 && a.bits != 8) || (a.head_dim != 64 && a.head_dim != 128)) return false;
     if (a.capacity % 64 != 0 || a.qprep == nullptr || a.dev_status == nullptr) return false;
     const int64_t units = (int64_t)a.batch * a.heads;
-    if (units * ((a.pos0 + 32) / 32) >= ((int64_t)1 << 31)) return false;  // flat chunk indices are int
+    const int64_t chunks = a.block_ids ? 2 * (int64_t)a.max_blocks : (a.pos0 + 32) / 32;
+    if (units * chunks >= ((int64_t)1 << 31)) return false;  // flat chunk indices are int
     return decode_workspace_floats(a.sm_count, units, a.head_dim, a.group) <= a.workspace_floats;
 }
 

@@ -99,6 +99,50 @@ __device__ __forceinline__ void v_inv(int dim, int &nt, int &col) {
     }
 }
 
+// ---- block lists -----------------------------------------------------------------
+// Unit of the cache (batch row, KV head) behind unit u of the launch, which is (query row, KV head):
+// with a block list a batch row has list_rows query rows, the first of the launch being row0.
+__device__ __forceinline__ int64_t kv_unit(const AttendArgs &a, int u) {
+    if (!a.block_ids) return u;
+    return (int64_t)((a.row0 + u / a.heads) / a.list_rows) * a.heads + u % a.heads;
+}
+
+// The chunks of CT tokens of a unit's listed blocks, laid end to end.
+struct BlockList {
+    const AttendArgs &a;
+    __device__ __forceinline__ explicit BlockList(const AttendArgs &args) : a(args) {}
+    // Position of the chunk's first token; past every position where the list has no block.
+    template <int CT>
+    __device__ __forceinline__ int64_t first(int u, int c) const {
+        constexpr int CPB = kBlockTokens / CT;
+        const int id = a.block_ids[(int64_t)u * a.max_blocks + c / CPB];
+        return id < 0 ? INT64_MAX : (int64_t)id * kBlockTokens + (c % CPB) * CT;
+    }
+    // Tokens of the chunk at or before the query's position.
+    template <int CT>
+    __device__ __forceinline__ int tokens(int u, int c) const {
+        const int64_t total = a.pos0 + (a.row0 + u / a.heads) % a.list_rows + 1, t = first<CT>(u, c);
+        return t >= total ? 0 : (int)(total - t < CT ? total - t : CT);
+    }
+    // Row of the cache that holds the chunk's first token (of a chunk with tokens).
+    template <int CT>
+    __device__ __forceinline__ int64_t row(int u, int c) const {
+        return kv_unit(a, u) * a.capacity + first<CT>(u, c);
+    }
+};
+
+// Below this the largest value scale of some tokens counts as this (the log2 of the reference).
+constexpr float kVScaleMin = 1.17549435e-38f;
+
+// Tokens that the query does not see (score -inf) take no part in the sums, whatever their metadata
+// holds; `some`: the chunk has such tokens.
+__device__ __forceinline__ void mask_unseen(bool some, const float (&s)[4], float (&vs)[4], float (&vz)[4]) {
+    if (!some) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (s[e] == -INFINITY) vs[e] = vz[e] = 0.0f;
+}
+
 // ---- stream-K records and their merge -------------------------------------------
 // Warp owning flat chunk f when F chunks are cut into W ranges
 // [w*F/W, (w+1)*F/W): the largest w with w*F/W <= f.
@@ -213,9 +257,10 @@ __device__ __forceinline__ void decode_merge_head(const AttendArgs &a, int ncu, 
     }
     L = warp_sum(L);
     Z = warp_sum(Z);
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const bool counts = L > 0.0f || (a.block_ids && L != 0.0f);  // a NaN sum spoils a row of a block list
+    const float inv = counts ? 1.0f / L : 0.0f;
 #pragma unroll
-    for (int rr = 0; rr < EPL; rr++) x[rr] = L > 0.0f ? (x[rr] + Z) * inv : 0.0f;
+    for (int rr = 0; rr < EPL; rr++) x[rr] = counts ? (x[rr] + Z) * inv : 0.0f;
     warp_wht_butterfly<EPL>(x, lane, D);
     const int h = u % a.heads;
 #pragma unroll

@@ -152,6 +152,9 @@ struct AttendArgs {
     // block lists (nullptr: off): [batch][seq_len][heads][max_blocks] ascending block ids, -1 = none
     const int32_t *block_ids;
     int max_blocks;
+    // tensor-core decode over block lists: batch = query rows of the launch (seq_len 1), list_rows
+    // of them per cache row, the launch's first being row0
+    int list_rows, row0;
 };
 
 // Moves drafted rows of every layer (sa_kv_cache_keep_drafts).

@@ -75,6 +75,29 @@ AttendArgs attend_args(kv_cache_impl *k, int32_t layer, const void *query, void 
     return a;
 }
 
+// Query rows of one launch of the tensor-core decode over block lists: bounds its workspace.
+constexpr int64_t kListUnits = 16384;
+
+int64_t list_rows_per_launch(const kv_cache_impl *k, int64_t rows) {
+    const int64_t most = kListUnits / k->cfg.kv_head_count > 0 ? kListUnits / k->cfg.kv_head_count : 1;
+    return rows < most ? rows : most;
+}
+
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Bytes of the partial records, and of the q digits behind them, of a launch of `rows` query rows.
+void list_workspace(const kv_cache_impl *k, int64_t rows, size_t *records, size_t *digits) {
+    const int64_t units = rows * k->cfg.kv_head_count;
+    *records = align256(decode_workspace_floats(k->sm_count, units, k->cfg.head_dim, k->group) * sizeof(float));
+    *digits = align256((size_t)units * decode_qprep_words(k->group) * sizeof(uint32_t));
+}
+
+// Whether block lists go to the tensor-core decode.
+bool list_decode_format(const kv_cache_impl *k) {
+    return (k->cfg.bits == 4 || k->cfg.bits == 8) && (k->cfg.head_dim == 64 || k->cfg.head_dim == 128) &&
+           k->group <= 8;
+}
+
 }  // namespace
 
 extern "C" {
@@ -223,8 +246,12 @@ int sa_gqa_select_blocks(sa_kv_cache *cache, int32_t layer, const void *query, i
 }
 
 int64_t sa_gqa_sparse_workspace_bytes(const sa_kv_cache *cache, int32_t seq_len) {
-    if (!cache || seq_len <= 0) return 0;
-    return 0;
+    const kv_cache_impl *k = reinterpret_cast<const kv_cache_impl *>(cache);
+    // one query token per sequence fits the cache's own workspace, which the decode step uses too
+    if (!cache || seq_len <= 1 || !list_decode_format(k)) return 0;
+    size_t records, digits;
+    list_workspace(k, list_rows_per_launch(k, (int64_t)k->cfg.batch * seq_len), &records, &digits);
+    return (int64_t)(records + digits);
 }
 
 int sa_gqa_sparse_attend(sa_kv_cache *cache, int32_t layer, const void *query, const int32_t *block_ids,
@@ -246,7 +273,31 @@ int sa_gqa_sparse_attend(sa_kv_cache *cache, int32_t layer, const void *query, c
     AttendArgs a = attend_args(k, layer, query, attn_out, dtype, batch, seq_len, has_scale, scale);
     a.block_ids = block_ids;
     a.max_blocks = max_blocks;
-    return launch_gqa_attend_generic(a, static_cast<cudaStream_t>(stream));
+    if (!list_decode_format(k)) return launch_gqa_attend_generic(a, static_cast<cudaStream_t>(stream));
+    const int64_t rows = (int64_t)batch * seq_len, per = seq_len == 1 ? rows : list_rows_per_launch(k, rows);
+    const int64_t row_bytes = (int64_t)a.heads * a.group * a.head_dim * (dtype == SA_DTYPE_FLOAT ? 4 : 2);
+    a.list_rows = seq_len;
+    a.seq_len = 1;
+    if (seq_len > 1) {
+        size_t records, digits;
+        list_workspace(k, per, &records, &digits);
+        a.workspace = static_cast<float *>(workspace);
+        a.workspace_floats = records / sizeof(float);
+        a.qprep = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + records);
+    }
+    for (int64_t r0 = 0; r0 < rows; r0 += per) {
+        a.batch = (int)(rows - r0 < per ? rows - r0 : per);
+        a.row0 = (int)r0;
+        a.query = static_cast<const char *>(query) + r0 * row_bytes;
+        a.out = static_cast<char *>(attn_out) + r0 * row_bytes;
+        a.block_ids = block_ids + r0 * a.heads * max_blocks;
+        if (a.batch > 65535 || !decode_fast_eligible(a))
+            return set_error(SA_ERR_UNSUPPORTED, "gqa_sparse_attend: %d rows of %d blocks in one launch", a.batch,
+                             max_blocks);
+        rc = launch_gqa_decode_fast(a, nullptr, static_cast<cudaStream_t>(stream));
+        if (rc != SA_OK) return rc;
+    }
+    return SA_OK;
 }
 
 }  // extern "C"
