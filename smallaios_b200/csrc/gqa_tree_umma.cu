@@ -1,0 +1,878 @@
+// Attention of a draft tree over the compressed cache on the 5th-generation
+// tensor cores: the R = nodes * G query rows of one KV head against the whole
+// context, in the rotated domain, with everything transposed -- tokens (then
+// dimensions) are the MMA's M, the query rows its N:
+//
+//   S^T[t][r]  = sum_d (c_td - C) q^_rd                      (M = 128 tokens, N = rows)
+//   s_tr       = ks_t S^T + (kz_t + C ks_t) sum(q^_r)         (log2 units; ks, kz: scale, zero point)
+//   u_tr       = vs_t 2^(s_tr - ref_r)
+//   O^T[d][r] += sum_t (c_td - C) u_tr                        (M = dimensions, N = rows)
+//   l_r += u_tr / vs_t,   z_r += u_tr (vz_t + C vs_t) / vs_t
+//   o'_r = (O_r + z_r) / l_r,   out = S.H.o' / sqrt(D)
+//
+// C = 8 or 128 centres the codes, so no sum carries the codes' mean, which the
+// zero point would have to cancel.  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
+// power of two common to the row block, in one fp16 plane (11 bits: bf16 callers)
+// or two (22 bits: f16 and f32), u in one (bf16, f16) or two (f32); sum(q^) is of
+// the rounded values, so their rounding only moves the query by its own.
+// Everything else is f32.
+//
+// Transposed, a thread of the softmax holds one token: its scale and zero point
+// are registers, not loads per score, and N follows the number of rows (16, 32 or
+// 64), so a tree of few rows costs few MMA columns.  The codes become fp16 in
+// tensor memory, as the A operands: an integer below 1024 or-ed into the mantissa
+// of 1024 is a float, one packed subtraction centres two.
+//
+// One persistent CTA per SM; roles by warp:
+//   4 * NG softmax warps (NG = NR / 16 groups of four): thread = token of the
+//     tile, 16 rows per group: tcgen05.ld of S^T, u, the sums l and z of its
+//     token, u to shared memory (the B operand, rows contiguous).  The reference
+//     ref_r is only raised when some score of the tile outgrows it by 2^8 (one
+//     vote per tile and group); then O is rescaled in tensor memory.
+//   4 K warps, 4 V warps: codes of the tile from shared memory to fp16 in tensor
+//     memory (thread = token for K, dimension for V), two buffers each.
+//   1 MMA warp: S^T(i), then O^T of tile i - 1.
+//   1 copy warp: codes and metadata of the tiles by bulk copies into a ring.
+// The tiles of all units (batch row, KV head) are laid end to end and cut into
+// equal ranges; row blocks beyond the first 64 rows run in CTAs of their own that
+// walk the same ranges at the same time, so the cache is read from HBM once.  A
+// CTA leaves one partial record per unit that it touches; a merge kernel joins
+// them, rotates back and stores.
+//
+// Every mbarrier wait is bounded (2 s); one that gives up sets the abort flag and
+// bit 0 of the cache's status word, every role leaves its loop, issued copies and
+// MMAs are waited for (bounded) and TMEM is freed; the records are then not valid.
+#include <type_traits>
+
+#include "sa_append.cuh"
+#include "sa_async.cuh"
+#include "sa_common.cuh"
+#include "sa_internal.h"
+#include "sa_tcgen05.cuh"
+
+namespace sa {
+
+namespace {
+
+constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
+constexpr int kCols = 16;       // query rows per softmax group
+constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
+constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
+constexpr int kPrepThreads = 256;
+constexpr int kMergeWarps = 8;
+
+template <int BITS, int D, int NR, int QP, int PP>
+struct Tg {
+    static constexpr int CB = D * BITS / 8;
+    static constexpr int NG = NR / kCols;                   // softmax groups
+    static constexpr int THREADS = 32 * (4 * NG + 10);
+    static constexpr int PBUF = PP * kTok * 128;            // u planes of a tile: [128 tokens][64 rows], 128-byte swizzle
+    static constexpr int QPLANE = NR * D * 2;               // D/64 tiles of [NR rows][128 B]
+    static constexpr int QREC = QP * QPLANE + NR * 4 + 16;  // planes, sum(q^) of the rows, power of two
+    static constexpr int QBUF = (QREC + 1023) / 1024 * 1024;
+    static constexpr int SLOT = kTok * (2 * CB + 16);       // K codes, V codes, K metadata, V metadata
+    static constexpr int P_OFF = 0, Q_OFF = 2 * PBUF, SLOT_OFF = Q_OFF + 2 * QBUF;
+    static constexpr int MISC = 6 * 1024;
+    static constexpr int ROOM = (226 * 1024 - SLOT_OFF - MISC) / SLOT;
+    static constexpr int NST = ROOM > 4 ? 4 : ROOM;         // ring slots
+    static constexpr int MISC_OFF = SLOT_OFF + NST * SLOT;
+    static constexpr int SMEM = MISC_OFF + MISC + 1024;     // + slack to align the base to 1024 B
+    // TMEM columns: K and V operands (two buffers each), S^T (two), O^T
+    static constexpr uint32_t KA = 0, VA = D, S = VA + kTok, O = S + 2 * NR;
+    static constexpr int REC = NR * D + 3 * NR;             // floats of a partial record: O rows, ref, l, z
+    static_assert(NST >= 2 && SMEM <= 227 * 1024 && O + NR <= 512, "tree kernel resources");
+};
+
+struct TreeArgs {
+    AttendArgs a;
+    const unsigned char *qimg;  // [unit][row block] query images
+    const uint64_t *path;       // [batch][64] ancestors and self of each node, 0: no node
+    float *records;
+    int rows;                   // nodes * group
+    int nb;                     // row blocks
+    int ntiles, F, groups;      // tiles per unit, of all units, ranges they are cut into
+};
+
+// Byte offset of 16-byte chunk c (0..7) of row r in a [rows][128 B] 128-byte-swizzle tile.
+__device__ __forceinline__ uint32_t sw128(int r, int c) {
+    return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
+}
+
+// Position along K of dimension e in the K operand, as the conversion of a 32-bit word leaves its
+// codes: 4 bits 0 4 1 5 2 6 3 7 of eight, 8 bits 0 2 1 3 of four.
+template <int BITS>
+__host__ __device__ __forceinline__ int k_position(int e) {
+    if (BITS == 4) return (e & ~7) | ((e & 3) << 1) | ((e >> 2) & 1);
+    return (e & ~3) | ((e & 1) << 1) | ((e >> 1) & 1);
+}
+
+// Position along K of token t in the V operand: 0 2 1 3 of every four.
+__device__ __forceinline__ int v_slot(int t) { return (t & ~3) | ((t & 1) << 1) | ((t >> 1) & 1); }
+
+// Instruction descriptor, kind::f16: D f32, A and B fp16, A K-major, M = 128, N = n; B K-major or
+// (mn != 0) with its rows contiguous.
+__host__ __device__ constexpr uint32_t tg_idesc(int n, uint32_t mn) {
+    return (1u << 4) | (mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTok >> 4) << 24);
+}
+
+// (x & mask) | magic -> 1024 + code (or 1024 + 16 code), two at once, then centred
+__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t mask, __half2 mul, __half2 add) {
+    const uint32_t biased = (x & mask) | 0x64006400u;
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&biased), mul, add);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+__device__ __forceinline__ float tg_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 ra, rb, rc, rd;\nmov.b64 ra, {%2, %3};\nmov.b64 rb, {%4, %5};\nmov.b64 rc, {%6, %7};\n"
+        "fma.rn.f32x2 rd, ra, rb, rc;\nmov.b64 {%0, %1}, rd;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// OR of `v` over the 128 threads of a softmax group (named barrier 1 + group).
+__device__ __forceinline__ bool group_or(int group, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.or.pred p, %2, 128, q;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(r)
+        : "r"((uint32_t)v), "r"(1 + group)
+        : "memory");
+    return r != 0;
+}
+
+// Sum (or maximum) over the warp of 16 values per lane: lane L returns that of value L & 15.
+template <typename Op>
+__device__ __forceinline__ float warp_columns(float (&v)[kCols], int lane, Op op) {
+#pragma unroll
+    for (int h = kCols / 2; h >= 1; h >>= 1) {
+        const bool up = lane & h;
+#pragma unroll
+        for (int i = 0; i < h; i++) {
+            const float mine = up ? v[i + h] : v[i], give = up ? v[i] : v[i + h];
+            v[i] = op(mine, __shfl_xor_sync(0xffffffffu, give, h));
+        }
+    }
+    return op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
+}
+
+// ---- query images --------------------------------------------------------------------------------
+// grid = units * row blocks.  Rows are query rows r = node * G + head of the KV head; a warp rotates
+// NR / 8 of them.
+template <typename T, int BITS, int D, int NR, int QP>
+__global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, unsigned char *qimg, uint64_t *path) {
+    using G0 = Tg<BITS, D, NR, QP, 1>;
+    constexpr int EPL = D / 32, RW = NR / (kPrepThreads / 32);
+    const AttendArgs &a = t.a;
+    extern __shared__ __align__(16) unsigned char img[];
+    __shared__ int s_max, s_par[kMaxDraftNodes];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int u = blockIdx.x / t.nb, rb = blockIdx.x % t.nb, h = u % a.heads, b = u / a.heads;
+    if (tid == 0) s_max = 0;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const int nodes = a.seq_len;
+    if (h == 0 && rb == 0 && tid < nodes) s_par[tid] = a.parents[(int64_t)b * nodes + tid];
+    __syncthreads();
+    if (h == 0 && rb == 0 && tid < nodes) path[(int64_t)b * kMaxDraftNodes + tid] = tree_path(s_par, tid);
+
+    const float *sg = a.signs + (int64_t)h * D + lane * EPL;
+    const float mul = a.wht_scale * a.scale * 1.4426950408889634f;
+    float x[RW][EPL], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+        const int r = rb * NR + warp * RW + i;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) x[i][e] = 0.0f;
+        if (r < t.rows) {
+            const int node = r / a.group, g = r % a.group;
+            const T *src = static_cast<const T *>(a.query) +
+                           (((int64_t)b * nodes + node) * (a.heads * a.group) + h * a.group + g) * D;
+            load_elems<T, EPL>(src + lane * EPL, x[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+#pragma unroll
+        for (int e = 0; e < EPL; e++) x[i][e] *= sg[e];
+        warp_wht_butterfly<EPL>(x[i], lane, D);
+#pragma unroll
+        for (int e = 0; e < EPL; e++) {
+            x[i][e] *= mul;
+            const float m = fabsf(x[i][e]);
+            if (m < INFINITY) top = fmaxf(top, m);
+        }
+    }
+    top = warp_max(top);
+    if (lane == 0) atomicMax(&s_max, __float_as_int(top));  // non-negative floats order as their bits
+    __syncthreads();
+    // the largest |q'| into [2^11, 2^12): a common power of two costs the scores no operation, and what
+    // a small row loses to it is small against the largest row's scores
+    const int ex = max(((s_max >> 23) & 0xff) - 126, -100);
+    const float up = __int_as_float((12 - ex + 127) << 23), down = __int_as_float((ex - 12 + 127) << 23);
+    const float *vtr = a.lr_vtr ? a.lr_vtr + (int64_t)u * D + lane * EPL : nullptr;
+    float *qsum = reinterpret_cast<float *>(img + QP * G0::QPLANE);
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+        const int row = warp * RW + i;
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) {
+            const float y = x[i][e] * up;
+            const __half hi = __float2half_rn(y);
+            const float hf = __half2float(hi);
+            const int p = k_position<BITS>(lane * EPL + e);
+            unsigned char *dst = img + (p >> 6) * (NR * 128) + sw128(row, (p & 63) >> 3) + (p & 7) * 2;
+            *reinterpret_cast<__half *>(dst) = hi;
+            float kept = hf;
+            if (QP == 2) {
+                const __half lo = __float2half_rn(y - hf);
+                *reinterpret_cast<__half *>(dst + G0::QPLANE) = lo;
+                kept += __half2float(lo);
+            }
+            sum += vtr ? kept * vtr[e] : kept;  // sum(q^), or q^.V^T with low-rank K
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) qsum[row] = sum * down;
+    }
+    if (tid < 4) qsum[NR + tid] = down;
+    __syncthreads();
+    uint4 *out = reinterpret_cast<uint4 *>(qimg + (int64_t)blockIdx.x * G0::QBUF);
+    for (int i = tid; i < G0::QREC / 16; i += kPrepThreads) out[i] = reinterpret_cast<const uint4 *>(img)[i];
+}
+
+// ---- attention -------------------------------------------------------------------------------------
+template <int BITS, int D, int NR, int QP, int PP>
+__global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma_kernel(TreeArgs t) {
+    using GG = Tg<BITS, D, NR, QP, PP>;
+    constexpr int CB = GG::CB, NST = GG::NST, NG = GG::NG, SM = 4 * NG;
+    constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
+    const AttendArgs &a = t.a;
+    extern __shared__ unsigned char tg_raw[];
+    unsigned char *smem = tg_raw + ((1024 - (smem_u32(tg_raw) & 1023)) & 1023);
+    unsigned char *slots = smem + GG::SLOT_OFF;
+    float *ref = reinterpret_cast<float *>(smem + GG::MISC_OFF);       // [NR], minus kShift
+    float *fac = ref + 64;                                             // [NR]
+    float *red = fac + 64;                                             // [SM warps][16][2]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 16 * kCols * 2);
+    uint64_t *raw_full = bars, *raw_empty = bars + 4, *ka_full = bars + 8, *va_full = bars + 10, *qk_done = bars + 12,
+             *pv_done = bars + 14, *s_empty = bars + 16, *p_full = bars + 18, *q_full = bars + 20, *q_empty = bars + 22,
+             *bar_fin = bars + 24;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 25);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 26);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int grp = blockIdx.x / t.nb, rb = blockIdx.x % t.nb;
+    const int f0 = (int)((int64_t)grp * t.F / t.groups), f1 = (int)((int64_t)(grp + 1) * t.F / t.groups);
+    const int n = f1 - f0, u0 = f0 / t.ntiles, k0 = f0 % t.ntiles;
+    const int total = (int)a.pos0 + a.seq_len;
+
+    if (tid == 0) {
+        for (int i = 0; i < NST; i++) {
+            mbar_init(raw_full + i, 1);
+            mbar_init(raw_empty + i, 8 + SM);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(ka_full + i, 4);
+            mbar_init(va_full + i, 4);
+            mbar_init(qk_done + i, 1);
+            mbar_init(pv_done + i, 1);
+            mbar_init(s_empty + i, SM);
+            mbar_init(p_full + i, SM);
+            mbar_init(q_full + i, 1);
+            mbar_init(q_empty + i, 1 + SM);
+        }
+        mbar_init(bar_fin, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(tslot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = *tslot;
+    const uint32_t tl = tbase + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's lane quarter
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the query images and node paths; the drafts in the cache
+
+    auto wait = [&](uint64_t *bar, int phase) {
+        return __all_sync(0xffffffffu, tc_wait_sleep(bar, (uint32_t)(phase & 1), abort_flag, a.dev_status));
+    };
+
+    if (warp == SM + 9) {
+        // ================= copies =================
+        int u = u0, kt = k0, units = 0, issued = 0;
+        for (int i = 0; i < n; i++) {
+            const int st = i % NST;
+            bool ok = i < NST || wait(raw_empty + st, i / NST - 1);
+            if (ok && (i == 0 || kt == 0)) {
+                const int qb = units & 1;
+                ok = units < 2 || wait(q_empty + qb, units / 2 - 1);
+                if (ok && lane == 0) {
+                    mbar_expect_tx(q_full + qb, GG::QREC);
+                    bulk_g2s(smem + GG::Q_OFF + qb * GG::QBUF, t.qimg + ((int64_t)u * t.nb + rb) * GG::QBUF, GG::QREC,
+                             q_full + qb);
+                }
+                units++;
+            }
+            if (!ok) break;
+            // the cache holds whole blocks of 64 tokens: a tile's second half may lie past them
+            const int t0 = kt * kTok, nt = min(kTok, a.capacity - t0);
+            const int64_t row = (int64_t)u * a.capacity + t0;
+            unsigned char *slot = slots + st * GG::SLOT;
+            if (lane == 0) mbar_expect_tx(raw_full + st, (uint32_t)nt * (2 * CB + 16));
+            __syncwarp();
+            if (lane == 0) bulk_g2s(slot, a.k_codes + row * CB, (uint32_t)nt * CB, raw_full + st);
+            if (lane == 1) bulk_g2s(slot + kTok * CB, a.v_codes + row * CB, (uint32_t)nt * CB, raw_full + st);
+            if (lane == 2) bulk_g2s(slot + 2 * kTok * CB, a.k_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
+            if (lane == 3) bulk_g2s(slot + 2 * kTok * CB + kTok * 8, a.v_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
+            issued = i + 1;
+            if (++kt == t.ntiles) {
+                kt = 0;
+                u++;
+            }
+        }
+        if (*abort_flag) {
+            // let the copies in flight land before the CTA ends (bounded)
+            for (int i = max(0, issued - NST); i < issued; i++) mbar_wait_bounded(raw_full + i % NST, (uint32_t)(i / NST) & 1);
+            for (int i = max(0, units - 2); i < units; i++) mbar_wait_bounded(q_full + (i & 1), (uint32_t)(i / 2) & 1);
+        }
+    } else if (warp == SM + 8) {
+        // ================= MMA =================
+        constexpr uint32_t id_s = tg_idesc(NR, 0), id_o = tg_idesc(NR, 1);
+        int kt = k0, units = 0;
+        bool first_prev = true;  // whether tile i - 1 was the first of its unit here
+        for (int i = 0; i <= n; i++) {
+            const bool starts = i == 0 || kt == 0;
+            if (i < n) {
+                bool ok = wait(ka_full + (i & 1), i >> 1);
+                if (ok && i >= 2) ok = wait(s_empty + (i & 1), (i >> 1) - 1);
+                if (ok && starts) {
+                    ok = wait(q_full + (units & 1), units >> 1);
+                    units++;
+                }
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t q = smem_u32(smem + GG::Q_OFF + ((units - 1) & 1) * GG::QBUF);
+#pragma unroll
+                    for (int pl = 0; pl < QP; pl++)
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; kk++)
+                            umma_ts(tbase + GG::S + (i & 1) * NR, tbase + GG::KA + (i & 1) * (D / 2) + 8 * kk,
+                                    sw128_kmajor_desc(q + pl * GG::QPLANE + (kk >> 2) * (NR * 128) + 32 * (kk & 3)), id_s,
+                                    (pl | kk) != 0 ? 1u : 0u);
+                    umma_commit(qk_done + (i & 1));
+                    if (kt == t.ntiles - 1) umma_commit(q_empty + ((units - 1) & 1));  // the unit's last use of q
+                }
+                __syncwarp();
+            }
+            if (i > 0) {
+                const int j = i - 1;
+                if (!(wait(p_full + (j & 1), j >> 1) && wait(va_full + (j & 1), j >> 1))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t p = smem_u32(smem + GG::P_OFF + (j & 1) * GG::PBUF);
+#pragma unroll
+                    for (int pl = 0; pl < PP; pl++)
+#pragma unroll
+                        for (int kk = 0; kk < kTok / 16; kk++)
+                            // B: rows contiguous, 8-token groups 1024 B apart, the same fields as a K-major tile
+                            umma_ts(tbase + GG::O, tbase + GG::VA + (j & 1) * (kTok / 2) + 8 * kk,
+                                    sw128_kmajor_desc(p + pl * (kTok * 128) + 2048 * kk), id_o,
+                                    (pl | kk) != 0 || !first_prev ? 1u : 0u);
+                    umma_commit(pv_done + (j & 1));
+                }
+                __syncwarp();
+            }
+            first_prev = starts;
+            if (++kt == t.ntiles) kt = 0;
+        }
+        // every issued MMA has completed before TMEM is freed
+        if (elect_one()) umma_commit(bar_fin);
+        __syncwarp();
+        const uint64_t tw = um_clock_ns();
+        while (!um_try(bar_fin, 0) && um_clock_ns() - tw < kTcWaitNs) {
+        }
+    } else if (warp >= SM + 4) {
+        // ================= V codes -> fp16, thread = dimension =================
+        const int dim = 32 * (warp & 3) + lane;
+        const bool live = 32 * (warp & 3) < D;
+        const int j = BITS == 4 ? dim >> 1 : dim;                           // byte of the token's codes
+        const bool odd = BITS == 4 && (dim & 1);
+        const uint32_t mask = BITS == 8 ? 0x00ff00ffu : odd ? 0x00f000f0u : 0x000f000fu;
+        const __half2 mul = __float2half2_rn(odd ? 0.0625f : 1.0f);
+        const __half2 add = __float2half2_rn(BITS == 8 ? -1152.0f : odd ? -72.0f : -1032.0f);
+        for (int i = 0; i < n; i++) {
+            const int st = i % NST;
+            if (!wait(raw_full + st, i / NST)) break;
+            if (i >= 2 && !wait(pv_done + (i & 1), (i >> 1) - 1)) break;
+            tc_fence_after();
+            if (live) {
+                const unsigned char *src = slots + st * GG::SLOT + kTok * CB + (j >> 2) * 64 + (j & 3) * 4;
+#pragma unroll
+                for (int blk = 0; blk < kTok / 16; blk += 2) {
+                    uint32_t v[16];
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const uint32_t w =
+                            *reinterpret_cast<const uint32_t *>(src + (blk + (g >> 2)) * (16 * CB) + (g & 3) * 16);
+                        v[2 * g] = centred(w, mask, mul, add);
+                        v[2 * g + 1] = centred(w >> 8, mask, mul, add);
+                    }
+                    tmem_st16(tl + GG::VA + (i & 1) * (kTok / 2) + blk * 8, v);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(va_full + (i & 1));
+                mbar_arrive(raw_empty + st);
+            }
+        }
+    } else if (warp >= SM) {
+        // ================= K codes -> fp16, thread = token =================
+        const int tok = 32 * (warp & 3) + lane;
+        const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
+        for (int i = 0; i < n; i++) {
+            const int st = i % NST;
+            if (!wait(raw_full + st, i / NST)) break;
+            if (i >= 2 && !wait(qk_done + (i & 1), (i >> 1) - 1)) break;
+            tc_fence_after();
+            const uint4 *src = reinterpret_cast<const uint4 *>(slots + st * GG::SLOT + tok * CB);
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {  // 32 dimensions: 16 columns
+                uint32_t v[16];
+                if constexpr (BITS == 4) {
+                    const uint4 x = src[c];
+                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        v[4 * q] = centred(w[q], 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                        v[4 * q + 1] = centred(w[q], 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                        v[4 * q + 2] = centred(w[q] >> 8, 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                        v[4 * q + 3] = centred(w[q] >> 8, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                    }
+                } else {
+                    const uint4 x = src[2 * c], y = src[2 * c + 1];
+                    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        v[2 * q] = centred(w[q], 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                        v[2 * q + 1] = centred(w[q] >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                    }
+                }
+                tmem_st16(tl + GG::KA + (i & 1) * (D / 2) + 16 * c, v);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(ka_full + (i & 1));
+                mbar_arrive(raw_empty + st);
+            }
+        }
+    } else {
+        // ================= softmax: thread = token, 16 rows per group =================
+        const int group = warp >> 2, wq = warp & 3, c0 = group * kCols;
+        const int tok = 32 * wq + lane, slot_row = v_slot(tok);
+        float *gref = ref + c0, *gfac = fac + c0;
+        float *my_red = red + warp * kCols * 2, *grp_red = red + group * 4 * kCols * 2;
+        int u = u0, kt = k0, units = 0;
+        float l[kCols], z[kCols];
+        for (int i = 0; i < n; i++) {
+            const int st = i % NST;
+            const bool starts = i == 0 || kt == 0;
+            const float *qsum = reinterpret_cast<const float *>(smem + GG::Q_OFF + ((starts ? units : units - 1) & 1) * GG::QBUF +
+                                                                QP * GG::QPLANE) + c0;
+            bool ok = wait(raw_full + st, i / NST) && wait(qk_done + (i & 1), i >> 1);
+            if (ok && i >= 2) ok = wait(pv_done + (i & 1), (i >> 1) - 1);  // u's buffer is free
+            if (starts) {
+                // the group's references start over once every thread is past the last unit's
+                if (ok) ok = wait(q_full + (units & 1), units >> 1);
+                units++;
+#pragma unroll
+                for (int c = 0; c < kCols; c++) l[c] = z[c] = 0.0f;
+                if (wq == 0 && lane < kCols) gref[lane] = -INFINITY;
+                if (group_or(group, !ok)) break;  // (also: the references are written)
+            }
+            tc_fence_after();
+            const unsigned char *slot = slots + st * GG::SLOT;
+            const float2 km = *reinterpret_cast<const float2 *>(slot + 2 * kTok * CB + tok * 8);
+            const float2 vm = *reinterpret_cast<const float2 *>(slot + 2 * kTok * CB + kTok * 8 + tok * 8);
+            const float down = qsum[NR - c0];
+            const float ks = km.x * down, kz = fmaf(kCentre, km.x, km.y);
+            const float vs = vm.x < 0x1p-100f ? 0x1p-100f : vm.x;
+            const float rv = 1.0f / vs, zv = fmaf(kCentre, vs, vm.y) * rv, lv = __log2f(vs);
+            const int pos = kt * kTok + tok;
+            const bool masked = (kt + 1) * kTok > a.pos0;  // the tile holds drafts, or tokens past them
+            // which of the group's rows see this token
+            uint32_t sees = 0xffffu;
+            if (masked && pos >= a.pos0) {
+                sees = 0;
+                if (pos < total) {
+                    const int b = u / a.heads, dj = pos - (int)a.pos0;
+#pragma unroll 1
+                    for (int c = 0; c < kCols; c++) {
+                        const int node = (rb * NR + c0 + c) / a.group;
+                        if (node < a.seq_len && ((t.path[(int64_t)b * kMaxDraftNodes + node] >> dj) & 1)) sees |= 1u << c;
+                    }
+                }
+            }
+            const uint32_t sbuf = tl + GG::S + (i & 1) * NR + c0;
+            float e[kCols];
+            // scores of the token relative to the references; returns the largest
+            auto scores = [&](bool relative) {
+                uint32_t v[16];
+                tmem_ld16(sbuf, v);
+                tmem_wait_ld();
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 4) {
+                    const float4 q4 = *reinterpret_cast<const float4 *>(qsum + c);
+                    float4 r4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (relative) r4 = *reinterpret_cast<const float4 *>(gref + c);
+                    const float2 kz2 = make_float2(kz, kz), ks2 = make_float2(ks, ks);
+                    const float2 b0 = fma2(kz2, make_float2(q4.x, q4.y), make_float2(lv - r4.x, lv - r4.y));
+                    const float2 b1 = fma2(kz2, make_float2(q4.z, q4.w), make_float2(lv - r4.z, lv - r4.w));
+                    const float2 s0 = fma2(make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), ks2, b0);
+                    const float2 s1 = fma2(make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), ks2, b1);
+                    e[c] = s0.x;
+                    e[c + 1] = s0.y;
+                    e[c + 2] = s1.x;
+                    e[c + 3] = s1.y;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) e[c] = (sees >> c) & 1 ? e[c] : -INFINITY;
+                }
+#pragma unroll
+                for (int c = 0; c < kCols; c++) top = fmaxf(top, e[c]);
+                return top;
+            };
+            const float top = scores(true);
+            if (group_or(group, !ok || top > kHead + kShift)) {
+                // some score outgrew its reference: raise the group's references to the tile's maxima
+                if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
+                if (group_or(group, !ok)) break;
+                tc_fence_after();
+                scores(false);
+                const float cm = warp_columns(e, lane, [](float x, float y) { return fmaxf(x, y); });
+                if (lane < kCols) my_red[lane] = cm;
+                group_or(group, false);
+                if (wq == 0 && lane < kCols) {
+                    float m = gref[lane] + kShift;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) m = fmaxf(m, grp_red[w * kCols * 2 + lane]);
+                    const float old = gref[lane], now = m - kShift;
+                    gfac[lane] = old == -INFINITY ? 0.0f : exp2f(old - now);
+                    gref[lane] = now;
+                }
+                group_or(group, false);
+#pragma unroll
+                for (int c = 0; c < kCols; c++) {
+                    l[c] *= gfac[c];
+                    z[c] *= gfac[c];
+                }
+                if (!starts) {
+                    uint32_t v[16];
+                    tmem_ld16(tl + GG::O + c0, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) v[c] = __float_as_uint(__uint_as_float(v[c]) * gfac[c]);
+                    tmem_st16(tl + GG::O + c0, v);
+                    tmem_wait_st();
+                }
+                scores(true);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_empty + (i & 1));
+            // u = vs 2^(s - ref), its planes to shared memory, the token's sums
+            unsigned char *pl = smem + GG::P_OFF + (i & 1) * GG::PBUF + (slot_row >> 3) * 1024 + (slot_row & 7) * 128;
+            const float2 rv2 = make_float2(rv, rv), zv2 = make_float2(zv, zv);
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                uint32_t uh[4], ul[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int c = 8 * hf + 2 * x;
+                    const float2 w = make_float2(tg_ex2(e[c]), tg_ex2(e[c + 1]));
+                    float2 l2 = fma2(w, rv2, make_float2(l[c], l[c + 1]));
+                    float2 z2 = fma2(w, zv2, make_float2(z[c], z[c + 1]));
+                    if (masked) {  // an unseen token takes no part, whatever its metadata holds
+                        if (!((sees >> c) & 1)) l2.x = l[c], z2.x = z[c];
+                        if (!((sees >> (c + 1)) & 1)) l2.y = l[c + 1], z2.y = z[c + 1];
+                    }
+                    l[c] = l2.x;
+                    l[c + 1] = l2.y;
+                    z[c] = z2.x;
+                    z[c + 1] = z2.y;
+                    const __half2 hh = __floats2half2_rn(w.x, w.y);
+                    uh[x] = *reinterpret_cast<const uint32_t *>(&hh);
+                    if (PP == 2) {
+                        const float2 back = __half22float2(hh);
+                        const __half2 ll = __floats2half2_rn(w.x - back.x, w.y - back.y);
+                        ul[x] = *reinterpret_cast<const uint32_t *>(&ll);
+                    }
+                }
+                const int ch = ((2 * group + hf) ^ (slot_row & 7)) << 4;
+                *reinterpret_cast<uint4 *>(pl + ch) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+                if (PP == 2) *reinterpret_cast<uint4 *>(pl + kTok * 128 + ch) = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(p_full + (i & 1));
+                mbar_arrive(raw_empty + st);
+            }
+            if (kt == t.ntiles - 1 || i == n - 1) {
+                // ---- the unit's partial record ----
+                const float lc = warp_columns(l, lane, [](float x, float y) { return x + y; });
+                const float zc = warp_columns(z, lane, [](float x, float y) { return x + y; });
+                if (lane < kCols) {
+                    my_red[lane] = lc;
+                    my_red[kCols + lane] = zc;
+                }
+                ok = wait(pv_done + (i & 1), i >> 1);
+                if (group_or(group, !ok)) break;
+                tc_fence_after();
+                float *rec = t.records + ((int64_t)(grp + u) * t.nb + rb) * GG::REC;
+                if (wq == 0 && lane < kCols) {
+                    float ls = 0.0f, zs = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        ls += grp_red[w * kCols * 2 + lane];
+                        zs += grp_red[w * kCols * 2 + kCols + lane];
+                    }
+                    rec[NR * D + c0 + lane] = gref[lane];
+                    rec[NR * D + NR + c0 + lane] = ls;
+                    rec[NR * D + 2 * NR + c0 + lane] = zs;
+                }
+                uint32_t v[16];
+                tmem_ld16(tl + GG::O + c0, v);
+                tmem_wait_ld();
+                if (tok < D) {  // tok is the lane of O: a dimension
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) rec[(c0 + c) * D + tok] = __uint_as_float(v[c]);
+                }
+                tc_fence_before();
+                group_or(group, false);  // my_red and gref are read before the next unit writes them
+                if (kt == t.ntiles - 1 && lane == 0) mbar_arrive(q_empty + ((units - 1) & 1));
+            }
+            if (++kt == t.ntiles) {
+                kt = 0;
+                u++;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tbase, 512);
+    }
+}
+
+// ---- merge -------------------------------------------------------------------------------------------
+// One warp per query row: joins the unit's records, rotates back and stores.
+template <typename T, int BITS, int D, int NR>
+__global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeArgs t) {
+    constexpr int EPL = D / 32, REC = NR * D + 3 * NR;
+    const AttendArgs &a = t.a;
+    const int lane = threadIdx.x & 31;
+    const int64_t id = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    if (id >= (int64_t)a.batch * a.heads * t.rows) return;
+    const int u = (int)(id / t.rows), r = (int)(id % t.rows), rb = r / NR, rr = r % NR;
+    const int h = u % a.heads, b = u / a.heads, node = r / a.group, g = r % a.group;
+    T *dst = static_cast<T *>(a.out) + (((int64_t)b * a.seq_len + node) * (a.heads * a.group) + h * a.group + g) * D +
+             lane * EPL;
+    if (t.path[(int64_t)b * kMaxDraftNodes + node] == 0) {  // no node in this slot
+#pragma unroll
+        for (int e = 0; e < EPL; e++) st_from_f32(dst + e, 0.0f);
+        return;
+    }
+    // ranges that touch tiles [u ntiles, (u + 1) ntiles)
+    const int64_t first = (int64_t)u * t.ntiles, last = first + t.ntiles - 1;
+    const int lo = (int)(((first + 1) * t.groups - 1) / t.F), hi = (int)(((last + 1) * t.groups - 1) / t.F);
+    float M = -INFINITY;
+    for (int w = lo + lane; w <= hi; w += 32)
+        M = fmaxf(M, t.records[((int64_t)(w + u) * t.nb + rb) * REC + NR * D + rr]);
+    M = warp_max(M);
+    float L = 0.0f, Z = 0.0f, x[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; e++) x[e] = 0.0f;
+    for (int w = lo; w <= hi; w++) {
+        const float *rec = t.records + ((int64_t)(w + u) * t.nb + rb) * REC;
+        const float m = rec[NR * D + rr], l = rec[NR * D + NR + rr];
+        if (l == 0.0f) continue;  // saw no token of this range
+        const float wt = exp2f(m - M);
+        L = fmaf(wt, l, L);
+        Z = fmaf(wt, rec[NR * D + 2 * NR + rr], Z);
+#pragma unroll
+        for (int e = 0; e < EPL; e++) x[e] = fmaf(wt, rec[rr * D + lane * EPL + e], x[e]);
+    }
+    const float inv = 1.0f / L;  // a node sees itself
+#pragma unroll
+    for (int e = 0; e < EPL; e++) x[e] = (x[e] + Z) * inv;
+    warp_wht_butterfly<EPL>(x, lane, D);
+    const float *sg = a.signs + (int64_t)h * D + lane * EPL;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) st_from_f32(dst + e, x[e] * (a.wht_scale * sg[e]));
+}
+
+// ---- host ----------------------------------------------------------------------------------------------
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Shape of a launch over `batch` sequences.
+struct TreePlan {
+    int nr, nb, groups, ntiles, F;
+    size_t records, qimg, path;  // workspace parts, in this order
+};
+
+int query_planes(int dtype) { return dtype == SA_DTYPE_BFLOAT16 ? 1 : 2; }
+
+TreePlan tree_plan(int64_t batch, int heads, int group, int head_dim, int sm_count, int64_t total, int nodes, int dtype) {
+    TreePlan p;
+    const int rows = nodes * group;
+    p.nr = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    p.nb = (rows + p.nr - 1) / p.nr;
+    p.ntiles = (int)((total + kTok - 1) / kTok);
+    const int64_t units = batch * heads;
+    p.F = (int)(units * p.ntiles);
+    const int most = sm_count / p.nb > 0 ? sm_count / p.nb : 1;
+    p.groups = p.F < most ? p.F : most;
+    p.records = up256((size_t)(p.groups + units) * p.nb * (p.nr * head_dim + 3 * p.nr) * sizeof(float));
+    const size_t image = ((size_t)query_planes(dtype) * p.nr * head_dim * 2 + p.nr * 4 + 16 + 1023) / 1024 * 1024;
+    p.qimg = (size_t)units * p.nb * image;
+    p.path = up256((size_t)batch * kMaxDraftNodes * sizeof(uint64_t));
+    return p;
+}
+
+// Sequences of one launch: bounds the workspace (a row block's record takes up to 33.5 KB).
+int64_t tree_batch(int64_t batch, int heads, int group, int nodes) {
+    const int64_t blocks = (int64_t)heads * ((nodes * group + 63) / 64);
+    const int64_t most = 4096 / blocks > 0 ? 4096 / blocks : 1;
+    return batch < most ? batch : most;
+}
+
+template <typename T, int BITS, int D, int NR, int QP, int PP>
+int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
+    using GG = Tg<BITS, D, NR, QP, PP>;
+    const int64_t units = (int64_t)t.a.batch * t.a.heads;
+    // each launch is a programmatic dependent of the one before it
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = stream;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(units * t.nb));
+    cfg.blockDim = dim3(kPrepThreads);
+    cfg.dynamicSmemBytes = GG::QREC;
+    int rc = check_cuda(cudaLaunchKernelEx(&cfg, tree_prep_kernel<T, BITS, D, NR, QP>, t, qimg, path),
+                        "gqa_tree_attend prep launch");
+    count_launch();
+    if (rc != SA_OK) return rc;
+    auto kern = tree_umma_kernel<BITS, D, NR, QP, PP>;
+    static int configured[64];  // of this kernel, by device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GG::SMEM);
+        if (e != cudaSuccess) return check_cuda(e, "gqa_tree_attend smem attribute");
+        if (dev >= 0 && dev < 64) __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
+    }
+    cfg.gridDim = dim3((unsigned)(t.groups * t.nb));
+    cfg.blockDim = dim3(GG::THREADS);
+    cfg.dynamicSmemBytes = GG::SMEM;
+    rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, t), "gqa_tree_attend launch");
+    count_launch();
+    if (rc != SA_OK) return rc;
+    cfg.gridDim = dim3((unsigned)((units * t.rows + kMergeWarps - 1) / kMergeWarps));
+    cfg.blockDim = dim3(32 * kMergeWarps);
+    cfg.dynamicSmemBytes = 0;
+    rc = check_cuda(cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, BITS, D, NR>, t), "gqa_tree_attend merge launch");
+    count_launch();
+    return rc;
+}
+
+template <typename T, int BITS, int D>
+int launch_format(const TreeArgs &t, int nr, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
+    constexpr int QP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PP = std::is_same<T, float>::value ? 2 : 1;
+    if (nr == 16) return launch_rows<T, BITS, D, 16, QP, PP>(t, qimg, path, stream);
+    if (nr == 32) return launch_rows<T, BITS, D, 32, QP, PP>(t, qimg, path, stream);
+    return launch_rows<T, BITS, D, 64, QP, PP>(t, qimg, path, stream);
+}
+
+template <typename T>
+int launch_type(const TreeArgs &t, int nr, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
+    if (t.a.bits == 4 && t.a.head_dim == 128) return launch_format<T, 4, 128>(t, nr, qimg, path, stream);
+    if (t.a.bits == 8 && t.a.head_dim == 128) return launch_format<T, 8, 128>(t, nr, qimg, path, stream);
+    if (t.a.bits == 4 && t.a.head_dim == 64) return launch_format<T, 4, 64>(t, nr, qimg, path, stream);
+    return launch_format<T, 8, 64>(t, nr, qimg, path, stream);
+}
+
+}  // namespace
+
+// Workspace of the tensor-core tree attention at any context up to `tokens` (0: another kernel's job).
+size_t tree_workspace_bytes(int batch, int heads, int group, int head_dim, int bits, int sm_count, int64_t tokens,
+                            int nodes, int dtype) {
+    if ((bits != 4 && bits != 8) || (head_dim != 64 && head_dim != 128)) return 0;
+    const int64_t per = tree_batch(batch, heads, group, nodes);
+    const TreePlan p = tree_plan(per, heads, group, head_dim, sm_count, tokens, nodes, dtype);
+    return p.records + p.qimg + p.path;
+}
+
+int launch_gqa_tree_umma(const AttendArgs &a, void *workspace, cudaStream_t stream) {
+    const int64_t per = tree_batch(a.batch, a.heads, a.group, a.seq_len);
+    const int64_t qrow = (int64_t)a.seq_len * a.heads * a.group * a.head_dim * (a.dtype == SA_DTYPE_FLOAT ? 4 : 2);
+    for (int64_t b0 = 0; b0 < a.batch; b0 += per) {
+        TreeArgs t{};
+        t.a = a;
+        t.a.batch = (int)(a.batch - b0 < per ? a.batch - b0 : per);
+        const int64_t unit0 = b0 * a.heads;
+        t.a.query = static_cast<const char *>(a.query) + b0 * qrow;
+        t.a.out = static_cast<char *>(a.out) + b0 * qrow;
+        t.a.parents = a.parents + b0 * a.seq_len;
+        t.a.k_codes = a.k_codes + unit0 * a.capacity * a.code_bytes;
+        t.a.v_codes = a.v_codes + unit0 * a.capacity * a.code_bytes;
+        t.a.k_meta = a.k_meta + unit0 * a.capacity * 2;
+        t.a.v_meta = a.v_meta + unit0 * a.capacity * 2;
+        if (a.lr_vtr) t.a.lr_vtr = a.lr_vtr + unit0 * a.head_dim;
+        const TreePlan p = tree_plan(t.a.batch, a.heads, a.group, a.head_dim, a.sm_count, a.pos0 + a.seq_len, a.seq_len,
+                                     a.dtype);
+        char *ws = static_cast<char *>(workspace);
+        t.records = reinterpret_cast<float *>(ws);
+        t.qimg = reinterpret_cast<unsigned char *>(ws + p.records);
+        t.path = reinterpret_cast<uint64_t *>(ws + p.records + p.qimg);
+        t.rows = a.seq_len * a.group;
+        t.nb = p.nb;
+        t.ntiles = p.ntiles;
+        t.F = p.F;
+        t.groups = p.groups;
+        unsigned char *qimg = reinterpret_cast<unsigned char *>(ws + p.records);
+        uint64_t *path = reinterpret_cast<uint64_t *>(ws + p.records + p.qimg);
+        int rc;
+        switch (a.dtype) {
+            case SA_DTYPE_FLOAT: rc = launch_type<float>(t, p.nr, qimg, path, stream); break;
+            case SA_DTYPE_FLOAT16: rc = launch_type<__half>(t, p.nr, qimg, path, stream); break;
+            default: rc = launch_type<__nv_bfloat16>(t, p.nr, qimg, path, stream); break;
+        }
+        if (rc != SA_OK) return rc;
+    }
+    return SA_OK;
+}
+
+}  // namespace sa

@@ -193,6 +193,9 @@ struct SelectArgs {
     int32_t *block_ids;
 };
 
+size_t tree_workspace_bytes(int batch, int heads, int group, int head_dim, int bits, int sm_count, int64_t tokens,
+                            int nodes, int dtype);
+int launch_gqa_tree_umma(const AttendArgs &a, void *workspace, cudaStream_t stream);
 int launch_keep_drafts(const KeepArgs &a, cudaStream_t stream);
 int launch_block_means(const MeansArgs &a, cudaStream_t stream);
 int launch_select_blocks(const SelectArgs &a, cudaStream_t stream);

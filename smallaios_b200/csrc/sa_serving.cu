@@ -103,8 +103,10 @@ bool list_decode_format(const kv_cache_impl *k) {
 extern "C" {
 
 int64_t sa_gqa_tree_workspace_bytes(const sa_kv_cache *cache, int32_t nodes, int32_t dtype) {
-    if (!cache || nodes <= 0 || !dtype_ok(dtype)) return 0;
-    return 0;
+    const kv_cache_impl *k = reinterpret_cast<const kv_cache_impl *>(cache);
+    if (!cache || nodes <= 0 || nodes > SA_MAX_DRAFT_NODES || !dtype_ok(dtype) || k->group > 8) return 0;
+    return (int64_t)tree_workspace_bytes(k->cfg.batch, k->cfg.kv_head_count, k->group, k->cfg.head_dim, k->cfg.bits,
+                                         k->sm_count, k->capacity, nodes, dtype);
 }
 
 int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, const int32_t *parents, void *attn_out,
@@ -119,11 +121,12 @@ int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, con
     if (nodes == 0) return SA_OK;
     if (!query || !parents || !attn_out)
         return set_error(SA_ERR_INVALID_ARGUMENT, "gqa_tree_attend: NULL query/parents/attn_out");
-    rc = check_workspace("gqa_tree_attend", workspace, workspace_bytes,
-                         sa_gqa_tree_workspace_bytes(cache, nodes, dtype));
+    const int64_t need = sa_gqa_tree_workspace_bytes(cache, nodes, dtype);
+    rc = check_workspace("gqa_tree_attend", workspace, workspace_bytes, need);
     if (rc != SA_OK) return rc;
     AttendArgs a = attend_args(k, layer, query, attn_out, dtype, batch, nodes, has_scale, scale);
     a.parents = parents;
+    if (need > 0) return launch_gqa_tree_umma(a, workspace, static_cast<cudaStream_t>(stream));
     return launch_gqa_attend_generic(a, static_cast<cudaStream_t>(stream));
 }
 
