@@ -24,13 +24,14 @@
 // of 1024 is a float, one packed subtraction centres two.
 //
 // One persistent CTA per SM; roles by warp:
-//   4 * NG softmax warps (NG = NR / 16 groups of four): thread = token of the
-//     tile, 16 rows per group: tcgen05.ld of S^T, u, the sums l and z of its
+//   4 or 8 softmax warps (groups of four, 16 or 32 rows each): thread = token of
+//     the tile, 16 rows at a time: tcgen05.ld of S^T, u, the sums l and z of its
 //     token, u to shared memory (the B operand, rows contiguous).  The reference
 //     ref_r is only raised when some score of the tile outgrows it by 2^8 (one
 //     vote per tile and group); then O is rescaled in tensor memory.
 //   4 K warps, 4 V warps: codes of the tile from shared memory to fp16 in tensor
-//     memory (thread = token for K, dimension for V), two buffers each.
+//     memory, two buffers each; the K warps also turn the tokens' scales and zero
+//     points into what the softmax needs.
 //   1 MMA warp: S^T(i), then O^T of tile i - 1.
 //   1 copy warp: codes and metadata of the tiles by bulk copies into a ring.
 // The tiles of all units (batch row, KV head) are laid end to end and cut into
@@ -55,7 +56,7 @@ namespace sa {
 namespace {
 
 constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
-constexpr int kCols = 16;       // query rows per softmax group
+constexpr int kCols = 16;       // query rows that a softmax thread works on at a time
 constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
 constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
 constexpr int kPrepThreads = 256;
@@ -64,17 +65,19 @@ constexpr int kMergeWarps = 8;
 template <int BITS, int D, int NR, int QP, int PP>
 struct Tg {
     static constexpr int CB = D * BITS / 8;
-    static constexpr int NG = NR / kCols;                   // softmax groups
+    static constexpr int NG = NR / kCols;                   // softmax groups of four warps
+    static constexpr int HC = NR / kCols / NG;              // 16-row parts per group
     static constexpr int THREADS = 32 * (4 * NG + 10);
     static constexpr int PBUF = PP * kTok * 128;            // u planes of a tile: [128 tokens][64 rows], 128-byte swizzle
     static constexpr int QPLANE = NR * D * 2;               // D/64 tiles of [NR rows][128 B]
     static constexpr int QREC = QP * QPLANE + NR * 4 + 16;  // planes, sum(q^) of the rows, power of two
     static constexpr int QBUF = (QREC + 1023) / 1024 * 1024;
-    static constexpr int SLOT = kTok * (2 * CB + 16);       // K codes, V codes, K metadata, V metadata
+    // ring slot: K codes, V codes, K metadata, V metadata; then what the softmax makes of a token's metadata
+    static constexpr int META = 2 * kTok * CB, CONST = META + kTok * 16, SLOT = CONST + kTok * 20;
     static constexpr int P_OFF = 0, Q_OFF = 2 * PBUF, SLOT_OFF = Q_OFF + 2 * QBUF;
     static constexpr int MISC = 6 * 1024;
     static constexpr int ROOM = (226 * 1024 - SLOT_OFF - MISC) / SLOT;
-    static constexpr int NST = ROOM > 4 ? 4 : ROOM;         // ring slots
+    static constexpr int NST = ROOM > 8 ? 8 : ROOM;         // ring slots
     static constexpr int MISC_OFF = SLOT_OFF + NST * SLOT;
     static constexpr int SMEM = MISC_OFF + MISC + 1024;     // + slack to align the base to 1024 B
     // TMEM columns: K and V operands (two buffers each), S^T (two), O^T
@@ -98,13 +101,23 @@ __device__ __forceinline__ uint32_t sw128(int r, int c) {
     return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
 }
 
-// Position along K of dimension e in the K operand, as the conversion of a 32-bit word leaves its
-// codes: 4 bits 0 4 1 5 2 6 3 7 of eight, 8 bits 0 2 1 3 of four.
-template <int BITS>
+// The operands in tensor memory are stored as fragments of 16 lanes x 8 columns: thread (Q, q) = (lane / 4,
+// lane % 4) holds columns 2q and 2q + 1 of lanes Q and Q + 8.
+//
+// K operand (lane = token): thread q takes the q-th quarter of a token's code bytes; its words become column
+// pairs as the conversion leaves the codes -- 4 bits: (0,4) (1,5) (2,6) (3,7) of a word's eight, 8 bits: (0,2)
+// (1,3) of four -- and its p-th column goes to column 8 (p / 2) + 2q + p % 2.  Position along K of dimension e:
+template <int BITS, int D>
 __host__ __device__ __forceinline__ int k_position(int e) {
-    if (BITS == 4) return (e & ~7) | ((e & 3) << 1) | ((e >> 2) & 1);
-    return (e & ~3) | ((e & 1) << 1) | ((e >> 1) & 1);
+    constexpr int W = 32 / BITS;              // codes per word
+    const int q = e / (D / 4), r = e % (D / 4);
+    const int p = r / W * (W / 2) + r % (W / 2);
+    return 2 * (8 * (p >> 1) + 2 * q + (p & 1)) + (r % W) / (W / 2);
 }
+
+// V operand: lane l of a quarter holds dimension 4 (l % 8) + l / 8, so that a thread's four lanes are the codes of
+// one 8-byte (4 bits) or 16-byte (8 bits) load of a group of four tokens.
+__device__ __forceinline__ int v_dimension(int l) { return 4 * (l & 7) + (l >> 3); }
 
 // Position along K of token t in the V operand: 0 2 1 3 of every four.
 __device__ __forceinline__ int v_slot(int t) { return (t & ~3) | ((t & 1) << 1) | ((t >> 1) & 1); }
@@ -135,6 +148,52 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
+}
+
+__device__ __forceinline__ float tg_rcp(float x) {  // within one ulp
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float tg_lg2(float x) {  // absolute error 2^-22
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 ra, rb, rd;\nmov.b64 ra, {%2, %3};\nmov.b64 rb, {%4, %5};\nadd.rn.f32x2 rd, ra, rb;\n"
+        "mov.b64 {%0, %1}, rd;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// Arrival of the warp's lane 0, without a branch.
+__device__ __forceinline__ void warp_arrive(uint64_t *bar, int lane) {
+    asm volatile("{\n.reg .pred p;\nsetp.eq.s32 p, %1, 0;\n@p mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(
+                     smem_u32(bar)),
+                 "r"(lane)
+                 : "memory");
+}
+
+// 16 lanes x 8N columns of tensor memory from fragments (see k_position): v[4m .. 4m + 3] = columns 8m + 2q, + 1
+// of lane Q, then of lane Q + 8.
+__device__ __forceinline__ void tmem_st_frag4(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};\n" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
 }
 
 // OR of `v` over the 128 threads of a softmax group (named barrier 1 + group).
@@ -228,7 +287,7 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
             const float y = x[i][e] * up;
             const __half hi = __float2half_rn(y);
             const float hf = __half2float(hi);
-            const int p = k_position<BITS>(lane * EPL + e);
+            const int p = k_position<BITS, D>(lane * EPL + e);
             unsigned char *dst = img + (p >> 6) * (NR * 128) + sw128(row, (p & 63) >> 3) + (p & 7) * 2;
             *reinterpret_cast<__half *>(dst) = hi;
             float kept = hf;
@@ -252,21 +311,20 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
 template <int BITS, int D, int NR, int QP, int PP>
 __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma_kernel(TreeArgs t) {
     using GG = Tg<BITS, D, NR, QP, PP>;
-    constexpr int CB = GG::CB, NST = GG::NST, NG = GG::NG, SM = 4 * NG;
+    constexpr int CB = GG::CB, NST = GG::NST, SM = 4 * GG::NG, HC = GG::HC;
     constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     const AttendArgs &a = t.a;
     extern __shared__ unsigned char tg_raw[];
     unsigned char *smem = tg_raw + ((1024 - (smem_u32(tg_raw) & 1023)) & 1023);
     unsigned char *slots = smem + GG::SLOT_OFF;
-    float *ref = reinterpret_cast<float *>(smem + GG::MISC_OFF);       // [NR], minus kShift
+    float *ref = reinterpret_cast<float *>(smem + GG::MISC_OFF);       // [NR], minus the reference
     float *fac = ref + 64;                                             // [NR]
-    float *red = fac + 64;                                             // [SM warps][16][2]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 16 * kCols * 2);
-    uint64_t *raw_full = bars, *raw_empty = bars + 4, *ka_full = bars + 8, *va_full = bars + 10, *qk_done = bars + 12,
-             *pv_done = bars + 14, *s_empty = bars + 16, *p_full = bars + 18, *q_full = bars + 20, *q_empty = bars + 22,
-             *bar_fin = bars + 24;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 25);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 26);
+    float *red = fac + 64;                                             // [softmax warps][HC][2][16]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 16 * 2 * kCols * HC);
+    uint64_t *raw_full = bars, *raw_empty = bars + 8, *ka_full = bars + 16, *va_full = bars + 18, *qk_done = bars + 20,
+             *pv_done = bars + 22, *p_full = bars + 24, *q_full = bars + 26, *q_empty = bars + 28, *bar_fin = bars + 30;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 31);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 32);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int grp = blockIdx.x / t.nb, rb = blockIdx.x % t.nb;
@@ -277,17 +335,16 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
     if (tid == 0) {
         for (int i = 0; i < NST; i++) {
             mbar_init(raw_full + i, 1);
-            mbar_init(raw_empty + i, 8 + SM);
+            mbar_init(raw_empty + i, 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(ka_full + i, 4);
             mbar_init(va_full + i, 4);
             mbar_init(qk_done + i, 1);
             mbar_init(pv_done + i, 1);
-            mbar_init(s_empty + i, SM);
             mbar_init(p_full + i, SM);
             mbar_init(q_full + i, 1);
-            mbar_init(q_empty + i, 1 + SM);
+            mbar_init(q_empty + i, 1);
         }
         mbar_init(bar_fin, 1);
         *abort_flag = 0;
@@ -303,7 +360,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
     asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the query images and node paths; the drafts in the cache
 
     auto wait = [&](uint64_t *bar, int phase) {
-        return __all_sync(0xffffffffu, tc_wait_sleep(bar, (uint32_t)(phase & 1), abort_flag, a.dev_status));
+        const bool ok = um_try(bar, (uint32_t)(phase & 1)) || tc_wait_sleep(bar, (uint32_t)(phase & 1), abort_flag, a.dev_status);
+        return (bool)__all_sync(0xffffffffu, ok);
     };
 
     if (warp == SM + 9) {
@@ -331,8 +389,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             __syncwarp();
             if (lane == 0) bulk_g2s(slot, a.k_codes + row * CB, (uint32_t)nt * CB, raw_full + st);
             if (lane == 1) bulk_g2s(slot + kTok * CB, a.v_codes + row * CB, (uint32_t)nt * CB, raw_full + st);
-            if (lane == 2) bulk_g2s(slot + 2 * kTok * CB, a.k_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
-            if (lane == 3) bulk_g2s(slot + 2 * kTok * CB + kTok * 8, a.v_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
+            if (lane == 2) bulk_g2s(slot + GG::META, a.k_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
+            if (lane == 3) bulk_g2s(slot + GG::META + kTok * 8, a.v_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
             issued = i + 1;
             if (++kt == t.ntiles) {
                 kt = 0;
@@ -349,11 +407,12 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         constexpr uint32_t id_s = tg_idesc(NR, 0), id_o = tg_idesc(NR, 1);
         int kt = k0, units = 0;
         bool first_prev = true;  // whether tile i - 1 was the first of its unit here
+        int prev_unit = 0;       // its unit
         for (int i = 0; i <= n; i++) {
             const bool starts = i == 0 || kt == 0;
             if (i < n) {
                 bool ok = wait(ka_full + (i & 1), i >> 1);
-                if (ok && i >= 2) ok = wait(s_empty + (i & 1), (i >> 1) - 1);
+                // (S^T's buffer: the softmax of tile i - 2 had read it before p_full(i - 2), seen below)
                 if (ok && starts) {
                     ok = wait(q_full + (units & 1), units >> 1);
                     units++;
@@ -370,7 +429,6 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                                     sw128_kmajor_desc(q + pl * GG::QPLANE + (kk >> 2) * (NR * 128) + 32 * (kk & 3)), id_s,
                                     (pl | kk) != 0 ? 1u : 0u);
                     umma_commit(qk_done + (i & 1));
-                    if (kt == t.ntiles - 1) umma_commit(q_empty + ((units - 1) & 1));  // the unit's last use of q
                 }
                 __syncwarp();
             }
@@ -389,10 +447,14 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                                     sw128_kmajor_desc(p + pl * (kTok * 128) + 2048 * kk), id_o,
                                     (pl | kk) != 0 || !first_prev ? 1u : 0u);
                     umma_commit(pv_done + (j & 1));
+                    // every role is past tile j: its ring slot, and after the unit's last tile its queries, are free
+                    umma_commit(raw_empty + j % NST);
+                    if (i == n || starts) umma_commit(q_empty + (prev_unit & 1));
                 }
                 __syncwarp();
             }
             first_prev = starts;
+            prev_unit = units - 1;
             if (++kt == t.ntiles) kt = 0;
         }
         // every issued MMA has completed before TMEM is freed
@@ -402,271 +464,340 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         while (!um_try(bar_fin, 0) && um_clock_ns() - tw < kTcWaitNs) {
         }
     } else if (warp >= SM + 4) {
-        // ================= V codes -> fp16, thread = dimension =================
-        const int dim = 32 * (warp & 3) + lane;
+        // ================= V codes -> fp16 =================
+        const int Q = lane >> 2, q = lane & 3;
         const bool live = 32 * (warp & 3) < D;
-        const int j = BITS == 4 ? dim >> 1 : dim;                           // byte of the token's codes
-        const bool odd = BITS == 4 && (dim & 1);
-        const uint32_t mask = BITS == 8 ? 0x00ff00ffu : odd ? 0x00f000f0u : 0x000f000fu;
-        const __half2 mul = __float2half2_rn(odd ? 0.0625f : 1.0f);
-        const __half2 add = __float2half2_rn(BITS == 8 ? -1152.0f : odd ? -72.0f : -1032.0f);
+        const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
         for (int i = 0; i < n; i++) {
             const int st = i % NST;
             if (!wait(raw_full + st, i / NST)) break;
             if (i >= 2 && !wait(pv_done + (i & 1), (i >> 1) - 1)) break;
             tc_fence_after();
             if (live) {
-                const unsigned char *src = slots + st * GG::SLOT + kTok * CB + (j >> 2) * 64 + (j & 3) * 4;
+                // group q of a 16-token block, dimensions 32 w + 4 Q .. + 3
+                const unsigned char *src = slots + st * GG::SLOT + kTok * CB + 16 * q +
+                                           (BITS == 4 ? (4 * (warp & 3) + (Q >> 1)) * 64 + (Q & 1) * 8
+                                                      : (8 * (warp & 3) + Q) * 64);
+                const uint32_t dst = tl + GG::VA + (i & 1) * (kTok / 2);
+#pragma unroll 1  // (the roles' loops share the instruction caches)
+                for (int half = 0; half < 2; half++) {
+                    uint32_t v0[16], v1[16];  // lanes Q and Q + 8; Q + 16 and Q + 24
 #pragma unroll
-                for (int blk = 0; blk < kTok / 16; blk += 2) {
-                    uint32_t v[16];
+                    for (int m = 0; m < 4; m++) {
+                        const unsigned char *blk = src + (4 * half + m) * (16 * CB);
+                        if constexpr (BITS == 4) {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(blk);
+                            v0[4 * m] = centred(w.x, 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                            v0[4 * m + 1] = centred(w.x >> 8, 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                            v0[4 * m + 2] = centred(w.x, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                            v0[4 * m + 3] = centred(w.x >> 8, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                            v1[4 * m] = centred(w.y, 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                            v1[4 * m + 1] = centred(w.y >> 8, 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                            v1[4 * m + 2] = centred(w.y, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                            v1[4 * m + 3] = centred(w.y >> 8, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                        } else {
+                            const uint4 w = *reinterpret_cast<const uint4 *>(blk);
+                            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int g = 0; g < 8; g++) {
-                        const uint32_t w =
-                            *reinterpret_cast<const uint32_t *>(src + (blk + (g >> 2)) * (16 * CB) + (g & 3) * 16);
-                        v[2 * g] = centred(w, mask, mul, add);
-                        v[2 * g + 1] = centred(w >> 8, mask, mul, add);
+                            for (int y = 0; y < 4; y++) {
+                                uint32_t *v = y < 2 ? v0 : v1;
+                                v[4 * m + 2 * (y & 1)] = centred(x[y], 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                                v[4 * m + 2 * (y & 1) + 1] =
+                                    centred(x[y] >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                            }
+                        }
                     }
-                    tmem_st16(tl + GG::VA + (i & 1) * (kTok / 2) + blk * 8, v);
+                    tmem_st_frag4(dst + 32 * half, v0);
+                    tmem_st_frag4(dst + 32 * half + (16u << 16), v1);
                 }
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(va_full + (i & 1));
-                mbar_arrive(raw_empty + st);
-            }
+            warp_arrive(va_full + (i & 1), lane);
         }
     } else if (warp >= SM) {
-        // ================= K codes -> fp16, thread = token =================
-        const int tok = 32 * (warp & 3) + lane;
+        // ================= K codes -> fp16, token constants =================
+        const int Q = lane >> 2, q = lane & 3, tok = 32 * (warp & 3) + lane;
+        constexpr int QB = CB / 4, NW = QB / 4;  // bytes and words of a quarter of a token's codes
         const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
         for (int i = 0; i < n; i++) {
             const int st = i % NST;
             if (!wait(raw_full + st, i / NST)) break;
             if (i >= 2 && !wait(qk_done + (i & 1), (i >> 1) - 1)) break;
             tc_fence_after();
-            const uint4 *src = reinterpret_cast<const uint4 *>(slots + st * GG::SLOT + tok * CB);
+            unsigned char *slot = slots + st * GG::SLOT;
+            {
+                const float2 km = *reinterpret_cast<const float2 *>(slot + GG::META + tok * 8);
+                const float2 vm = *reinterpret_cast<const float2 *>(slot + GG::META + kTok * 8 + tok * 8);
+                const float vs = vm.x < 0x1p-100f ? 0x1p-100f : vm.x, rv = tg_rcp(vs);
+                *reinterpret_cast<float4 *>(slot + GG::CONST + tok * 16) =
+                    make_float4(km.x, fmaf(kCentre, km.x, km.y), tg_lg2(vs), rv);
+                *reinterpret_cast<float *>(slot + GG::CONST + kTok * 16 + tok * 4) = fmaf(kCentre, vs, vm.y) * rv;
+            }
+            const unsigned char *src = slot + (32 * (warp & 3) + Q) * CB + q * QB;
+            const uint32_t dst = tl + GG::KA + (i & 1) * (D / 2);
+            // tokens Q, Q + 8 of 16 at a time, 16 registers (8 columns by 4 column blocks) at a time
+#pragma unroll 1
+            for (int half = 0; half < 2; half++) {
+                uint32_t w[2][NW];
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {  // 32 dimensions: 16 columns
-                uint32_t v[16];
-                if constexpr (BITS == 4) {
-                    const uint4 x = src[c];
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                for (int y = 0; y < 2; y++) {
+                    const unsigned char *row = src + (16 * half + 8 * y) * CB;
+                    if constexpr (QB == 8) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(row);
+                        w[y][0] = x.x;
+                        w[y][1] = x.y;
+                    } else {
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        v[4 * q] = centred(w[q], 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                        v[4 * q + 1] = centred(w[q], 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
-                        v[4 * q + 2] = centred(w[q] >> 8, 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                        v[4 * q + 3] = centred(w[q] >> 8, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
-                    }
-                } else {
-                    const uint4 x = src[2 * c], y = src[2 * c + 1];
-                    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        v[2 * q] = centred(w[q], 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
-                        v[2 * q + 1] = centred(w[q] >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                        for (int x = 0; x < QB / 16; x++) {
+                            const uint4 t4 = reinterpret_cast<const uint4 *>(row)[x];
+                            w[y][4 * x] = t4.x;
+                            w[y][4 * x + 1] = t4.y;
+                            w[y][4 * x + 2] = t4.z;
+                            w[y][4 * x + 3] = t4.w;
+                        }
                     }
                 }
-                tmem_st16(tl + GG::KA + (i & 1) * (D / 2) + 16 * c, v);
+                // columns 2m, 2m + 1 of the thread (of D / 8 in all) go to column block m
+#pragma unroll
+                for (int m0 = 0; m0 < D / 16; m0 += 4) {
+                    uint32_t v[16];
+#pragma unroll
+                    for (int m = 0; m < 4; m++)
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            if constexpr (BITS == 4) {
+                                const uint32_t x = w[y][(m0 + m) >> 1] >> ((m & 1) * 8);
+                                v[4 * m + 2 * y] = centred(x, 0x000f000fu, one, __float2half2_rn(-1032.0f));
+                                v[4 * m + 2 * y + 1] = centred(x, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                            } else {
+                                const uint32_t x = w[y][m0 + m];
+                                v[4 * m + 2 * y] = centred(x, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                                v[4 * m + 2 * y + 1] = centred(x >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                            }
+                        }
+                    tmem_st_frag4(dst + 8 * m0 + (half ? 16u << 16 : 0u), v);
+                }
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(ka_full + (i & 1));
-                mbar_arrive(raw_empty + st);
-            }
+            warp_arrive(ka_full + (i & 1), lane);
         }
     } else {
-        // ================= softmax: thread = token, 16 rows per group =================
-        const int group = warp >> 2, wq = warp & 3, c0 = group * kCols;
+        // ================= softmax: thread = token, HC times 16 rows per group =================
+        const int group = warp >> 2, wq = warp & 3, c0 = group * HC * kCols;
         const int tok = 32 * wq + lane, slot_row = v_slot(tok);
         float *gref = ref + c0, *gfac = fac + c0;
-        float *my_red = red + warp * kCols * 2, *grp_red = red + group * 4 * kCols * 2;
+        constexpr int kRed = HC * 2 * kCols;
+        float *my_red = red + warp * kRed, *grp_red = red + group * 4 * kRed;
         int u = u0, kt = k0, units = 0;
-        float l[kCols], z[kCols];
+        float l[HC][kCols], z[HC][kCols];
         for (int i = 0; i < n; i++) {
             const int st = i % NST;
             const bool starts = i == 0 || kt == 0;
             const float *qsum = reinterpret_cast<const float *>(smem + GG::Q_OFF + ((starts ? units : units - 1) & 1) * GG::QBUF +
                                                                 QP * GG::QPLANE) + c0;
-            bool ok = wait(raw_full + st, i / NST) && wait(qk_done + (i & 1), i >> 1);
-            if (ok && i >= 2) ok = wait(pv_done + (i & 1), (i >> 1) - 1);  // u's buffer is free
+            // S^T(i); with it the token constants are in place (the K warps wrote them before) and O^T(i - 2),
+            // issued before, is complete: u's buffer is free
+            bool ok = wait(qk_done + (i & 1), i >> 1);
             if (starts) {
                 // the group's references start over once every thread is past the last unit's
                 if (ok) ok = wait(q_full + (units & 1), units >> 1);
                 units++;
 #pragma unroll
-                for (int c = 0; c < kCols; c++) l[c] = z[c] = 0.0f;
-                if (wq == 0 && lane < kCols) gref[lane] = -INFINITY;
+                for (int p = 0; p < HC; p++)
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) l[p][c] = z[p][c] = 0.0f;
+                if (wq == 0 && lane < HC * kCols) gref[lane] = INFINITY;
                 if (group_or(group, !ok)) break;  // (also: the references are written)
             }
             tc_fence_after();
             const unsigned char *slot = slots + st * GG::SLOT;
-            const float2 km = *reinterpret_cast<const float2 *>(slot + 2 * kTok * CB + tok * 8);
-            const float2 vm = *reinterpret_cast<const float2 *>(slot + 2 * kTok * CB + kTok * 8 + tok * 8);
-            const float down = qsum[NR - c0];
-            const float ks = km.x * down, kz = fmaf(kCentre, km.x, km.y);
-            const float vs = vm.x < 0x1p-100f ? 0x1p-100f : vm.x;
-            const float rv = 1.0f / vs, zv = fmaf(kCentre, vs, vm.y) * rv, lv = __log2f(vs);
-            const int pos = kt * kTok + tok;
-            const bool masked = (kt + 1) * kTok > a.pos0;  // the tile holds drafts, or tokens past them
-            // which of the group's rows see this token
-            uint32_t sees = 0xffffu;
-            if (masked && pos >= a.pos0) {
-                sees = 0;
-                if (pos < total) {
-                    const int b = u / a.heads, dj = pos - (int)a.pos0;
-#pragma unroll 1
-                    for (int c = 0; c < kCols; c++) {
-                        const int node = (rb * NR + c0 + c) / a.group;
-                        if (node < a.seq_len && ((t.path[(int64_t)b * kMaxDraftNodes + node] >> dj) & 1)) sees |= 1u << c;
-                    }
-                }
-            }
+            const float4 tc = *reinterpret_cast<const float4 *>(slot + GG::CONST + tok * 16);
+            const float zv = *reinterpret_cast<const float *>(slot + GG::CONST + kTok * 16 + tok * 4);
+            const float ks = tc.x * qsum[NR - c0], kz = tc.y, lv = tc.z, rv = tc.w;
             const uint32_t sbuf = tl + GG::S + (i & 1) * NR + c0;
-            float e[kCols];
-            // scores of the token relative to the references; returns the largest
-            auto scores = [&](bool relative) {
-                uint32_t v[16];
-                tmem_ld16(sbuf, v);
-                tmem_wait_ld();
-                float top = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < kCols; c += 4) {
-                    const float4 q4 = *reinterpret_cast<const float4 *>(qsum + c);
-                    float4 r4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (relative) r4 = *reinterpret_cast<const float4 *>(gref + c);
-                    const float2 kz2 = make_float2(kz, kz), ks2 = make_float2(ks, ks);
-                    const float2 b0 = fma2(kz2, make_float2(q4.x, q4.y), make_float2(lv - r4.x, lv - r4.y));
-                    const float2 b1 = fma2(kz2, make_float2(q4.z, q4.w), make_float2(lv - r4.z, lv - r4.w));
-                    const float2 s0 = fma2(make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), ks2, b0);
-                    const float2 s1 = fma2(make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), ks2, b1);
-                    e[c] = s0.x;
-                    e[c + 1] = s0.y;
-                    e[c + 2] = s1.x;
-                    e[c + 3] = s1.y;
-                }
-                if (masked) {
-#pragma unroll
-                    for (int c = 0; c < kCols; c++) e[c] = (sees >> c) & 1 ? e[c] : -INFINITY;
-                }
-#pragma unroll
-                for (int c = 0; c < kCols; c++) top = fmaxf(top, e[c]);
-                return top;
-            };
-            const float top = scores(true);
-            if (group_or(group, !ok || top > kHead + kShift)) {
-                // some score outgrew its reference: raise the group's references to the tile's maxima
-                if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
-                if (group_or(group, !ok)) break;
-                tc_fence_after();
-                scores(false);
-                const float cm = warp_columns(e, lane, [](float x, float y) { return fmaxf(x, y); });
-                if (lane < kCols) my_red[lane] = cm;
-                group_or(group, false);
-                if (wq == 0 && lane < kCols) {
-                    float m = gref[lane] + kShift;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) m = fmaxf(m, grp_red[w * kCols * 2 + lane]);
-                    const float old = gref[lane], now = m - kShift;
-                    gfac[lane] = old == -INFINITY ? 0.0f : exp2f(old - now);
-                    gref[lane] = now;
-                }
-                group_or(group, false);
-#pragma unroll
-                for (int c = 0; c < kCols; c++) {
-                    l[c] *= gfac[c];
-                    z[c] *= gfac[c];
-                }
-                if (!starts) {
-                    uint32_t v[16];
-                    tmem_ld16(tl + GG::O + c0, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < kCols; c++) v[c] = __float_as_uint(__uint_as_float(v[c]) * gfac[c]);
-                    tmem_st16(tl + GG::O + c0, v);
-                    tmem_wait_st();
-                }
-                scores(true);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty + (i & 1));
-            // u = vs 2^(s - ref), its planes to shared memory, the token's sums
             unsigned char *pl = smem + GG::P_OFF + (i & 1) * GG::PBUF + (slot_row >> 3) * 1024 + (slot_row & 7) * 128;
-            const float2 rv2 = make_float2(rv, rv), zv2 = make_float2(zv, zv);
+            // 16 rows of the tile, from row p0 of the group; `masked`: it holds drafts, or tokens past them (sees:
+            // the rows that see this token)
+            auto part = [&](auto masked, auto which, uint32_t sees) {
+                constexpr bool MASK = decltype(masked)::value;
+                constexpr int P = decltype(which)::value, p0 = P * kCols;
+                const float2 kz2 = make_float2(kz, kz), ks2 = make_float2(ks, ks), lv2 = make_float2(lv, lv);
+                const float2 rv2 = make_float2(rv, rv), zv2 = make_float2(zv, zv);
+                float w[kCols];
+                // A unit's first tile, and one with a score that outgrew its reference, first raise the references
+                // to the tile's maxima.  u is computed before the vote on that, so that the exponentials overlap the
+                // scores' arithmetic; a raise does it over.
+                // w: the scores (raising), or u, which also goes to shared memory; returns the largest score
+                auto pass = [&](auto raising) {
+                    constexpr bool RAISE = decltype(raising)::value;
+                    float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                uint32_t uh[4], ul[4];
+                    for (int hf = 0; hf < 2; hf++) {
+                        uint32_t v[8], uh[4], ul[4];
+                        tmem_ld8(sbuf + p0 + 8 * hf, v);
+                        tmem_wait_ld();
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int c = 8 * hf + 2 * x;
-                    const float2 w = make_float2(tg_ex2(e[c]), tg_ex2(e[c + 1]));
-                    float2 l2 = fma2(w, rv2, make_float2(l[c], l[c + 1]));
-                    float2 z2 = fma2(w, zv2, make_float2(z[c], z[c + 1]));
-                    if (masked) {  // an unseen token takes no part, whatever its metadata holds
-                        if (!((sees >> c) & 1)) l2.x = l[c], z2.x = z[c];
-                        if (!((sees >> (c + 1)) & 1)) l2.y = l[c + 1], z2.y = z[c + 1];
+                        for (int c = 8 * hf; c < 8 * hf + 8; c += 4) {
+                            const float4 q4 = *reinterpret_cast<const float4 *>(qsum + p0 + c);
+                            float4 r4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (!RAISE) r4 = *reinterpret_cast<const float4 *>(gref + p0 + c);  // minus the reference
+                            const float2 b0 = fma2(kz2, make_float2(q4.x, q4.y), add2(make_float2(r4.x, r4.y), lv2));
+                            const float2 b1 = fma2(kz2, make_float2(q4.z, q4.w), add2(make_float2(r4.z, r4.w), lv2));
+                            const float2 s0 =
+                                fma2(make_float2(__uint_as_float(v[c & 7]), __uint_as_float(v[(c & 7) + 1])), ks2, b0);
+                            const float2 s1 =
+                                fma2(make_float2(__uint_as_float(v[(c & 7) + 2]), __uint_as_float(v[(c & 7) + 3])), ks2, b1);
+                            float e[4] = {s0.x, s0.y, s1.x, s1.y};
+                            if (MASK) {
+#pragma unroll
+                                for (int x = 0; x < 4; x++)
+                                    if (!((sees >> (c + x)) & 1)) e[x] = -INFINITY;
+                            }
+                            top0 = fmaxf(top0, fmaxf(e[0], e[1]));
+                            top1 = fmaxf(top1, fmaxf(e[2], e[3]));
+#pragma unroll
+                            for (int x = 0; x < 4; x++) w[c + x] = RAISE ? e[x] : tg_ex2(e[x]);
+                            if (RAISE) continue;
+#pragma unroll
+                            for (int x = 0; x < 4; x += 2) {
+                                const int k = ((c & 7) + x) / 2;
+                                const __half2 hh = __floats2half2_rn(w[c + x], w[c + x + 1]);
+                                uh[k] = *reinterpret_cast<const uint32_t *>(&hh);
+                                if (PP == 2) {
+                                    const float2 back = __half22float2(hh);
+                                    const __half2 ll = __floats2half2_rn(w[c + x] - back.x, w[c + x + 1] - back.y);
+                                    ul[k] = *reinterpret_cast<const uint32_t *>(&ll);
+                                }
+                            }
+                        }
+                        if (RAISE) continue;
+                        const int ch = ((2 * (HC * group + P) + hf) ^ (slot_row & 7)) << 4;
+                        *reinterpret_cast<uint4 *>(pl + ch) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+                        if (PP == 2)
+                            *reinterpret_cast<uint4 *>(pl + kTok * 128 + ch) = make_uint4(ul[0], ul[1], ul[2], ul[3]);
                     }
-                    l[c] = l2.x;
-                    l[c + 1] = l2.y;
-                    z[c] = z2.x;
-                    z[c + 1] = z2.y;
-                    const __half2 hh = __floats2half2_rn(w.x, w.y);
-                    uh[x] = *reinterpret_cast<const uint32_t *>(&hh);
-                    if (PP == 2) {
-                        const float2 back = __half22float2(hh);
-                        const __half2 ll = __floats2half2_rn(w.x - back.x, w.y - back.y);
-                        ul[x] = *reinterpret_cast<const uint32_t *>(&ll);
+                    return fmaxf(top0, top1);
+                };
+                for (bool raise = starts;;) {
+                    if (!raise) {
+                        const float top = pass(std::false_type{});
+                        raise = group_or(group, !ok || top > kHead + kShift);
+                        if (!raise) break;
+                        if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
+                        if (group_or(group, !ok)) return false;
+                        tc_fence_after();
+                    }
+                    pass(std::true_type{});
+                    const float cm = warp_columns(w, lane, [](float x, float y) { return fmaxf(x, y); });
+                    if (lane < kCols) my_red[lane] = cm;  // (the group's last reads of it are behind a barrier)
+                    group_or(group, false);
+                    if (wq == 0 && lane < kCols) {
+                        const float old = -gref[p0 + lane];
+                        float m = old + kShift;
+#pragma unroll
+                        for (int x = 0; x < 4; x++) m = fmaxf(m, grp_red[x * kRed + lane]);
+                        gfac[p0 + lane] = old == -INFINITY ? 0.0f : exp2f(old - (m - kShift));
+                        gref[p0 + lane] = kShift - m;
+                    }
+                    group_or(group, false);
+                    if (!starts) {
+                        uint32_t o[16];
+                        tmem_ld16(tl + GG::O + c0 + p0, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < kCols; c++) {
+                            const float f = gfac[p0 + c];
+                            l[P][c] *= f;
+                            z[P][c] *= f;
+                            o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+                        }
+                        tmem_st16(tl + GG::O + c0 + p0, o);
+                        tmem_wait_st();
+                    }
+                    raise = false;
+                }
+                // the token's sums; an unseen token takes no part, whatever its metadata holds
+#pragma unroll
+                for (int c = 0; c < kCols; c += 2) {
+                    const float2 w2 = make_float2(w[c], w[c + 1]);
+                    const float2 l2 = fma2(w2, rv2, make_float2(l[P][c], l[P][c + 1]));
+                    const float2 z2 = fma2(w2, zv2, make_float2(z[P][c], z[P][c + 1]));
+                    const bool s0 = !MASK || (sees >> c) & 1, s1 = !MASK || (sees >> (c + 1)) & 1;
+                    l[P][c] = s0 ? l2.x : l[P][c];
+                    l[P][c + 1] = s1 ? l2.y : l[P][c + 1];
+                    z[P][c] = s0 ? z2.x : z[P][c];
+                    z[P][c + 1] = s1 ? z2.y : z[P][c + 1];
+                }
+                return true;
+            };
+            using First = std::integral_constant<int, 0>;
+            using Second = std::integral_constant<int, HC - 1>;
+            bool done;
+            if ((kt + 1) * kTok <= a.pos0) {
+                done = part(std::false_type{}, First{}, 0u);
+                if (HC == 2 && done) done = part(std::false_type{}, Second{}, 0u);
+            } else {
+                const int pos = kt * kTok + tok, dj = pos - (int)a.pos0;
+                uint32_t sees = dj < 0 ? 0xffffffffu : 0u;
+                if (dj >= 0 && pos < total) {
+                    const uint64_t *path = t.path + (int64_t)(u / a.heads) * kMaxDraftNodes;
+#pragma unroll 1
+                    for (int c = 0; c < HC * kCols; c++) {
+                        const int node = (rb * NR + c0 + c) / a.group;
+                        if (node < a.seq_len && ((path[node] >> dj) & 1)) sees |= 1u << c;
                     }
                 }
-                const int ch = ((2 * group + hf) ^ (slot_row & 7)) << 4;
-                *reinterpret_cast<uint4 *>(pl + ch) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
-                if (PP == 2) *reinterpret_cast<uint4 *>(pl + kTok * 128 + ch) = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+                done = part(std::true_type{}, First{}, sees);
+                if (HC == 2 && done) done = part(std::true_type{}, Second{}, sees >> kCols);
             }
+            if (!done) break;
+            tc_fence_before();
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(p_full + (i & 1));
-                mbar_arrive(raw_empty + st);
-            }
+            warp_arrive(p_full + (i & 1), lane);
             if (kt == t.ntiles - 1 || i == n - 1) {
                 // ---- the unit's partial record ----
-                const float lc = warp_columns(l, lane, [](float x, float y) { return x + y; });
-                const float zc = warp_columns(z, lane, [](float x, float y) { return x + y; });
-                if (lane < kCols) {
-                    my_red[lane] = lc;
-                    my_red[kCols + lane] = zc;
+#pragma unroll
+                for (int p = 0; p < HC; p++) {
+                    const float lc = warp_columns(l[p], lane, [](float x, float y) { return x + y; });
+                    const float zc = warp_columns(z[p], lane, [](float x, float y) { return x + y; });
+                    if (lane < kCols) {
+                        my_red[p * kCols + lane] = lc;
+                        my_red[(HC + p) * kCols + lane] = zc;
+                    }
                 }
                 ok = wait(pv_done + (i & 1), i >> 1);
                 if (group_or(group, !ok)) break;
                 tc_fence_after();
                 float *rec = t.records + ((int64_t)(grp + u) * t.nb + rb) * GG::REC;
-                if (wq == 0 && lane < kCols) {
+                if (wq == 0 && lane < HC * kCols) {
                     float ls = 0.0f, zs = 0.0f;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
-                        ls += grp_red[w * kCols * 2 + lane];
-                        zs += grp_red[w * kCols * 2 + kCols + lane];
+                        ls += grp_red[w * kRed + lane];
+                        zs += grp_red[w * kRed + HC * kCols + lane];
                     }
-                    rec[NR * D + c0 + lane] = gref[lane];
+                    rec[NR * D + c0 + lane] = -gref[lane];
                     rec[NR * D + NR + c0 + lane] = ls;
                     rec[NR * D + 2 * NR + c0 + lane] = zs;
                 }
-                uint32_t v[16];
-                tmem_ld16(tl + GG::O + c0, v);
-                tmem_wait_ld();
-                if (tok < D) {  // tok is the lane of O: a dimension
 #pragma unroll
-                    for (int c = 0; c < kCols; c++) rec[(c0 + c) * D + tok] = __uint_as_float(v[c]);
+                for (int p = 0; p < HC; p++) {
+                    uint32_t v[16];
+                    tmem_ld16(tl + GG::O + c0 + p * kCols, v);
+                    tmem_wait_ld();
+                    if (tok < D) {  // tok is the lane of O
+                        const int dim = 32 * wq + v_dimension(lane);
+#pragma unroll
+                        for (int c = 0; c < kCols; c++) rec[(c0 + p * kCols + c) * D + dim] = __uint_as_float(v[c]);
+                    }
                 }
                 tc_fence_before();
                 group_or(group, false);  // my_red and gref are read before the next unit writes them
-                if (kt == t.ntiles - 1 && lane == 0) mbar_arrive(q_empty + ((units - 1) & 1));
             }
             if (++kt == t.ntiles) {
                 kt = 0;
