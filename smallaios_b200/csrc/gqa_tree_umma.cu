@@ -32,7 +32,7 @@
 //   4 K warps, 4 V warps: codes of the tile from shared memory to fp16 in tensor
 //     memory, two buffers each; the K warps also turn the tokens' scales and zero
 //     points into what the softmax needs.
-//   1 MMA warp: S^T(i), then O^T of tile i - 1.
+//   2 MMA warps: one issues S^T, the other O^T.
 //   1 copy warp: codes and metadata of the tiles by bulk copies into a ring.
 // The tiles of all units (batch row, KV head) are laid end to end and cut into
 // equal ranges; row blocks beyond the first 64 rows run in CTAs of their own that
@@ -59,6 +59,9 @@ constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
 constexpr int kCols = 16;       // query rows that a softmax thread works on at a time
 constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
 constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
+// With four softmax groups the 864 threads are launched with 72 registers each; the 256 threads of the K and V
+// warps hand theirs on to the softmax: 512 * 88 + 256 * 40 + 96 * 72 = 864 * 72.
+constexpr int kSoftRegs = 88, kStageRegs = 40;
 constexpr int kPrepThreads = 256;
 constexpr int kMergeWarps = 8;
 
@@ -67,7 +70,8 @@ struct Tg {
     static constexpr int CB = D * BITS / 8;
     static constexpr int NG = NR / kCols;                   // softmax groups of four warps
     static constexpr int HC = NR / kCols / NG;              // 16-row parts per group
-    static constexpr int THREADS = 32 * (4 * NG + 10);
+    static constexpr int THREADS = 32 * (4 * NG + 11);
+    static constexpr bool SPLIT = NG == 4;                  // registers handed on (kSoftRegs)
     static constexpr int PBUF = PP * kTok * 128;            // u planes of a tile: [128 tokens][64 rows], 128-byte swizzle
     static constexpr int QPLANE = NR * D * 2;               // D/64 tiles of [NR rows][128 B]
     static constexpr int QREC = QP * QPLANE + NR * 4 + 16;  // planes, sum(q^) of the rows, power of two
@@ -194,6 +198,16 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                  : "r"(taddr));
+}
+
+// Registers per thread of this warpgroup (all four warps execute it).
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
 }
 
 // OR of `v` over the 128 threads of a softmax group (named barrier 1 + group).
@@ -323,8 +337,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
     uint64_t *bars = reinterpret_cast<uint64_t *>(red + 16 * 2 * kCols * HC);
     uint64_t *raw_full = bars, *raw_empty = bars + 8, *ka_full = bars + 16, *va_full = bars + 18, *qk_done = bars + 20,
              *pv_done = bars + 22, *p_full = bars + 24, *q_full = bars + 26, *q_empty = bars + 28, *bar_fin = bars + 30;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 31);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 32);
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 32);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 33);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int grp = blockIdx.x / t.nb, rb = blockIdx.x % t.nb;
@@ -347,6 +361,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             mbar_init(q_empty + i, 1);
         }
         mbar_init(bar_fin, 1);
+        mbar_init(bar_fin + 1, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -364,107 +379,121 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         return (bool)__all_sync(0xffffffffu, ok);
     };
 
-    if (warp == SM + 9) {
-        // ================= copies =================
-        int u = u0, kt = k0, units = 0, issued = 0;
-        for (int i = 0; i < n; i++) {
-            const int st = i % NST;
-            bool ok = i < NST || wait(raw_empty + st, i / NST - 1);
-            if (ok && (i == 0 || kt == 0)) {
-                const int qb = units & 1;
-                ok = units < 2 || wait(q_empty + qb, units / 2 - 1);
-                if (ok && lane == 0) {
+    // one thread's waits (the single-thread roles)
+    auto wait1 = [&](uint64_t *bar, int phase) {
+        return um_try(bar, (uint32_t)(phase & 1)) || tc_wait_sleep(bar, (uint32_t)(phase & 1), abort_flag, a.dev_status);
+    };
+    // every MMA this thread issued has completed (before TMEM is freed)
+    auto drain = [&](uint64_t *bar) {
+        umma_commit(bar);
+        const uint64_t tw = um_clock_ns();
+        while (!um_try(bar, 0) && um_clock_ns() - tw < kTcWaitNs) {
+        }
+    };
+    if (warp == SM + 8) {
+        // ================= copies: one thread =================
+        if (lane == 0) {
+            int u = u0, kt = k0, units = 0, issued = 0, st = 0, ph = -1;
+            const unsigned char *q = t.qimg + ((int64_t)u0 * t.nb + rb) * GG::QBUF;
+            int64_t row = (int64_t)u0 * a.capacity + (int64_t)k0 * kTok;
+            for (int i = 0; i < n; i++) {
+                if (i >= NST && !wait1(raw_empty + st, ph)) break;
+                if (i == 0 || kt == 0) {
+                    const int qb = units & 1;
+                    if (units >= 2 && !wait1(q_empty + qb, units / 2 - 1)) break;
                     mbar_expect_tx(q_full + qb, GG::QREC);
-                    bulk_g2s(smem + GG::Q_OFF + qb * GG::QBUF, t.qimg + ((int64_t)u * t.nb + rb) * GG::QBUF, GG::QREC,
-                             q_full + qb);
-                }
-                units++;
-            }
-            if (!ok) break;
-            // the cache holds whole blocks of 64 tokens: a tile's second half may lie past them
-            const int t0 = kt * kTok, nt = min(kTok, a.capacity - t0);
-            const int64_t row = (int64_t)u * a.capacity + t0;
-            unsigned char *slot = slots + st * GG::SLOT;
-            if (lane == 0) mbar_expect_tx(raw_full + st, (uint32_t)nt * (2 * CB + 16));
-            __syncwarp();
-            if (lane == 0) bulk_g2s(slot, a.k_codes + row * CB, (uint32_t)nt * CB, raw_full + st);
-            if (lane == 1) bulk_g2s(slot + kTok * CB, a.v_codes + row * CB, (uint32_t)nt * CB, raw_full + st);
-            if (lane == 2) bulk_g2s(slot + GG::META, a.k_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
-            if (lane == 3) bulk_g2s(slot + GG::META + kTok * 8, a.v_meta + row * 2, (uint32_t)nt * 8, raw_full + st);
-            issued = i + 1;
-            if (++kt == t.ntiles) {
-                kt = 0;
-                u++;
-            }
-        }
-        if (*abort_flag) {
-            // let the copies in flight land before the CTA ends (bounded)
-            for (int i = max(0, issued - NST); i < issued; i++) mbar_wait_bounded(raw_full + i % NST, (uint32_t)(i / NST) & 1);
-            for (int i = max(0, units - 2); i < units; i++) mbar_wait_bounded(q_full + (i & 1), (uint32_t)(i / 2) & 1);
-        }
-    } else if (warp == SM + 8) {
-        // ================= MMA =================
-        constexpr uint32_t id_s = tg_idesc(NR, 0), id_o = tg_idesc(NR, 1);
-        int kt = k0, units = 0;
-        bool first_prev = true;  // whether tile i - 1 was the first of its unit here
-        int prev_unit = 0;       // its unit
-        for (int i = 0; i <= n; i++) {
-            const bool starts = i == 0 || kt == 0;
-            if (i < n) {
-                bool ok = wait(ka_full + (i & 1), i >> 1);
-                // (S^T's buffer: the softmax of tile i - 2 had read it before p_full(i - 2), seen below)
-                if (ok && starts) {
-                    ok = wait(q_full + (units & 1), units >> 1);
+                    bulk_g2s(smem + GG::Q_OFF + qb * GG::QBUF, q, GG::QREC, q_full + qb);
+                    q += (int64_t)t.nb * GG::QBUF;
                     units++;
                 }
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t q = smem_u32(smem + GG::Q_OFF + ((units - 1) & 1) * GG::QBUF);
-#pragma unroll
-                    for (int pl = 0; pl < QP; pl++)
-#pragma unroll
-                        for (int kk = 0; kk < D / 16; kk++)
-                            umma_ts(tbase + GG::S + (i & 1) * NR, tbase + GG::KA + (i & 1) * (D / 2) + 8 * kk,
-                                    sw128_kmajor_desc(q + pl * GG::QPLANE + (kk >> 2) * (NR * 128) + 32 * (kk & 3)), id_s,
-                                    (pl | kk) != 0 ? 1u : 0u);
-                    umma_commit(qk_done + (i & 1));
+                // the cache holds whole blocks of 64 tokens: a tile's second half may lie past them
+                const uint32_t nt = (uint32_t)min(kTok, a.capacity - kt * kTok);
+                unsigned char *slot = slots + st * GG::SLOT;
+                uint64_t *bar = raw_full + st;
+                mbar_expect_tx(bar, nt * (2 * CB + 16));
+                bulk_g2s(slot, a.k_codes + row * CB, nt * CB, bar);
+                bulk_g2s(slot + kTok * CB, a.v_codes + row * CB, nt * CB, bar);
+                bulk_g2s(slot + GG::META, a.k_meta + row * 2, nt * 8, bar);
+                bulk_g2s(slot + GG::META + kTok * 8, a.v_meta + row * 2, nt * 8, bar);
+                issued = i + 1;
+                row += kTok;
+                if (++kt == t.ntiles) {
+                    kt = 0;
+                    row = (int64_t)++u * a.capacity;
                 }
-                __syncwarp();
-            }
-            if (i > 0) {
-                const int j = i - 1;
-                if (!(wait(p_full + (j & 1), j >> 1) && wait(va_full + (j & 1), j >> 1))) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t p = smem_u32(smem + GG::P_OFF + (j & 1) * GG::PBUF);
-#pragma unroll
-                    for (int pl = 0; pl < PP; pl++)
-#pragma unroll
-                        for (int kk = 0; kk < kTok / 16; kk++)
-                            // B: rows contiguous, 8-token groups 1024 B apart, the same fields as a K-major tile
-                            umma_ts(tbase + GG::O, tbase + GG::VA + (j & 1) * (kTok / 2) + 8 * kk,
-                                    sw128_kmajor_desc(p + pl * (kTok * 128) + 2048 * kk), id_o,
-                                    (pl | kk) != 0 || !first_prev ? 1u : 0u);
-                    umma_commit(pv_done + (j & 1));
-                    // every role is past tile j: its ring slot, and after the unit's last tile its queries, are free
-                    umma_commit(raw_empty + j % NST);
-                    if (i == n || starts) umma_commit(q_empty + (prev_unit & 1));
+                if (++st == NST) {
+                    st = 0;
+                    ph++;
                 }
-                __syncwarp();
             }
-            first_prev = starts;
-            prev_unit = units - 1;
-            if (++kt == t.ntiles) kt = 0;
+            if (*abort_flag) {
+                // let the copies in flight land before the CTA ends (bounded)
+                for (int i = max(0, issued - NST); i < issued; i++)
+                    mbar_wait_bounded(raw_full + i % NST, (uint32_t)(i / NST) & 1);
+                for (int i = max(0, units - 2); i < units; i++) mbar_wait_bounded(q_full + (i & 1), (uint32_t)(i / 2) & 1);
+            }
         }
-        // every issued MMA has completed before TMEM is freed
-        if (elect_one()) umma_commit(bar_fin);
-        __syncwarp();
-        const uint64_t tw = um_clock_ns();
-        while (!um_try(bar_fin, 0) && um_clock_ns() - tw < kTcWaitNs) {
+    } else if (warp == SM + 9) {
+        // ================= S^T: one thread =================
+        if (lane == 0) {
+            constexpr uint32_t id_s = tg_idesc(NR, 0);
+            int kt = k0, units = 0;
+            const uint64_t q0 = sw128_kmajor_desc(smem_u32(smem + GG::Q_OFF));
+            for (int i = 0; i < n; i++) {
+                if (!wait1(ka_full + (i & 1), i >> 1)) break;
+                // O^T(i - 2) complete: the softmax had read S^T(i - 2), whose buffer this takes, and with S^T(i) the
+                // softmax knows that u's buffer is free
+                if (i >= 2 && !wait1(pv_done + (i & 1), (i >> 1) - 1)) break;
+                if (i == 0 || kt == 0) {
+                    if (!wait1(q_full + (units & 1), units >> 1)) break;
+                    units++;
+                }
+                tc_fence_after();
+                const uint64_t q = q0 + (((units - 1) & 1) * (GG::QBUF >> 4));  // start addresses count 16 bytes
+                const uint32_t d = tbase + GG::S + (i & 1) * NR, k = tbase + GG::KA + (i & 1) * (D / 2);
+#pragma unroll
+                for (int pl = 0; pl < QP; pl++)
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk++)
+                        umma_ts(d, k + 8 * kk, q + ((pl * GG::QPLANE + (kk >> 2) * (NR * 128) + 32 * (kk & 3)) >> 4), id_s,
+                                (pl | kk) != 0 ? 1u : 0u);
+                umma_commit(qk_done + (i & 1));
+                if (++kt == t.ntiles) kt = 0;
+            }
+            drain(bar_fin);
+        }
+    } else if (warp == SM + 10) {
+        // ================= O^T: one thread =================
+        if (lane == 0) {
+            constexpr uint32_t id_o = tg_idesc(NR, 1);
+            int kt = k0, units = 0, st = 0;
+            const uint64_t p0 = sw128_kmajor_desc(smem_u32(smem + GG::P_OFF));
+            for (int i = 0; i < n; i++) {
+                const bool starts = i == 0 || kt == 0;
+                if (starts) units++;
+                if (!wait1(va_full + (i & 1), i >> 1) || !wait1(p_full + (i & 1), i >> 1)) break;
+                tc_fence_after();
+                // B: rows contiguous, 8-token groups 1024 B apart -- the same fields as a K-major tile
+                const uint64_t p = p0 + ((i & 1) * (GG::PBUF >> 4));
+                const uint32_t v = tbase + GG::VA + (i & 1) * (kTok / 2);
+#pragma unroll
+                for (int pl = 0; pl < PP; pl++)
+#pragma unroll
+                    for (int kk = 0; kk < kTok / 16; kk++)
+                        umma_ts(tbase + GG::O, v + 8 * kk, p + ((pl * (kTok * 128) + 2048 * kk) >> 4), id_o,
+                                (pl | kk) != 0 || !starts ? 1u : 0u);
+                umma_commit(pv_done + (i & 1));
+                // every role is past tile i: its ring slot, and after the unit's last tile its queries, are free
+                umma_commit(raw_empty + st);
+                if (kt == t.ntiles - 1) umma_commit(q_empty + ((units - 1) & 1));
+                if (++kt == t.ntiles) kt = 0;
+                if (++st == NST) st = 0;
+            }
+            drain(bar_fin + 1);
         }
     } else if (warp >= SM + 4) {
         // ================= V codes -> fp16 =================
+        if constexpr (GG::SPLIT) reg_dec<kStageRegs>();
         const int Q = lane >> 2, q = lane & 3;
         const bool live = 32 * (warp & 3) < D;
         const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
@@ -518,6 +547,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         }
     } else if (warp >= SM) {
         // ================= K codes -> fp16, token constants =================
+        if constexpr (GG::SPLIT) reg_dec<kStageRegs>();
         const int Q = lane >> 2, q = lane & 3, tok = 32 * (warp & 3) + lane;
         constexpr int QB = CB / 4, NW = QB / 4;  // bytes and words of a quarter of a token's codes
         const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
@@ -587,6 +617,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         }
     } else {
         // ================= softmax: thread = token, HC times 16 rows per group =================
+        if constexpr (GG::SPLIT) reg_inc<kSoftRegs>();
         const int group = warp >> 2, wq = warp & 3, c0 = group * HC * kCols;
         const int tok = 32 * wq + lane, slot_row = v_slot(tok);
         float *gref = ref + c0, *gfac = fac + c0;
@@ -602,7 +633,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             // S^T(i); with it the token constants are in place (the K warps wrote them before) and O^T(i - 2),
             // issued before, is complete: u's buffer is free
             bool ok = wait(qk_done + (i & 1), i >> 1);
-            if (starts) {
+            if (__builtin_expect(starts, 0)) {
                 // the group's references start over once every thread is past the last unit's
                 if (ok) ok = wait(q_full + (units & 1), units >> 1);
                 units++;
@@ -637,7 +668,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++) {
-                        uint32_t v[8], uh[4], ul[4];
+                        uint32_t v[8];
+                        [[maybe_unused]] uint32_t uh[4], ul[4];
                         tmem_ld8(sbuf + p0 + 8 * hf, v);
                         tmem_wait_ld();
 #pragma unroll
@@ -661,32 +693,34 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                             top1 = fmaxf(top1, fmaxf(e[2], e[3]));
 #pragma unroll
                             for (int x = 0; x < 4; x++) w[c + x] = RAISE ? e[x] : tg_ex2(e[x]);
-                            if (RAISE) continue;
+                            if constexpr (!RAISE) {
 #pragma unroll
-                            for (int x = 0; x < 4; x += 2) {
-                                const int k = ((c & 7) + x) / 2;
-                                const __half2 hh = __floats2half2_rn(w[c + x], w[c + x + 1]);
-                                uh[k] = *reinterpret_cast<const uint32_t *>(&hh);
-                                if (PP == 2) {
-                                    const float2 back = __half22float2(hh);
-                                    const __half2 ll = __floats2half2_rn(w[c + x] - back.x, w[c + x + 1] - back.y);
-                                    ul[k] = *reinterpret_cast<const uint32_t *>(&ll);
+                                for (int x = 0; x < 4; x += 2) {
+                                    const int k = ((c & 7) + x) / 2;
+                                    const __half2 hh = __floats2half2_rn(w[c + x], w[c + x + 1]);
+                                    uh[k] = *reinterpret_cast<const uint32_t *>(&hh);
+                                    if constexpr (PP == 2) {
+                                        const float2 back = __half22float2(hh);
+                                        const __half2 ll = __floats2half2_rn(w[c + x] - back.x, w[c + x + 1] - back.y);
+                                        ul[k] = *reinterpret_cast<const uint32_t *>(&ll);
+                                    }
                                 }
                             }
                         }
-                        if (RAISE) continue;
-                        const int ch = ((2 * (HC * group + P) + hf) ^ (slot_row & 7)) << 4;
-                        *reinterpret_cast<uint4 *>(pl + ch) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
-                        if (PP == 2)
-                            *reinterpret_cast<uint4 *>(pl + kTok * 128 + ch) = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+                        if constexpr (!RAISE) {
+                            const int ch = ((2 * (HC * group + P) + hf) ^ (slot_row & 7)) << 4;
+                            *reinterpret_cast<uint4 *>(pl + ch) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+                            if constexpr (PP == 2)
+                                *reinterpret_cast<uint4 *>(pl + kTok * 128 + ch) = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+                        }
                     }
                     return fmaxf(top0, top1);
                 };
                 for (bool raise = starts;;) {
-                    if (!raise) {
+                    if (__builtin_expect(!raise, 1)) {
                         const float top = pass(std::false_type{});
                         raise = group_or(group, !ok || top > kHead + kShift);
-                        if (!raise) break;
+                        if (__builtin_expect(!raise, 1)) break;
                         if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
                         if (group_or(group, !ok)) return false;
                         tc_fence_after();
@@ -737,7 +771,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             using First = std::integral_constant<int, 0>;
             using Second = std::integral_constant<int, HC - 1>;
             bool done;
-            if ((kt + 1) * kTok <= a.pos0) {
+            if (__builtin_expect((kt + 1) * kTok <= a.pos0, 1)) {
                 done = part(std::false_type{}, First{}, 0u);
                 if (HC == 2 && done) done = part(std::false_type{}, Second{}, 0u);
             } else {
@@ -759,7 +793,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             warp_arrive(p_full + (i & 1), lane);
-            if (kt == t.ntiles - 1 || i == n - 1) {
+            if (__builtin_expect(kt == t.ntiles - 1 || i == n - 1, 0)) {
                 // ---- the unit's partial record ----
 #pragma unroll
                 for (int p = 0; p < HC; p++) {
