@@ -25,7 +25,7 @@
 //
 // One persistent CTA per SM; roles by warp:
 //   4 or 8 softmax warps (groups of four, 16 or 32 rows each): thread = token of
-//     the tile, 16 rows at a time: tcgen05.ld of S^T, u, the sums l and z of its
+//     the tile: tcgen05.ld of S^T, u, the sums l and z of its
 //     token, u to shared memory (the B operand, rows contiguous).  The reference
 //     ref_r is only raised when some score of the tile outgrows it by 2^8 (one
 //     vote per tile and group); then O is rescaled in tensor memory.
@@ -56,22 +56,22 @@ namespace sa {
 namespace {
 
 constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
-constexpr int kCols = 16;       // query rows that a softmax thread works on at a time
 constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
 constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
-// With four softmax groups the 864 threads are launched with 72 registers each; the 256 threads of the K and V
-// warps hand theirs on to the softmax: 512 * 88 + 256 * 40 + 96 * 72 = 864 * 72.
-constexpr int kSoftRegs = 88, kStageRegs = 40;
 constexpr int kPrepThreads = 256;
 constexpr int kMergeWarps = 8;
 
 template <int BITS, int D, int NR, int QP, int PP>
 struct Tg {
     static constexpr int CB = D * BITS / 8;
-    static constexpr int NG = NR / kCols;                   // softmax groups of four warps
-    static constexpr int HC = NR / kCols / NG;              // 16-row parts per group
+    static constexpr int NC = 16;                           // query rows of a softmax group of four warps
+    static constexpr int NG = NR / NC;
     static constexpr int THREADS = 32 * (4 * NG + 11);
-    static constexpr bool SPLIT = NG == 4;                  // registers handed on (kSoftRegs)
+    // With four groups the 864 threads are launched with 72 registers each, and the 256 threads of the K and V warps
+    // hand some of theirs on to the softmax: 512 * 88 + 256 * 40 + 96 * 72 = 864 * 72 (launch_rows checks the 72).
+    static constexpr bool SPLIT = NG == 4;
+    static constexpr int LAUNCH = 72, SOFT = 88, STAGE = 40;
+    static_assert(!SPLIT || 128 * NG * SOFT + 256 * STAGE + 96 * LAUNCH <= THREADS * LAUNCH, "register split");
     static constexpr int PBUF = PP * kTok * 128;            // u planes of a tile: [128 tokens][64 rows], 128-byte swizzle
     static constexpr int QPLANE = NR * D * 2;               // D/64 tiles of [NR rows][128 B]
     static constexpr int QREC = QP * QPLANE + NR * 4 + 16;  // planes, sum(q^) of the rows, power of two
@@ -221,11 +221,11 @@ __device__ __forceinline__ bool group_or(int group, bool v) {
     return r != 0;
 }
 
-// Sum (or maximum) over the warp of 16 values per lane: lane L returns that of value L & 15.
-template <typename Op>
-__device__ __forceinline__ float warp_columns(float (&v)[kCols], int lane, Op op) {
+// Sum (or maximum) over the warp of N values per lane: lane L returns that of value L % N.
+template <int N, typename Op>
+__device__ __forceinline__ float warp_columns(float (&v)[N], int lane, Op op) {
 #pragma unroll
-    for (int h = kCols / 2; h >= 1; h >>= 1) {
+    for (int h = N / 2; h >= 1; h >>= 1) {
         const bool up = lane & h;
 #pragma unroll
         for (int i = 0; i < h; i++) {
@@ -233,7 +233,9 @@ __device__ __forceinline__ float warp_columns(float (&v)[kCols], int lane, Op op
             v[i] = op(mine, __shfl_xor_sync(0xffffffffu, give, h));
         }
     }
-    return op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
+#pragma unroll
+    for (int h = N; h < 32; h <<= 1) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], h));
+    return v[0];
 }
 
 // ---- query images --------------------------------------------------------------------------------
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
 template <int BITS, int D, int NR, int QP, int PP>
 __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma_kernel(TreeArgs t) {
     using GG = Tg<BITS, D, NR, QP, PP>;
-    constexpr int CB = GG::CB, NST = GG::NST, SM = 4 * GG::NG, HC = GG::HC;
+    constexpr int CB = GG::CB, NST = GG::NST, NC = GG::NC, SM = 4 * GG::NG;
     constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     const AttendArgs &a = t.a;
     extern __shared__ unsigned char tg_raw[];
@@ -333,8 +335,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
     unsigned char *slots = smem + GG::SLOT_OFF;
     float *ref = reinterpret_cast<float *>(smem + GG::MISC_OFF);       // [NR], minus the reference
     float *fac = ref + 64;                                             // [NR]
-    float *red = fac + 64;                                             // [softmax warps][HC][2][16]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 16 * 2 * kCols * HC);
+    float *red = fac + 64;                                             // [softmax warps][2][NC]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 16 * 2 * NC);
     uint64_t *raw_full = bars, *raw_empty = bars + 8, *ka_full = bars + 16, *va_full = bars + 18, *qk_done = bars + 20,
              *pv_done = bars + 22, *p_full = bars + 24, *q_full = bars + 26, *q_empty = bars + 28, *bar_fin = bars + 30;
     uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 32);
@@ -493,13 +495,12 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         }
     } else if (warp >= SM + 4) {
         // ================= V codes -> fp16 =================
-        if constexpr (GG::SPLIT) reg_dec<kStageRegs>();
+        if constexpr (GG::SPLIT) reg_dec<GG::STAGE>();
         const int Q = lane >> 2, q = lane & 3;
         const bool live = 32 * (warp & 3) < D;
         const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
-        for (int i = 0; i < n; i++) {
-            const int st = i % NST;
-            if (!wait(raw_full + st, i / NST)) break;
+        for (int i = 0, st = 0, ph = 0; i < n; i++) {
+            if (!wait(raw_full + st, ph)) break;
             if (i >= 2 && !wait(pv_done + (i & 1), (i >> 1) - 1)) break;
             tc_fence_after();
             if (live) {
@@ -544,16 +545,16 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             tc_fence_before();
             __syncwarp();
             warp_arrive(va_full + (i & 1), lane);
+            if (++st == NST) st = 0, ph ^= 1;
         }
     } else if (warp >= SM) {
         // ================= K codes -> fp16, token constants =================
-        if constexpr (GG::SPLIT) reg_dec<kStageRegs>();
+        if constexpr (GG::SPLIT) reg_dec<GG::STAGE>();
         const int Q = lane >> 2, q = lane & 3, tok = 32 * (warp & 3) + lane;
         constexpr int QB = CB / 4, NW = QB / 4;  // bytes and words of a quarter of a token's codes
         const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
-        for (int i = 0; i < n; i++) {
-            const int st = i % NST;
-            if (!wait(raw_full + st, i / NST)) break;
+        for (int i = 0, st = 0, ph = 0; i < n; i++) {
+            if (!wait(raw_full + st, ph)) break;
             if (i >= 2 && !wait(qk_done + (i & 1), (i >> 1) - 1)) break;
             tc_fence_after();
             unsigned char *slot = slots + st * GG::SLOT;
@@ -614,228 +615,240 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             tc_fence_before();
             __syncwarp();
             warp_arrive(ka_full + (i & 1), lane);
+            if (++st == NST) st = 0, ph ^= 1;
         }
     } else {
-        // ================= softmax: thread = token, HC times 16 rows per group =================
-        if constexpr (GG::SPLIT) reg_inc<kSoftRegs>();
-        const int group = warp >> 2, wq = warp & 3, c0 = group * HC * kCols;
+        // ================= softmax: thread = token, NC rows =================
+        if constexpr (GG::SPLIT) reg_inc<GG::SOFT>();
+        const int group = warp >> 2, wq = warp & 3, c0 = group * NC;
         const int tok = 32 * wq + lane, slot_row = v_slot(tok);
         float *gref = ref + c0, *gfac = fac + c0;
-        constexpr int kRed = HC * 2 * kCols;
-        float *my_red = red + warp * kRed, *grp_red = red + group * 4 * kRed;
+        float *my_red = red + warp * 2 * NC, *grp_red = red + group * 8 * NC;
+        unsigned char *pl = smem + GG::P_OFF + (slot_row >> 3) * 1024 + (slot_row & 7) * 128;
+        const int ch0 = (group * (NC / 8)) << 4, chx = (slot_row & 7) << 4;  // 16-byte chunk c of its row: (ch0 + 16 c) ^ chx
+        const unsigned char *consts = slots + GG::CONST;  // of the tile's ring slot
+        const float *qsum = nullptr;
         int u = u0, kt = k0, units = 0;
-        float l[HC][kCols], z[HC][kCols];
+        float l[NC], z[NC];
         for (int i = 0; i < n; i++) {
-            const int st = i % NST;
             const bool starts = i == 0 || kt == 0;
-            const float *qsum = reinterpret_cast<const float *>(smem + GG::Q_OFF + ((starts ? units : units - 1) & 1) * GG::QBUF +
-                                                                QP * GG::QPLANE) + c0;
             // S^T(i); with it the token constants are in place (the K warps wrote them before) and O^T(i - 2),
-            // issued before, is complete: u's buffer is free
+            // which the S^T warp waited for, is complete: u's buffer is free
             bool ok = wait(qk_done + (i & 1), i >> 1);
             if (__builtin_expect(starts, 0)) {
-                // the group's references start over once every thread is past the last unit's
                 if (ok) ok = wait(q_full + (units & 1), units >> 1);
+                qsum = reinterpret_cast<const float *>(smem + GG::Q_OFF + (units & 1) * GG::QBUF + QP * GG::QPLANE) + c0;
                 units++;
 #pragma unroll
-                for (int p = 0; p < HC; p++)
-#pragma unroll
-                    for (int c = 0; c < kCols; c++) l[p][c] = z[p][c] = 0.0f;
-                if (wq == 0 && lane < HC * kCols) gref[lane] = INFINITY;
+                for (int c = 0; c < NC; c++) l[c] = z[c] = 0.0f;
+                if (wq == 0 && lane < NC) gref[lane] = INFINITY;  // no token seen yet
                 if (group_or(group, !ok)) break;  // (also: the references are written)
             }
             tc_fence_after();
-            const unsigned char *slot = slots + st * GG::SLOT;
-            const float4 tc = *reinterpret_cast<const float4 *>(slot + GG::CONST + tok * 16);
-            const float zv = *reinterpret_cast<const float *>(slot + GG::CONST + kTok * 16 + tok * 4);
-            const float ks = tc.x * qsum[NR - c0], kz = tc.y, lv = tc.z, rv = tc.w;
-            const uint32_t sbuf = tl + GG::S + (i & 1) * NR + c0;
-            unsigned char *pl = smem + GG::P_OFF + (i & 1) * GG::PBUF + (slot_row >> 3) * 1024 + (slot_row & 7) * 128;
-            // 16 rows of the tile, from row p0 of the group; `masked`: it holds drafts, or tokens past them (sees:
-            // the rows that see this token)
-            auto part = [&](auto masked, auto which, uint32_t sees) {
-                constexpr bool MASK = decltype(masked)::value;
-                constexpr int P = decltype(which)::value, p0 = P * kCols;
-                const float2 kz2 = make_float2(kz, kz), ks2 = make_float2(ks, ks), lv2 = make_float2(lv, lv);
-                const float2 rv2 = make_float2(rv, rv), zv2 = make_float2(zv, zv);
-                float w[kCols];
-                // A unit's first tile, and one with a score that outgrew its reference, first raise the references
-                // to the tile's maxima.  u is computed before the vote on that, so that the exponentials overlap the
-                // scores' arithmetic; a raise does it over.
-                // w: the scores (raising), or u, which also goes to shared memory; returns the largest score
-                auto pass = [&](auto raising) {
-                    constexpr bool RAISE = decltype(raising)::value;
-                    float top0 = -INFINITY, top1 = -INFINITY;
+            uint32_t v[NC];
+            auto load = [&]() { tmem_ld16(tl + GG::S + (i & 1) * NR + c0, v); };
+            load();
+            // drafts in the tile, or tokens past them: bit c of `sees`: row c sees this token
+            const bool masked = (kt + 1) * kTok > a.pos0;
+            uint32_t sees = 0xffffffffu;
+            if (__builtin_expect(masked, 0)) {
+                const int pos = kt * kTok + tok, dj = pos - (int)a.pos0;
+                if (dj >= 0) {
+                    const uint64_t *path = t.path + (int64_t)(u / a.heads) * kMaxDraftNodes;
+                    sees = 0;
+                    if (pos < total) {
+#pragma unroll 1
+                        for (int c = 0; c < NC; c++) {
+                            const int node = (rb * NR + c0 + c) / a.group;
+                            if (node < a.seq_len && ((path[node] >> dj) & 1)) sees |= 1u << c;
+                        }
+                    }
+                }
+            }
+            const float4 tc = *reinterpret_cast<const float4 *>(consts + tok * 16);
+            const float zv = *reinterpret_cast<const float *>(consts + kTok * 16 + tok * 4);
+            const float ks = tc.x * qsum[NR - c0], rv = tc.w;
+            const float2 ks2 = make_float2(ks, ks), kz2 = make_float2(tc.y, tc.y), lv2 = make_float2(tc.z, tc.z);
+            unsigned char *dst = pl + (i & 1) * GG::PBUF;
+            // w = u = vs 2^(s - ref), which also goes to shared memory -- or, raising, the scores themselves; returns the
+            // largest score.  u is computed before the vote on its range, so that the exponentials overlap the scores'
+            // arithmetic (1.15 times as fast at 64 rows); a raise does it over.
+            float w[NC];
+            auto pass = [&](auto raising, auto masking) {
+                constexpr bool RAISE = decltype(raising)::value, MASK = decltype(masking)::value;
+                float top0 = -INFINITY, top1 = -INFINITY;
+                tmem_wait_ld();
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        uint32_t v[8];
-                        [[maybe_unused]] uint32_t uh[4], ul[4];
-                        tmem_ld8(sbuf + p0 + 8 * hf, v);
-                        tmem_wait_ld();
+                for (int hf = 0; hf < NC / 8; hf++) {
+                    [[maybe_unused]] uint32_t uh[4], ul[4];
 #pragma unroll
-                        for (int c = 8 * hf; c < 8 * hf + 8; c += 4) {
-                            const float4 q4 = *reinterpret_cast<const float4 *>(qsum + p0 + c);
-                            float4 r4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (!RAISE) r4 = *reinterpret_cast<const float4 *>(gref + p0 + c);  // minus the reference
-                            const float2 b0 = fma2(kz2, make_float2(q4.x, q4.y), add2(make_float2(r4.x, r4.y), lv2));
-                            const float2 b1 = fma2(kz2, make_float2(q4.z, q4.w), add2(make_float2(r4.z, r4.w), lv2));
-                            const float2 s0 =
-                                fma2(make_float2(__uint_as_float(v[c & 7]), __uint_as_float(v[(c & 7) + 1])), ks2, b0);
-                            const float2 s1 =
-                                fma2(make_float2(__uint_as_float(v[(c & 7) + 2]), __uint_as_float(v[(c & 7) + 3])), ks2, b1);
-                            float e[4] = {s0.x, s0.y, s1.x, s1.y};
-                            if (MASK) {
+                    for (int c = 0; c < 8; c += 4) {
+                        const float4 q4 = *reinterpret_cast<const float4 *>(qsum + 8 * hf + c);
+                        float4 r4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (!RAISE) r4 = *reinterpret_cast<const float4 *>(gref + 8 * hf + c);  // minus the reference
+                        const float2 b0 = fma2(kz2, make_float2(q4.x, q4.y), add2(make_float2(r4.x, r4.y), lv2));
+                        const float2 b1 = fma2(kz2, make_float2(q4.z, q4.w), add2(make_float2(r4.z, r4.w), lv2));
+                        const float2 s0 = fma2(make_float2(__uint_as_float(v[8 * hf + c]), __uint_as_float(v[8 * hf + c + 1])), ks2, b0);
+                        const float2 s1 = fma2(make_float2(__uint_as_float(v[8 * hf + c + 2]), __uint_as_float(v[8 * hf + c + 3])), ks2, b1);
+                        float e[4] = {s0.x, s0.y, s1.x, s1.y};
+                        if constexpr (MASK) {
 #pragma unroll
-                                for (int x = 0; x < 4; x++)
-                                    if (!((sees >> (c + x)) & 1)) e[x] = -INFINITY;
-                            }
-                            top0 = fmaxf(top0, fmaxf(e[0], e[1]));
-                            top1 = fmaxf(top1, fmaxf(e[2], e[3]));
+                            for (int x = 0; x < 4; x++)
+                                if (!((sees >> (8 * hf + c + x)) & 1)) e[x] = -INFINITY;
+                        }
+                        top0 = fmaxf(top0, fmaxf(e[0], e[1]));
+                        top1 = fmaxf(top1, fmaxf(e[2], e[3]));
 #pragma unroll
-                            for (int x = 0; x < 4; x++) w[c + x] = RAISE ? e[x] : tg_ex2(e[x]);
-                            if constexpr (!RAISE) {
+                        for (int x = 0; x < 4; x++) w[8 * hf + c + x] = RAISE ? e[x] : tg_ex2(e[x]);
+                        if constexpr (!RAISE) {
 #pragma unroll
-                                for (int x = 0; x < 4; x += 2) {
-                                    const int k = ((c & 7) + x) / 2;
-                                    const __half2 hh = __floats2half2_rn(w[c + x], w[c + x + 1]);
-                                    uh[k] = *reinterpret_cast<const uint32_t *>(&hh);
-                                    if constexpr (PP == 2) {
-                                        const float2 back = __half22float2(hh);
-                                        const __half2 ll = __floats2half2_rn(w[c + x] - back.x, w[c + x + 1] - back.y);
-                                        ul[k] = *reinterpret_cast<const uint32_t *>(&ll);
-                                    }
+                            for (int x = 0; x < 4; x += 2) {
+                                const float2 u2 = make_float2(w[8 * hf + c + x], w[8 * hf + c + x + 1]);
+                                const __half2 hh = __floats2half2_rn(u2.x, u2.y);
+                                uh[(c + x) / 2] = *reinterpret_cast<const uint32_t *>(&hh);
+                                if constexpr (PP == 2) {
+                                    const float2 back = __half22float2(hh);
+                                    const __half2 ll = __floats2half2_rn(u2.x - back.x, u2.y - back.y);
+                                    ul[(c + x) / 2] = *reinterpret_cast<const uint32_t *>(&ll);
                                 }
                             }
                         }
-                        if constexpr (!RAISE) {
-                            const int ch = ((2 * (HC * group + P) + hf) ^ (slot_row & 7)) << 4;
-                            *reinterpret_cast<uint4 *>(pl + ch) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
-                            if constexpr (PP == 2)
-                                *reinterpret_cast<uint4 *>(pl + kTok * 128 + ch) = make_uint4(ul[0], ul[1], ul[2], ul[3]);
-                        }
                     }
-                    return fmaxf(top0, top1);
-                };
-                for (bool raise = starts;;) {
-                    if (__builtin_expect(!raise, 1)) {
-                        const float top = pass(std::false_type{});
-                        raise = group_or(group, !ok || top > kHead + kShift);
-                        if (__builtin_expect(!raise, 1)) break;
-                        if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
-                        if (group_or(group, !ok)) return false;
-                        tc_fence_after();
+                    if constexpr (!RAISE) {
+                        *reinterpret_cast<uint4 *>(dst + ((ch0 + 16 * hf) ^ chx)) = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+                        if constexpr (PP == 2)
+                            *reinterpret_cast<uint4 *>(dst + kTok * 128 + ((ch0 + 16 * hf) ^ chx)) =
+                                make_uint4(ul[0], ul[1], ul[2], ul[3]);
                     }
-                    pass(std::true_type{});
-                    const float cm = warp_columns(w, lane, [](float x, float y) { return fmaxf(x, y); });
-                    if (lane < kCols) my_red[lane] = cm;  // (the group's last reads of it are behind a barrier)
-                    group_or(group, false);
-                    if (wq == 0 && lane < kCols) {
-                        const float old = -gref[p0 + lane];
-                        float m = old + kShift;
+                }
+                return fmaxf(top0, top1);
+            };
+            // A unit's first tile, and one with a score that outgrew its reference, raise the references to the tile's
+            // maxima first (so do tiles where rows may see their first token).
+            bool failed = false;
+            for (bool raise = starts || masked;;) {
+                if (__builtin_expect(!raise, 1)) {
+                    const float top = pass(std::false_type{}, std::false_type{});  // (a masked tile raises)
+                    if (__builtin_expect(!group_or(group, !ok || top > kHead + kShift), 1)) break;
+                }
+                if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
+                if (group_or(group, !ok)) {
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+                load();
+                if (masked) pass(std::true_type{}, std::true_type{});
+                else pass(std::true_type{}, std::false_type{});
+                // (8 columns at a time: few registers beside the hot path's)
 #pragma unroll
-                        for (int x = 0; x < 4; x++) m = fmaxf(m, grp_red[x * kRed + lane]);
-                        gfac[p0 + lane] = old == -INFINITY ? 0.0f : exp2f(old - (m - kShift));
-                        gref[p0 + lane] = kShift - m;
-                    }
-                    group_or(group, false);
-                    if (!starts) {
-                        uint32_t o[16];
-                        tmem_ld16(tl + GG::O + c0 + p0, o);
+                for (int c = 0; c < NC; c += 8) {
+                    float m[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) m[k] = w[c + k];
+                    const float cm = warp_columns(m, lane, [](float x, float y) { return fmaxf(x, y); });
+                    if (lane < 8) my_red[c + lane] = cm;  // (the group's last reads of it are behind a barrier)
+                }
+                group_or(group, false);
+                if (wq == 0 && lane < NC) {
+                    const float old = -gref[lane];
+                    float m = old + kShift;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) m = fmaxf(m, grp_red[x * 2 * NC + lane]);
+                    gfac[lane] = old == -INFINITY ? 0.0f : exp2f(old - (m - kShift));
+                    gref[lane] = kShift - m;
+                }
+                group_or(group, false);
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    l[c] *= gfac[c];
+                    z[c] *= gfac[c];
+                }
+                if (!starts) {
+#pragma unroll 1
+                    for (int c = 0; c < NC; c += 8) {
+                        uint32_t o[8];
+                        tmem_ld8(tl + GG::O + c0 + c, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int c = 0; c < kCols; c++) {
-                            const float f = gfac[p0 + c];
-                            l[P][c] *= f;
-                            z[P][c] *= f;
-                            o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-                        }
-                        tmem_st16(tl + GG::O + c0 + p0, o);
-                        tmem_wait_st();
+                        for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * gfac[c + k]);
+                        tmem_st8(tl + GG::O + c0 + c, o);
                     }
-                    raise = false;
+                    tmem_wait_st();
                 }
-                // the token's sums; an unseen token takes no part, whatever its metadata holds
-#pragma unroll
-                for (int c = 0; c < kCols; c += 2) {
-                    const float2 w2 = make_float2(w[c], w[c + 1]);
-                    const float2 l2 = fma2(w2, rv2, make_float2(l[P][c], l[P][c + 1]));
-                    const float2 z2 = fma2(w2, zv2, make_float2(z[P][c], z[P][c + 1]));
-                    const bool s0 = !MASK || (sees >> c) & 1, s1 = !MASK || (sees >> (c + 1)) & 1;
-                    l[P][c] = s0 ? l2.x : l[P][c];
-                    l[P][c + 1] = s1 ? l2.y : l[P][c + 1];
-                    z[P][c] = s0 ? z2.x : z[P][c];
-                    z[P][c + 1] = s1 ? z2.y : z[P][c + 1];
-                }
-                return true;
-            };
-            using First = std::integral_constant<int, 0>;
-            using Second = std::integral_constant<int, HC - 1>;
-            bool done;
-            if (__builtin_expect((kt + 1) * kTok <= a.pos0, 1)) {
-                done = part(std::false_type{}, First{}, 0u);
-                if (HC == 2 && done) done = part(std::false_type{}, Second{}, 0u);
-            } else {
-                const int pos = kt * kTok + tok, dj = pos - (int)a.pos0;
-                uint32_t sees = dj < 0 ? 0xffffffffu : 0u;
-                if (dj >= 0 && pos < total) {
-                    const uint64_t *path = t.path + (int64_t)(u / a.heads) * kMaxDraftNodes;
-#pragma unroll 1
-                    for (int c = 0; c < HC * kCols; c++) {
-                        const int node = (rb * NR + c0 + c) / a.group;
-                        if (node < a.seq_len && ((path[node] >> dj) & 1)) sees |= 1u << c;
-                    }
-                }
-                done = part(std::true_type{}, First{}, sees);
-                if (HC == 2 && done) done = part(std::true_type{}, Second{}, sees >> kCols);
+                load();
+                if (masked) pass(std::false_type{}, std::true_type{});
+                else pass(std::false_type{}, std::false_type{});
+                break;
             }
-            if (!done) break;
+            if (failed) break;
             tc_fence_before();
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            warp_arrive(p_full + (i & 1), lane);
-            if (__builtin_expect(kt == t.ntiles - 1 || i == n - 1, 0)) {
-                // ---- the unit's partial record ----
+            warp_arrive(p_full + (i & 1), lane);  // (and the last reads of the ring slot are behind)
+            const float2 rv2 = make_float2(rv, rv), zv2 = make_float2(zv, zv);
+            // ---- the token's sums; an unseen token takes no part, whatever its metadata holds ----
+            if (__builtin_expect(masked, 0)) {
 #pragma unroll
-                for (int p = 0; p < HC; p++) {
-                    const float lc = warp_columns(l[p], lane, [](float x, float y) { return x + y; });
-                    const float zc = warp_columns(z[p], lane, [](float x, float y) { return x + y; });
-                    if (lane < kCols) {
-                        my_red[p * kCols + lane] = lc;
-                        my_red[(HC + p) * kCols + lane] = zc;
+                for (int c = 0; c < NC; c++)
+                    if ((sees >> c) & 1) {
+                        l[c] = fmaf(w[c], rv, l[c]);
+                        z[c] = fmaf(w[c], zv, z[c]);
                     }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c += 2) {
+                    const float2 w2 = make_float2(w[c], w[c + 1]);
+                    const float2 l2 = fma2(w2, rv2, make_float2(l[c], l[c + 1]));
+                    const float2 z2 = fma2(w2, zv2, make_float2(z[c], z[c + 1]));
+                    l[c] = l2.x;
+                    l[c + 1] = l2.y;
+                    z[c] = z2.x;
+                    z[c + 1] = z2.y;
                 }
-                ok = wait(pv_done + (i & 1), i >> 1);
+            }
+            consts = consts + GG::SLOT == slots + GG::CONST + NST * GG::SLOT ? slots + GG::CONST : consts + GG::SLOT;
+            kt++;
+            if (__builtin_expect(kt == t.ntiles || i == n - 1, 0)) {
+                // ---- the unit's partial record ----
+                const float lc = warp_columns(l, lane, [](float x, float y) { return x + y; });
+                const float zc = warp_columns(z, lane, [](float x, float y) { return x + y; });
+                if (lane < NC) {
+                    my_red[lane] = lc;
+                    my_red[NC + lane] = zc;
+                }
+                ok = ok && wait(pv_done + (i & 1), i >> 1);
                 if (group_or(group, !ok)) break;
                 tc_fence_after();
                 float *rec = t.records + ((int64_t)(grp + u) * t.nb + rb) * GG::REC;
-                if (wq == 0 && lane < HC * kCols) {
+                if (wq == 0 && lane < NC) {
                     float ls = 0.0f, zs = 0.0f;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
-                        ls += grp_red[w * kRed + lane];
-                        zs += grp_red[w * kRed + HC * kCols + lane];
+                        ls += grp_red[w * 2 * NC + lane];
+                        zs += grp_red[w * 2 * NC + NC + lane];
                     }
                     rec[NR * D + c0 + lane] = -gref[lane];
                     rec[NR * D + NR + c0 + lane] = ls;
                     rec[NR * D + 2 * NR + c0 + lane] = zs;
                 }
-#pragma unroll
-                for (int p = 0; p < HC; p++) {
-                    uint32_t v[16];
-                    tmem_ld16(tl + GG::O + c0 + p * kCols, v);
+                const int dim = 32 * wq + v_dimension(lane);
+#pragma unroll 1
+                for (int c = 0; c < NC; c += 8) {
+                    uint32_t v[8];
+                    tmem_ld8(tl + GG::O + c0 + c, v);
                     tmem_wait_ld();
                     if (tok < D) {  // tok is the lane of O
-                        const int dim = 32 * wq + v_dimension(lane);
 #pragma unroll
-                        for (int c = 0; c < kCols; c++) rec[(c0 + p * kCols + c) * D + dim] = __uint_as_float(v[c]);
+                        for (int k = 0; k < 8; k++) rec[(c0 + c + k) * D + dim] = __uint_as_float(v[k]);
                     }
                 }
                 tc_fence_before();
                 group_or(group, false);  // my_red and gref are read before the next unit writes them
-            }
-            if (++kt == t.ntiles) {
-                kt = 0;
-                u++;
+                if (kt == t.ntiles) {
+                    kt = 0;
+                    u++;
+                }
             }
         }
     }
@@ -955,7 +968,12 @@ int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStre
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GG::SMEM);
+        cudaFuncAttributes fa;
+        cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+        if (e == cudaSuccess && GG::SPLIT && fa.numRegs < GG::LAUNCH)  // the split would wait for registers that are not there
+            return set_error(SA_ERR_CUDA, "gqa_tree_attend: compiled to %d registers, the split needs %d", fa.numRegs,
+                             GG::LAUNCH);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GG::SMEM);
         if (e != cudaSuccess) return check_cuda(e, "gqa_tree_attend smem attribute");
         if (dev >= 0 && dev < 64) __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
     }
