@@ -161,6 +161,8 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
     using GG = G8Geo<BITS, D>;
     using RG = RecGeo<D, 8>;
     constexpr int KB = GG::KB, CT = GG::CT, SCS = GG::SCS;
+    // f32 outputs of a block list: centred value sums (kCodeCentre)
+    constexpr bool CENTRED = LIST && std::is_same<T, float>::value;
 
     extern __shared__ __align__(128) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -404,6 +406,7 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
         // ---------------- phase 2: values, one half of the heads at a time ----------------
 #pragma unroll
         for (int hh = 0; hh < 2; hh++) {
+            int pones[4] = {0, 0, 0, 0};  // sums of the digits themselves
             int pacc[GG::NTV][4];
             const float *sch = scw + (4 * hh + ph) * SCS;
 #pragma unroll
@@ -427,6 +430,7 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
                             const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
                             float vs[4] = {m01.x, m01.z, m23.x, m23.z}, vz[4] = {m01.y, m01.w, m23.y, m23.w};
                             if constexpr (LIST) mask_unseen(n_c[cc] < CT, sv, vs, vz);
+                            if constexpr (CENTRED) centre_zero_points<BITS>(vs, vz);
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const float ee = ex2_approx(sv[e] - Rq[hh]);
@@ -447,6 +451,7 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
                         const uint32_t pa1 = r < 4 ? tile[(r + 8) * kTileW + q] : 0u;
                         const uint32_t pa3 = r < 4 ? tile[(r + 8) * kTileW + 4 + q] : 0u;
                         __syncwarp();
+                        if constexpr (CENTRED) mma_u8u8(pones, pa0, pa1, pa2, pa3, 0x01010101u, 0x01010101u);
 #pragma unroll
                         for (int v = 0; v < GG::VV; v++) {
                             const unsigned char *vb0 = st + (2 * sp) * (KB * kVBlock) + (8 * v + r) * 64 + 16 * q;
@@ -494,6 +499,7 @@ __global__ void __launch_bounds__(kNW8 * 32, 1)
 #pragma unroll
                         for (int x = 0; x < 4; x++) pacc[2 * np][x] -= pacc[2 * np + 1][x];
                     }
+                    if constexpr (CENTRED) centre_sums<BITS>(pacc[2 * np], pacc[2 * np + 1], pones);
 #pragma unroll
                     for (int cc = 0; cc < 2; cc++) {
                         // rows 12-15 of the P tile are zero, so c2/c3 of lanes >= 16 add nothing

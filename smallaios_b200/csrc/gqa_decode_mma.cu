@@ -190,6 +190,8 @@ __global__ void __launch_bounds__(kNW * 32, 2)
                          const float *__restrict__ qscal) {
     using GG = WGeo<BITS, D>;
     constexpr int KB = GG::KB, CT = GG::CT, SCS = GG::SCS;
+    // f32 outputs of a block list: centred value sums (kCodeCentre)
+    constexpr bool CENTRED = LIST && std::is_same<T, float>::value;
 
     extern __shared__ __align__(128) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -428,6 +430,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
         }
 
         // ---------------- phase 2: values ----------------
+        int pones[4] = {0, 0, 0, 0};  // sums of the digits themselves
         int pacc[GG::NTV][4];  // started by the first 32-token step (chunk 0 always holds tokens)
 #pragma unroll
         for (int cc = 0; cc < 2; cc++) {
@@ -450,6 +453,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
                         const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
                         float vs[4] = {m01.x, m01.z, m23.x, m23.z}, vz[4] = {m01.y, m01.w, m23.y, m23.w};
                         if constexpr (LIST) mask_unseen(n_c[cc] < CT, sv, vs, vz);
+                        if constexpr (CENTRED) centre_zero_points<BITS>(vs, vz);
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float ee = ex2_approx(sv[e] - Rq);  // kUMax * 2^(s - R)
@@ -473,6 +477,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
                     const uint32_t pa1 = r < 4 ? tile[(r + 8) * kTileW + q] : 0u;
                     const uint32_t pa3 = r < 4 ? tile[(r + 8) * kTileW + 4 + q] : 0u;
                     __syncwarp();
+                    if constexpr (CENTRED) mma_u8u8(pones, pa0, pa1, pa2, pa3, 0x01010101u, 0x01010101u);
                     // V words of token group q of 16-token blocks 2sp (b0) and 2sp+1 (b1)
 #pragma unroll
                     for (int v = 0; v < GG::VV; v++) {
@@ -526,6 +531,7 @@ __global__ void __launch_bounds__(kNW * 32, 2)
 #pragma unroll
                     for (int x = 0; x < 4; x++) pacc[2 * np][x] -= pacc[2 * np + 1][x];  // low nibbles
                 }
+                if constexpr (CENTRED) centre_sums<BITS>(pacc[2 * np], pacc[2 * np + 1], pones);
 #pragma unroll
                 for (int cc = 0; cc < 2; cc++) {
                     // rows 12-15 of the P tile are zero, so c2/c3 of lanes >= 16 add nothing

@@ -3,7 +3,10 @@
 // to the first slots after the prefix.
 //
 // One CTA per (layer, batch row, KV head) reads the n rows into shared memory,
-// then writes them, so a path may name its rows in any order.
+// then writes them, so a path may name its rows in any order.  A thread keeps
+// its byte (V: bytes of a token lie 4 apart) or word (K) of the row and steps
+// over the rows, so an element costs one load, one store and no division.
+// Bound by the latency of its two round trips to L2 and HBM.
 #include "sa_common.cuh"
 #include "sa_internal.h"
 
@@ -11,11 +14,12 @@ namespace sa {
 
 namespace {
 
-constexpr int kKeepThreads = 128;
+constexpr int kKeepThreads = 256;
 
 // Bytes of shared memory per row: K and V codes, their scale and zero point, and the QJL residuals.
 __host__ __device__ __forceinline__ int keep_row_bytes(int cb, int qb) { return 2 * cb + 16 + (qb ? 2 * qb + 8 : 0); }
 
+// a.bytes, a.words: the row's code bytes and words, up to a power of two (at most 256).
 __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int s_path[kMaxDraftNodes];
@@ -41,10 +45,20 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
     uint8_t *s_k = reinterpret_cast<uint8_t *>(s_mag + (qb ? 2 * n : 0));
     uint8_t *s_v = s_k + n * cb, *s_kq = s_v + n * cb, *s_vq = s_kq + n * qb;
     const int64_t pos0 = a.pos0;
-    for (int i = tid; i < n * cb; i += kKeepThreads) {
-        const int64_t t = pos0 + s_path[i / cb];
-        s_k[i] = kc[t * cb + i % cb];
-        s_v[i] = vc[v_byte_offset(t, i % cb, cb)];
+    // K: word jw of row i; V: byte jv of row i
+    const int cw = cb / 4, jw = tid & (a.words - 1), jv = tid & (a.bytes - 1);
+    const int iw = tid / a.words, iv = tid / a.bytes, dw = kKeepThreads / a.words, dv = kKeepThreads / a.bytes;
+    const uint32_t *kw = reinterpret_cast<const uint32_t *>(kc);
+    uint32_t *s_kw = reinterpret_cast<uint32_t *>(s_k);
+    const int64_t vat = (jv >> 2) * 64 + (jv & 3) * 4;  // of byte jv within a 16-token block
+    auto v_row = [&](int64_t t) { return (t >> 4) * (16 * cb) + ((t >> 2) & 3) * 16 + (t & 3) + vat; };
+    if (jw < cw) {
+#pragma unroll 4
+        for (int i = iw; i < n; i += dw) s_kw[i * cw + jw] = kw[(pos0 + s_path[i]) * cw + jw];
+    }
+    if (jv < cb) {
+#pragma unroll 4
+        for (int i = iv; i < n; i += dv) s_v[i * cb + jv] = vc[v_row(pos0 + s_path[i])];
     }
     for (int i = tid; i < n; i += kKeepThreads) {
         const int64_t t = pos0 + s_path[i];
@@ -61,10 +75,13 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
         s_vq[i] = vq[t * qb + i % qb];
     }
     __syncthreads();
-    for (int i = tid; i < n * cb; i += kKeepThreads) {
-        const int64_t t = pos0 + i / cb;
-        kc[t * cb + i % cb] = s_k[i];
-        vc[v_byte_offset(t, i % cb, cb)] = s_v[i];
+    if (jw < cw) {
+#pragma unroll 4
+        for (int i = iw; i < n; i += dw) reinterpret_cast<uint32_t *>(kc)[(pos0 + i) * cw + jw] = s_kw[i * cw + jw];
+    }
+    if (jv < cb) {
+#pragma unroll 4
+        for (int i = iv; i < n; i += dv) vc[v_row(pos0 + i)] = s_v[i * cb + jv];
     }
     for (int i = tid; i < n; i += kKeepThreads) {
         const int64_t t = pos0 + i;
@@ -90,7 +107,10 @@ int launch_keep_drafts(const KeepArgs &a, cudaStream_t stream) {
         return set_error(SA_ERR_UNSUPPORTED, "kv_cache_keep_drafts: %lld units", (long long)units);
     // at most 64 rows of 2 * 256 code bytes and 88 others: 38400 bytes, below the default limit
     const size_t smem = (size_t)a.n * keep_row_bytes(a.code_bytes, a.k_qjl_bits ? a.head_dim / 8 : 0);
-    keep_drafts_kernel<<<(unsigned)units, kKeepThreads, smem, stream>>>(a);
+    KeepArgs k = a;
+    for (k.bytes = 4; k.bytes < a.code_bytes;) k.bytes *= 2;
+    k.words = k.bytes / 4;
+    keep_drafts_kernel<<<(unsigned)units, kKeepThreads, smem, stream>>>(k);
     count_launch();
     return check_cuda(cudaGetLastError(), "kv_cache_keep_drafts launch");
 }
