@@ -2,11 +2,13 @@
 // accepted drafts (codes, scale, zero point and QJL residual of K and V) move
 // to the first slots after the prefix.
 //
-// One CTA per (layer, batch row, KV head) reads the n rows into shared memory,
-// then writes them, so a path may name its rows in any order.  A thread keeps
-// its byte (V: bytes of a token lie 4 apart) or word (K) of the row and steps
-// over the rows, so an element costs one load, one store and no division.
-// Bound by the latency of its two round trips to L2 and HBM.
+// One CTA per (layer, batch row, KV head) reads before it writes, so a path may
+// name its rows in any order.  K rows move as 16-byte pieces.  A token's V bytes
+// lie 4 apart among those of its neighbours (16-token blocks), so the drafts' V
+// blocks are read whole -- their addresses do not depend on the path, and row by
+// row each byte would cost a 4-byte access and each row half the sectors of its
+// block -- the bytes move in shared memory, and the 16-byte pieces that hold a
+// kept token are written back.
 #include "sa_common.cuh"
 #include "sa_internal.h"
 
@@ -14,12 +16,19 @@ namespace sa {
 
 namespace {
 
-constexpr int kKeepThreads = 256;
+// Two warps per unit: many units in flight, several loads of a thread under way at once.
+constexpr int kKeepThreads = 64;
 
-// Bytes of shared memory per row: K and V codes, their scale and zero point, and the QJL residuals.
-__host__ __device__ __forceinline__ int keep_row_bytes(int cb, int qb) { return 2 * cb + 16 + (qb ? 2 * qb + 8 : 0); }
+// Shared memory: the drafts' V blocks, the kept V bytes, K rows, metadata and QJL residuals.
+__host__ __device__ __forceinline__ int keep_blocks(int64_t pos0, int drafted) {
+    return (int)(((pos0 + drafted - 1) >> 4) - (pos0 >> 4)) + 1;
+}
+__host__ __device__ __forceinline__ size_t keep_smem(int64_t pos0, int drafted, int n, int cb, int qb) {
+    return (size_t)keep_blocks(pos0, drafted) * 16 * cb + (size_t)n * (2 * cb + 16 + (qb ? 2 * qb + 8 : 0));
+}
 
-// a.bytes, a.words: the row's code bytes and words, up to a power of two (at most 256).
+// U: the widest aligned access of the K rows; 2^piece_bits of them, or 2^byte_bits bytes, cover a row.
+template <typename U>
 __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int s_path[kMaxDraftNodes];
@@ -27,38 +36,39 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
     const int64_t unit = blockIdx.x;  // (layer * batch + b) * heads + h
     const int b = (int)(unit / a.heads % a.batch);
     const int cb = a.code_bytes, n = a.n, qb = a.k_qjl_bits ? a.head_dim / 8 : 0;
-    if (tid < n) {
-        const int p = a.path[(int64_t)b * n + tid];
-        const bool ok = p >= 0 && p < a.drafted;
-        if (!ok) atomicOr(a.dev_status, 2);
-        s_path[tid] = ok ? p : tid;
-    }
-    __syncthreads();
-    const int64_t row0 = unit * a.capacity;
-    uint8_t *kc = a.k_codes + row0 * cb, *vc = a.v_codes + row0 * cb;
+    const int64_t pos0 = a.pos0, row0 = unit * a.capacity;
+    const int nblk = keep_blocks(pos0, a.drafted);
+    uint8_t *kc = a.k_codes + row0 * cb;
+    uint4 *vblk = reinterpret_cast<uint4 *>(a.v_codes + row0 * cb + (pos0 >> 4) * (16 * cb));
     float2 *km = reinterpret_cast<float2 *>(a.k_meta) + row0, *vm = reinterpret_cast<float2 *>(a.v_meta) + row0;
     uint8_t *kq = qb ? a.k_qjl_bits + row0 * qb : nullptr, *vq = qb ? a.v_qjl_bits + row0 * qb : nullptr;
     float *kg = qb ? a.k_qjl_mag + row0 : nullptr, *vg = qb ? a.v_qjl_mag + row0 : nullptr;
-    // shared arrays, [n] rows each
-    float2 *s_meta = reinterpret_cast<float2 *>(smem);  // K, then V
-    float *s_mag = reinterpret_cast<float *>(s_meta + 2 * n);
-    uint8_t *s_k = reinterpret_cast<uint8_t *>(s_mag + (qb ? 2 * n : 0));
-    uint8_t *s_v = s_k + n * cb, *s_kq = s_v + n * cb, *s_vq = s_kq + n * qb;
-    const int64_t pos0 = a.pos0;
-    // K: word jw of row i; V: byte jv of row i
-    const int cw = cb / 4, jw = tid & (a.words - 1), jv = tid & (a.bytes - 1);
-    const int iw = tid / a.words, iv = tid / a.bytes, dw = kKeepThreads / a.words, dv = kKeepThreads / a.bytes;
-    const uint32_t *kw = reinterpret_cast<const uint32_t *>(kc);
-    uint32_t *s_kw = reinterpret_cast<uint32_t *>(s_k);
-    const int64_t vat = (jv >> 2) * 64 + (jv & 3) * 4;  // of byte jv within a 16-token block
-    auto v_row = [&](int64_t t) { return (t >> 4) * (16 * cb) + ((t >> 2) & 3) * 16 + (t & 3) + vat; };
-    if (jw < cw) {
-#pragma unroll 4
-        for (int i = iw; i < n; i += dw) s_kw[i * cw + jw] = kw[(pos0 + s_path[i]) * cw + jw];
+    uint4 *s_blk = reinterpret_cast<uint4 *>(smem);
+    float2 *s_meta = reinterpret_cast<float2 *>(smem + nblk * 16 * cb);  // K, then V
+    uint8_t *s_k = reinterpret_cast<uint8_t *>(s_meta + 2 * n);
+    uint8_t *s_v = s_k + n * cb;
+    float *s_mag = reinterpret_cast<float *>(s_v + n * cb);
+    uint8_t *s_kq = reinterpret_cast<uint8_t *>(s_mag + (qb ? 2 * n : 0)), *s_vq = s_kq + n * qb;
+
+    for (int i = tid; i < n; i += kKeepThreads) {
+        const int p = a.path[(int64_t)b * n + i];
+        const bool ok = p >= 0 && p < a.drafted;
+        if (!ok) atomicOr(a.dev_status, 2);
+        s_path[i] = ok ? p : i;
     }
-    if (jv < cb) {
 #pragma unroll 4
-        for (int i = iv; i < n; i += dv) s_v[i * cb + jv] = vc[v_row(pos0 + s_path[i])];
+    for (int i = tid; i < nblk * cb; i += kKeepThreads) s_blk[i] = vblk[i];
+    __syncthreads();
+    // x counts pieces (K) or bytes (V) of the rows, a row's number of them rounded up to a power of two
+    const int np = cb / (int)sizeof(U), off = (int)(pos0 & 15);
+    auto v_at = [&](int row, int j) {
+        const int t = off + row;
+        return (t >> 4) * (16 * cb) + ((t >> 2) & 3) * 16 + (t & 3) + (j >> 2) * 64 + (j & 3) * 4;
+    };
+#pragma unroll 4
+    for (int x = tid; x < n << a.piece_bits; x += kKeepThreads) {
+        const int i = x >> a.piece_bits, j = x & ((1 << a.piece_bits) - 1);
+        if (j < np) reinterpret_cast<U *>(s_k)[i * np + j] = reinterpret_cast<const U *>(kc)[(pos0 + s_path[i]) * np + j];
     }
     for (int i = tid; i < n; i += kKeepThreads) {
         const int64_t t = pos0 + s_path[i];
@@ -74,14 +84,21 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
         s_kq[i] = kq[t * qb + i % qb];
         s_vq[i] = vq[t * qb + i % qb];
     }
-    __syncthreads();
-    if (jw < cw) {
 #pragma unroll 4
-        for (int i = iw; i < n; i += dw) reinterpret_cast<uint32_t *>(kc)[(pos0 + i) * cw + jw] = s_kw[i * cw + jw];
+    for (int x = tid; x < n << a.byte_bits; x += kKeepThreads) {
+        const int i = x >> a.byte_bits, j = x & ((1 << a.byte_bits) - 1);
+        if (j < cb) s_v[i * cb + j] = smem[v_at(s_path[i], j)];
     }
-    if (jv < cb) {
+    __syncthreads();
 #pragma unroll 4
-        for (int i = iv; i < n; i += dv) vc[v_row(pos0 + i)] = s_v[i * cb + jv];
+    for (int x = tid; x < n << a.byte_bits; x += kKeepThreads) {
+        const int i = x >> a.byte_bits, j = x & ((1 << a.byte_bits) - 1);
+        if (j < cb) smem[v_at(i, j)] = s_v[i * cb + j];
+    }
+#pragma unroll 4
+    for (int x = tid; x < n << a.piece_bits; x += kKeepThreads) {
+        const int i = x >> a.piece_bits, j = x & ((1 << a.piece_bits) - 1);
+        if (j < np) reinterpret_cast<U *>(kc)[(pos0 + i) * np + j] = reinterpret_cast<const U *>(s_k)[i * np + j];
     }
     for (int i = tid; i < n; i += kKeepThreads) {
         const int64_t t = pos0 + i;
@@ -97,6 +114,12 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(KeepArgs a) {
         kq[t * qb + i % qb] = s_kq[i];
         vq[t * qb + i % qb] = s_vq[i];
     }
+    __syncthreads();
+    // piece i: token group i % 4 of block i / cb (a block has cb pieces)
+    for (int i = tid; i < keep_blocks(pos0, n) * cb; i += kKeepThreads) {
+        const int t = (i / cb) * 16 + (i & 3) * 4 - off;  // the group's first token, from the first draft
+        if (t + 3 >= 0 && t < n) vblk[i] = s_blk[i];
+    }
 }
 
 }  // namespace
@@ -105,12 +128,18 @@ int launch_keep_drafts(const KeepArgs &a, cudaStream_t stream) {
     const int64_t units = (int64_t)a.layers * a.batch * a.heads;
     if (units > 0x7fffffff)
         return set_error(SA_ERR_UNSUPPORTED, "kv_cache_keep_drafts: %lld units", (long long)units);
-    // at most 64 rows of 2 * 256 code bytes and 88 others: 38400 bytes, below the default limit
-    const size_t smem = (size_t)a.n * keep_row_bytes(a.code_bytes, a.k_qjl_bits ? a.head_dim / 8 : 0);
+    const int qb = a.k_qjl_bits ? a.head_dim / 8 : 0;
+    const size_t smem = keep_smem(a.pos0, a.drafted, a.n, a.code_bytes, qb);  // at most 58 KB
     KeepArgs k = a;
-    for (k.bytes = 4; k.bytes < a.code_bytes;) k.bytes *= 2;
-    k.words = k.bytes / 4;
-    keep_drafts_kernel<<<(unsigned)units, kKeepThreads, smem, stream>>>(k);
+    const bool wide = a.code_bytes % 16 == 0;
+    while ((1 << k.byte_bits) < a.code_bytes) k.byte_bits++;
+    while (((wide ? 16 : 4) << k.piece_bits) < a.code_bytes) k.piece_bits++;
+    auto kern = wide ? keep_drafts_kernel<uint4> : keep_drafts_kernel<uint32_t>;
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return check_cuda(e, "kv_cache_keep_drafts smem attribute");
+    }
+    kern<<<(unsigned)units, kKeepThreads, smem, stream>>>(k);
     count_launch();
     return check_cuda(cudaGetLastError(), "kv_cache_keep_drafts launch");
 }
