@@ -562,7 +562,8 @@ DecodeGrid8 decode8_grid(const AttendArgs &a) {
     const int64_t total = a.block_ids ? (int64_t)a.max_blocks * kBlockTokens : a.pos0 + 1;
     g.ncu = (int)((total + GG::CT - 1) / GG::CT);
     g.F = a.batch * a.heads * g.ncu;
-    g.W = min(a.sm_count * kNW8, g.F);
+    // a block list's ranges have two chunks at least, one copied with the other: half the records to merge
+    g.W = min(a.sm_count * kNW8, a.block_ids ? (g.F + 1) / 2 : g.F);
     g.ctas = (g.W + kNW8 - 1) / kNW8;
     return g;
 }

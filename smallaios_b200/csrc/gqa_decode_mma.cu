@@ -593,7 +593,8 @@ DecodeGrid decode_grid(const AttendArgs &a) {
     const int64_t total = a.block_ids ? (int64_t)a.max_blocks * kBlockTokens : a.pos0 + 1;
     g.ncu = (int)((total + GG::CT - 1) / GG::CT);
     g.F = a.batch * a.heads * g.ncu;  // fits int: decode_fast_eligible bounds it
-    g.W = min(2 * a.sm_count * kNW, g.F);
+    // a block list's ranges have two chunks at least, one copied with the other: half the records to merge
+    g.W = min(2 * a.sm_count * kNW, a.block_ids ? (g.F + 1) / 2 : g.F);
     g.ctas = (g.W + kNW - 1) / kNW;
     return g;
 }

@@ -261,16 +261,19 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
     const float *sg = a.signs + (int64_t)h * D + lane * EPL;
     const float mul = a.wht_scale * a.scale * 1.4426950408889634f;
     float x[RW][EPL], top = 0.0f;
+    // row r of the KV head is query head g = r % G of node r / G: step over them without a division per row
+    const T *src = static_cast<const T *>(a.query) + ((int64_t)b * nodes * a.heads + h) * a.group * D + lane * EPL;
+    int g = (rb * NR + warp * RW) % a.group;
+    src += ((int64_t)((rb * NR + warp * RW) / a.group) * a.heads * a.group + g) * D;
 #pragma unroll
     for (int i = 0; i < RW; i++) {
-        const int r = rb * NR + warp * RW + i;
 #pragma unroll
         for (int e = 0; e < EPL; e++) x[i][e] = 0.0f;
-        if (r < t.rows) {
-            const int node = r / a.group, g = r % a.group;
-            const T *src = static_cast<const T *>(a.query) +
-                           (((int64_t)b * nodes + node) * (a.heads * a.group) + h * a.group + g) * D;
-            load_elems<T, EPL>(src + lane * EPL, x[i]);
+        if (rb * NR + warp * RW + i < t.rows) load_elems<T, EPL>(src, x[i]);
+        src += D;
+        if (++g == a.group) {
+            g = 0;
+            src += (int64_t)(a.heads - 1) * a.group * D;
         }
     }
 #pragma unroll
@@ -298,21 +301,52 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
     for (int i = 0; i < RW; i++) {
         const int row = warp * RW + i;
         float sum = 0.0f;
+        uint32_t hs[EPL];  // hi, and lo above it
 #pragma unroll
         for (int e = 0; e < EPL; e++) {
             const float y = x[i][e] * up;
             const __half hi = __float2half_rn(y);
             const float hf = __half2float(hi);
-            const int p = k_position<BITS, D>(lane * EPL + e);
-            unsigned char *dst = img + (p >> 6) * (NR * 128) + sw128(row, (p & 63) >> 3) + (p & 7) * 2;
-            *reinterpret_cast<__half *>(dst) = hi;
             float kept = hf;
+            hs[e] = __half_as_ushort(hi);
             if (QP == 2) {
                 const __half lo = __float2half_rn(y - hf);
-                *reinterpret_cast<__half *>(dst + G0::QPLANE) = lo;
+                hs[e] |= (uint32_t)__half_as_ushort(lo) << 16;
                 kept += __half2float(lo);
             }
             sum += vtr ? kept * vtr[e] : kept;  // sum(q^), or q^.V^T with low-rank K
+        }
+        if constexpr (D == 128) {
+            // The lane's four dimensions (and, 4 bits, its neighbour's) make pairs of adjacent 32-bit words:
+            // 4 bits: lanes 2m and 2m + 1 hold the halves of four words, each stores two; 8 bits: a lane holds both.
+            uint32_t first[2], second[2];  // lower and upper halves of the two words
+            if constexpr (BITS == 4) {
+                const bool odd = lane & 1;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? hs[k] : hs[2 + k], 1);
+                    first[k] = odd ? got : hs[k];
+                    second[k] = odd ? hs[2 + k] : got;
+                }
+            } else {
+                first[0] = hs[0], first[1] = hs[1];
+                second[0] = hs[2], second[1] = hs[3];
+            }
+            const int p = k_position<BITS, D>(BITS == 4 ? (lane & ~1) * 4 + 2 * (lane & 1) : lane * 4);
+            unsigned char *dst = img + (p >> 6) * (NR * 128) + sw128(row, (p & 63) >> 3) + (p & 7) * 2;
+            *reinterpret_cast<uint2 *>(dst) =
+                make_uint2(__byte_perm(first[0], second[0], 0x5410), __byte_perm(first[1], second[1], 0x5410));
+            if (QP == 2)
+                *reinterpret_cast<uint2 *>(dst + G0::QPLANE) =
+                    make_uint2(__byte_perm(first[0], second[0], 0x7632), __byte_perm(first[1], second[1], 0x7632));
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL; e++) {
+                const int p = k_position<BITS, D>(lane * EPL + e);
+                unsigned char *dst = img + (p >> 6) * (NR * 128) + sw128(row, (p & 63) >> 3) + (p & 7) * 2;
+                *reinterpret_cast<uint16_t *>(dst) = (uint16_t)hs[e];
+                if (QP == 2) *reinterpret_cast<uint16_t *>(dst + G0::QPLANE) = (uint16_t)(hs[e] >> 16);
+            }
         }
         sum = warp_sum(sum);
         if (lane == 0) qsum[row] = sum * down;
@@ -861,52 +895,98 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
 }
 
 // ---- merge -------------------------------------------------------------------------------------------
-// One warp per query row: joins the unit's records, rotates back and stores.
+// Range that holds flat tile f when F tiles are cut into `groups` ranges [w F / groups, (w + 1) F / groups).
+__device__ __forceinline__ int range_of(int64_t f, int F, int groups) {
+    const int64_t x = (f + 1) * groups - 1;
+    int w = (int)((float)x / (float)F);  // the guess is off by one at most per 2^23: stepped to the exact one
+    while ((int64_t)(w + 1) * F <= x) w++;
+    while ((int64_t)w * F > x) w--;
+    return w;
+}
+
+// One warp per query row: joins the unit's records, rotates back and stores.  Four records' loads at a time.
 template <typename T, int BITS, int D, int NR>
 __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeArgs t) {
-    constexpr int EPL = D / 32, REC = NR * D + 3 * NR;
+    constexpr int EPL = D / 32, REC = NR * D + 3 * NR, BATCH = 4;
     const AttendArgs &a = t.a;
     const int lane = threadIdx.x & 31;
-    const int64_t id = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    const int u = blockIdx.x, h = u % a.heads, b = u / a.heads;
+    const int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), rb = r / NR, rr = r % NR;
+    const float *sg = a.signs + (int64_t)h * D + lane * EPL;
+    float sgw[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; e++) sgw[e] = a.wht_scale * sg[e];
+    // ranges that touch tiles [u ntiles, (u + 1) ntiles)
+    const int lo = range_of((int64_t)u * t.ntiles, t.F, t.groups);
+    const int hi = range_of((int64_t)(u + 1) * t.ntiles - 1, t.F, t.groups);
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    if (id >= (int64_t)a.batch * a.heads * t.rows) return;
-    const int u = (int)(id / t.rows), r = (int)(id % t.rows), rb = r / NR, rr = r % NR;
-    const int h = u % a.heads, b = u / a.heads, node = r / a.group, g = r % a.group;
+    if (r >= t.rows) return;
+    const int node = r / a.group, g = r % a.group;
     T *dst = static_cast<T *>(a.out) + (((int64_t)b * a.seq_len + node) * (a.heads * a.group) + h * a.group + g) * D +
              lane * EPL;
-    if (t.path[(int64_t)b * kMaxDraftNodes + node] == 0) {  // no node in this slot
-#pragma unroll
-        for (int e = 0; e < EPL; e++) st_from_f32(dst + e, 0.0f);
-        return;
-    }
-    // ranges that touch tiles [u ntiles, (u + 1) ntiles)
-    const int64_t first = (int64_t)u * t.ntiles, last = first + t.ntiles - 1;
-    const int lo = (int)(((first + 1) * t.groups - 1) / t.F), hi = (int)(((last + 1) * t.groups - 1) / t.F);
-    float M = -INFINITY;
-    for (int w = lo + lane; w <= hi; w += 32)
-        M = fmaxf(M, t.records[((int64_t)(w + u) * t.nb + rb) * REC + NR * D + rr]);
-    M = warp_max(M);
-    float L = 0.0f, Z = 0.0f, x[EPL];
+    const bool present = t.path[(int64_t)b * kMaxDraftNodes + node] != 0;
+    const float *rec0 = t.records + ((int64_t)(lo + u) * t.nb + rb) * REC;
+    const int64_t step = (int64_t)t.nb * REC;
+    float M = -INFINITY, L = 0.0f, Z = 0.0f, x[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; e++) x[e] = 0.0f;
-    for (int w = lo; w <= hi; w++) {
-        const float *rec = t.records + ((int64_t)(w + u) * t.nb + rb) * REC;
-        const float m = rec[NR * D + rr], l = rec[NR * D + NR + rr];
-        if (l == 0.0f) continue;  // saw no token of this range
-        const float wt = exp2f(m - M);
-        L = fmaf(wt, l, L);
-        Z = fmaf(wt, rec[NR * D + 2 * NR + rr], Z);
+    for (int w0 = lo; w0 <= hi; w0 += BATCH, rec0 += BATCH * step) {
+        float m[BATCH], l[BATCH], z[BATCH], y[BATCH][EPL];
 #pragma unroll
-        for (int e = 0; e < EPL; e++) x[e] = fmaf(wt, rec[rr * D + lane * EPL + e], x[e]);
+        for (int k = 0; k < BATCH; k++) {
+            m[k] = -INFINITY;
+            l[k] = z[k] = 0.0f;
+            if (w0 + k <= hi) {
+                const float *rec = rec0 + k * step;
+                m[k] = rec[NR * D + rr];
+                l[k] = rec[NR * D + NR + rr];
+                z[k] = rec[NR * D + 2 * NR + rr];
+                load_elems<float, EPL>(rec + rr * D + lane * EPL, y[k]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < EPL; e++) y[k][e] = 0.0f;
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < BATCH; k++)
+            if (l[k] != 0.0f) top = fmaxf(top, m[k]);  // (a range that showed the row no token has a sum of zero)
+        const float f = M == -INFINITY ? 0.0f : exp2f(M - top);
+        L *= f;
+        Z *= f;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) x[e] *= f;
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+            const float wt = l[k] == 0.0f ? 0.0f : exp2f(m[k] - top);
+            L = fmaf(wt, l[k], L);
+            if (wt != 0.0f) {  // (what a row without tokens left is not read)
+                Z = fmaf(wt, z[k], Z);
+#pragma unroll
+                for (int e = 0; e < EPL; e++) x[e] = fmaf(wt, y[k][e], x[e]);
+            }
+        }
+        M = top;
     }
     const float inv = 1.0f / L;  // a node sees itself
 #pragma unroll
     for (int e = 0; e < EPL; e++) x[e] = (x[e] + Z) * inv;
     warp_wht_butterfly<EPL>(x, lane, D);
-    const float *sg = a.signs + (int64_t)h * D + lane * EPL;
 #pragma unroll
-    for (int e = 0; e < EPL; e++) st_from_f32(dst + e, x[e] * (a.wht_scale * sg[e]));
+    for (int e = 0; e < EPL; e++) x[e] = present ? x[e] * sgw[e] : 0.0f;  // zero where the slot holds no node
+    if (EPL == 4 && sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+        union {
+            T t[4];
+            uint2 v;
+        } o;
+#pragma unroll
+        for (int e = 0; e < EPL && e < 4; e++) o.t[e] = DT<T>::from_f32(x[e]);
+        *reinterpret_cast<uint2 *>(dst) = o.v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < EPL; e++) st_from_f32(dst + e, x[e]);
+    }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------
@@ -983,7 +1063,7 @@ int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStre
     rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, t), "gqa_tree_attend launch");
     count_launch();
     if (rc != SA_OK) return rc;
-    cfg.gridDim = dim3((unsigned)((units * t.rows + kMergeWarps - 1) / kMergeWarps));
+    cfg.gridDim = dim3((unsigned)units, (unsigned)((t.rows + kMergeWarps - 1) / kMergeWarps));
     cfg.blockDim = dim3(32 * kMergeWarps);
     cfg.dynamicSmemBytes = 0;
     rc = check_cuda(cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, BITS, D, NR>, t), "gqa_tree_attend merge launch");

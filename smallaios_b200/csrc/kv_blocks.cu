@@ -224,38 +224,43 @@ __global__ void __launch_bounds__(32 * kMeansWarps) block_means_warp_kernel(Mean
 // The 8-bit queries of the G heads of one KV head, as floats [G][d] in shared memory.  Warp g takes head g.
 template <typename T, int EPL>
 __device__ __forceinline__ void select_queries(const SelectArgs &a, const T *src, const float *sg, float *s_q,
-                                               int *s_max) {
+                                               float (*s_top)[8]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.head_dim;
     const bool active = lane * EPL < d;
-    if (threadIdx.x < 2) s_max[threadIdx.x] = 0;
-    __syncthreads();
-    float x[EPL];
+    float x[EPL], sgn[EPL];
     float top = 0.0f;
     if (warp < a.group) {
 #pragma unroll
+        for (int r = 0; r < EPL; r++) x[r] = 0.0f;
+        if (active) load_elems<T, EPL>(src + (int64_t)warp * d + lane * EPL, x);
+#pragma unroll
         for (int r = 0; r < EPL; r++) {
-            x[r] = active ? grid_value(ld_f32(src + (int64_t)warp * d + lane * EPL + r)) : 0.0f;
+            sgn[r] = active ? sg[lane * EPL + r] : 0.0f;
+            x[r] = grid_value(x[r]);
             top = fmaxf(top, fabsf(x[r]));
         }
         top = warp_max(top);
-        if (lane == 0) atomicMax(&s_max[0], __float_as_int(top));  // non-negative floats order as their bits
+        if (lane == 0) s_top[0][warp] = top;
     }
     __syncthreads();
     if (warp < a.group) {
-        const float f = power_of_two(12 - grid_exponent(__int_as_float(s_max[0])));
+        top = 0.0f;
+        for (int g = 0; g < a.group; g++) top = fmaxf(top, s_top[0][g]);
+        const float f = power_of_two(12 - grid_exponent(top));
 #pragma unroll
-        for (int r = 0; r < EPL; r++) x[r] = active ? rintf(x[r] * f) * sg[lane * EPL + r] : 0.0f;
+        for (int r = 0; r < EPL; r++) x[r] = rintf(x[r] * f) * sgn[r];
         warp_wht_butterfly<EPL>(x, lane, d);
         top = 0.0f;
 #pragma unroll
         for (int r = 0; r < EPL; r++) top = fmaxf(top, active ? fabsf(x[r]) : 0.0f);
         top = warp_max(top);
-        if (lane == 0) atomicMax(&s_max[1], __float_as_int(top));
+        if (lane == 0) s_top[1][warp] = top;
     }
     __syncthreads();
     if (warp < a.group && active) {
-        const int sh = max(0, grid_exponent(__int_as_float(s_max[1])) - 7);
-        const float f = power_of_two(-sh);
+        top = 0.0f;
+        for (int g = 0; g < a.group; g++) top = fmaxf(top, s_top[1][g]);
+        const float f = power_of_two(-max(0, grid_exponent(top) - 7));
 #pragma unroll
         for (int r = 0; r < EPL; r++)
             s_q[warp * d + lane * EPL + r] = fminf(fmaxf(rintf(x[r] * f), -127.0f), 127.0f);
@@ -267,38 +272,42 @@ __device__ __forceinline__ void select_queries(const SelectArgs &a, const T *src
 // products and sums are whole numbers below 2^24 times the block's power of two).  Thread (g, q) reads 8 dimensions
 // (16 bytes) of blocks g and g + 8 at a time; bq holds the columns' values in the same order of dimensions.
 template <int D>
-__device__ __forceinline__ void block_scores(const __nv_bfloat16 *means, int nb, const uint32_t (&bq)[D / 8], int lane,
-                                             float &s0, float &s1) {
-    const int g = lane >> 2, q = lane & 3;
-    const uint4 *r0 = reinterpret_cast<const uint4 *>(means + (int64_t)min(g, nb - 1) * D) + q;
-    const uint4 *r1 = reinterpret_cast<const uint4 *>(means + (int64_t)min(g + 8, nb - 1) * D) + q;
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+struct BlockRows {
     uint4 x[D / 32], y[D / 32];
+    // blocks g and g + 8 of `means` (nb > 0 of them are there)
+    __device__ __forceinline__ void load(const __nv_bfloat16 *means, int nb, int lane) {
+        const int g = lane >> 2, q = lane & 3;
+        const uint4 *r0 = reinterpret_cast<const uint4 *>(means + (int64_t)min(g, nb - 1) * D) + q;
+        const uint4 *r1 = reinterpret_cast<const uint4 *>(means + (int64_t)min(g + 8, nb - 1) * D) + q;
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) {
-        x[j] = r0[4 * j];
-        y[j] = r1[4 * j];
+        for (int j = 0; j < D / 32; j++) {
+            x[j] = r0[4 * j];
+            y[j] = r1[4 * j];
+        }
     }
+    __device__ __forceinline__ void scores(const uint32_t (&bq)[D / 8], float &s0, float &s1) const {
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) {
-        const uint32_t a[2][4] = {{x[j].x, y[j].x, x[j].y, y[j].y}, {x[j].z, y[j].z, x[j].w, y[j].w}};
+        for (int j = 0; j < D / 32; j++) {
+            const uint32_t a[2][4] = {{x[j].x, y[j].x, x[j].y, y[j].y}, {x[j].z, y[j].z, x[j].w, y[j].w}};
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-            asm volatile(
-                "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                "{%0, %1, %2, %3};\n"
-                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                : "r"(a[h][0]), "r"(a[h][1]), "r"(a[h][2]), "r"(a[h][3]), "r"(bq[4 * j + 2 * h]),
-                  "r"(bq[4 * j + 2 * h + 1]));
+            for (int h = 0; h < 2; h++)
+                asm volatile(
+                    "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                    "{%0, %1, %2, %3};\n"
+                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                    : "r"(a[h][0]), "r"(a[h][1]), "r"(a[h][2]), "r"(a[h][3]), "r"(bq[4 * j + 2 * h]),
+                      "r"(bq[4 * j + 2 * h + 1]));
+        }
+        s0 = fmaxf(c[0], c[1]);
+        s1 = fmaxf(c[2], c[3]);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            s0 = fmaxf(s0, __shfl_xor_sync(0xffffffffu, s0, o));
+            s1 = fmaxf(s1, __shfl_xor_sync(0xffffffffu, s1, o));
+        }
     }
-    s0 = fmaxf(c[0], c[1]);
-    s1 = fmaxf(c[2], c[3]);
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        s0 = fmaxf(s0, __shfl_xor_sync(0xffffffffu, s0, o));
-        s1 = fmaxf(s1, __shfl_xor_sync(0xffffffffu, s1, o));
-    }
-}
+};
 
 // grid = (heads, seq_len, batch): one CTA per query token and KV head.  The scores by tensor core (the means are read
 // once, 16 blocks per warp step), then the k-th largest key bit by bit from the top -- one block-wide count per bit,
@@ -309,7 +318,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
     constexpr int EPL = D >= 32 ? D / 32 : 1, NW = kSelectThreads / 32;
     extern __shared__ uint32_t s_key[];  // one key per candidate block, in unsigned order
     __shared__ float s_q[8 * D];
-    __shared__ int s_max[2], s_scan[NW];
+    __shared__ float s_top[2][8];
+    __shared__ int s_scan[NW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int h = blockIdx.x, s = blockIdx.y, b = blockIdx.z;
     const int64_t row = (int64_t)b * a.seq_len + s;
@@ -322,11 +332,13 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
         for (int i = tid; i < k; i += kSelectThreads) out[i] = i < nb ? i : -1;
         return;
     }
-    select_queries<T, EPL>(a, src, a.signs + (int64_t)h * D, s_q, s_max);
-
     // ---- scores as order-preserving integers; the forced blocks above all ----
     const __nv_bfloat16 *means = static_cast<const __nv_bfloat16 *>(a.means) + ((int64_t)b * a.heads + h) * a.row_stride;
     if constexpr (D >= 32) {
+        BlockRows<D> rows;  // loaded a step ahead, the first ones before the queries
+        int i0 = warp * 16;
+        if (i0 < own) rows.load(means + (int64_t)i0 * D, own - i0, lane);
+        select_queries<T, EPL>(a, src, a.signs + (int64_t)h * D, s_q, s_top);
         uint32_t bq[D / 8];  // query column g (heads past the group repeat the first)
         const float *qg = s_q + ((lane >> 2) < a.group ? lane >> 2 : 0) * D + 8 * (lane & 3);
 #pragma unroll
@@ -336,9 +348,11 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
                 const __nv_bfloat162 v = __floats2bfloat162_rn(qg[32 * j + 2 * p], qg[32 * j + 2 * p + 1]);  // exact
                 bq[4 * j + p] = *reinterpret_cast<const uint32_t *>(&v);
             }
-        for (int i0 = warp * 16; i0 < own; i0 += NW * 16) {  // the means of blocks before the query's own
+        for (; i0 < own; i0 += NW * 16) {  // the means of blocks before the query's own
+            const BlockRows<D> now = rows;
+            if (i0 + NW * 16 < own) rows.load(means + (int64_t)(i0 + NW * 16) * D, own - i0 - NW * 16, lane);
             float s0, s1;
-            block_scores<D>(means + (int64_t)i0 * D, own - i0, bq, lane, s0, s1);
+            now.scores(bq, s0, s1);
             const int i = i0 + (lane >> 2) + ((lane & 1) ? 8 : 0);
             if ((lane & 3) < 2 && i < own) {
                 const bool forced = i < a.sink || i > own - a.local;
@@ -346,6 +360,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
             }
         }
     } else {
+        select_queries<T, EPL>(a, src, a.signs + (int64_t)h * D, s_q, s_top);
         for (int i = warp; i < own; i += NW) {
             float best = -INFINITY;
             const float m = lane < D ? __bfloat162float(means[(int64_t)i * D + lane]) : 0.0f;
@@ -360,10 +375,12 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
     // ---- the largest threshold that at least k keys reach ----
     uint32_t least = 0;
     int reach = nb;  // keys at or above it
+    const uint32_t mine = tid < nb ? s_key[tid] : 0u;  // t > 0: a thread without a key never counts
     for (uint32_t bit = 0x80000000u; bit != 0 && reach != k; bit >>= 1) {
         const uint32_t t = least | bit;
-        int n = 0;
-        for (int i = tid; i - tid < nb; i += kSelectThreads) n += __syncthreads_count(i < nb && s_key[i] >= t);
+        int n = __syncthreads_count(mine >= t);
+        for (int i = tid + kSelectThreads; i - tid < nb; i += kSelectThreads)
+            n += __syncthreads_count(i < nb && s_key[i] >= t);
         if (n >= k) {
             least = t;
             reach = n;
