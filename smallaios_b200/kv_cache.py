@@ -132,6 +132,10 @@ class GpuKvCache:
         with torch.cuda.device(self.device):
             check(lib.sa_kv_cache_create(ctypes.byref(cfg), ctypes.byref(self._handle)))
         self.config = cfg
+        # width of a query token: the query heads of the KV heads held here
+        self.query_width = cfg.num_heads // cfg.num_kv_heads * cfg.kv_head_count * cfg.head_dim
+        self.row_shape = (cfg.batch, cfg.kv_head_count, cfg.head_dim)
+        self._tree_bytes: dict = {}
 
     # -- GpuKvCache API ------------------------------------------------------
     @classmethod
@@ -196,6 +200,14 @@ class GpuKvCache:
         rc = lib.sa_kv_cache_keep_drafts(self.handle, path.data_ptr(), path.shape[0], path.shape[1], int(drafted),
                                          _stream_handle(stream, self.device))
         _raise_op(rc, "keep_drafts")
+
+    def tree_workspace_bytes(self, nodes: int, dtype_code: int) -> int:
+        """sa_gqa_tree_workspace_bytes, which a cache's configuration fixes."""
+        key = (nodes, dtype_code)
+        n = self._tree_bytes.get(key)
+        if n is None:
+            n = self._tree_bytes[key] = lib.sa_gqa_tree_workspace_bytes(self.handle, nodes, dtype_code)
+        return n
 
     def view(self, layer: int) -> LayerView:
         """The layer's arrays.  The tensors keep the cache alive; ``close()`` ends them all the same."""

@@ -80,8 +80,18 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 def _stream_handle(stream, device) -> int:
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        return _current_stream_handle(device)
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _current_stream_handle(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object (a microsecond less)
+    def _current_stream_handle(device) -> int:  # noqa: F811
+        index = device.index
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def _cuda(t, what):
@@ -176,13 +186,14 @@ def gqa_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, *, num_heads:
 def _rotated_query(op: str, query, cache: GpuKvCache, out):
     """Checks of (B, S, Hq_local*D) query tokens already rotated to their positions; returns out."""
     _cuda(query, "query")
-    cfg = cache.config
     if query.dim() != 3:
         raise ShapeMismatch(f"{op}: query must be rank-3")
-    if query.shape[2] != cfg.num_heads // cfg.num_kv_heads * cfg.kv_head_count * cfg.head_dim:
+    if query.shape[2] != cache.query_width:
         raise ShapeMismatch(f"{op}: hidden size does not match the cache's heads/head_dim")
     if out is None:
         return torch.empty_like(query)
+    if out is query:
+        return out
     _cuda(out, "out")
     if out.shape != query.shape or out.dtype != query.dtype:
         raise ShapeMismatch(f"{op}: out must have query's shape and dtype")
@@ -219,7 +230,7 @@ def gqa_tree_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, parents:
     b, n, _ = query.shape
     _int32("gqa_tree_attend", parents, (b, n), "parents")
     code = _dtype_code(query)
-    workspace = _workspace(workspace, lib.sa_gqa_tree_workspace_bytes(cache.handle, n, code), query.device)
+    workspace = _workspace(workspace, cache.tree_workspace_bytes(n, code), query.device)
     rc = lib.sa_gqa_tree_attend(cache.handle, layer, query.data_ptr(), parents.data_ptr(), out.data_ptr(), code, b, n,
                                 int(num_heads), int(scale is not None), float(scale or 0.0),
                                 None if workspace is None else workspace.data_ptr(),
@@ -230,15 +241,17 @@ def gqa_tree_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, parents:
 
 def _means_rows(op: str, means, cache: GpuKvCache):
     """(blocks, row stride) of bf16 block means (B, H, blocks, D), which may be a slice of blocks."""
-    cfg = cache.config
     if not isinstance(means, torch.Tensor) or not means.is_cuda:
         raise TypeError("means must be a CUDA tensor")
     if means.dtype != torch.bfloat16:
         raise UnsupportedOp(f"{op}: means must be bfloat16")
-    b, h, d = cfg.batch, cfg.kv_head_count, cfg.head_dim
-    if means.dim() != 4 or means.shape[:2] != (b, h) or means.shape[3] != d:
-        raise ShapeMismatch(f"{op}: means must be ({b}, {h}, blocks, {d}), got {tuple(means.shape)}")
-    blocks = means.shape[2]
+    b, h, d = cache.row_shape
+    shape = means.shape
+    if len(shape) != 4 or shape[0] != b or shape[1] != h or shape[3] != d:
+        raise ShapeMismatch(f"{op}: means must be ({b}, {h}, blocks, {d}), got {tuple(shape)}")
+    blocks = shape[2]
+    if means.is_contiguous():
+        return blocks, blocks * d
     row = means.stride(1) if h > 1 else means.stride(0) if b > 1 else blocks * d
     if means.stride(3) != 1 or (blocks > 1 and means.stride(2) != d) or (h > 1 and b > 1 and
                                                                          means.stride(0) != h * row):
@@ -253,13 +266,14 @@ def kv_block_means(cache: GpuKvCache, layer: int, block_begin: int, block_end: i
     A serving loop keeps one tensor of all blocks per layer and updates the ones that filled up:
     ``kv_block_means(cache, layer, i, j, out=means[:, :, i:j])``.
     """
-    cfg = cache.config
     n = max(int(block_end) - int(block_begin), 0)
     if out is None:
-        out = torch.empty(cfg.batch, cfg.kv_head_count, n, cfg.head_dim, dtype=torch.bfloat16, device=cache.device)
-    blocks, row = _means_rows("kv_block_means", out, cache)
-    if blocks != n:
-        raise ShapeMismatch(f"kv_block_means: out holds {blocks} blocks, not {n}")
+        b, h, d = cache.row_shape
+        out, row = torch.empty((b, h, n, d), dtype=torch.bfloat16, device=cache.device), n * d
+    else:
+        blocks, row = _means_rows("kv_block_means", out, cache)
+        if blocks != n:
+            raise ShapeMismatch(f"kv_block_means: out holds {blocks} blocks, not {n}")
     rc = lib.sa_kv_block_means(cache.handle, layer, out.data_ptr(), row, int(block_begin), int(block_end),
                                _stream_handle(stream, cache.device))
     _raise_op(rc, "kv_block_means")
@@ -278,7 +292,7 @@ def gqa_select_blocks(query: torch.Tensor, cache: GpuKvCache, layer: int, means:
     _rotated_query("gqa_select_blocks", query, cache, query)
     b, s, _ = query.shape
     blocks, row = _means_rows("gqa_select_blocks", means, cache)
-    shape = (b, s, cache.config.kv_head_count, max(int(max_blocks), 0))
+    shape = (b, s, cache.row_shape[1], max(int(max_blocks), 0))
     if out is None:
         out = torch.empty(shape, dtype=torch.int32, device=query.device)
     else:
@@ -303,8 +317,9 @@ def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_
     b, s, _ = query.shape
     if not isinstance(block_ids, torch.Tensor) or block_ids.dim() != 4:
         raise ShapeMismatch("gqa_sparse_attend: block_ids must be rank-4")
-    _int32("gqa_sparse_attend", block_ids, (b, s, cache.config.kv_head_count, block_ids.shape[3]), "block_ids")
-    workspace = _workspace(workspace, lib.sa_gqa_sparse_workspace_bytes(cache.handle, s), query.device)
+    _int32("gqa_sparse_attend", block_ids, (b, s, cache.row_shape[1], block_ids.shape[3]), "block_ids")
+    # (one query token per sequence needs none)
+    workspace = _workspace(workspace, lib.sa_gqa_sparse_workspace_bytes(cache.handle, s) if s > 1 else 0, query.device)
     rc = lib.sa_gqa_sparse_attend(cache.handle, layer, query.data_ptr(), block_ids.data_ptr(), block_ids.shape[3],
                                   out.data_ptr(), _dtype_code(query), b, s, int(num_heads), int(scale is not None),
                                   float(scale or 0.0), None if workspace is None else workspace.data_ptr(),
