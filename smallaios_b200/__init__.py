@@ -12,7 +12,7 @@ from .ops import (CapacityError, InternalError, InvalidAttribute, KvCacheDispatc
                   gqa_select_blocks, gqa_sparse_attend, gqa_tree_attend, group_query_attention, kv_block_means,
                   matmul_nbits, matmul_nbits_packed, qkv_project_append, rms_norm,
                   rotary_device_status, rotary_embedding, silu_mul, supports_op)
-from .layer import LayerWeights, decoder_layer_step, prefill_layer_step
+from .layer import LayerWeights, decoder_layer_step, prefill_layer_step, tree_layer_step
 
 __all__ = [
     "DEFAULT_SEED", "GpuKvCache", "LayerView", "CapacityError", "InternalError", "InvalidAttribute",
@@ -20,5 +20,5 @@ __all__ = [
     "gqa_attend", "group_query_attention", "matmul_nbits", "matmul_nbits_packed", "PackedNBitsWeight",
     "qkv_project_append", "rms_norm", "silu_mul", "supports_op", "LayerWeights", "decoder_layer_step", "prefill_layer_step",
     "qjl_correction", "rotary_embedding", "rotary_device_status", "gqa_tree_attend", "kv_block_means",
-    "gqa_select_blocks", "gqa_sparse_attend",
+    "gqa_select_blocks", "gqa_sparse_attend", "tree_layer_step",
 ]
