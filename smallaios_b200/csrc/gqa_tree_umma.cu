@@ -126,6 +126,13 @@ __device__ __forceinline__ int v_dimension(int l) { return 4 * (l & 7) + (l >> 3
 // Position along K of token t in the V operand: 0 2 1 3 of every four.
 __device__ __forceinline__ int v_slot(int t) { return (t & ~3) | ((t & 1) << 1) | ((t >> 1) & 1); }
 
+// Scores keep the codes' mean unless u has two planes (f32): S^T then carries C sum(q^), a few times the score
+// itself, whose f32 rounding bf16 and f16 callers cannot see -- and the bare code, zero-extended to 16 bits, is
+// the fp16 number c 2^-24, so the K operand takes one operation per pair.  The odd codes of a byte stay in place
+// as 16 c, with q^ / 16.
+template <typename T>
+constexpr bool kCentredScores = std::is_same<T, float>::value;
+
 // Instruction descriptor, kind::f16: D f32, A and B fp16, A K-major, M = 128, N = n; B K-major or
 // (mn != 0) with its rows contiguous.
 __host__ __device__ constexpr uint32_t tg_idesc(int n, uint32_t mn) {
@@ -304,7 +311,9 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
         uint32_t hs[EPL];  // hi, and lo above it
 #pragma unroll
         for (int e = 0; e < EPL; e++) {
-            const float y = x[i][e] * up;
+            // (the odd dimensions of 4-bit codes: see kCentredScores)
+            const bool sixteenth = BITS == 4 && !kCentredScores<T> && ((lane * EPL + e) & 1);
+            const float y = x[i][e] * (sixteenth ? up * 0.0625f : up);
             const __half hi = __float2half_rn(y);
             const float hf = __half2float(hi);
             float kept = hf;
@@ -314,6 +323,7 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
                 hs[e] |= (uint32_t)__half_as_ushort(lo) << 16;
                 kept += __half2float(lo);
             }
+            if (sixteenth) kept *= 16.0f;
             sum += vtr ? kept * vtr[e] : kept;  // sum(q^), or q^.V^T with low-rank K
         }
         if constexpr (D == 128) {
@@ -586,6 +596,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         if constexpr (GG::SPLIT) reg_dec<GG::STAGE>();
         const int Q = lane >> 2, q = lane & 3, tok = 32 * (warp & 3) + lane;
         constexpr int QB = CB / 4, NW = QB / 4;  // bytes and words of a quarter of a token's codes
+        constexpr bool KC = PP == 2;             // kCentredScores
         const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
         for (int i = 0, st = 0, ph = 0; i < n; i++) {
             if (!wait(raw_full + st, ph)) break;
@@ -597,7 +608,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 const float2 vm = *reinterpret_cast<const float2 *>(slot + GG::META + kTok * 8 + tok * 8);
                 const float vs = vm.x < 0x1p-100f ? 0x1p-100f : vm.x, rv = tg_rcp(vs);
                 *reinterpret_cast<float4 *>(slot + GG::CONST + tok * 16) =
-                    make_float4(km.x, fmaf(kCentre, km.x, km.y), tg_lg2(vs), rv);
+                    KC ? make_float4(km.x, fmaf(kCentre, km.x, km.y), tg_lg2(vs), rv)
+                       : make_float4(km.x * 0x1p24f, km.y, tg_lg2(vs), rv);
                 *reinterpret_cast<float *>(slot + GG::CONST + kTok * 16 + tok * 4) = fmaf(kCentre, vs, vm.y) * rv;
             }
             const unsigned char *src = slot + (32 * (warp & 3) + Q) * CB + q * QB;
@@ -634,12 +646,14 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                         for (int y = 0; y < 2; y++) {
                             if constexpr (BITS == 4) {
                                 const uint32_t x = w[y][(m0 + m) >> 1] >> ((m & 1) * 8);
-                                v[4 * m + 2 * y] = centred(x, 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                                v[4 * m + 2 * y + 1] = centred(x, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                                v[4 * m + 2 * y] = KC ? centred(x, 0x000f000fu, one, __float2half2_rn(-1032.0f)) : x & 0x000f000fu;
+                                v[4 * m + 2 * y + 1] =
+                                    KC ? centred(x, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f)) : x & 0x00f000f0u;
                             } else {
                                 const uint32_t x = w[y][m0 + m];
-                                v[4 * m + 2 * y] = centred(x, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
-                                v[4 * m + 2 * y + 1] = centred(x >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                                v[4 * m + 2 * y] = KC ? centred(x, 0x00ff00ffu, one, __float2half2_rn(-1152.0f)) : x & 0x00ff00ffu;
+                                v[4 * m + 2 * y + 1] = KC ? centred(x >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f))
+                                                          : __byte_perm(x, 0, 0x4341);
                             }
                         }
                     tmem_st_frag4(dst + 8 * m0 + (half ? 16u << 16 : 0u), v);
@@ -660,15 +674,18 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         float *my_red = red + warp * 2 * NC, *grp_red = red + group * 8 * NC;
         unsigned char *pl = smem + GG::P_OFF + (slot_row >> 3) * 1024 + (slot_row & 7) * 128;
         const int ch0 = (group * (NC / 8)) << 4, chx = (slot_row & 7) << 4;  // 16-byte chunk c of its row: (ch0 + 16 c) ^ chx
-        const unsigned char *consts = slots + GG::CONST;  // of the tile's ring slot
-        const float *qsum = nullptr;
+        const int prefix_tiles = (int)(a.pos0 / kTok);     // tiles that every row sees whole
         int u = u0, kt = k0, units = 0;
+        int slot = 0;                                      // ring slot of the tile
+        int buf = 0, phase = 0;                            // buffer i & 1 and its phase (i >> 1) & 1
+        int left = min(n, t.ntiles - k0), rest = n - left;  // tiles to the end of the unit, or of the range; after it
+        bool starts = true;                                // the unit's first tile here
+        const float *qsum = nullptr;
         float l[NC], z[NC];
-        for (int i = 0; i < n; i++) {
-            const bool starts = i == 0 || kt == 0;
+        while (left > 0) {
             // S^T(i); with it the token constants are in place (the K warps wrote them before) and O^T(i - 2),
             // which the S^T warp waited for, is complete: u's buffer is free
-            bool ok = wait(qk_done + (i & 1), i >> 1);
+            bool ok = wait(qk_done + buf, phase);
             if (__builtin_expect(starts, 0)) {
                 if (ok) ok = wait(q_full + (units & 1), units >> 1);
                 qsum = reinterpret_cast<const float *>(smem + GG::Q_OFF + (units & 1) * GG::QBUF + QP * GG::QPLANE) + c0;
@@ -679,11 +696,12 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 if (group_or(group, !ok)) break;  // (also: the references are written)
             }
             tc_fence_after();
+            const unsigned char *consts = slots + slot * GG::SLOT + GG::CONST;
             uint32_t v[NC];
-            auto load = [&]() { tmem_ld16(tl + GG::S + (i & 1) * NR + c0, v); };
+            auto load = [&]() { tmem_ld16(tl + GG::S + buf * NR + c0, v); };
             load();
             // drafts in the tile, or tokens past them: bit c of `sees`: row c sees this token
-            const bool masked = (kt + 1) * kTok > a.pos0;
+            const bool masked = kt >= prefix_tiles;
             uint32_t sees = 0xffffffffu;
             if (__builtin_expect(masked, 0)) {
                 const int pos = kt * kTok + tok, dj = pos - (int)a.pos0;
@@ -703,7 +721,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             const float zv = *reinterpret_cast<const float *>(consts + kTok * 16 + tok * 4);
             const float ks = tc.x * qsum[NR - c0], rv = tc.w;
             const float2 ks2 = make_float2(ks, ks), kz2 = make_float2(tc.y, tc.y), lv2 = make_float2(tc.z, tc.z);
-            unsigned char *dst = pl + (i & 1) * GG::PBUF;
+            unsigned char *dst = pl + buf * GG::PBUF;
             // w = u = vs 2^(s - ref), which also goes to shared memory -- or, raising, the scores themselves; returns the
             // largest score.  u is computed before the vote on its range, so that the exponentials overlap the scores'
             // arithmetic (1.15 times as fast at 64 rows); a raise does it over.
@@ -765,7 +783,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     const float top = pass(std::false_type{}, std::false_type{});  // (a masked tile raises)
                     if (__builtin_expect(!group_or(group, !ok || top > kHead + kShift), 1)) break;
                 }
-                if (ok && !starts) ok = wait(pv_done + ((i - 1) & 1), (i - 1) >> 1);  // O is at rest
+                if (ok && !starts) ok = wait(pv_done + (buf ^ 1), phase ^ (buf ^ 1));  // O^T(i - 1): O is at rest
                 if (group_or(group, !ok)) {
                     failed = true;
                     break;
@@ -819,7 +837,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             tc_fence_before();
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            warp_arrive(p_full + (i & 1), lane);  // (and the last reads of the ring slot are behind)
+            warp_arrive(p_full + buf, lane);  // (and the last reads of the ring slot are behind)
             const float2 rv2 = make_float2(rv, rv), zv2 = make_float2(zv, zv);
             // ---- the token's sums; an unseen token takes no part, whatever its metadata holds ----
             if (__builtin_expect(masked, 0)) {
@@ -841,9 +859,10 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     z[c + 1] = z2.y;
                 }
             }
-            consts = consts + GG::SLOT == slots + GG::CONST + NST * GG::SLOT ? slots + GG::CONST : consts + GG::SLOT;
             kt++;
-            if (__builtin_expect(kt == t.ntiles || i == n - 1, 0)) {
+            if (++slot == NST) slot = 0;
+            starts = false;
+            if (__builtin_expect(--left == 0, 0)) {
                 // ---- the unit's partial record ----
                 const float lc = warp_columns(l, lane, [](float x, float y) { return x + y; });
                 const float zc = warp_columns(z, lane, [](float x, float y) { return x + y; });
@@ -851,7 +870,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     my_red[lane] = lc;
                     my_red[NC + lane] = zc;
                 }
-                ok = ok && wait(pv_done + (i & 1), i >> 1);
+                ok = ok && wait(pv_done + buf, phase);
                 if (group_or(group, !ok)) break;
                 tc_fence_after();
                 float *rec = t.records + ((int64_t)(grp + u) * t.nb + rb) * GG::REC;
@@ -879,11 +898,14 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 }
                 tc_fence_before();
                 group_or(group, false);  // my_red and gref are read before the next unit writes them
-                if (kt == t.ntiles) {
-                    kt = 0;
-                    u++;
-                }
+                kt = 0;
+                u++;
+                left = min(rest, t.ntiles);
+                rest -= left;
+                starts = true;
             }
+            phase ^= buf;
+            buf ^= 1;
         }
     }
     tc_fence_before();
