@@ -926,14 +926,16 @@ __device__ __forceinline__ int range_of(int64_t f, int F, int groups) {
     return w;
 }
 
-// One warp per query row: joins the unit's records, rotates back and stores.  Four records' loads at a time.
-template <typename T, int BITS, int D, int NR>
+// A warp joins the records of PER query rows, rotates back and stores: one row where warps are few, four
+// records' loads at a time; four rows where they are many, whose loads go out together when the unit has one
+// record (a tree of 448 rows over 255 tokens, 440 units: 109 us with one row per warp, 57 with four).
+template <typename T, int BITS, int D, int NR, int PER>
 __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeArgs t) {
     constexpr int EPL = D / 32, REC = NR * D + 3 * NR, BATCH = 4;
     const AttendArgs &a = t.a;
     const int lane = threadIdx.x & 31;
     const int u = blockIdx.x, h = u % a.heads, b = u / a.heads;
-    const int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), rb = r / NR, rr = r % NR;
+    const int r0 = (blockIdx.y * kMergeWarps + (threadIdx.x >> 5)) * PER;
     const float *sg = a.signs + (int64_t)h * D + lane * EPL;
     float sgw[EPL];
 #pragma unroll
@@ -943,71 +945,104 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeArgs t
     const int hi = range_of((int64_t)(u + 1) * t.ntiles - 1, t.F, t.groups);
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    if (r >= t.rows) return;
-    const int node = r / a.group, g = r % a.group;
-    T *dst = static_cast<T *>(a.out) + (((int64_t)b * a.seq_len + node) * (a.heads * a.group) + h * a.group + g) * D +
-             lane * EPL;
-    const bool present = t.path[(int64_t)b * kMaxDraftNodes + node] != 0;
-    const float *rec0 = t.records + ((int64_t)(lo + u) * t.nb + rb) * REC;
-    const int64_t step = (int64_t)t.nb * REC;
-    float M = -INFINITY, L = 0.0f, Z = 0.0f, x[EPL];
+    if (r0 >= t.rows) return;
+    const float *unit = t.records + (int64_t)(lo + u) * t.nb * REC;
+    // row r's place in the output, and whether its slot holds a node: asked for before the records
+    auto place = [&](int r, T *&dst, bool &present) {
+        const int node = r / a.group, g = r % a.group;
+        dst = static_cast<T *>(a.out) + (((int64_t)b * a.seq_len + node) * (a.heads * a.group) + h * a.group + g) * D +
+              lane * EPL;
+        present = t.path[(int64_t)b * kMaxDraftNodes + node] != 0;
+    };
+    auto finish = [&](T *dst, bool present, float (&x)[EPL], float L, float Z) {
+        const float inv = 1.0f / L;  // a node sees itself
 #pragma unroll
-    for (int e = 0; e < EPL; e++) x[e] = 0.0f;
-    for (int w0 = lo; w0 <= hi; w0 += BATCH, rec0 += BATCH * step) {
-        float m[BATCH], l[BATCH], z[BATCH], y[BATCH][EPL];
+        for (int e = 0; e < EPL; e++) x[e] = (x[e] + Z) * inv;
+        warp_wht_butterfly<EPL>(x, lane, D);
 #pragma unroll
-        for (int k = 0; k < BATCH; k++) {
-            m[k] = -INFINITY;
-            l[k] = z[k] = 0.0f;
-            if (w0 + k <= hi) {
-                const float *rec = rec0 + k * step;
-                m[k] = rec[NR * D + rr];
-                l[k] = rec[NR * D + NR + rr];
-                z[k] = rec[NR * D + 2 * NR + rr];
-                load_elems<float, EPL>(rec + rr * D + lane * EPL, y[k]);
-            } else {
+        for (int e = 0; e < EPL; e++) x[e] = present ? x[e] * sgw[e] : 0.0f;  // zero where the slot holds no node
+        if (EPL == 4 && sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+            union {
+                T t[4];
+                uint2 v;
+            } o;
 #pragma unroll
-                for (int e = 0; e < EPL; e++) y[k][e] = 0.0f;
-            }
+            for (int e = 0; e < EPL && e < 4; e++) o.t[e] = DT<T>::from_f32(x[e]);
+            *reinterpret_cast<uint2 *>(dst) = o.v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL; e++) st_from_f32(dst + e, x[e]);
         }
-        float top = M;
+    };
+    if (PER > 1 && lo == hi) {
+        float l[PER], z[PER], y[PER][EPL];
+        T *dst[PER];
+        bool present[PER];
 #pragma unroll
-        for (int k = 0; k < BATCH; k++)
-            if (l[k] != 0.0f) top = fmaxf(top, m[k]);  // (a range that showed the row no token has a sum of zero)
-        const float f = M == -INFINITY ? 0.0f : exp2f(M - top);
-        L *= f;
-        Z *= f;
-#pragma unroll
-        for (int e = 0; e < EPL; e++) x[e] *= f;
-#pragma unroll
-        for (int k = 0; k < BATCH; k++) {
-            const float wt = l[k] == 0.0f ? 0.0f : exp2f(m[k] - top);
-            L = fmaf(wt, l[k], L);
-            if (wt != 0.0f) {  // (what a row without tokens left is not read)
-                Z = fmaf(wt, z[k], Z);
-#pragma unroll
-                for (int e = 0; e < EPL; e++) x[e] = fmaf(wt, y[k][e], x[e]);
-            }
+        for (int k = 0; k < PER; k++) {
+            const int r = min(r0 + k, t.rows - 1), rb = r / NR, rr = r % NR;
+            const float *rec = unit + (int64_t)rb * REC;
+            place(r, dst[k], present[k]);
+            l[k] = rec[NR * D + NR + rr];
+            z[k] = rec[NR * D + 2 * NR + rr];
+            load_elems<float, EPL>(rec + rr * D + lane * EPL, y[k]);
         }
-        M = top;
+#pragma unroll
+        for (int k = 0; k < PER; k++)
+            if (r0 + k < t.rows) finish(dst[k], present[k], y[k], l[k], z[k]);
+        return;
     }
-    const float inv = 1.0f / L;  // a node sees itself
+    const int64_t step = (int64_t)t.nb * REC;
+#pragma unroll 1
+    for (int r = r0; r < r0 + PER; r++) {
+        if (PER > 1 && r >= t.rows) return;
+        const int rb = r / NR, rr = r % NR;
+        const float *rec0 = unit + (int64_t)rb * REC;
+        T *dst;
+        bool present;
+        place(r, dst, present);
+        float M = -INFINITY, L = 0.0f, Z = 0.0f, x[EPL];
 #pragma unroll
-    for (int e = 0; e < EPL; e++) x[e] = (x[e] + Z) * inv;
-    warp_wht_butterfly<EPL>(x, lane, D);
+        for (int e = 0; e < EPL; e++) x[e] = 0.0f;
+        for (int w0 = lo; w0 <= hi; w0 += BATCH, rec0 += BATCH * step) {
+            float m[BATCH], l[BATCH], z[BATCH], y[BATCH][EPL];
 #pragma unroll
-    for (int e = 0; e < EPL; e++) x[e] = present ? x[e] * sgw[e] : 0.0f;  // zero where the slot holds no node
-    if (EPL == 4 && sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
-        union {
-            T t[4];
-            uint2 v;
-        } o;
+            for (int k = 0; k < BATCH; k++) {
+                m[k] = -INFINITY;
+                l[k] = z[k] = 0.0f;
+                if (w0 + k <= hi) {
+                    const float *rec = rec0 + k * step;
+                    m[k] = rec[NR * D + rr];
+                    l[k] = rec[NR * D + NR + rr];
+                    z[k] = rec[NR * D + 2 * NR + rr];
+                    load_elems<float, EPL>(rec + rr * D + lane * EPL, y[k]);
+                } else {
 #pragma unroll
-        for (int e = 0; e < EPL && e < 4; e++) o.t[e] = DT<T>::from_f32(x[e]);
-        *reinterpret_cast<uint2 *>(dst) = o.v;
-    } else {
+                    for (int e = 0; e < EPL; e++) y[k][e] = 0.0f;
+                }
+            }
+            float top = M;
 #pragma unroll
-        for (int e = 0; e < EPL; e++) st_from_f32(dst + e, x[e]);
+            for (int k = 0; k < BATCH; k++)
+                if (l[k] != 0.0f) top = fmaxf(top, m[k]);  // (a range that showed the row no token has a sum of zero)
+            const float f = M == -INFINITY ? 0.0f : exp2f(M - top);
+            L *= f;
+            Z *= f;
+#pragma unroll
+            for (int e = 0; e < EPL; e++) x[e] *= f;
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const float wt = l[k] == 0.0f ? 0.0f : exp2f(m[k] - top);
+                L = fmaf(wt, l[k], L);
+                if (wt != 0.0f) {  // (what a row without tokens left is not read)
+                    Z = fmaf(wt, z[k], Z);
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) x[e] = fmaf(wt, y[k][e], x[e]);
+                }
+            }
+            M = top;
+        }
+        finish(dst, present, x, L, Z);
     }
 }
 
@@ -1085,10 +1120,13 @@ int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStre
     rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, t), "gqa_tree_attend launch");
     count_launch();
     if (rc != SA_OK) return rc;
-    cfg.gridDim = dim3((unsigned)units, (unsigned)((t.rows + kMergeWarps - 1) / kMergeWarps));
+    const bool many = units * t.rows > 128 * t.a.sm_count;  // (a GPU of warps, twice over)
+    const int rows = kMergeWarps * (many ? 4 : 1);
+    cfg.gridDim = dim3((unsigned)units, (unsigned)((t.rows + rows - 1) / rows));
     cfg.blockDim = dim3(32 * kMergeWarps);
     cfg.dynamicSmemBytes = 0;
-    rc = check_cuda(cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, BITS, D, NR>, t), "gqa_tree_attend merge launch");
+    rc = check_cuda(cudaLaunchKernelEx(&cfg, many ? tree_merge_kernel<T, BITS, D, NR, 4> : tree_merge_kernel<T, BITS, D, NR, 1>, t),
+                    "gqa_tree_attend merge launch");
     count_launch();
     return rc;
 }
