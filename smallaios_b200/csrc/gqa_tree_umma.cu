@@ -10,8 +10,10 @@
 //   l_r += u_tr / vs_t,   z_r += u_tr (vz_t + C vs_t) / vs_t
 //   o'_r = (O_r + z_r) / l_r,   out = S.H.o' / sqrt(D)
 //
-// C = 8 or 128 centres the codes, so no sum carries the codes' mean, which the
-// zero point would have to cancel.  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
+// C = 7.5 or 127.5, the middle of the codes, so that no sum carries the codes' mean,
+// which the zero point would have to cancel: the tensor cores' f32 sums round toward
+// zero at every step, and with C = 8 the half that is left cost f32 callers a factor
+// of three at 16,000 tokens (3.3e-6 against 1.0e-6 of the output's norm).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
 // power of two common to the row block, in one fp16 plane (11 bits: bf16 callers)
 // or two (22 bits: f16 and f32), u in one (bf16, f16) or two (f32); sum(q^) is of
 // the rounded values, so their rounding only moves the query by its own.
@@ -139,10 +141,14 @@ __host__ __device__ constexpr uint32_t tg_idesc(int n, uint32_t mn) {
     return (1u << 4) | (mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTok >> 4) << 24);
 }
 
-// (x & mask) | magic -> 1024 + code (or 1024 + 16 code), two at once, then centred
-__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t mask, __half2 mul, __half2 add) {
-    const uint32_t biased = (x & mask) | 0x64006400u;
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&biased), mul, add);
+// Two codes to fp16, less their middle C: a code (or 16 times one) zero-extended to 16 bits is the fp16 number
+// c 2^-24 (16 c 2^-24), and (c - C) 2^-9, a half-integer of at most 8 bits, is exact.
+constexpr float kCodeUnit = 0x1p-9f;
+template <int BITS>
+__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t mask, __half2 up) {
+    const uint32_t bare = x & mask;
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&bare), up,
+                              __float2half2_rn(BITS == 4 ? -7.5f * kCodeUnit : -127.5f * kCodeUnit));
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
@@ -372,7 +378,7 @@ template <int BITS, int D, int NR, int QP, int PP>
 __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma_kernel(TreeArgs t) {
     using GG = Tg<BITS, D, NR, QP, PP>;
     constexpr int CB = GG::CB, NST = GG::NST, NC = GG::NC, SM = 4 * GG::NG;
-    constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
+    constexpr float kCentre = BITS == 4 ? 7.5f : 127.5f;
     const AttendArgs &a = t.a;
     extern __shared__ unsigned char tg_raw[];
     unsigned char *smem = tg_raw + ((1024 - (smem_u32(tg_raw) & 1023)) & 1023);
@@ -498,11 +504,11 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 const uint64_t q = q0 + (((units - 1) & 1) * (GG::QBUF >> 4));  // start addresses count 16 bytes
                 const uint32_t d = tbase + GG::S + (i & 1) * NR, k = tbase + GG::KA + (i & 1) * (D / 2);
 #pragma unroll
-                for (int pl = 0; pl < QP; pl++)
+                for (int pl = QP - 1; pl >= 0; pl--)  // the low plane first, while the sums that its steps round are small
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++)
                         umma_ts(d, k + 8 * kk, q + ((pl * GG::QPLANE + (kk >> 2) * (NR * 128) + 32 * (kk & 3)) >> 4), id_s,
-                                (pl | kk) != 0 ? 1u : 0u);
+                                pl != QP - 1 || kk != 0 ? 1u : 0u);
                 umma_commit(qk_done + (i & 1));
                 if (++kt == t.ntiles) kt = 0;
             }
@@ -542,7 +548,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         if constexpr (GG::SPLIT) reg_dec<GG::STAGE>();
         const int Q = lane >> 2, q = lane & 3;
         const bool live = 32 * (warp & 3) < D;
-        const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
+        const __half2 low = __float2half2_rn(0x1p15f), high = __float2half2_rn(0x1p11f);  // of a byte's codes
         for (int i = 0, st = 0, ph = 0; i < n; i++) {
             if (!wait(raw_full + st, ph)) break;
             if (i >= 2 && !wait(pv_done + (i & 1), (i >> 1) - 1)) break;
@@ -561,23 +567,23 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                         const unsigned char *blk = src + (4 * half + m) * (16 * CB);
                         if constexpr (BITS == 4) {
                             const uint2 w = *reinterpret_cast<const uint2 *>(blk);
-                            v0[4 * m] = centred(w.x, 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                            v0[4 * m + 1] = centred(w.x >> 8, 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                            v0[4 * m + 2] = centred(w.x, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
-                            v0[4 * m + 3] = centred(w.x >> 8, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
-                            v1[4 * m] = centred(w.y, 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                            v1[4 * m + 1] = centred(w.y >> 8, 0x000f000fu, one, __float2half2_rn(-1032.0f));
-                            v1[4 * m + 2] = centred(w.y, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
-                            v1[4 * m + 3] = centred(w.y >> 8, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f));
+                            v0[4 * m] = centred<BITS>(w.x, 0x000f000fu, low);
+                            v0[4 * m + 1] = centred<BITS>(w.x >> 8, 0x000f000fu, low);
+                            v0[4 * m + 2] = centred<BITS>(w.x, 0x00f000f0u, high);
+                            v0[4 * m + 3] = centred<BITS>(w.x >> 8, 0x00f000f0u, high);
+                            v1[4 * m] = centred<BITS>(w.y, 0x000f000fu, low);
+                            v1[4 * m + 1] = centred<BITS>(w.y >> 8, 0x000f000fu, low);
+                            v1[4 * m + 2] = centred<BITS>(w.y, 0x00f000f0u, high);
+                            v1[4 * m + 3] = centred<BITS>(w.y >> 8, 0x00f000f0u, high);
                         } else {
                             const uint4 w = *reinterpret_cast<const uint4 *>(blk);
                             const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                             for (int y = 0; y < 4; y++) {
                                 uint32_t *v = y < 2 ? v0 : v1;
-                                v[4 * m + 2 * (y & 1)] = centred(x[y], 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                                v[4 * m + 2 * (y & 1)] = centred<BITS>(x[y], 0x00ff00ffu, low);
                                 v[4 * m + 2 * (y & 1) + 1] =
-                                    centred(x[y] >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f));
+                                    centred<BITS>(x[y] >> 8, 0x00ff00ffu, low);
                             }
                         }
                     }
@@ -597,7 +603,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         const int Q = lane >> 2, q = lane & 3, tok = 32 * (warp & 3) + lane;
         constexpr int QB = CB / 4, NW = QB / 4;  // bytes and words of a quarter of a token's codes
         constexpr bool KC = PP == 2;             // kCentredScores
-        const __half2 one = __float2half2_rn(1.0f), sixteenth = __float2half2_rn(0.0625f);
+        const __half2 low = __float2half2_rn(0x1p15f), high = __float2half2_rn(0x1p11f);  // of a byte's codes
         for (int i = 0, st = 0, ph = 0; i < n; i++) {
             if (!wait(raw_full + st, ph)) break;
             if (i >= 2 && !wait(qk_done + (i & 1), (i >> 1) - 1)) break;
@@ -608,7 +614,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 const float2 vm = *reinterpret_cast<const float2 *>(slot + GG::META + kTok * 8 + tok * 8);
                 const float vs = vm.x < 0x1p-100f ? 0x1p-100f : vm.x, rv = tg_rcp(vs);
                 *reinterpret_cast<float4 *>(slot + GG::CONST + tok * 16) =
-                    KC ? make_float4(km.x, fmaf(kCentre, km.x, km.y), tg_lg2(vs), rv)
+                    KC ? make_float4(km.x * (1.0f / kCodeUnit), fmaf(kCentre, km.x, km.y), tg_lg2(vs), rv)
                        : make_float4(km.x * 0x1p24f, km.y, tg_lg2(vs), rv);
                 *reinterpret_cast<float *>(slot + GG::CONST + kTok * 16 + tok * 4) = fmaf(kCentre, vs, vm.y) * rv;
             }
@@ -646,13 +652,13 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                         for (int y = 0; y < 2; y++) {
                             if constexpr (BITS == 4) {
                                 const uint32_t x = w[y][(m0 + m) >> 1] >> ((m & 1) * 8);
-                                v[4 * m + 2 * y] = KC ? centred(x, 0x000f000fu, one, __float2half2_rn(-1032.0f)) : x & 0x000f000fu;
+                                v[4 * m + 2 * y] = KC ? centred<BITS>(x, 0x000f000fu, low) : x & 0x000f000fu;
                                 v[4 * m + 2 * y + 1] =
-                                    KC ? centred(x, 0x00f000f0u, sixteenth, __float2half2_rn(-72.0f)) : x & 0x00f000f0u;
+                                    KC ? centred<BITS>(x, 0x00f000f0u, high) : x & 0x00f000f0u;
                             } else {
                                 const uint32_t x = w[y][m0 + m];
-                                v[4 * m + 2 * y] = KC ? centred(x, 0x00ff00ffu, one, __float2half2_rn(-1152.0f)) : x & 0x00ff00ffu;
-                                v[4 * m + 2 * y + 1] = KC ? centred(x >> 8, 0x00ff00ffu, one, __float2half2_rn(-1152.0f))
+                                v[4 * m + 2 * y] = KC ? centred<BITS>(x, 0x00ff00ffu, low) : x & 0x00ff00ffu;
+                                v[4 * m + 2 * y + 1] = KC ? centred<BITS>(x >> 8, 0x00ff00ffu, low)
                                                           : __byte_perm(x, 0, 0x4341);
                             }
                         }
@@ -893,7 +899,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     tmem_wait_ld();
                     if (tok < D) {  // tok is the lane of O
 #pragma unroll
-                        for (int k = 0; k < 8; k++) rec[(c0 + c + k) * D + dim] = __uint_as_float(v[k]);
+                        for (int k = 0; k < 8; k++) rec[(c0 + c + k) * D + dim] = __uint_as_float(v[k]) * (1.0f / kCodeUnit);
                     }
                 }
                 tc_fence_before();

@@ -59,6 +59,9 @@ TREES = [  # bits, d, g, dtype, b, h, past, n
     (4, 128, 4, "f16", 1, 2, 63, 2),     # the drafts straddle a block
     (4, 128, 4, "f32", 40, 4, 300, 4),   # more units than SMs
     (4, 128, 2, "f32", 1, 1, 9000, 3),   # few rows, long context
+    (4, 64, 1, "bf16", 600, 8, 70, 2),   # more row blocks than one launch takes
+    (4, 128, 8, "bf16", 11, 8, 199, 56), # many rows over a short context: several per warp of the merge
+    (8, 64, 2, "f16", 30, 8, 300, 40),   # the same with units cut between ranges
     (3, 64, 4, "f32", 2, 2, 100, 9),     # formats of the general kernel
     (4, 32, 4, "f16", 2, 2, 77, 5),
     (8, 16, 2, "f32", 2, 2, 40, 6),
@@ -358,6 +361,7 @@ SPARSE = [  # bits, d, g, dtype, b, h, past, s, k
     (4, 64, 7, "f32", 1, 1, 64 * 9 + 5, 5, 20),     # longer lists than blocks
     (4, 128, 4, "f32", 1, 1, 0, 1, 1),              # one token
     (4, 128, 2, "f32", 20, 4, 64 * 6 + 1, 4, 3),    # more units than SMs
+    (4, 64, 1, "f32", 3, 4, 10, 1400, 2),           # more query rows than one launch takes
     (3, 64, 4, "f32", 1, 2, 64 * 8 + 9, 2, 3),      # formats of the general kernel
     (4, 256, 2, "f16", 1, 2, 64 * 8 + 9, 2, 3),
     (8, 32, 8, "f32", 1, 2, 64 * 8 + 9, 2, 3),
