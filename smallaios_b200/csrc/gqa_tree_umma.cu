@@ -13,7 +13,9 @@
 // C = 7.5 or 127.5, the middle of the codes, so that no sum carries the codes' mean,
 // which the zero point would have to cancel: the tensor cores' f32 sums round toward
 // zero at every step, and with C = 8 the half that is left cost f32 callers a factor
-// of three at 16,000 tokens (3.3e-6 against 1.0e-6 of the output's norm).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
+// of three at 16,000 tokens (3.3e-6 against 1.0e-6 of the output's norm).  For the same
+// reason O^T holds one tile at a time for f32 callers, and the softmax warps add it up
+// (summed in tensor memory over the 110 tiles of a range: 2.6e-5; so: 5.9e-7).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
 // power of two common to the row block, in one fp16 plane (11 bits: bf16 callers)
 // or two (22 bits: f16 and f32), u in one (bf16, f16) or two (f32); sum(q^) is of
 // the rounded values, so their rounding only moves the query by its own.
@@ -22,8 +24,8 @@
 // Transposed, a thread of the softmax holds one token: its scale and zero point
 // are registers, not loads per score, and N follows the number of rows (16, 32 or
 // 64), so a tree of few rows costs few MMA columns.  The codes become fp16 in
-// tensor memory, as the A operands: an integer below 1024 or-ed into the mantissa
-// of 1024 is a float, one packed subtraction centres two.
+// tensor memory, as the A operands: a code zero-extended to 16 bits is an fp16 number, and one
+// packed multiply-add centres two.
 //
 // One persistent CTA per SM; roles by warp:
 //   4 or 8 softmax warps (groups of four, 16 or 32 rows each): thread = token of
@@ -86,10 +88,12 @@ struct Tg {
     static constexpr int NST = ROOM > 8 ? 8 : ROOM;         // ring slots
     static constexpr int MISC_OFF = SLOT_OFF + NST * SLOT;
     static constexpr int SMEM = MISC_OFF + MISC + 1024;     // + slack to align the base to 1024 B
+    // f32: the softmax warps sum the tiles' O^T themselves, from two buffers
+    static constexpr bool FOLD = PP == 2;
     // TMEM columns: K and V operands (two buffers each), S^T (two), O^T
     static constexpr uint32_t KA = 0, VA = D, S = VA + kTok, O = S + 2 * NR;
     static constexpr int REC = NR * D + 3 * NR;             // floats of a partial record: O rows, ref, l, z
-    static_assert(NST >= 2 && SMEM <= 227 * 1024 && O + NR <= 512, "tree kernel resources");
+    static_assert(NST >= 2 && SMEM <= 227 * 1024 && O + (FOLD ? 2 : 1) * NR <= 512, "tree kernel resources");
 };
 
 struct TreeArgs {
@@ -529,11 +533,12 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 const uint64_t p = p0 + ((i & 1) * (GG::PBUF >> 4));
                 const uint32_t v = tbase + GG::VA + (i & 1) * (kTok / 2);
 #pragma unroll
-                for (int pl = 0; pl < PP; pl++)
+                for (int pl = PP - 1; pl >= 0; pl--)
 #pragma unroll
                     for (int kk = 0; kk < kTok / 16; kk++)
-                        umma_ts(tbase + GG::O, v + 8 * kk, p + ((pl * (kTok * 128) + 2048 * kk) >> 4), id_o,
-                                (pl | kk) != 0 || !starts ? 1u : 0u);
+                        umma_ts(tbase + GG::O + (GG::FOLD ? (i & 1) * NR : 0), v + 8 * kk,
+                                p + ((pl * (kTok * 128) + 2048 * kk) >> 4), id_o,
+                                pl != PP - 1 || kk != 0 || !(GG::FOLD || starts) ? 1u : 0u);
                 umma_commit(pv_done + (i & 1));
                 // every role is past tile i: its ring slot, and after the unit's last tile its queries, are free
                 umma_commit(raw_empty + st);
@@ -688,6 +693,17 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         bool starts = true;                                // the unit's first tile here
         const float *qsum = nullptr;
         float l[NC], z[NC];
+        [[maybe_unused]] float o[GG::FOLD ? NC : 8];       // FOLD: the unit's O of dimension `tok`
+        auto fold = [&](int b) {
+#pragma unroll
+            for (int c = 0; c < (GG::FOLD ? NC : 8); c += 8) {
+                uint32_t x[8];
+                tmem_ld8(tl + GG::O + b * NR + c0 + c, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 8; k++) o[c + k] += __uint_as_float(x[k]);
+            }
+        };
         while (left > 0) {
             // S^T(i); with it the token constants are in place (the K warps wrote them before) and O^T(i - 2),
             // which the S^T warp waited for, is complete: u's buffer is free
@@ -698,6 +714,10 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                 units++;
 #pragma unroll
                 for (int c = 0; c < NC; c++) l[c] = z[c] = 0.0f;
+                if constexpr (GG::FOLD) {
+#pragma unroll
+                    for (int c = 0; c < NC; c++) o[c] = 0.0f;
+                }
                 if (wq == 0 && lane < NC) gref[lane] = INFINITY;  // no token seen yet
                 if (group_or(group, !ok)) break;  // (also: the references are written)
             }
@@ -783,7 +803,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
             };
             // A unit's first tile, and one with a score that outgrew its reference, raise the references to the tile's
             // maxima first (so do tiles where rows may see their first token).
-            bool failed = false;
+            bool failed = false, folded = starts;
             for (bool raise = starts || masked;;) {
                 if (__builtin_expect(!raise, 1)) {
                     const float top = pass(std::false_type{}, std::false_type{});  // (a masked tile raises)
@@ -795,6 +815,10 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     break;
                 }
                 tc_fence_after();
+                if constexpr (GG::FOLD) {
+                    if (!starts) fold(buf ^ 1);
+                    folded = true;
+                }
                 load();
                 if (masked) pass(std::true_type{}, std::true_type{});
                 else pass(std::true_type{}, std::false_type{});
@@ -822,7 +846,10 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     l[c] *= gfac[c];
                     z[c] *= gfac[c];
                 }
-                if (!starts) {
+                if constexpr (GG::FOLD) {
+#pragma unroll
+                    for (int c = 0; c < NC; c++) o[c] *= gfac[c];
+                } else if (!starts) {
 #pragma unroll 1
                     for (int c = 0; c < NC; c += 8) {
                         uint32_t o[8];
@@ -865,6 +892,13 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     z[c + 1] = z2.y;
                 }
             }
+            if constexpr (GG::FOLD) {
+                if (!folded) {
+                    ok = wait(pv_done + (buf ^ 1), phase ^ (buf ^ 1));  // O^T(i - 1)
+                    tc_fence_after();
+                    fold(buf ^ 1);  // (the next arrival at p_full orders it before O^T(i + 1))
+                }
+            }
             kt++;
             if (++slot == NST) slot = 0;
             starts = false;
@@ -892,14 +926,23 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
                     rec[NR * D + 2 * NR + c0 + lane] = zs;
                 }
                 const int dim = 32 * wq + v_dimension(lane);
-#pragma unroll 1
-                for (int c = 0; c < NC; c += 8) {
-                    uint32_t v[8];
-                    tmem_ld8(tl + GG::O + c0 + c, v);
-                    tmem_wait_ld();
+                if constexpr (GG::FOLD) {
+                    fold(buf);
                     if (tok < D) {  // tok is the lane of O
 #pragma unroll
-                        for (int k = 0; k < 8; k++) rec[(c0 + c + k) * D + dim] = __uint_as_float(v[k]) * (1.0f / kCodeUnit);
+                        for (int c = 0; c < NC; c++) rec[(c0 + c) * D + dim] = o[c] * (1.0f / kCodeUnit);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < NC; c += 8) {
+                        uint32_t v[8];
+                        tmem_ld8(tl + GG::O + c0 + c, v);
+                        tmem_wait_ld();
+                        if (tok < D) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                rec[(c0 + c + k) * D + dim] = __uint_as_float(v[k]) * (1.0f / kCodeUnit);
+                        }
                     }
                 }
                 tc_fence_before();
@@ -1066,7 +1109,7 @@ int query_planes(int dtype) { return dtype == SA_DTYPE_BFLOAT16 ? 1 : 2; }
 TreePlan tree_plan(int64_t batch, int heads, int group, int head_dim, int sm_count, int64_t total, int nodes, int dtype) {
     TreePlan p;
     const int rows = nodes * group;
-    p.nr = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    p.nr = rows <= 16 ? 16 : rows <= 32 || dtype == SA_DTYPE_FLOAT ? 32 : 64;  // (f32: the sums of O take the registers of the other 32)
     p.nb = (rows + p.nr - 1) / p.nr;
     p.ntiles = (int)((total + kTok - 1) / kTok);
     const int64_t units = batch * heads;
@@ -1142,7 +1185,8 @@ int launch_format(const TreeArgs &t, int nr, unsigned char *qimg, uint64_t *path
     constexpr int QP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PP = std::is_same<T, float>::value ? 2 : 1;
     if (nr == 16) return launch_rows<T, BITS, D, 16, QP, PP>(t, qimg, path, stream);
     if (nr == 32) return launch_rows<T, BITS, D, 32, QP, PP>(t, qimg, path, stream);
-    return launch_rows<T, BITS, D, 64, QP, PP>(t, qimg, path, stream);
+    if constexpr (PP == 1) return launch_rows<T, BITS, D, 64, QP, PP>(t, qimg, path, stream);
+    return set_error(SA_ERR_CUDA, "gqa_tree_attend: no kernel of %d rows", nr);
 }
 
 template <typename T>
