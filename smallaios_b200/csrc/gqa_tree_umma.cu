@@ -28,11 +28,11 @@
 // packed multiply-add centres two.
 //
 // One persistent CTA per SM; roles by warp:
-//   4 or 8 softmax warps (groups of four, 16 or 32 rows each): thread = token of
-//     the tile: tcgen05.ld of S^T, u, the sums l and z of its
-//     token, u to shared memory (the B operand, rows contiguous).  The reference
-//     ref_r is only raised when some score of the tile outgrows it by 2^8 (one
-//     vote per tile and group); then O is rescaled in tensor memory.
+//   4, 8 or 16 softmax warps (groups of four, 16 rows each): thread = token of
+//     the tile: tcgen05.ld of S^T, u, the sums l and z of its token, u to shared
+//     memory (the B operand, rows contiguous).  The reference ref_r is only raised
+//     when some score of the tile outgrows it by 2^8 (one vote per tile and
+//     group); then O is rescaled, in tensor memory or the threads' registers.
 //   4 K warps, 4 V warps: codes of the tile from shared memory to fp16 in tensor
 //     memory, two buffers each; the K warps also turn the tokens' scales and zero
 //     points into what the softmax needs.

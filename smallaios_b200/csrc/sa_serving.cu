@@ -1,7 +1,8 @@
 // C entry points of the serving operators: attention of a draft tree, keeping
 // the accepted drafts, block means, block selection and block-sparse attention
-// (argument checks and workspace layout; the kernels are in gqa_attend.cu,
-// kv_keep.cu and kv_blocks.cu).
+// (argument checks and workspace layout; the kernels are in gqa_tree_umma.cu,
+// gqa_attend.cu, kv_keep.cu, kv_blocks.cu, gqa_decode_mma.cu and
+// gqa_decode_g8.cu).
 #include "sa_common.cuh"
 #include "sa_internal.h"
 
