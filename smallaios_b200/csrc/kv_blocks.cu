@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kMeansThreads) block_means_kernel(MeansArgs a)
 // L / CPT + (32 / CPT) i, so a warp's loads are contiguous.  Two tokens' codes of a dimension, interleaved as
 // bytes, are contracted with their two 16-bit scales by one dp2a: about one instruction per product.  The
 // lanes' sums join by halving exchanges, and the rounding needs one maximum over the warp.
-// Bound by HBM: 8 x 8 heads x 32768 int8 tokens of 128 dimensions (294 MB) in 53 us, 5.5 TB/s.
+// Bound by HBM: 8 x 8 heads x 32768 int8 tokens of 128 dimensions (294 MB) in 49 us, 6.0 TB/s.
 constexpr int kMeansWarps = 8;
 
 __device__ __forceinline__ int dp2a_lo(uint32_t s, uint32_t c, int acc) {
@@ -311,8 +311,8 @@ struct BlockRows {
 
 // grid = (heads, seq_len, batch): one CTA per query token and KV head.  The scores by tensor core (the means are read
 // once, 16 blocks per warp step), then the k-th largest key bit by bit from the top -- one block-wide count per bit,
-// ending as soon as a bit leaves exactly k -- and an ordered compaction.  Bound by latency at small contexts, by the
-// means' bytes at large ones.
+// ending as soon as a bit leaves exactly k -- and an ordered compaction.  Bound by the latency of that chain: 32
+// sequences of 8 heads, 127 candidates, 8.6 MB of means in 10.9 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArgs a) {
     constexpr int EPL = D >= 32 ? D / 32 : 1, NW = kSelectThreads / 32;

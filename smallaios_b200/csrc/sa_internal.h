@@ -168,7 +168,7 @@ struct KeepArgs {
     int n, drafted;
     int64_t pos0;
     int *dev_status;
-    int byte_bits, piece_bits;  // set by the launcher
+    int piece_bits;  // set by the launcher
 };
 
 // Block means of one layer (sa_kv_block_means).
