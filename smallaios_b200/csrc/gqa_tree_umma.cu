@@ -69,7 +69,7 @@ namespace {
 constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
 constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
 constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
-constexpr int kPrepThreads = 256;
+constexpr int kPrepThreads = 512;
 constexpr int kMergeWarps = 8;
 
 template <int BITS, int D, int NR, int QP, int PP>
