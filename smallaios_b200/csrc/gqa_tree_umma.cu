@@ -47,7 +47,7 @@
 //
 // Bound by instruction issue (60% of the cycles; about 5,700 warp instructions per
 // tile of 128 tokens and 64 rows, more than half of them the softmax's; tensor pipe
-// 20%): 16 sequences of 8 KV heads, 8176 int4 tokens, 64 bf16 rows, 155 MB, 90 us with
+// 20%): 16 sequences of 8 KV heads, 8176 int4 tokens, 64 bf16 rows, 155 MB, 88 us with
 // prep and merge; 64 sequences 314 us.  Groups of 16 rows: with 32 a group's
 // registers leave room for half the warps (113 us).
 //
