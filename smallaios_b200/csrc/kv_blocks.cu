@@ -20,7 +20,6 @@ namespace sa {
 namespace {
 
 constexpr int kMeansThreads = 128;
-constexpr int kSelectThreads = 256;
 constexpr float kGridMax = 1.2676506002282294e30f;  // 2^100: larger values (and NaN) count as zero
 
 __device__ __forceinline__ float grid_value(float x) { return fabsf(x) < kGridMax ? x : 0.0f; }
@@ -312,10 +311,15 @@ struct BlockRows {
 // grid = (heads, seq_len, batch): one CTA per query token and KV head.  The scores by tensor core (the means are read
 // once, 16 blocks per warp step), then the k-th largest key bit by bit from the top -- one block-wide count per bit,
 // ending as soon as a bit leaves exactly k -- and an ordered compaction.  Bound by the latency of that chain: 32
-// sequences of 8 heads, 127 candidates, 8.6 MB of means in 10.9 us.
-template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArgs a) {
-    constexpr int EPL = D >= 32 ? D / 32 : 1, NW = kSelectThreads / 32;
+// sequences of 8 heads, 127 candidates, 8.6 MB of means in 10.9 us alone, 7 among others.  Warp g also prepares head
+// g's query.
+//
+// Eight warps, or four for groups of up to four heads where a warp has two steps at most (128 blocks) and CTAs of
+// eight warps (two per SM) would come in waves: 512 CTAs, 127 candidates 7.4 us instead of 10.4, 1024 CTAs 11.4
+// instead of 18.7.  At 255 candidates both take 11.9 us; 256 CTAs at 511 take 18.5 with four warps, 11.3 with eight.
+template <typename T, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) select_blocks_kernel(SelectArgs a) {
+    constexpr int EPL = D >= 32 ? D / 32 : 1, NW = THREADS / 32;
     extern __shared__ uint32_t s_key[];  // one key per candidate block, in unsigned order
     __shared__ float s_q[8 * D];
     __shared__ float s_top[2][8];
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     if (nb <= k) {  // every block
-        for (int i = tid; i < k; i += kSelectThreads) out[i] = i < nb ? i : -1;
+        for (int i = tid; i < k; i += THREADS) out[i] = i < nb ? i : -1;
         return;
     }
     // ---- scores as order-preserving integers; the forced blocks above all ----
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
     for (uint32_t bit = 0x80000000u; bit != 0 && reach != k; bit >>= 1) {
         const uint32_t t = least | bit;
         int n = __syncthreads_count(mine >= t);
-        for (int i = tid + kSelectThreads; i - tid < nb; i += kSelectThreads)
+        for (int i = tid + THREADS; i - tid < nb; i += THREADS)
             n += __syncthreads_count(i < nb && s_key[i] >= t);
         if (n >= k) {
             least = t;
@@ -389,11 +393,11 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
     // ---- ascending ids of the keys above it, and of the lowest blocks that equal it ----
     int above = 0;
     if (reach != k) {
-        for (int i = tid; i - tid < nb; i += kSelectThreads) above += __syncthreads_count(i < nb && s_key[i] > least);
+        for (int i = tid; i - tid < nb; i += THREADS) above += __syncthreads_count(i < nb && s_key[i] > least);
     }
     const int left = reach == k ? 0x7fffffff : k - above;  // how many that equal it
     int taken = 0, equal = 0;  // counts before this round of blocks
-    for (int i0 = 0; i0 < nb; i0 += kSelectThreads) {
+    for (int i0 = 0; i0 < nb; i0 += THREADS) {
         const int i = i0 + tid;
         const uint32_t u = i < nb ? s_key[i] : 0u;
         const bool gt = i < nb && u > least, eq = i < nb && u == least;
@@ -419,8 +423,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_blocks_kernel(SelectArg
 
 template <typename T, int D>
 int launch_select_t(const SelectArgs &a, cudaStream_t stream) {
-    auto kern = select_blocks_kernel<T, D>;
     const int64_t blocks = (a.pos0 + a.seq_len - 1) / kBlockTokens + 1;
+    const bool four = a.group <= 4 && blocks <= 128 && (int64_t)a.heads * a.seq_len * a.batch > 2 * a.sm_count;
+    auto kern = four ? select_blocks_kernel<T, D, 128> : select_blocks_kernel<T, D, 256>;
     const size_t smem = (size_t)blocks * sizeof(int);
     if (smem > 192 * 1024)
         return set_error(SA_ERR_UNSUPPORTED, "gqa_select_blocks: %lld blocks, at most 49152", (long long)blocks);
@@ -436,7 +441,7 @@ int launch_select_t(const SelectArgs &a, cudaStream_t stream) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.heads, a.seq_len, a.batch);
-    cfg.blockDim = dim3(kSelectThreads);
+    cfg.blockDim = dim3(four ? 128 : 256);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = pdl;

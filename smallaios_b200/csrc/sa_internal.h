@@ -186,6 +186,7 @@ struct SelectArgs {
     const void *query;
     int dtype;
     int batch, seq_len, heads, group, head_dim;
+    int sm_count;
     int64_t pos0;
     const float *signs;
     const void *means;  // bf16

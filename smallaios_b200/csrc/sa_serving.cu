@@ -238,6 +238,7 @@ int sa_gqa_select_blocks(sa_kv_cache *cache, int32_t layer, const void *query, i
     a.heads = v.kv_heads;
     a.group = k->group;
     a.head_dim = v.head_dim;
+    a.sm_count = k->sm_count;
     a.pos0 = k->position;
     a.signs = v.signs;
     a.means = means;

@@ -303,6 +303,11 @@ SELECT = [  # d, g, dtype, b, h, past, s, k, sink, local
     (128, 4, "f32", 2, 2, 0, 1, 2, 1, 1),            # the first token
     (64, 4, "f32", 1, 2, 64 * 9, 1, 1, 0, 1),        # its own block only
     (128, 4, "f32", 1, 2, 64 * 1100 + 9, 1, 33, 1, 1),
+    (128, 4, "bf16", 40, 8, 64 * 127 + 63, 1, 32, 1, 1),  # more CTAs than fit at once, up to 128 blocks
+    (128, 8, "bf16", 40, 8, 64 * 127 + 63, 1, 32, 1, 1),
+    (64, 2, "f32", 20, 8, 64 * 60 + 62, 3, 5, 1, 2),
+    (16, 1, "f16", 76, 4, 64 * 30, 1, 4, 1, 1),
+    (32, 3, "f32", 76, 4, 64 * 128, 1, 4, 1, 1),          # 129 blocks
 ]
 
 
