@@ -11,8 +11,8 @@
 //   o'_r = (O_r + z_r) / l_r,   out = S.H.o' / sqrt(D)
 //
 // C = 7.5 or 127.5, the middle of the codes, so that no sum carries the codes' mean,
-// which the zero point would have to cancel: the tensor cores' f32 sums round toward
-// zero at every step, and with C = 8 the half that is left cost f32 callers a factor
+// which the zero point would have to cancel: the tensor cores' f32 sums lose bits at
+// every step, and with C = 8 the half that is left cost f32 callers a factor
 // of three at 16,000 tokens (3.3e-6 against 1.0e-6 of the output's norm).  For the same
 // reason O^T holds one tile at a time for f32 callers, and the softmax warps add it up
 // (summed in tensor memory over the 110 tiles of a range: 2.6e-5; so: 5.9e-7).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
