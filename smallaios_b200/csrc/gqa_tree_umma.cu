@@ -16,10 +16,13 @@
 // of three at 16,000 tokens (3.3e-6 against 1.0e-6 of the output's norm).  For the same
 // reason O^T holds one tile at a time for f32 callers, and the softmax warps add it up
 // (summed in tensor memory over the 110 tiles of a range: 2.6e-5; so: 5.9e-7).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
-// power of two common to the row block, in one fp16 plane (11 bits: bf16 callers)
-// or two (22 bits: f16 and f32), u in one (bf16, f16) or two (f32); sum(q^) is of
-// the rounded values, so their rounding only moves the query by its own.
-// Everything else is f32.
+// power of two common to the row block; q^ and u are held in one fp16 plane each
+// (11 bits) for bf16 callers, whose outputs' own rounding is eight times as coarse
+// (the error against 64 bits grows by 2.2%), and in two (22 bits) for f16 and f32:
+// with one plane of u the error of f16 outputs was 1.37 times that of f32 arithmetic
+// rounded once, at 1,316 instead of 1,377 us in the widest case.  sum(q^) is of the
+// rounded values, so their rounding only moves the query by its own.  Everything
+// else is f32.
 //
 // Transposed, a thread of the softmax holds one token: its scale and zero point
 // are registers, not loads per score, and N follows the number of rows (16, 32 or
@@ -72,7 +75,8 @@ constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
 constexpr int kPrepThreads = 512;
 constexpr int kMergeWarps = 8;
 
-template <int BITS, int D, int NR, int QP, int PP>
+// QP, PP: fp16 planes of q^ and u.  F32: the caller's type is f32 (see the top).
+template <int BITS, int D, int NR, int QP, int PP, bool F32>
 struct Tg {
     static constexpr int CB = D * BITS / 8;
     static constexpr int NC = 16;                           // query rows of a softmax group of four warps
@@ -96,7 +100,7 @@ struct Tg {
     static constexpr int MISC_OFF = SLOT_OFF + NST * SLOT;
     static constexpr int SMEM = MISC_OFF + MISC + 1024;     // + slack to align the base to 1024 B
     // f32: the softmax warps sum the tiles' O^T themselves, from two buffers
-    static constexpr bool FOLD = PP == 2;
+    static constexpr bool FOLD = F32;
     // TMEM columns: K and V operands (two buffers each), S^T (two), O^T
     static constexpr uint32_t KA = 0, VA = D, S = VA + kTok, O = S + 2 * NR;
     static constexpr int REC = NR * D + 3 * NR;             // floats of a partial record: O rows, ref, l, z
@@ -139,7 +143,7 @@ __device__ __forceinline__ int v_dimension(int l) { return 4 * (l & 7) + (l >> 3
 // Position along K of token t in the V operand: 0 2 1 3 of every four.
 __device__ __forceinline__ int v_slot(int t) { return (t & ~3) | ((t & 1) << 1) | ((t >> 1) & 1); }
 
-// Scores keep the codes' mean unless u has two planes (f32): S^T then carries C sum(q^), a few times the score
+// Scores keep the codes' mean unless the caller's type is f32: S^T then carries C sum(q^), a few times the score
 // itself, whose f32 rounding bf16 and f16 callers cannot see -- and the bare code, zero-extended to 16 bits, is
 // the fp16 number c 2^-24, so the K operand takes one operation per pair.  The odd codes of a byte stay in place
 // as 16 c, with q^ / 16.
@@ -267,7 +271,7 @@ __device__ __forceinline__ float warp_columns(float (&v)[N], int lane, Op op) {
 // NR / 8 of them.
 template <typename T, int BITS, int D, int NR, int QP>
 __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, unsigned char *qimg, uint64_t *path) {
-    using G0 = Tg<BITS, D, NR, QP, 1>;
+    using G0 = Tg<BITS, D, NR, QP, 1, false>;
     constexpr int EPL = D / 32, RW = NR / (kPrepThreads / 32);
     const AttendArgs &a = t.a;
     extern __shared__ __align__(16) unsigned char img[];
@@ -385,9 +389,9 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
 }
 
 // ---- attention -------------------------------------------------------------------------------------
-template <int BITS, int D, int NR, int QP, int PP>
-__global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma_kernel(TreeArgs t) {
-    using GG = Tg<BITS, D, NR, QP, PP>;
+template <int BITS, int D, int NR, int QP, int PP, bool F32>
+__global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree_umma_kernel(TreeArgs t) {
+    using GG = Tg<BITS, D, NR, QP, PP, F32>;
     constexpr int CB = GG::CB, NST = GG::NST, NC = GG::NC, SM = 4 * GG::NG;
     constexpr float kCentre = BITS == 4 ? 7.5f : 127.5f;
     const AttendArgs &a = t.a;
@@ -614,7 +618,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP>::THREADS, 1) tree_umma
         if constexpr (GG::SPLIT) reg_dec<GG::STAGE>();
         const int Q = lane >> 2, q = lane & 3, tok = 32 * (warp & 3) + lane;
         constexpr int QB = CB / 4, NW = QB / 4;  // bytes and words of a quarter of a token's codes
-        constexpr bool KC = PP == 2;             // kCentredScores
+        constexpr bool KC = F32;                 // kCentredScores
         const __half2 low = __float2half2_rn(0x1p15f), high = __float2half2_rn(0x1p11f);  // of a byte's codes
         for (int i = 0, st = 0, ph = 0; i < n; i++) {
             if (!wait(raw_full + st, ph)) break;
@@ -1139,7 +1143,8 @@ int64_t tree_batch(int64_t batch, int heads, int group, int nodes) {
 
 template <typename T, int BITS, int D, int NR, int QP, int PP>
 int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
-    using GG = Tg<BITS, D, NR, QP, PP>;
+    constexpr bool F32 = std::is_same<T, float>::value;
+    using GG = Tg<BITS, D, NR, QP, PP, F32>;
     const int64_t units = (int64_t)t.a.batch * t.a.heads;
     // each launch is a programmatic dependent of the one before it
     cudaLaunchAttribute pdl[1];
@@ -1156,7 +1161,7 @@ int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStre
                         "gqa_tree_attend prep launch");
     count_launch();
     if (rc != SA_OK) return rc;
-    auto kern = tree_umma_kernel<BITS, D, NR, QP, PP>;
+    auto kern = tree_umma_kernel<BITS, D, NR, QP, PP, F32>;
     static int configured[64];  // of this kernel, by device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1189,10 +1194,10 @@ int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStre
 
 template <typename T, int BITS, int D>
 int launch_format(const TreeArgs &t, int nr, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
-    constexpr int QP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PP = std::is_same<T, float>::value ? 2 : 1;
+    constexpr int QP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PP = QP;
     if (nr == 16) return launch_rows<T, BITS, D, 16, QP, PP>(t, qimg, path, stream);
     if (nr == 32) return launch_rows<T, BITS, D, 32, QP, PP>(t, qimg, path, stream);
-    if constexpr (PP == 1) return launch_rows<T, BITS, D, 64, QP, PP>(t, qimg, path, stream);
+    if constexpr (!std::is_same<T, float>::value) return launch_rows<T, BITS, D, 64, QP, PP>(t, qimg, path, stream);
     return set_error(SA_ERR_CUDA, "gqa_tree_attend: no kernel of %d rows", nr);
 }
 
