@@ -464,7 +464,14 @@ int sa_rotary_embedding(const void *x, void *y, int32_t dtype, int32_t layout, i
  *   query, attn_out  (batch, nodes, q_heads_local * head_dim) in dtype
  *
  * Node i attends to the prefix [0, p), to its ancestors and to itself.  Rows
- * of slots without a node are zero. */
+ * of slots without a node are zero.
+ *
+ * Precision: queries and weights are held to 22 bits, for bf16 callers to 11,
+ * which adds about 2% to the rounding of the output's own type.
+ * sa_kv_cache_set_tree_precision(cache, 1) gives bf16 callers 22 bits too (the
+ * precision of the decode and prefill paths, about a quarter more time); it
+ * changes what sa_gqa_tree_workspace_bytes says.  0 is the default. */
+int sa_kv_cache_set_tree_precision(sa_kv_cache *cache, int32_t full);
 int64_t sa_gqa_tree_workspace_bytes(const sa_kv_cache *cache, int32_t nodes, int32_t dtype);
 int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, const int32_t *parents,
                        void *attn_out, int32_t dtype, int32_t batch, int32_t nodes, int64_t num_heads,

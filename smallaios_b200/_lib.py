@@ -37,7 +37,7 @@ EXPORTED = [
     "sa_kv_append", "sa_gqa_attend", "sa_group_query_attention", "sa_matmul_nbits", "sa_gqa_attend_no_alloc",
     "sa_matmul_nbits_packed_bytes", "sa_matmul_nbits_prepack", "sa_matmul_nbits_packed",
     "sa_qkv_project_append", "sa_rms_norm", "sa_silu_mul", "sa_rotary_embedding",
-    "sa_gqa_tree_workspace_bytes", "sa_gqa_tree_attend", "sa_kv_cache_keep_drafts", "sa_kv_block_means",
+    "sa_gqa_tree_workspace_bytes", "sa_gqa_tree_attend", "sa_kv_cache_set_tree_precision", "sa_kv_cache_keep_drafts", "sa_kv_block_means",
     "sa_gqa_select_blocks", "sa_gqa_sparse_workspace_bytes", "sa_gqa_sparse_attend",
 ]
 SA_MAX_DRAFT_NODES = 64
@@ -152,6 +152,8 @@ def _declare(l: ctypes.CDLL) -> None:
                                       _I64, _I64, _I32, _I32, _P, _P]
     l.sa_gqa_tree_workspace_bytes.restype = _I64
     l.sa_gqa_tree_workspace_bytes.argtypes = [_P, _I32, _I32]
+    l.sa_kv_cache_set_tree_precision.restype = ctypes.c_int
+    l.sa_kv_cache_set_tree_precision.argtypes = [_P, _I32]
     l.sa_gqa_tree_attend.restype = ctypes.c_int
     l.sa_gqa_tree_attend.argtypes = [_P, _I32, _P, _P, _P, _I32, _I32, _I32, _I64, _I32, _F, _P, _I64, _P]
     l.sa_kv_cache_keep_drafts.restype = ctypes.c_int

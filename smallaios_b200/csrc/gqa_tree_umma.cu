@@ -18,7 +18,8 @@
 // (summed in tensor memory over the 110 tiles of a range: 2.6e-5; so: 5.9e-7).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
 // power of two common to the row block; q^ and u are held in one fp16 plane each
 // (11 bits) for bf16 callers, whose outputs' own rounding is eight times as coarse
-// (the error against 64 bits grows by 2.2%), and in two (22 bits) for f16 and f32:
+// (the error against 64 bits grows by 2.2%; with two planes, the cache's choice, by
+// nothing, at 384 instead of 308 us), and in two (22 bits) for f16 and f32:
 // with one plane of u the error of f16 outputs was 1.37 times that of f32 arithmetic
 // rounded once, at 1,316 instead of 1,377 us in the widest case.  sum(q^) is of the
 // rounded values, so their rounding only moves the query by its own.  Everything
@@ -1115,9 +1116,11 @@ struct TreePlan {
     size_t records, qimg, path;  // workspace parts, in this order
 };
 
-int query_planes(int dtype) { return dtype == SA_DTYPE_BFLOAT16 ? 1 : 2; }
+// Planes of q^ and u.
+int tree_planes(int dtype, int full) { return dtype == SA_DTYPE_BFLOAT16 && !full ? 1 : 2; }
 
-TreePlan tree_plan(int64_t batch, int heads, int group, int head_dim, int sm_count, int64_t total, int nodes, int dtype) {
+TreePlan tree_plan(int64_t batch, int heads, int group, int head_dim, int sm_count, int64_t total, int nodes, int dtype,
+                   int full) {
     TreePlan p;
     const int rows = nodes * group;
     p.nr = rows <= 16 ? 16 : rows <= 32 || dtype == SA_DTYPE_FLOAT ? 32 : 64;  // (f32: the sums of O take the registers of the other 32)
@@ -1128,7 +1131,7 @@ TreePlan tree_plan(int64_t batch, int heads, int group, int head_dim, int sm_cou
     const int most = sm_count / p.nb > 0 ? sm_count / p.nb : 1;
     p.groups = p.F < most ? p.F : most;
     p.records = up256((size_t)(p.groups + units) * p.nb * (p.nr * head_dim + 3 * p.nr) * sizeof(float));
-    const size_t image = ((size_t)query_planes(dtype) * p.nr * head_dim * 2 + p.nr * 4 + 16 + 1023) / 1024 * 1024;
+    const size_t image = ((size_t)tree_planes(dtype, full) * p.nr * head_dim * 2 + p.nr * 4 + 16 + 1023) / 1024 * 1024;
     p.qimg = (size_t)units * p.nb * image;
     p.path = up256((size_t)batch * kMaxDraftNodes * sizeof(uint64_t));
     return p;
@@ -1192,31 +1195,30 @@ int launch_rows(const TreeArgs &t, unsigned char *qimg, uint64_t *path, cudaStre
     return rc;
 }
 
-template <typename T, int BITS, int D>
+template <typename T, int PL, int BITS, int D>
 int launch_format(const TreeArgs &t, int nr, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
-    constexpr int QP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PP = QP;
-    if (nr == 16) return launch_rows<T, BITS, D, 16, QP, PP>(t, qimg, path, stream);
-    if (nr == 32) return launch_rows<T, BITS, D, 32, QP, PP>(t, qimg, path, stream);
-    if constexpr (!std::is_same<T, float>::value) return launch_rows<T, BITS, D, 64, QP, PP>(t, qimg, path, stream);
+    if (nr == 16) return launch_rows<T, BITS, D, 16, PL, PL>(t, qimg, path, stream);
+    if (nr == 32) return launch_rows<T, BITS, D, 32, PL, PL>(t, qimg, path, stream);
+    if constexpr (!std::is_same<T, float>::value) return launch_rows<T, BITS, D, 64, PL, PL>(t, qimg, path, stream);
     return set_error(SA_ERR_CUDA, "gqa_tree_attend: no kernel of %d rows", nr);
 }
 
-template <typename T>
+template <typename T, int PL>
 int launch_type(const TreeArgs &t, int nr, unsigned char *qimg, uint64_t *path, cudaStream_t stream) {
-    if (t.a.bits == 4 && t.a.head_dim == 128) return launch_format<T, 4, 128>(t, nr, qimg, path, stream);
-    if (t.a.bits == 8 && t.a.head_dim == 128) return launch_format<T, 8, 128>(t, nr, qimg, path, stream);
-    if (t.a.bits == 4 && t.a.head_dim == 64) return launch_format<T, 4, 64>(t, nr, qimg, path, stream);
-    return launch_format<T, 8, 64>(t, nr, qimg, path, stream);
+    if (t.a.bits == 4 && t.a.head_dim == 128) return launch_format<T, PL, 4, 128>(t, nr, qimg, path, stream);
+    if (t.a.bits == 8 && t.a.head_dim == 128) return launch_format<T, PL, 8, 128>(t, nr, qimg, path, stream);
+    if (t.a.bits == 4 && t.a.head_dim == 64) return launch_format<T, PL, 4, 64>(t, nr, qimg, path, stream);
+    return launch_format<T, PL, 8, 64>(t, nr, qimg, path, stream);
 }
 
 }  // namespace
 
 // Workspace of the tensor-core tree attention at any context up to `tokens` (0: another kernel's job).
 size_t tree_workspace_bytes(int batch, int heads, int group, int head_dim, int bits, int sm_count, int64_t tokens,
-                            int nodes, int dtype) {
+                            int nodes, int dtype, int full) {
     if ((bits != 4 && bits != 8) || (head_dim != 64 && head_dim != 128)) return 0;
     const int64_t per = tree_batch(batch, heads, group, nodes);
-    const TreePlan p = tree_plan(per, heads, group, head_dim, sm_count, tokens, nodes, dtype);
+    const TreePlan p = tree_plan(per, heads, group, head_dim, sm_count, tokens, nodes, dtype, full);
     return p.records + p.qimg + p.path;
 }
 
@@ -1237,7 +1239,7 @@ int launch_gqa_tree_umma(const AttendArgs &a, void *workspace, cudaStream_t stre
         t.a.v_meta = a.v_meta + unit0 * a.capacity * 2;
         if (a.lr_vtr) t.a.lr_vtr = a.lr_vtr + unit0 * a.head_dim;
         const TreePlan p = tree_plan(t.a.batch, a.heads, a.group, a.head_dim, a.sm_count, a.pos0 + a.seq_len, a.seq_len,
-                                     a.dtype);
+                                     a.dtype, a.tree_full);
         char *ws = static_cast<char *>(workspace);
         t.records = reinterpret_cast<float *>(ws);
         t.qimg = reinterpret_cast<unsigned char *>(ws + p.records);
@@ -1251,9 +1253,12 @@ int launch_gqa_tree_umma(const AttendArgs &a, void *workspace, cudaStream_t stre
         uint64_t *path = reinterpret_cast<uint64_t *>(ws + p.records + p.qimg);
         int rc;
         switch (a.dtype) {
-            case SA_DTYPE_FLOAT: rc = launch_type<float>(t, p.nr, qimg, path, stream); break;
-            case SA_DTYPE_FLOAT16: rc = launch_type<__half>(t, p.nr, qimg, path, stream); break;
-            default: rc = launch_type<__nv_bfloat16>(t, p.nr, qimg, path, stream); break;
+            case SA_DTYPE_FLOAT: rc = launch_type<float, 2>(t, p.nr, qimg, path, stream); break;
+            case SA_DTYPE_FLOAT16: rc = launch_type<__half, 2>(t, p.nr, qimg, path, stream); break;
+            default:
+                rc = a.tree_full ? launch_type<__nv_bfloat16, 2>(t, p.nr, qimg, path, stream)
+                                 : launch_type<__nv_bfloat16, 1>(t, p.nr, qimg, path, stream);
+                break;
         }
         if (rc != SA_OK) return rc;
     }

@@ -79,6 +79,7 @@ struct kv_cache_impl {
     uint32_t *qprep;   // [B*H] x decode_qprep_words(group): q-digit words, then score constants
     int *dev_status;   // one int: device-side status bits
     GatherOut gather;  // head-sharded output buffers (n = 0: off)
+    int tree_full;     // tree attention of bf16 callers: two planes of q^ and u, as for f16
     size_t layer_codes_bytes;  // B*H*T*CB
     size_t layer_meta_floats;  // B*H*T*2
     uint8_t *k_qjl_bits;       // [L][B][H][T][D/8], nullptr unless cfg.qjl_residual
@@ -149,6 +150,7 @@ struct AttendArgs {
     const float *lr_vtr;
     // draft tree (nullptr: off): [batch][seq_len] parents, the query tokens are the tree's nodes
     const int32_t *parents;
+    int tree_full;  // kv_cache_impl::tree_full
     // block lists (nullptr: off): [batch][seq_len][heads][max_blocks] ascending block ids, -1 = none
     const int32_t *block_ids;
     int max_blocks;
@@ -196,7 +198,7 @@ struct SelectArgs {
 };
 
 size_t tree_workspace_bytes(int batch, int heads, int group, int head_dim, int bits, int sm_count, int64_t tokens,
-                            int nodes, int dtype);
+                            int nodes, int dtype, int full);
 int launch_gqa_tree_umma(const AttendArgs &a, void *workspace, cudaStream_t stream);
 int launch_keep_drafts(const KeepArgs &a, cudaStream_t stream);
 int launch_block_means(const MeansArgs &a, cudaStream_t stream);

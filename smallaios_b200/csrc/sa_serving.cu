@@ -107,7 +107,13 @@ int64_t sa_gqa_tree_workspace_bytes(const sa_kv_cache *cache, int32_t nodes, int
     const kv_cache_impl *k = reinterpret_cast<const kv_cache_impl *>(cache);
     if (!cache || nodes <= 0 || nodes > SA_MAX_DRAFT_NODES || !dtype_ok(dtype) || k->group > 8) return 0;
     return (int64_t)tree_workspace_bytes(k->cfg.batch, k->cfg.kv_head_count, k->group, k->cfg.head_dim, k->cfg.bits,
-                                         k->sm_count, k->capacity, nodes, dtype);
+                                         k->sm_count, k->capacity, nodes, dtype, k->tree_full);
+}
+
+int sa_kv_cache_set_tree_precision(sa_kv_cache *cache, int32_t full) {
+    if (!cache) return set_error(SA_ERR_INVALID_ARGUMENT, "kv_cache_set_tree_precision: NULL cache");
+    reinterpret_cast<kv_cache_impl *>(cache)->tree_full = full != 0;
+    return SA_OK;
 }
 
 int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, const int32_t *parents, void *attn_out,
@@ -127,6 +133,7 @@ int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, con
     if (rc != SA_OK) return rc;
     AttendArgs a = attend_args(k, layer, query, attn_out, dtype, batch, nodes, has_scale, scale);
     a.parents = parents;
+    a.tree_full = k->tree_full;
     if (need > 0) return launch_gqa_tree_umma(a, workspace, static_cast<cudaStream_t>(stream));
     return launch_gqa_attend_generic(a, static_cast<cudaStream_t>(stream));
 }

@@ -201,8 +201,14 @@ class GpuKvCache:
                                          _stream_handle(stream, self.device))
         _raise_op(rc, "keep_drafts")
 
+    def set_tree_precision(self, full: bool) -> None:
+        """Bits of queries and weights in ``gqa_tree_attend`` for bf16 callers (sa_kv_cache_set_tree_precision):
+        22 with ``full``, as f16 and f32 callers and the decode path have; else 11, the default."""
+        check(lib.sa_kv_cache_set_tree_precision(self.handle, int(bool(full))))
+        self._tree_bytes.clear()
+
     def tree_workspace_bytes(self, nodes: int, dtype_code: int) -> int:
-        """sa_gqa_tree_workspace_bytes, which a cache's configuration fixes."""
+        """sa_gqa_tree_workspace_bytes, which a cache's configuration and tree precision fix."""
         key = (nodes, dtype_code)
         n = self._tree_bytes.get(key)
         if n is None:

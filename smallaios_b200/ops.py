@@ -223,7 +223,8 @@ def gqa_tree_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, parents:
     ``query`` (B, N, Hq*D), N <= 64 drafts rotated to position + depth, whose keys and values have been
     appended at the cache position (not advanced).  ``parents`` int32 (B, N) on the device: -1 a node that
     follows the prefix, j < i a node that follows node j, anything else no node (zero output, as for the
-    nodes below it).  Each node sees the prefix, its ancestors and itself.  ``workspace``: uint8, at least
+    nodes below it).  Each node sees the prefix, its ancestors and itself.  ``cache.set_tree_precision`` sets the
+    bits that bf16 callers get.  ``workspace``: uint8, at least
     ``sa_gqa_tree_workspace_bytes``; allocated when not given.
     """
     out = _rotated_query("gqa_tree_attend", query, cache, out)
