@@ -16,7 +16,8 @@
 // of three at 16,000 tokens (3.3e-6 against 1.0e-6 of the output's norm).  For the same
 // reason O^T holds one tile at a time for f32 callers, and the softmax warps add it up
 // (summed in tensor memory over the 110 tiles of a range: 2.6e-5; so: 5.9e-7).  q^ is q' = H.S.q scale log2(e) / D^(1/2) on a
-// power of two common to the row block; q^ and u are held in one fp16 plane each
+// power of two common to the row block, or, in a block whose rows lie more than 2^14
+// apart, on one of its own row (kSpread); q^ and u are held in one fp16 plane each
 // (11 bits) for bf16 callers, whose outputs' own rounding is eight times as coarse
 // (the error against 64 bits grows by 2.2%; with two planes, the cache's choice, by
 // nothing, at 384 instead of 308 us), and in two (22 bits) for f16 and f32:
@@ -73,6 +74,11 @@ namespace {
 constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
 constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
 constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
+// Rows whose largest |q'| is within 2^kSpread of the block's keep all 22 bits of two planes on the block's power of
+// two: the block's largest is put into [2^11, 2^12), and fp16 numbers are multiples of 2^-24.  A block that spreads
+// further has a power of two per row, so that no query, however large, costs other rows bits; each of its tiles takes
+// the path that raises references.  A scale per row in every tile takes 324 instead of 308 us.
+constexpr int kSpread = 14;
 constexpr int kPrepThreads = 512;
 constexpr int kMergeWarps = 8;
 
@@ -90,7 +96,8 @@ struct Tg {
     static_assert(!SPLIT || 128 * NG * SOFT + 256 * STAGE + 96 * LAUNCH <= THREADS * LAUNCH, "register split");
     static constexpr int PBUF = PP * kTok * 128;            // u planes of a tile: [128 tokens][64 rows], 128-byte swizzle
     static constexpr int QPLANE = NR * D * 2;               // D/64 tiles of [NR rows][128 B]
-    static constexpr int QREC = QP * QPLANE + NR * 4 + 16;  // planes, sum(q^) of the rows, power of two
+    // planes, sum(q^) of the rows, their powers of two, the common one (0: the rows have their own)
+    static constexpr int QREC = QP * QPLANE + NR * 8 + 16;
     static constexpr int QBUF = (QREC + 1023) / 1024 * 1024;
     // ring slot: K codes, V codes, K metadata, V metadata; then what the softmax makes of a token's metadata
     static constexpr int META = 2 * kTok * CB, CONST = META + kTok * 16, SLOT = CONST + kTok * 20;
@@ -269,39 +276,51 @@ __device__ __forceinline__ float warp_columns(float (&v)[N], int lane, Op op) {
 
 // ---- query images --------------------------------------------------------------------------------
 // grid = units * row blocks.  Rows are query rows r = node * G + head of the KV head; a warp rotates
-// NR / 8 of them.
+// NR / 16 of them.
 template <typename T, int BITS, int D, int NR, int QP>
 __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, unsigned char *qimg, uint64_t *path) {
     using G0 = Tg<BITS, D, NR, QP, 1, false>;
     constexpr int EPL = D / 32, RW = NR / (kPrepThreads / 32);
     const AttendArgs &a = t.a;
     extern __shared__ __align__(16) unsigned char img[];
-    __shared__ int s_max, s_par[kMaxDraftNodes];
+    __shared__ int s_max, s_min, s_par[kMaxDraftNodes];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int u = blockIdx.x / t.nb, rb = blockIdx.x % t.nb, h = u % a.heads, b = u / a.heads;
-    if (tid == 0) s_max = 0;
+    if (tid == 0) {
+        s_max = 0;
+        s_min = 0x7f800000;
+    }
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int nodes = a.seq_len;
-    if (h == 0 && rb == 0 && tid < nodes) s_par[tid] = a.parents[(int64_t)b * nodes + tid];
+    const int32_t *parents = a.parents + (int64_t)b * nodes;
+    if (h == 0 && rb == 0 && tid < nodes) s_par[tid] = parents[tid];
     __syncthreads();
     if (h == 0 && rb == 0 && tid < nodes) path[(int64_t)b * kMaxDraftNodes + tid] = tree_path(s_par, tid);
 
     const float *sg = a.signs + (int64_t)h * D + lane * EPL;
     const float mul = a.wht_scale * a.scale * 1.4426950408889634f;
-    float x[RW][EPL], top = 0.0f;
+    float x[RW][EPL];
+    int row_top[RW];  // largest finite |q'| (non-negative floats order as their bits)
+    bool present[RW];
     // row r of the KV head is query head g = r % G of node r / G: step over them without a division per row
     const T *src = static_cast<const T *>(a.query) + ((int64_t)b * nodes * a.heads + h) * a.group * D + lane * EPL;
-    int g = (rb * NR + warp * RW) % a.group;
-    src += ((int64_t)((rb * NR + warp * RW) / a.group) * a.heads * a.group + g) * D;
+    int g = (rb * NR + warp * RW) % a.group, node = (rb * NR + warp * RW) / a.group;
+    src += ((int64_t)node * a.heads * a.group + g) * D;
 #pragma unroll
     for (int i = 0; i < RW; i++) {
 #pragma unroll
         for (int e = 0; e < EPL; e++) x[i][e] = 0.0f;
-        if (rb * NR + warp * RW + i < t.rows) load_elems<T, EPL>(src, x[i]);
+        present[i] = false;
+        if (node < nodes) {
+            load_elems<T, EPL>(src, x[i]);
+            const int up = parents[node];
+            present[i] = up >= -1 && up < node;
+        }
         src += D;
         if (++g == a.group) {
             g = 0;
+            node++;
             src += (int64_t)(a.heads - 1) * a.group * D;
         }
     }
@@ -310,25 +329,37 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
 #pragma unroll
         for (int e = 0; e < EPL; e++) x[i][e] *= sg[e];
         warp_wht_butterfly<EPL>(x[i], lane, D);
+        float top = 0.0f;
 #pragma unroll
         for (int e = 0; e < EPL; e++) {
-            x[i][e] *= mul;
+            x[i][e] = present[i] ? x[i][e] * mul : 0.0f;  // (what a slot without a node holds takes no part)
             const float m = fabsf(x[i][e]);
             if (m < INFINITY) top = fmaxf(top, m);
         }
+        row_top[i] = __reduce_max_sync(0xffffffffu, __float_as_int(top));
     }
-    top = warp_max(top);
-    if (lane == 0) atomicMax(&s_max, __float_as_int(top));  // non-negative floats order as their bits
+    int most = 0, least = 0x7f800000;
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+        most = max(most, row_top[i]);
+        least = min(least, row_top[i] > 0 ? row_top[i] : 0x7f800000);
+    }
+    if (lane == 0) {
+        atomicMax(&s_max, most);
+        atomicMin(&s_min, least);
+    }
     __syncthreads();
-    // the largest |q'| into [2^11, 2^12): a common power of two costs the scores no operation, and what
-    // a small row loses to it is small against the largest row's scores
-    const int ex = max(((s_max >> 23) & 0xff) - 126, -100);
-    const float up = __int_as_float((12 - ex + 127) << 23), down = __int_as_float((ex - 12 + 127) << 23);
+    // the block's largest |q'| into [2^11, 2^12)
+    auto exponent = [](int bits) { return max(((bits >> 23) & 0xff) - 126, -100); };
+    const int common = exponent(s_max);
+    const bool apart = common - exponent(s_min) > kSpread;  // (rows of zeros aside)
     const float *vtr = a.lr_vtr ? a.lr_vtr + (int64_t)u * D + lane * EPL : nullptr;
     float *qsum = reinterpret_cast<float *>(img + QP * G0::QPLANE);
 #pragma unroll
     for (int i = 0; i < RW; i++) {
         const int row = warp * RW + i;
+        const int ex = apart ? exponent(row_top[i]) : common;
+        const float up = __int_as_float((12 - ex + 127) << 23), down = __int_as_float((ex - 12 + 127) << 23);
         float sum = 0.0f;
         uint32_t hs[EPL];  // hi, and lo above it
 #pragma unroll
@@ -381,9 +412,12 @@ __global__ void __launch_bounds__(kPrepThreads) tree_prep_kernel(TreeArgs t, uns
             }
         }
         sum = warp_sum(sum);
-        if (lane == 0) qsum[row] = sum * down;
+        if (lane == 0) {
+            qsum[row] = sum * down;
+            qsum[NR + row] = down;
+        }
     }
-    if (tid < 4) qsum[NR + tid] = down;
+    if (tid < 4) qsum[2 * NR + tid] = apart ? 0.0f : __int_as_float((common - 12 + 127) << 23);
     __syncthreads();
     uint4 *out = reinterpret_cast<uint4 *>(qimg + (int64_t)blockIdx.x * G0::QBUF);
     for (int i = tid; i < G0::QREC / 16; i += kPrepThreads) out[i] = reinterpret_cast<const uint4 *>(img)[i];
@@ -697,7 +731,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
         float *my_red = red + warp * 2 * NC, *grp_red = red + group * 8 * NC;
         unsigned char *pl = smem + GG::P_OFF + (slot_row >> 3) * 1024 + (slot_row & 7) * 128;
         const int ch0 = (group * (NC / 8)) << 4, chx = (slot_row & 7) << 4;  // 16-byte chunk c of its row: (ch0 + 16 c) ^ chx
-        const int prefix_tiles = (int)(a.pos0 / kTok);     // tiles that every row sees whole
+        int plain_tiles = 0;                               // tiles of the unit that need no raise of themselves
         int u = u0, kt = k0, units = 0;
         int slot = 0;                                      // ring slot of the tile
         int buf = 0, phase = 0;                            // buffer i & 1 and its phase (i >> 1) & 1
@@ -724,6 +758,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
                 if (ok) ok = wait(q_full + (units & 1), units >> 1);
                 qsum = reinterpret_cast<const float *>(smem + GG::Q_OFF + (units & 1) * GG::QBUF + QP * GG::QPLANE) + c0;
                 units++;
+                if (ok) plain_tiles = qsum[2 * NR - c0] == 0.0f ? 0 : (int)a.pos0 / kTok;
 #pragma unroll
                 for (int c = 0; c < NC; c++) l[c] = z[c] = 0.0f;
                 if constexpr (GG::FOLD) {
@@ -737,9 +772,16 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
             const unsigned char *consts = slots + slot * GG::SLOT + GG::CONST;
             uint32_t v[NC];
             auto load = [&]() { tmem_ld16(tl + GG::S + buf * NR + c0, v); };
+            // S^T in the rows' own powers of two
+            auto load_by_row = [&]() {
+                load();
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < NC; c++) v[c] = __float_as_uint(__uint_as_float(v[c]) * qsum[NR + c]);
+            };
             load();
             // drafts in the tile, or tokens past them: bit c of `sees`: row c sees this token
-            const bool masked = kt >= prefix_tiles;
+            const bool masked = (kt + 1) * kTok > (int)a.pos0;  // (the tiles before are seen whole)
             uint32_t sees = 0xffffffffu;
             if (__builtin_expect(masked, 0)) {
                 const int pos = kt * kTok + tok, dj = pos - (int)a.pos0;
@@ -757,8 +799,9 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
             }
             const float4 tc = *reinterpret_cast<const float4 *>(consts + tok * 16);
             const float zv = *reinterpret_cast<const float *>(consts + kTok * 16 + tok * 4);
-            const float ks = tc.x * qsum[NR - c0], rv = tc.w;
-            const float2 ks2 = make_float2(ks, ks), kz2 = make_float2(tc.y, tc.y), lv2 = make_float2(tc.z, tc.z);
+            const float rv = tc.w;
+            float ks = tc.x * qsum[2 * NR - c0];
+            const float2 kz2 = make_float2(tc.y, tc.y), lv2 = make_float2(tc.z, tc.z);
             unsigned char *dst = pl + buf * GG::PBUF;
             // w = u = vs 2^(s - ref), which also goes to shared memory -- or, raising, the scores themselves; returns the
             // largest score.  u is computed before the vote on its range, so that the exponentials overlap the scores'
@@ -766,6 +809,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
             float w[NC];
             auto pass = [&](auto raising, auto masking) {
                 constexpr bool RAISE = decltype(raising)::value, MASK = decltype(masking)::value;
+                const float2 ks2 = make_float2(ks, ks);
                 float top0 = -INFINITY, top1 = -INFINITY;
                 tmem_wait_ld();
 #pragma unroll
@@ -814,9 +858,9 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
                 return fmaxf(top0, top1);
             };
             // A unit's first tile, and one with a score that outgrew its reference, raise the references to the tile's
-            // maxima first (so do tiles where rows may see their first token).
+            // maxima first (so do tiles where rows may see their first token, and all of a row block spread wide).
             bool failed = false, folded = starts;
-            for (bool raise = starts || masked;;) {
+            for (bool raise = starts || kt >= plain_tiles;;) {
                 if (__builtin_expect(!raise, 1)) {
                     const float top = pass(std::false_type{}, std::false_type{});  // (a masked tile raises)
                     if (__builtin_expect(!group_or(group, !ok || top > kHead + kShift), 1)) break;
@@ -831,7 +875,8 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
                     if (!starts) fold(buf ^ 1);
                     folded = true;
                 }
-                load();
+                load_by_row();
+                ks = *reinterpret_cast<const float *>(consts + tok * 16);
                 if (masked) pass(std::true_type{}, std::true_type{});
                 else pass(std::true_type{}, std::false_type{});
                 // (8 columns at a time: few registers beside the hot path's)
@@ -873,7 +918,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
                     }
                     tmem_wait_st();
                 }
-                load();
+                load_by_row();
                 if (masked) pass(std::false_type{}, std::true_type{});
                 else pass(std::false_type{}, std::false_type{});
                 break;
@@ -1131,7 +1176,7 @@ TreePlan tree_plan(int64_t batch, int heads, int group, int head_dim, int sm_cou
     const int most = sm_count / p.nb > 0 ? sm_count / p.nb : 1;
     p.groups = p.F < most ? p.F : most;
     p.records = up256((size_t)(p.groups + units) * p.nb * (p.nr * head_dim + 3 * p.nr) * sizeof(float));
-    const size_t image = ((size_t)tree_planes(dtype, full) * p.nr * head_dim * 2 + p.nr * 4 + 16 + 1023) / 1024 * 1024;
+    const size_t image = ((size_t)tree_planes(dtype, full) * p.nr * head_dim * 2 + p.nr * 8 + 16 + 1023) / 1024 * 1024;
     p.qimg = (size_t)units * p.nb * image;
     p.path = up256((size_t)batch * kMaxDraftNodes * sizeof(uint64_t));
     return p;
