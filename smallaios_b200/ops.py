@@ -16,6 +16,7 @@ Errors map the library's status codes onto the reference's OpError variants.
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass, field
 
 import torch
@@ -92,6 +93,23 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a 
     def _current_stream_handle(device) -> int:  # noqa: F811
         index = device.index
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+_AS_IS = contextlib.nullcontext()
+
+
+def _owned_by(stream, device):
+    """Context whose allocations belong to the stream that a call launches on.
+
+    A block of another stream's pool could be in that stream's use before the launch, or be handed out there
+    again while the kernels still run.
+    """
+    if stream is None:
+        return _AS_IS
+    if not hasattr(stream, "cuda_stream"):
+        handle = int(stream)
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
 
 
 def _cuda(t, what):
@@ -183,7 +201,7 @@ def gqa_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, *, num_heads:
 
 
 # ---- serving operators: draft trees and block-sparse attention ------------------
-def _rotated_query(op: str, query, cache: GpuKvCache, out):
+def _rotated_query(op: str, query, cache: GpuKvCache, out, stream):
     """Checks of (B, S, Hq_local*D) query tokens already rotated to their positions; returns out."""
     _cuda(query, "query")
     if query.dim() != 3:
@@ -191,7 +209,8 @@ def _rotated_query(op: str, query, cache: GpuKvCache, out):
     if query.shape[2] != cache.query_width:
         raise ShapeMismatch(f"{op}: hidden size does not match the cache's heads/head_dim")
     if out is None:
-        return torch.empty_like(query)
+        with _owned_by(stream, query.device):
+            return torch.empty_like(query)
     if out is query:
         return out
     _cuda(out, "out")
@@ -208,10 +227,11 @@ def _int32(op: str, t, shape: tuple, what: str):
         raise ShapeMismatch(f"{op}: {what} must be {shape}, got {tuple(t.shape)}")
 
 
-def _workspace(workspace, nbytes: int, device):
-    """``workspace``, or a buffer of the stream-ordered allocator where the call needs one."""
+def _workspace(workspace, nbytes: int, device, stream):
+    """``workspace``, or a buffer of the launch stream's pool where the call needs one."""
     if workspace is None and nbytes:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        with _owned_by(stream, device):
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return _cuda(workspace, "workspace")
 
 
@@ -227,11 +247,11 @@ def gqa_tree_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, parents:
     bits that bf16 callers get.  ``workspace``: uint8, at least
     ``sa_gqa_tree_workspace_bytes``; allocated when not given.
     """
-    out = _rotated_query("gqa_tree_attend", query, cache, out)
+    out = _rotated_query("gqa_tree_attend", query, cache, out, stream)
     b, n, _ = query.shape
     _int32("gqa_tree_attend", parents, (b, n), "parents")
     code = _dtype_code(query)
-    workspace = _workspace(workspace, cache.tree_workspace_bytes(n, code), query.device)
+    workspace = _workspace(workspace, cache.tree_workspace_bytes(n, code), query.device, stream)
     rc = lib.sa_gqa_tree_attend(cache.handle, layer, query.data_ptr(), parents.data_ptr(), out.data_ptr(), code, b, n,
                                 int(num_heads), int(scale is not None), float(scale or 0.0),
                                 None if workspace is None else workspace.data_ptr(),
@@ -270,7 +290,8 @@ def kv_block_means(cache: GpuKvCache, layer: int, block_begin: int, block_end: i
     n = max(int(block_end) - int(block_begin), 0)
     if out is None:
         b, h, d = cache.row_shape
-        out, row = torch.empty((b, h, n, d), dtype=torch.bfloat16, device=cache.device), n * d
+        with _owned_by(stream, cache.device):
+            out, row = torch.empty((b, h, n, d), dtype=torch.bfloat16, device=cache.device), n * d
     else:
         blocks, row = _means_rows("kv_block_means", out, cache)
         if blocks != n:
@@ -290,12 +311,13 @@ def gqa_select_blocks(query: torch.Tensor, cache: GpuKvCache, layer: int, means:
     up to the query's own block at least.  The first ``sink_blocks`` and the last ``local_blocks`` blocks, and
     of the others those with the largest exact scores, ties to the lower block (sa_gqa_select_blocks).
     """
-    _rotated_query("gqa_select_blocks", query, cache, query)
+    _rotated_query("gqa_select_blocks", query, cache, query, stream)
     b, s, _ = query.shape
     blocks, row = _means_rows("gqa_select_blocks", means, cache)
     shape = (b, s, cache.row_shape[1], max(int(max_blocks), 0))
     if out is None:
-        out = torch.empty(shape, dtype=torch.int32, device=query.device)
+        with _owned_by(stream, query.device):
+            out = torch.empty(shape, dtype=torch.int32, device=query.device)
     else:
         _int32("gqa_select_blocks", out, shape, "out")
     rc = lib.sa_gqa_select_blocks(cache.handle, layer, query.data_ptr(), _dtype_code(query), b, s, int(num_heads),
@@ -314,13 +336,14 @@ def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_
     ``block_ids`` int32 (B, S, H, max_blocks), distinct ids, -1 = none (gqa_select_blocks).  Tokens after the
     query's own position are masked; a query without blocks gives zeros.
     """
-    out = _rotated_query("gqa_sparse_attend", query, cache, out)
+    out = _rotated_query("gqa_sparse_attend", query, cache, out, stream)
     b, s, _ = query.shape
     if not isinstance(block_ids, torch.Tensor) or block_ids.dim() != 4:
         raise ShapeMismatch("gqa_sparse_attend: block_ids must be rank-4")
     _int32("gqa_sparse_attend", block_ids, (b, s, cache.row_shape[1], block_ids.shape[3]), "block_ids")
     # (one query token per sequence needs none)
-    workspace = _workspace(workspace, lib.sa_gqa_sparse_workspace_bytes(cache.handle, s) if s > 1 else 0, query.device)
+    workspace = _workspace(workspace, lib.sa_gqa_sparse_workspace_bytes(cache.handle, s) if s > 1 else 0, query.device,
+                           stream)
     rc = lib.sa_gqa_sparse_attend(cache.handle, layer, query.data_ptr(), block_ids.data_ptr(), block_ids.shape[3],
                                   out.data_ptr(), _dtype_code(query), b, s, int(num_heads), int(scale is not None),
                                   float(scale or 0.0), None if workspace is None else workspace.data_ptr(),
