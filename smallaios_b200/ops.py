@@ -551,9 +551,10 @@ def rotary_embedding(x: torch.Tensor, cos_cache: torch.Tensor, sin_cache: torch.
     if position_ids is not None:
         if position_ids.dtype not in _POS_DTYPES:
             raise ShapeMismatch("RotaryEmbedding: position_ids must be int32 or int64")
-        if not position_ids.is_cuda:
-            position_ids = position_ids.to(x.device, non_blocking=True)
-        position_ids = position_ids.contiguous()
+        with _owned_by(stream, x.device):
+            if not position_ids.is_cuda:
+                position_ids = position_ids.to(x.device, non_blocking=True)
+            position_ids = position_ids.contiguous()
         pos_ptr, pos_dtype, pos_count = position_ids.data_ptr(), _POS_DTYPES[position_ids.dtype], position_ids.numel()
     if out is None:
         out = torch.empty_like(x)

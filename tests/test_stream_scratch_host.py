@@ -75,3 +75,30 @@ def test_outputs_and_scratch_belong_to_the_launch_stream(recorded, stream):
 def test_without_a_stream_they_belong_to_the_current_one(recorded):
     _calls(None)
     assert {s for _, s in recorded} == {None}
+
+
+@pytest.mark.parametrize("host", [True, False])
+def test_position_ids_are_made_ready_on_the_launch_stream(recorded, monkeypatch, host):
+    """Ids on the host, or strided, are copied by the stream that reads the copy."""
+    from smallaios_b200 import ops
+
+    made = []
+
+    class Ids(_Fake):
+        is_cuda = not host
+
+        def to(self, *a, **kw):
+            torch.empty(1)
+            made.append(recorded[-1][1])
+            return _fake(self)
+
+        def contiguous(self):
+            torch.empty(1)
+            made.append(recorded[-1][1])
+            return _fake(self)
+
+    monkeypatch.setattr(ops, "_rotary_status_word", lambda device: _fake(torch.zeros(1, dtype=torch.int32)))
+    x, table = _fake(torch.zeros(1, 2, 64)), _fake(torch.zeros(4, 8))
+    ids = torch.zeros(2, dtype=torch.int32).as_subclass(Ids)
+    ops.rotary_embedding(x, table, table, position_ids=ids, num_heads=4, out=x, stream=SimpleNamespace(cuda_stream=77))
+    assert made and set(made) == {77}
