@@ -131,8 +131,10 @@ struct BlockList {
     }
 };
 
-// Below this the largest value scale of some tokens counts as this (the log2 of the reference).
-constexpr float kVScaleMin = 1.17549435e-38f;
+// Below this the largest value scale of some tokens counts as this (the log2 of the reference): the weights
+// 2^24 2^(s - R) that the sums add up then stay below 2^24 / kVScaleMin = 2^88, their sums with zero points far from
+// f32's 2^128.  Values of such scales lose at most 2^-24 of this each, whatever they are: 255 steps of 3e-27.
+constexpr float kVScaleMin = 0x1p-64f;
 
 // Tokens that the query does not see (score -inf) take no part in the sums, whatever their metadata
 // holds; `some`: the chunk has such tokens.
