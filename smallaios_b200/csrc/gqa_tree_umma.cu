@@ -73,6 +73,9 @@ namespace {
 
 constexpr int kTok = 128;       // tokens per tile: M of S^T, K of O^T
 constexpr float kHead = 8.0f;   // octaves a score may outgrow its reference before that moves
+// Smaller value scales (constant vectors have 0) count as this, at 255 times it in the outputs at most.  The sums of
+// u / vs then reach 2^(7 + 80) times the tokens and, in z, the zero points: far from f32's 2^128 at any context.
+constexpr float kScaleMin = 0x1p-80f;
 constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
 // Rows whose largest |q'| is within 2^kSpread of the block's keep all 22 bits of two planes on the block's power of
 // two: the block's largest is put into [2^11, 2^12), and fp16 numbers are multiples of 2^-24.  A block that spreads
@@ -663,7 +666,7 @@ __global__ void __launch_bounds__(Tg<BITS, D, NR, QP, PP, F32>::THREADS, 1) tree
             {
                 const float2 km = *reinterpret_cast<const float2 *>(slot + GG::META + tok * 8);
                 const float2 vm = *reinterpret_cast<const float2 *>(slot + GG::META + kTok * 8 + tok * 8);
-                const float vs = vm.x < 0x1p-100f ? 0x1p-100f : vm.x, rv = tg_rcp(vs);
+                const float vs = vm.x < kScaleMin ? kScaleMin : vm.x, rv = tg_rcp(vs);
                 *reinterpret_cast<float4 *>(slot + GG::CONST + tok * 16) =
                     KC ? make_float4(km.x * (1.0f / kCodeUnit), fmaf(kCentre, km.x, km.y), tg_lg2(vs), rv)
                        : make_float4(km.x * 0x1p24f, km.y, tg_lg2(vs), rv);
