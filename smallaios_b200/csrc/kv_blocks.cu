@@ -426,14 +426,16 @@ int launch_select_t(const SelectArgs &a, cudaStream_t stream) {
     const int64_t blocks = (a.pos0 + a.seq_len - 1) / kBlockTokens + 1;
     const bool four = a.group <= 4 && blocks <= 128 && (int64_t)a.heads * a.seq_len * a.batch > 2 * a.sm_count;
     auto kern = four ? select_blocks_kernel<T, D, 128> : select_blocks_kernel<T, D, 256>;
+    constexpr size_t kMost = 192 * 1024, kPlain = 32 * 1024;  // keys; without the attribute (static memory beside them)
     const size_t smem = (size_t)blocks * sizeof(int);
-    if (smem > 192 * 1024)
+    if (smem > kMost)
         return set_error(SA_ERR_UNSUPPORTED, "gqa_select_blocks: %lld blocks, at most 49152", (long long)blocks);
     if (a.seq_len > 65535 || a.batch > 65535)
         return set_error(SA_ERR_UNSUPPORTED, "gqa_select_blocks: %d x %d query rows, at most 65535 each", a.batch,
                          a.seq_len);
-    if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > kPlain) {
+        // always the most, so that a call of another thread between this and the launch changes nothing
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
         if (e != cudaSuccess) return check_cuda(e, "gqa_select_blocks smem attribute");
     }
     cudaLaunchAttribute pdl[1];

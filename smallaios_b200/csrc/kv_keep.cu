@@ -131,15 +131,12 @@ int launch_keep_drafts(const KeepArgs &a, cudaStream_t stream) {
     if (units > 0x7fffffff)
         return set_error(SA_ERR_UNSUPPORTED, "kv_cache_keep_drafts: %lld units", (long long)units);
     const int qb = a.k_qjl_bits ? a.head_dim / 8 : 0;
-    const size_t smem = keep_smem(a.pos0, a.drafted, a.n, a.code_bytes, qb);  // at most 58 KB
+    // at most 42.5 KB (64 drafts over five V blocks, head_dim 256, 8 bits, QJL): no attribute needed
+    const size_t smem = keep_smem(a.pos0, a.drafted, a.n, a.code_bytes, qb);
     KeepArgs k = a;
     const bool wide = a.code_bytes % 16 == 0;
     while (((wide ? 16 : 4) << k.piece_bits) < a.code_bytes) k.piece_bits++;
     auto kern = wide ? keep_drafts_kernel<uint4> : keep_drafts_kernel<uint32_t>;
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return check_cuda(e, "kv_cache_keep_drafts smem attribute");
-    }
     kern<<<(unsigned)units, kKeepThreads, smem, stream>>>(k);
     count_launch();
     return check_cuda(cudaGetLastError(), "kv_cache_keep_drafts launch");
