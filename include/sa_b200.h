@@ -446,9 +446,14 @@ int sa_rotary_embedding(const void *x, void *y, int32_t dtype, int32_t layout, i
  * positions (sa_qkv_project_append and sa_rotary_embedding do it).  A cache
  * with a gather set (sa_kv_cache_set_gather) is SA_ERR_UNSUPPORTED here.
  *
- * Workspaces are the caller's: `workspace` (device, 256-byte aligned) holds
- * at least what the matching *_workspace_bytes says; NULL is fine where that
- * is 0.  Concurrent calls on one cache need one each.
+ * `workspace` (device, 256-byte aligned) holds at least what the matching
+ * *_workspace_bytes says, and is the call's alone until its kernels have run.
+ * Where that is 0 (NULL is fine then: one query token per sequence of the
+ * sparse attention, and the formats of the general kernel, 3 bits or head_dim
+ * 16, 32 and 256) the call uses the workspace inside the cache, as
+ * sa_gqa_attend and sa_group_query_attention do, so its kernels and theirs on
+ * one cache must be ordered on the device: one stream, or streams joined by
+ * events.  Calls on one handle are serialised by the caller in any case.
  * ====================================================================== */
 #define SA_MAX_DRAFT_NODES 64
 #define SA_BLOCK_TOKENS 64

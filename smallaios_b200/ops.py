@@ -245,7 +245,8 @@ def gqa_tree_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, parents:
     follows the prefix, j < i a node that follows node j, anything else no node (zero output, as for the
     nodes below it).  Each node sees the prefix, its ancestors and itself.  ``cache.set_tree_precision`` sets the
     bits that bf16 callers get.  ``workspace``: uint8, at least
-    ``sa_gqa_tree_workspace_bytes``; allocated when not given.
+    ``sa_gqa_tree_workspace_bytes``; allocated when not given.  Where that is 0 the call uses the cache's own
+    workspace, and must not overlap on the device with other attention calls on the cache.
     """
     out = _rotated_query("gqa_tree_attend", query, cache, out, stream)
     b, n, _ = query.shape
@@ -334,7 +335,8 @@ def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_
 
     ``query`` (B, S, Hq*D) rotated to positions p + s, own keys and values appended (position not advanced);
     ``block_ids`` int32 (B, S, H, max_blocks), distinct ids, -1 = none (gqa_select_blocks).  Tokens after the
-    query's own position are masked; a query without blocks gives zeros.
+    query's own position are masked; a query without blocks gives zeros.  With S = 1 the call uses the cache's own
+    workspace, and must not overlap on the device with other attention calls on the cache.
     """
     out = _rotated_query("gqa_sparse_attend", query, cache, out, stream)
     b, s, _ = query.shape
