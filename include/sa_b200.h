@@ -526,7 +526,8 @@ int sa_gqa_select_blocks(sa_kv_cache *cache, int32_t layer, const void *query, i
 
 /* Attention of query token s, at position p + s, over the cached tokens at or
  * before its position of its listed blocks (block_ids as above; distinct ids;
- * entries outside the cache's blocks count as -1; an empty list gives zeros).
+ * entries outside the cache's blocks count as -1; an empty list gives zeros;
+ * max_blocks below 2^25).
  * The query tokens' own keys and values have been appended; the position has
  * not moved. */
 int64_t sa_gqa_sparse_workspace_bytes(const sa_kv_cache *cache, int32_t seq_len);

@@ -276,6 +276,10 @@ int sa_gqa_sparse_attend(sa_kv_cache *cache, int32_t layer, const void *query, c
     if (rc != SA_OK) return rc;
     if (max_blocks < 1)
         return set_error(SA_ERR_INVALID_ATTRIBUTE, "gqa_sparse_attend: max_blocks must be > 0 (got %d)", max_blocks);
+    // tokens along a list are counted in 32 bits; no cache has more blocks
+    if (max_blocks > INT32_MAX / SA_BLOCK_TOKENS)
+        return set_error(SA_ERR_UNSUPPORTED, "gqa_sparse_attend: lists of %d blocks, at most %d", max_blocks,
+                         INT32_MAX / SA_BLOCK_TOKENS);
     if (seq_len == 0) return SA_OK;
     if (!query || !block_ids || !attn_out)
         return set_error(SA_ERR_INVALID_ARGUMENT, "gqa_sparse_attend: NULL query/block_ids/attn_out");
