@@ -95,9 +95,6 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a 
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-_AS_IS = contextlib.nullcontext()
-
-
 def _owned_by(stream, device):
     """Context whose allocations belong to the stream that a call launches on.
 
@@ -105,11 +102,18 @@ def _owned_by(stream, device):
     again while the kernels still run.
     """
     if stream is None:
-        return _AS_IS
+        return contextlib.nullcontext()
     if not hasattr(stream, "cuda_stream"):
         handle = int(stream)
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
     return torch.cuda.stream(stream)
+
+
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    if stream is None:  # (a context costs half a microsecond)
+        return torch.empty(shape, dtype=dtype, device=device)
+    with _owned_by(stream, device):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _cuda(t, what):
@@ -209,8 +213,7 @@ def _rotated_query(op: str, query, cache: GpuKvCache, out, stream):
     if query.shape[2] != cache.query_width:
         raise ShapeMismatch(f"{op}: hidden size does not match the cache's heads/head_dim")
     if out is None:
-        with _owned_by(stream, query.device):
-            return torch.empty_like(query)
+        return torch.empty_like(query) if stream is None else _empty(query.shape, query.dtype, query.device, stream)
     if out is query:
         return out
     _cuda(out, "out")
@@ -230,8 +233,7 @@ def _int32(op: str, t, shape: tuple, what: str):
 def _workspace(workspace, nbytes: int, device, stream):
     """``workspace``, or a buffer of the launch stream's pool where the call needs one."""
     if workspace is None and nbytes:
-        with _owned_by(stream, device):
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        workspace = _empty(nbytes, torch.uint8, device, stream)
     return _cuda(workspace, "workspace")
 
 
@@ -291,8 +293,7 @@ def kv_block_means(cache: GpuKvCache, layer: int, block_begin: int, block_end: i
     n = max(int(block_end) - int(block_begin), 0)
     if out is None:
         b, h, d = cache.row_shape
-        with _owned_by(stream, cache.device):
-            out, row = torch.empty((b, h, n, d), dtype=torch.bfloat16, device=cache.device), n * d
+        out, row = _empty((b, h, n, d), torch.bfloat16, cache.device, stream), n * d
     else:
         blocks, row = _means_rows("kv_block_means", out, cache)
         if blocks != n:
@@ -317,8 +318,7 @@ def gqa_select_blocks(query: torch.Tensor, cache: GpuKvCache, layer: int, means:
     blocks, row = _means_rows("gqa_select_blocks", means, cache)
     shape = (b, s, cache.row_shape[1], max(int(max_blocks), 0))
     if out is None:
-        with _owned_by(stream, query.device):
-            out = torch.empty(shape, dtype=torch.int32, device=query.device)
+        out = _empty(shape, torch.int32, query.device, stream)
     else:
         _int32("gqa_select_blocks", out, shape, "out")
     rc = lib.sa_gqa_select_blocks(cache.handle, layer, query.data_ptr(), _dtype_code(query), b, s, int(num_heads),
