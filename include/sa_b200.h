@@ -489,7 +489,8 @@ int sa_gqa_tree_attend(sa_kv_cache *cache, int32_t layer, const void *query, con
  * (batch, n), device, nodes in [0, drafted); drafted <= SA_MAX_DRAFT_NODES.
  * An entry outside [0, drafted) leaves its destination as it was and sets bit 1
  * of sa_kv_cache_device_status.  Does not advance the position: the caller
- * advances it by n.  Not for low-rank K (its state follows writes in order). */
+ * advances it by n, one n for all sequences (those that accepted more draft
+ * the rest again).  Not for low-rank K (its state follows writes in order). */
 int sa_kv_cache_keep_drafts(sa_kv_cache *cache, const int32_t *path, int32_t batch, int32_t n, int32_t drafted,
                             sa_stream_t stream);
 

@@ -20,9 +20,9 @@
 // apart, on one of its own row (kSpread); q^ and u are held in one fp16 plane each
 // (11 bits) for bf16 callers, whose outputs' own rounding is eight times as coarse
 // (the error against 64 bits grows by 2.2%; with two planes, the cache's choice, by
-// nothing, at 384 instead of 308 us), and in two (22 bits) for f16 and f32:
+// nothing, at 388 instead of 300 us for 64 sequences), and in two (22 bits) for f16 and f32:
 // with one plane of u the error of f16 outputs was 1.37 times that of f32 arithmetic
-// rounded once, at 1,316 instead of 1,377 us in the widest case.  sum(q^) is of the
+// rounded once, at 1,316 instead of 1,412 us in the widest case.  sum(q^) is of the
 // rounded values, so their rounding only moves the query by its own.  Everything
 // else is f32.
 //
@@ -49,11 +49,10 @@
 // CTA leaves one partial record per unit that it touches; a merge kernel joins
 // them, rotates back and stores.
 //
-//
-// Bound by instruction issue (60% of the cycles; about 5,700 warp instructions per
+// Bound by instruction issue (62% of the cycles; about 5,900 warp instructions per
 // tile of 128 tokens and 64 rows, more than half of them the softmax's; tensor pipe
 // 20%): 16 sequences of 8 KV heads, 8176 int4 tokens, 64 bf16 rows, 155 MB, 88 us with
-// prep and merge; 64 sequences 314 us.  Groups of 16 rows: with 32 a group's
+// prep and merge (f16, two planes: 110); 64 sequences 300 us.  Groups of 16 rows: with 32 a group's
 // registers leave room for half the warps (113 us).
 //
 // Every mbarrier wait is bounded (2 s); one that gives up sets the abort flag and
@@ -80,7 +79,8 @@ constexpr float kShift = 7.0f;  // u <= 2^(kHead + kShift), below fp16's 65504
 // Rows whose largest |q'| is within 2^kSpread of the block's keep all 22 bits of two planes on the block's power of
 // two: the block's largest is put into [2^11, 2^12), and fp16 numbers are multiples of 2^-24.  A block that spreads
 // further has a power of two per row, so that no query, however large, costs other rows bits; each of its tiles takes
-// the path that raises references.  A scale per row in every tile takes 324 instead of 308 us.
+// the path that raises references (145 instead of 88 us for 16 sequences in bf16).  A scale per row in every tile
+// cost all callers 5%.
 constexpr int kSpread = 14;
 constexpr int kPrepThreads = 512;
 constexpr int kMergeWarps = 8;

@@ -187,7 +187,8 @@ class GpuKvCache:
         """Move the accepted drafts of a verified tree to the front, in every layer (sa_kv_cache_keep_drafts).
 
         ``path`` int32 (B, n) on the device: node path[b][i] of the ``drafted`` appended ones becomes token
-        position + i.  The position is not advanced (``advance_position(n)`` does).  An entry outside
+        position + i.  The position is not advanced (``advance_position(n)`` does), and is one for all sequences: n is
+        the smallest number accepted.  An entry outside
         [0, drafted) moves nothing and sets bit 1 of ``device_status``.
         """
         from .ops import ShapeMismatch, UnsupportedOp, _cuda, _raise_op, _stream_handle
