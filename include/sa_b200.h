@@ -537,6 +537,117 @@ int sa_gqa_sparse_attend(sa_kv_cache *cache, int32_t layer, const void *query, c
                          int64_t num_heads, int32_t has_scale, float scale, void *workspace,
                          int64_t workspace_bytes, sa_stream_t stream);
 
+/* ======================================================================
+ * Paged serving: a pool of pages of SA_PAGE_TOKENS tokens in the compressed
+ * format of sa_kv_cache, for sequences of different lengths, and beam search
+ * over it.  The reference has neither (its cache holds one sequence,
+ * onnx-rt/src/cuda/kv_cache.rs:111-193); codes, scales and zero points of a
+ * vector are those of sa_kv_append (kv_compression.rs:216-267), and attention
+ * has sa_gqa_attend's semantics.
+ *
+ * Everything that changes from step to step lives on the device, so that a
+ * captured step can be replayed:
+ *   page_table  int32 (batch, max_pages), rows table_stride elements apart:
+ *               page j of row b holds its tokens [64 j, 64 j + 64).  A page may
+ *               stand in several rows.  Entries past a row's tokens are not read.
+ *   seq_lens    int32 (batch): tokens that row b holds before the call's new
+ *               ones.  Below 0: the row takes no part.
+ *   counts      NULL, or int32 (batch): of the call's seq_len new tokens, row
+ *               b's first counts[b] exist (values are clamped to [0, seq_len]).
+ * What a call cannot check on the host sets bits of sa_kv_pages_device_status.
+ *
+ * Layout, per layer: record (page p, local KV head h) of
+ * SA_PAGE_TOKENS * (2 CB + 16) bytes at (p * kv_heads + h) * record bytes:
+ *   K codes [64][CB], K {scale, zero point} [64][2] f32, V {scale, zero point}
+ *   [64][2] f32, V codes in sa_kv_cache's 16-token blocks, so that a whole
+ *   record is one contiguous copy.  bits 4 or 8, head_dim 64 or 128.
+ *
+ * Calls allocate nothing and wait for nothing; calls that write pages, tables
+ * or lengths and calls that read them are ordered by the caller (one stream, or
+ * events).  Attention calls on one pool may overlap on the device if each has a
+ * workspace of its own.  The calls read the handle only: any threads.
+ * ====================================================================== */
+#define SA_PAGE_TOKENS 64
+#define SA_MAX_BEAMS 32
+#define SA_MAX_BEAM_KEEP 64
+
+typedef struct sa_kv_pages sa_kv_pages;
+
+typedef struct sa_kv_pages_config {
+    int32_t num_layers;
+    int32_t num_pages;
+    int32_t num_heads;     /* query heads of the model */
+    int32_t num_kv_heads;  /* as in sa_kv_cache_config, with the head range held here */
+    int32_t kv_head_begin;
+    int32_t kv_head_count;
+    int32_t head_dim;      /* 64 or 128 */
+    int32_t bits;          /* 4 or 8 */
+    uint64_t seed;         /* signs as sa_kv_cache draws them */
+} sa_kv_pages_config;
+
+typedef struct sa_kv_pages_view {
+    uint8_t *records;        /* [num_pages][kv_heads][record_bytes] of the layer */
+    const float *signs;      /* [kv_heads][head_dim] */
+    int32_t num_pages;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t bits;
+    int32_t code_bytes;      /* CB */
+    int32_t record_bytes;
+    int32_t k_meta_offset;   /* K codes are at 0 */
+    int32_t v_meta_offset;
+    int32_t v_codes_offset;
+    float wht_scale;
+} sa_kv_pages_view;
+
+/* Allocates every layer's pages on the current device, zero-filled; the only
+ * call here that allocates.  destroy frees them (NULL is ok). */
+int sa_kv_pages_create(const sa_kv_pages_config *config, sa_kv_pages **out);
+int sa_kv_pages_destroy(sa_kv_pages *pages);
+int sa_kv_pages_get_config(const sa_kv_pages *pages, sa_kv_pages_config *config);
+int sa_kv_pages_layer_view(const sa_kv_pages *pages, int32_t layer, sa_kv_pages_view *view);
+/* 0, or bits of what the kernels on this pool met: 1 a bounded wait gave up
+ * (the output is not valid); 2 a page id outside the pool, or a row with more
+ * tokens than its table has pages (such tokens were not written, and are not
+ * attended to); 4 a position outside the cos/sin tables (not written; zero
+ * output); 8 beams of one group with different lengths, or a parent outside the
+ * group (the group, or the beam, stays as it was).  Synchronises with the
+ * device; `clear` resets it. */
+int sa_kv_pages_device_status(sa_kv_pages *pages, int32_t *status, int32_t clear);
+
+/* Quantize-on-append of seq_len new tokens per row: token s of row b goes to
+ * position seq_lens[b] + s of its pages (s < counts[b]), K rotated to that
+ * position when do_rotary is set (tables as for sa_kv_append).  key / value:
+ * row b, token s at + b * batch_stride + s * token_stride elements of `dtype`,
+ * kv_heads * head_dim consecutive values.  Bit-exact with sa_kv_append.  Rows
+ * that share a page must not write the same token of it.  seq_lens is not
+ * changed: a forward pass appends in every layer and then raises it once. */
+int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const void *value,
+                       int64_t batch_stride, int64_t token_stride, int32_t dtype, int32_t batch, int32_t seq_len,
+                       const int32_t *page_table, int64_t table_stride, int32_t max_pages,
+                       const int32_t *seq_lens, const int32_t *counts, const float *cos_cache,
+                       const float *sin_cache, int32_t cache_rows, int32_t do_rotary,
+                       int32_t rotary_interleaved, sa_stream_t stream);
+
+/* Attention of the new tokens over the pages: token s of row b, at position
+ * seq_lens[b] + s, attends to the row's tokens [0, seq_lens[b] + s] (its own
+ * K/V included: append first).  query: as key above, q_heads_local * head_dim
+ * values, rotated in the kernel when do_rotary is set; attn_out: (batch,
+ * seq_len, q_heads_local * head_dim), contiguous, zero for tokens that do not
+ * exist and rows without tokens.  A row's pages are read once per new token:
+ * this is the decode step, for one new token or a few.
+ * Precision: queries and weights are held to 16 bits for f16 and bf16 callers
+ * (weights relative to the largest of each 32 or 64 tokens), to 24 for f32.
+ * `workspace` (device, 256-byte aligned, at least what
+ * sa_gqa_paged_workspace_bytes says) is the call's alone until it has run. */
+int64_t sa_gqa_paged_workspace_bytes(const sa_kv_pages *pages, int32_t batch, int32_t seq_len, int32_t dtype);
+int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, int64_t batch_stride,
+                        int64_t token_stride, void *attn_out, int32_t dtype, int32_t batch, int32_t seq_len,
+                        int64_t num_heads, int32_t has_scale, float scale, const int32_t *page_table,
+                        int64_t table_stride, int32_t max_pages, const int32_t *seq_lens, const int32_t *counts,
+                        const float *cos_cache, const float *sin_cache, int32_t cache_rows, int32_t do_rotary,
+                        int32_t rotary_interleaved, void *workspace, int64_t workspace_bytes, sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

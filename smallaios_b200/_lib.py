@@ -39,9 +39,14 @@ EXPORTED = [
     "sa_qkv_project_append", "sa_rms_norm", "sa_silu_mul", "sa_rotary_embedding",
     "sa_gqa_tree_workspace_bytes", "sa_gqa_tree_attend", "sa_kv_cache_set_tree_precision", "sa_kv_cache_keep_drafts", "sa_kv_block_means",
     "sa_gqa_select_blocks", "sa_gqa_sparse_workspace_bytes", "sa_gqa_sparse_attend",
+    "sa_kv_pages_create", "sa_kv_pages_destroy", "sa_kv_pages_get_config", "sa_kv_pages_layer_view",
+    "sa_kv_pages_device_status", "sa_kv_pages_append", "sa_gqa_paged_workspace_bytes", "sa_gqa_paged_attend",
 ]
 SA_MAX_DRAFT_NODES = 64
 SA_BLOCK_TOKENS = 64
+SA_PAGE_TOKENS = 64
+SA_MAX_BEAMS = 32
+SA_MAX_BEAM_KEEP = 64
 SA_STATIC_SCRATCH_BYTES = 8 << 20
 
 
@@ -84,6 +89,37 @@ class KvLayerView(ctypes.Structure):
         ("lr_us", ctypes.c_void_p),
         ("lr_kmeta", ctypes.c_void_p),
         ("lr_vtr", ctypes.c_void_p),
+    ]
+
+
+class KvPagesConfig(ctypes.Structure):
+    _fields_ = [
+        ("num_layers", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("kv_head_begin", ctypes.c_int32),
+        ("kv_head_count", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
+        ("seed", ctypes.c_uint64),
+    ]
+
+
+class KvPagesView(ctypes.Structure):
+    _fields_ = [
+        ("records", ctypes.c_void_p),
+        ("signs", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
+        ("code_bytes", ctypes.c_int32),
+        ("record_bytes", ctypes.c_int32),
+        ("k_meta_offset", ctypes.c_int32),
+        ("v_meta_offset", ctypes.c_int32),
+        ("v_codes_offset", ctypes.c_int32),
+        ("wht_scale", ctypes.c_float),
     ]
 
 
@@ -166,6 +202,24 @@ def _declare(l: ctypes.CDLL) -> None:
     l.sa_gqa_sparse_workspace_bytes.argtypes = [_P, _I32]
     l.sa_gqa_sparse_attend.restype = ctypes.c_int
     l.sa_gqa_sparse_attend.argtypes = [_P, _I32, _P, _P, _I32, _P, _I32, _I32, _I32, _I64, _I32, _F, _P, _I64, _P]
+    l.sa_kv_pages_create.restype = ctypes.c_int
+    l.sa_kv_pages_create.argtypes = [ctypes.POINTER(KvPagesConfig), ctypes.POINTER(_P)]
+    l.sa_kv_pages_destroy.restype = ctypes.c_int
+    l.sa_kv_pages_destroy.argtypes = [_P]
+    l.sa_kv_pages_get_config.restype = ctypes.c_int
+    l.sa_kv_pages_get_config.argtypes = [_P, ctypes.POINTER(KvPagesConfig)]
+    l.sa_kv_pages_layer_view.restype = ctypes.c_int
+    l.sa_kv_pages_layer_view.argtypes = [_P, _I32, ctypes.POINTER(KvPagesView)]
+    l.sa_kv_pages_device_status.restype = ctypes.c_int
+    l.sa_kv_pages_device_status.argtypes = [_P, ctypes.POINTER(_I32), _I32]
+    l.sa_kv_pages_append.restype = ctypes.c_int
+    l.sa_kv_pages_append.argtypes = [_P, _I32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _P, _P, _P, _I32,
+                                     _I32, _I32, _P]
+    l.sa_gqa_paged_workspace_bytes.restype = _I64
+    l.sa_gqa_paged_workspace_bytes.argtypes = [_P, _I32, _I32, _I32]
+    l.sa_gqa_paged_attend.restype = ctypes.c_int
+    l.sa_gqa_paged_attend.argtypes = [_P, _I32, _P, _I64, _I64, _P, _I32, _I32, _I32, _I64, _I32, _F, _P, _I64, _I32, _P,
+                                      _P, _P, _P, _I32, _I32, _I32, _P, _I64, _P]
     l.sa_qkv_project_append.restype = ctypes.c_int
     l.sa_qkv_project_append.argtypes = [_P, _I32, _P, _P, _P, _I32, _I32, _I64, _P, _P, _I32, _I32, _I32, _P, _P,
                                         _P, _P]

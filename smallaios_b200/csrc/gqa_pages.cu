@@ -1,0 +1,706 @@
+// Decode attention over pages: one query token per row, rows of any lengths,
+// 4/8-bit codes, head_dim 64/128.
+//
+// pages_attend_kernel: every SM runs one CTA of twelve independent warps.  The
+// chunks (64 tokens, or 32 where a token has 128 code bytes) of all units (row,
+// KV head, block of query heads) lie end to end and each warp owns an equal
+// range, so rows of very different lengths keep all SMs busy; a warp streams its
+// chunks through a ring of shared-memory stages, one bulk copy per chunk (a
+// record's K codes, metadata and V codes are contiguous).
+//
+// The arithmetic of a chunk stays in registers.  With A = the query digits (row r
+// of the MMA: head r's high byte, row r + 8 its low byte) and B = K codes (columns:
+// tokens), lane (r, q) of the accumulator holds head r's scores of tokens; with the
+// tokens assigned to columns as tok() says, these are exactly the tokens whose
+// weights the lane has to supply as the A operand of the value product, whose
+// B operand is a word of the V layout.  So scores become weights without passing
+// through shared memory, and one MMA carries eight query heads: 16 rows = 8 heads x
+// 2 digits.  f32 callers get three digits and four heads (12 rows).
+//
+//   s_t = ks_t (q'.c_t) + kz_t sum(q')           (log2 units, scale folded in)
+//   R = max s + log2 max vs,  u_t = 2^(s_t - R) vs_t in (0, 1], 16 or 24 bits of it
+//   L = sum 2^(s_t - R), Z = sum 2^(s_t - R) vz_t, X = sum u_t c_t
+//   out = S.H.((X + Z) / L) / sqrt(D)
+//
+// R is each chunk's own, and its sums are moved to the running reference when they
+// are added: a weight far below the context's largest keeps 16 bits relative to its
+// neighbours, not to that largest one.  Codes enter both products less their middle
+// (8 or 128), their zero points raised by as much, so that the large common part of
+// q'.c and of X need not cancel after both were rounded.
+//
+// Products are exact integers; the int8 MMAs, one ex2 and some fifteen other
+// instructions per (head pair, token) fit below the copy time of a chunk.
+//
+// pages_merge_kernel: per unit, the sum of its warps' partial records, the
+// division, the inverse rotation and the store.
+#include "sa_async.cuh"
+#include "sa_decode_common.cuh"
+#include "sa_pages.cuh"
+
+namespace sa {
+
+namespace {
+
+using namespace dec;
+
+constexpr int kNWP = 12;         // warps per CTA, one CTA per SM
+constexpr int kMaxRows = 1024;   // rows of a launch: its prefix sums fit in 4 KB
+constexpr int64_t kMaxUnits = 16384;  // units of a launch: bounds the workspace
+
+template <int BITS, int D, int ND>
+struct PGeo {
+    static constexpr int KB = D * BITS / 8;
+    static constexpr int CT = KB > 64 ? 32 : 64;    // tokens per chunk
+    static constexpr int CPP = kPageTokens / CT;    // chunks per page
+    static constexpr int STAGE = CT * (2 * KB + 16);
+    static constexpr int NST = 2;                   // stages per warp
+    static constexpr int HB = ND == 2 ? 8 : 4;      // query heads per unit
+    static constexpr int NCH = D / 32;              // QK k-steps
+    static constexpr int SEGW = KB / 16;            // K words per lane and token
+    static constexpr int NPR = CT / 16;             // token pairs of tiles: 16 tokens each
+    static constexpr int VV = KB / 32;              // 16-byte V loads per 16-token block
+    static constexpr int NF = D / 4;                // value sums per lane
+    static constexpr int REC = HB * (D + 4);        // floats per partial record: values, then R, L, Z (and padding)
+    static constexpr int SMEM = kNWP * NST * STAGE + kNWP * NST * 8;
+    static constexpr float UMAX = ND == 2 ? 65535.0f : 16777215.0f;
+    static constexpr float LOG2UMAX = ND == 2 ? 15.99997798605f : 23.99999991400867f;
+    static constexpr int QMAX = ND == 2 ? 32639 : 8355711;  // 127 in the top digit
+    static constexpr float CENTRE = BITS == 4 ? 8.0f : 128.0f;
+    static constexpr float UNIT = BITS == 4 ? 0.0625f : 1.0f;  // 4-bit codes enter the products as 16 (c - 8)
+    static_assert(SMEM + (kMaxRows + 1) * 4 + 256 <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void mma_s8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_u8s8_w(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Codes of a word as signed bytes less their middle: of 8 bits, or 16 times the low / high nibbles.
+__device__ __forceinline__ uint32_t centred8(uint32_t w) { return w ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t centred_lo(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t centred_hi(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
+
+// Where a range is: chunk c of unit k of row r, whose units have n chunks.
+struct Place {
+    int r, k, c, n;
+};
+
+// Tokens that query row r (row0 + r of batch x seq_len) attends to.
+__device__ __forceinline__ int visible(const PagesAttendArgs &a, int row, bool report) {
+    const int b = row / a.seq_len, s = row - b * a.seq_len;
+    int64_t pos0;
+    if (s >= row_tokens(a.rows, b, a.seq_len, pos0)) return 0;
+    const int64_t pos = pos0 + s;
+    if (a.rope.on && pos >= a.rope.rows) {
+        if (report) atomicOr(a.rows.dev_status, kPagesBadPosition);
+        return 0;
+    }
+    const int64_t most = (int64_t)a.rows.max_pages * kPageTokens;
+    if (pos >= most) {
+        if (report) atomicOr(a.rows.dev_status, kPagesBadPage);
+        return (int)most;
+    }
+    return (int)pos + 1;
+}
+
+// Warps that share F chunks: at least two chunks each, so that a warp's copies overlap its work and half the
+// partial records are left to merge.
+__host__ __device__ __forceinline__ int sharing_warps(int F, int warps) { return min(warps, (F + 1) / 2); }
+
+template <typename T, int BITS, int D, int ND>
+__global__ void __launch_bounds__(kNWP * 32, 1)
+    pages_attend_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, int *prefix_out, float *records) {
+    using G = PGeo<BITS, D, ND>;
+    constexpr int KB = G::KB, CT = G::CT, N = D / 4;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int s_prefix[kMaxRows + 1];
+    __shared__ int s_warp[kNWP];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r = lane >> 2, q = lane & 3;
+    unsigned char *ring = smem + warp * G::NST * G::STAGE;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kNWP * G::NST * G::STAGE) + warp * G::NST;
+    if (lane == 0)
+        for (int i = 0; i < G::NST; i++) mbar_init(bars + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    griddep_launch_dependents();
+    griddep_wait();  // pages, table, lengths and the query may come from the kernels before
+
+    // prefix sums of the rows' chunks
+    {
+        int carry = 0;
+        if (tid == 0) s_prefix[0] = 0;
+        for (int base = 0; base < rows; base += kNWP * 32) {
+            const int i = base + tid;
+            int v = i < rows ? (visible(a, row0 + i, blockIdx.x == 0) + CT - 1) / CT : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += up;
+            }
+            if (lane == 31) s_warp[warp] = v;
+            __syncthreads();
+            int before = carry;
+#pragma unroll
+            for (int w = 0; w < kNWP; w++) {
+                if (w < warp) before += s_warp[w];
+                carry += s_warp[w];
+            }
+            if (i < rows) s_prefix[i + 1] = before + v;
+            __syncthreads();
+        }
+    }
+    const int upr = a.heads * hblocks;  // units per row
+    if (blockIdx.x == 0)
+        for (int i = tid; i <= rows; i += kNWP * 32) prefix_out[i] = s_prefix[i];
+    const int F = s_prefix[rows] * upr;  // fits: the launch bounds it
+    const int W = sharing_warps(F, (int)gridDim.x * kNWP);
+    const int w = warp * (int)gridDim.x + blockIdx.x;  // neighbours in the flat order run on different SMs
+    if (w >= W) return;  // warps are independent from here on
+    const int f0 = (int)((int64_t)w * F / W), f1 = (int)((int64_t)(w + 1) * F / W);
+
+    Place cur;
+    {
+        // the last row that begins at or before f0 and has chunks
+        int lo = 0, hi = rows;
+        const int target = f0 / upr;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_prefix[mid] <= target) lo = mid;
+            else hi = mid;
+        }
+        cur.r = lo;
+        cur.n = s_prefix[lo + 1] - s_prefix[lo];
+        const int off = f0 - s_prefix[lo] * upr;
+        cur.k = off / cur.n;
+        cur.c = off - cur.k * cur.n;
+    }
+    auto advance = [&](Place &p) {
+        if (++p.c < p.n) return;
+        p.c = 0;
+        if (++p.k < upr) return;
+        p.k = 0;
+        do {
+            if (++p.r >= rows) {  // past the last chunk: never used again
+                p.r = rows - 1;
+                return;
+            }
+            p.n = s_prefix[p.r + 1] - s_prefix[p.r];
+        } while (p.n == 0);
+    };
+    auto page_of = [&](const Place &p) {
+        return a.rows.table[(int64_t)((row0 + p.r) / a.seq_len) * a.rows.table_stride + p.c / G::CPP];
+    };
+
+    // copies run NST chunks ahead; the page of the next chunk to copy is fetched one step before
+    Place ahead = cur;
+    int fa = f0, page = page_of(ahead);
+    unsigned pend = 0, bad = 0;
+    bool failed = false;
+    auto issue = [&](int st) {
+        if (fa < f1) {
+            uint64_t *bar = bars + st;
+            if (page < 0 || page >= a.rows.num_pages) {
+                bad |= 1u << st;
+                if (lane == 0) {
+                    atomicOr(a.rows.dev_status, kPagesBadPage);
+                    mbar_arrive(bar);
+                }
+            } else {
+                bad &= ~(1u << st);
+                const uint8_t *rec = a.records + ((int64_t)page * a.heads + ahead.k / hblocks) * page_record(KB);
+                unsigned char *dst = ring + st * G::STAGE;
+                if (lane == 0) mbar_expect_tx(bar, G::STAGE);
+                if constexpr (G::CPP == 1) {
+                    if (lane == 0) {
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // after the warp's reads of the stage
+                        bulk_g2s(dst, rec, G::STAGE, bar);
+                    }
+                } else if (lane < 4) {
+                    const int part = ahead.c % G::CPP;
+                    const bool codes = lane == 0 || lane == 3;
+                    const uint32_t nb = codes ? CT * KB : CT * 8;
+                    const int from = lane == 0 ? 0 : lane == 1 ? page_k_meta(KB) : lane == 2 ? page_v_meta(KB) : page_v_codes(KB);
+                    const int to = lane == 0 ? 0 : CT * KB + (lane - 1) * CT * 8;
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    bulk_g2s(dst + to, rec + from + part * nb, nb, bar);
+                }
+            }
+            pend |= 1u << st;
+            if (++fa < f1) {
+                advance(ahead);
+                page = page_of(ahead);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < G::NST; i++) issue(i);
+
+    uint32_t qa[G::NCH][4];       // query digits, A fragments
+    float c1 = 0.0f, c2 = 0.0f;   // score constants of the lane's head
+    float facc[G::NF];            // value sums in the frame of R
+    float R = -INFINITY, L = 0.0f, Z = 0.0f;
+    int len = 0;
+    bool fresh = true;
+    int st = 0;
+    uint32_t phase = 0;
+    for (int f = f0; f < f1; f++) {
+        if (fresh) {
+            // ---- a new unit: the lane's quarter of its head's query, rotated, as digits ----
+            fresh = false;
+            R = -INFINITY;
+            L = Z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < G::NF; i++) facc[i] = 0.0f;
+            const int row = row0 + cur.r, b = row / a.seq_len, s = row - b * a.seq_len;
+            len = visible(a, row, false);
+            const int h = cur.k / hblocks, g = (cur.k - h * hblocks) * G::HB + (ND == 2 ? r : (r & 3));
+            const bool on = g < a.group;
+            float x[N];
+            if (on) {
+                const T *src = static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
+                               ((int64_t)h * a.group + g) * D + q * N;
+                load_run<T, N>(src, a.aligned, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] = 0.0f;
+            }
+            if (a.rope.on) {
+                const int64_t pos = (int64_t)a.rows.lens[b] + s;
+                if (a.rope.interleaved) {
+                    const float *cs = a.rope.cos_cache + pos * (D / 2) + q * (N / 2);
+                    const float *sn = a.rope.sin_cache + pos * (D / 2) + q * (N / 2);
+#pragma unroll
+                    for (int i = 0; i < N / 2; i++) {
+                        const float co = cs[i], si = sn[i], x0 = x[2 * i], x1 = x[2 * i + 1];
+                        x[2 * i] = __fsub_rn(__fmul_rn(co, x0), __fmul_rn(si, x1));
+                        x[2 * i + 1] = __fadd_rn(__fmul_rn(si, x0), __fmul_rn(co, x1));
+                    }
+                } else {
+                    // the partner of dimension d is d +- D/2, the lane two away
+                    const float *cs = a.rope.cos_cache + pos * (D / 2) + (q & 1) * N;
+                    const float *sn = a.rope.sin_cache + pos * (D / 2) + (q & 1) * N;
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const float co = cs[i], si = sn[i], other = __shfl_xor_sync(0xffffffffu, x[i], 2);
+                        const float own = __fmul_rn(co, x[i]), cross = __fmul_rn(si, other);
+                        x[i] = (q & 2) ? __fadd_rn(cross, own) : __fsub_rn(own, cross);
+                    }
+                }
+            }
+            const float *sg = a.signs + (int64_t)h * D + q * N;
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] *= sg[i];
+#pragma unroll
+            for (int hs = 1; hs < N; hs <<= 1)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if ((i & hs) == 0) {
+                        const float p0 = x[i], p1 = x[i + hs];
+                        x[i] = p0 + p1;
+                        x[i + hs] = p0 - p1;
+                    }
+#pragma unroll
+            for (int lm = 1; lm < 4; lm <<= 1)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const float other = __shfl_xor_sync(0xffffffffu, x[i], lm);
+                    x[i] = (q & lm) ? other - x[i] : x[i] + other;
+                }
+            float sum = 0.0f, mabs = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                x[i] *= a.wht_scale;
+                sum += x[i];
+                mabs = fmaxf(mabs, fabsf(x[i]));
+            }
+#pragma unroll
+            for (int lm = 1; lm < 4; lm <<= 1) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, lm);
+                mabs = fmaxf(mabs, __shfl_xor_sync(0xffffffffu, mabs, lm));
+            }
+            const float sigma = mabs > 0.0f ? mabs / (float)G::QMAX : 1.0f;
+            const float inv = 1.0f / sigma, sl2 = a.scale * kLog2eF;
+            c1 = sigma * sl2 * G::UNIT;
+            c2 = sum * sl2;
+#pragma unroll
+            for (int k = 0; k < G::NCH; k++) {
+                qa[k][0] = qa[k][1] = qa[k][2] = qa[k][3] = 0u;
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        // byte e of k-group hf: dimension as the K words hold it (even and odd nibbles, or bytes)
+                        const int i = 8 * k + (BITS == 4 ? 2 * e + hf : 4 * hf + e);
+                        const int v = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
+                        const int d2 = (int)(int8_t)(v & 0xff), rest = (v - d2) >> 8;
+                        if constexpr (ND == 2) {
+                            qa[k][2 * hf] |= ((uint32_t)rest & 0xffu) << (8 * e);
+                            qa[k][2 * hf + 1] |= ((uint32_t)d2 & 0xffu) << (8 * e);
+                        } else {
+                            const int d1 = (int)(int8_t)(rest & 0xff), d0 = (rest - d1) >> 8;
+                            qa[k][2 * hf] |= ((uint32_t)(r < 4 ? d0 : d1) & 0xffu) << (8 * e);
+                            qa[k][2 * hf + 1] |= (r < 4 ? (uint32_t)d2 & 0xffu : 0u) << (8 * e);
+                        }
+                    }
+            }
+        }
+        if (!mbar_wait_bounded(bars + st, phase)) failed = true;
+        if (__any_sync(0xffffffffu, failed)) {
+            failed = true;
+            break;
+        }
+        pend &= ~(1u << st);
+        const int n_tok = (bad >> st) & 1u ? 0 : min(CT, len - cur.c * CT);
+        if (n_tok > 0) {
+            const unsigned char *sp = ring + st * G::STAGE;
+            const unsigned char *vmeta = sp + CT * (KB + 8), *vcodes = sp + CT * (KB + 16);
+            // ---- scores: tile pair p holds tokens 16 p + 4 q + e of the lane's head ----
+            float sc[4 * G::NPR];
+            float smax = -INFINITY, vmax = 0.0f;
+#pragma unroll
+            for (int p = 0; p < G::NPR; p++) {
+                int acc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const unsigned char *kp = sp + (16 * p + 4 * (r >> 1) + 2 * j + (r & 1)) * KB + q * (KB / 4);
+                    uint32_t wv[G::SEGW];
+                    if constexpr (G::SEGW == 2) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+                        wv[0] = v.x;
+                        wv[1] = v.y;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < G::SEGW / 4; i++) {
+                            const uint4 v = reinterpret_cast<const uint4 *>(kp)[i];
+                            wv[4 * i] = v.x;
+                            wv[4 * i + 1] = v.y;
+                            wv[4 * i + 2] = v.z;
+                            wv[4 * i + 3] = v.w;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < G::NCH; k++) {
+                        if constexpr (BITS == 4) mma_s8s8(acc[j], qa[k], centred_lo(wv[k]), centred_hi(wv[k]));
+                        else mma_s8s8(acc[j], qa[k], centred8(wv[2 * k]), centred8(wv[2 * k + 1]));
+                    }
+                }
+                const float4 km0 = *reinterpret_cast<const float4 *>(sp + CT * KB + (16 * p + 4 * q) * 8);
+                const float4 km1 = *reinterpret_cast<const float4 *>(sp + CT * KB + (16 * p + 4 * q) * 8 + 16);
+                const float4 vm0 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8);
+                const float4 vm1 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8 + 16);
+                const float ks[4] = {km0.x, km0.z, km1.x, km1.z}, kz[4] = {km0.y, km0.w, km1.y, km1.w};
+                const float vs[4] = {vm0.x, vm0.z, vm1.x, vm1.z};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = e >> 1, x = e & 1;
+                    float dot;
+                    if constexpr (ND == 2) {
+                        dot = (float)(acc[j][x] * 256 + acc[j][2 + x]);
+                    } else {
+                        const float part = r < 4 ? fmaf((float)acc[j][x], 65536.0f, (float)acc[j][2 + x])
+                                                 : (float)acc[j][x] * 256.0f;
+                        dot = part + __shfl_xor_sync(0xffffffffu, part, 16);
+                    }
+                    float s = fmaf(ks[e] * c1, dot, fmaf(G::CENTRE, ks[e], kz[e]) * c2);
+                    float v = vs[e];
+                    if (n_tok < CT && 16 * p + 4 * q + e >= n_tok) {
+                        s = -INFINITY;
+                        v = 0.0f;
+                    }
+                    sc[4 * p + e] = s;
+                    smax = fmaxf(smax, s);
+                    vmax = fmaxf(vmax, v);
+                }
+            }
+#pragma unroll
+            for (int lm = 1; lm < 4; lm <<= 1) {
+                smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, lm));
+                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, lm));
+            }
+            // the chunk's reference, the running one, and the factors that bring both sums to the latter
+            const float Rc = smax + __log2f(fmaxf(vmax, kVScaleMin));
+            const float Rn = fmaxf(R, Rc);
+            const float fo = R == -INFINITY ? 0.0f : exp2f(R - Rn), fn = Rc == -INFINITY ? 0.0f : exp2f(Rc - Rn);
+            R = Rn;
+            const float base = Rc == -INFINITY ? 0.0f : Rc - G::LOG2UMAX;
+            // ---- weights: u = 2^(s - Rc) vs as UMAX fixed-point digits, A fragments of 32 tokens each ----
+            uint32_t ua[CT / 32][4];
+            float lc = 0.0f, zc = 0.0f;
+#pragma unroll
+            for (int p = 0; p < G::NPR; p++) {
+                const float4 vm0 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8);
+                const float4 vm1 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8 + 16);
+                float vs[4] = {vm0.x, vm0.z, vm1.x, vm1.z}, vz[4] = {vm0.y, vm0.w, vm1.y, vm1.w};
+                uint32_t U[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (n_tok < CT && 16 * p + 4 * q + e >= n_tok) vs[e] = vz[e] = 0.0f;  // whatever a page holds there
+                    const float ee = ex2_approx(sc[4 * p + e] - base);
+                    lc += ee;
+                    zc = fmaf(ee, fmaf(G::CENTRE, vs[e], vz[e]), zc);
+                    U[e] = __float2uint_rn(fminf(ee * vs[e], G::UMAX));
+                }
+                if constexpr (ND == 2) {
+                    const uint32_t p01 = __byte_perm(U[0], U[1], 0x5410), p23 = __byte_perm(U[2], U[3], 0x5410);
+                    ua[p >> 1][2 * (p & 1)] = __byte_perm(p01, p23, 0x7531);
+                    ua[p >> 1][2 * (p & 1) + 1] = __byte_perm(p01, p23, 0x6420);
+                } else {
+                    const uint32_t top = r < 4 ? 0x0062u : 0x0051u;
+                    ua[p >> 1][2 * (p & 1)] =
+                        __byte_perm(__byte_perm(U[0], U[1], top), __byte_perm(U[2], U[3], top), 0x5410);
+                    ua[p >> 1][2 * (p & 1) + 1] =
+                        r < 4 ? __byte_perm(__byte_perm(U[0], U[1], 0x0040), __byte_perm(U[2], U[3], 0x0040), 0x5410)
+                              : 0u;
+                }
+            }
+            L = fmaf(L, fo, lc * fn);
+            Z = fmaf(Z, fo, zc * fn);
+            if (__any_sync(0xffffffffu, fo != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < G::NF; i++) facc[i] *= fo;
+            }
+            // ---- values: 16-byte piece v of the V blocks at a time, its integer sums folded at once ----
+            const float fu = fn * G::UNIT;
+#pragma unroll
+            for (int v = 0; v < G::VV; v++) {
+                constexpr int NJ = BITS == 4 ? 8 : 4;  // n-tiles of the piece
+                int acc[NJ][4];
+#pragma unroll
+                for (int j = 0; j < NJ; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
+#pragma unroll
+                for (int t = 0; t < CT / 32; t++) {
+                    const unsigned char *vb = vcodes + 2 * t * (16 * KB) + (8 * v + r) * 64 + 16 * q;
+                    const uint4 x0 = *reinterpret_cast<const uint4 *>(vb);
+                    const uint4 x1 = *reinterpret_cast<const uint4 *>(vb + 16 * KB);
+                    const uint32_t y0[4] = {x0.x, x0.y, x0.z, x0.w}, y1[4] = {x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if constexpr (BITS == 4) {
+                            mma_u8s8_w(acc[2 * j], ua[t], centred_lo(y0[j]), centred_lo(y1[j]));
+                            mma_u8s8_w(acc[2 * j + 1], ua[t], centred_hi(y0[j]), centred_hi(y1[j]));
+                        } else {
+                            mma_u8s8_w(acc[j], ua[t], centred8(y0[j]), centred8(y1[j]));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        float val;
+                        if constexpr (ND == 2)
+                            val = (float)(acc[j][x] * 256 + acc[j][2 + x]);
+                        else
+                            val = r < 4 ? fmaf((float)acc[j][x], 65536.0f, (float)acc[j][2 + x])
+                                        : (float)acc[j][x] * 256.0f;
+                        float &dst = facc[(v * NJ + j) * 2 + x];
+                        dst = fmaf(val, fu, dst);
+                    }
+            }
+        }
+        __syncwarp();
+        issue(st);
+        if (++st == G::NST) {
+            st = 0;
+            phase ^= 1u;
+        }
+        const Place was = cur;
+        advance(cur);
+        if (f + 1 == f1 || cur.c == 0) {
+            // ---- the unit's partial record ----
+#pragma unroll
+            for (int lm = 1; lm < 4; lm <<= 1) {
+                L += __shfl_xor_sync(0xffffffffu, L, lm);
+                Z += __shfl_xor_sync(0xffffffffu, Z, lm);
+            }
+            if constexpr (ND == 3) {  // the two lanes of a head hold sums of different digits
+#pragma unroll
+                for (int i = 0; i < G::NF; i++) facc[i] += __shfl_xor_sync(0xffffffffu, facc[i], 16);
+            }
+            if (r < G::HB) {
+                float *rec = records + ((int64_t)w + (int64_t)was.r * upr + was.k) * G::REC;
+                float4 *dst = reinterpret_cast<float4 *>(rec + r * D + q * N);
+#pragma unroll
+                for (int i = 0; i < N / 4; i++)
+                    dst[i] = make_float4(facc[4 * i], facc[4 * i + 1], facc[4 * i + 2], facc[4 * i + 3]);
+                if (q == 0) *reinterpret_cast<float4 *>(rec + G::HB * D + 4 * r) = make_float4(R, L, Z, 0.0f);
+            }
+            fresh = true;
+        }
+    }
+    if (failed) {
+        if (lane == 0) {
+            atomicOr(a.rows.dev_status, kPagesTimeout);
+            // nothing was issued since: let this warp's copies in flight land (bounded)
+            for (int i = 0; i < G::NST; i++)
+                if (pend & (1u << i)) mbar_wait_bounded(bars + i, i < st ? phase ^ 1u : phase);
+        }
+    }
+}
+
+// One CTA per unit, one warp per query head.
+template <typename T, int BITS, int D, int ND>
+__global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
+    pages_merge_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, int warps, const int *prefix,
+                       const float *records) {
+    using G = PGeo<BITS, D, ND>;
+    constexpr int EPL = D / 32;
+    __shared__ float s_x[G::HB][D];
+    const int lane = threadIdx.x & 31, hl = threadIdx.x >> 5;
+    const int upr = a.heads * hblocks;
+    const int u = blockIdx.x, row = u / upr, k = u - row * upr, h = k / hblocks, g = (k - h * hblocks) * G::HB + hl;
+    griddep_launch_dependents();
+    float sg[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; e++) sg[e] = a.wht_scale * a.signs[(int64_t)h * D + lane * EPL + e];
+    griddep_wait();
+    if (g >= a.group) return;
+    const int p0 = prefix[row], n = prefix[row + 1] - p0;
+    float x[EPL], L = 0.0f, Z = 0.0f;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) x[e] = 0.0f;
+    if (n > 0) {
+        const int F = prefix[rows] * upr, W = sharing_warps(F, warps);
+        const int f0 = p0 * upr + k * n;
+        const int w_lo = warp_of_chunk(f0, F, W), w_hi = warp_of_chunk(f0 + n - 1, F, W);
+        const float *base = records + ((int64_t)u + w_lo) * G::REC;
+        const int nrec = w_hi - w_lo + 1;
+        float M = -INFINITY;
+        for (int i = lane; i < nrec; i += 32) M = fmaxf(M, base[(int64_t)i * G::REC + G::HB * D + 4 * hl]);
+        M = warp_max(M);
+        for (int i0 = 0; i0 < nrec; i0 += 32) {
+            float wt = 0.0f;
+            if (i0 + lane < nrec) {
+                const float4 m = *reinterpret_cast<const float4 *>(base + (int64_t)(i0 + lane) * G::REC + G::HB * D + 4 * hl);
+                wt = m.x == -INFINITY ? 0.0f : exp2f(m.x - M);
+                L = fmaf(wt, m.y, L);
+                Z = fmaf(wt, m.z, Z);
+                if (m.x == -INFINITY) L += m.y;  // NaN sums spoil the row
+            }
+            const int cnt = min(32, nrec - i0);
+#pragma unroll 8
+            for (int j = 0; j < cnt; j++) {
+                const float wj = __shfl_sync(0xffffffffu, wt, j);
+                const float *src = base + (int64_t)(i0 + j) * G::REC + hl * D + lane * EPL;
+#pragma unroll
+                for (int e = 0; e < EPL; e++) x[e] = fmaf(wj, src[e], x[e]);
+            }
+        }
+    }
+    L = warp_sum(L);
+    Z = warp_sum(Z);
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    // records hold a lane's sums in its order: entry (q, v, n-tile, column pair) -> dimension
+#pragma unroll
+    for (int e = 0; e < EPL; e++) {
+        const int i = lane * EPL + e, q = i / (D / 4), rest = i % (D / 4);
+        constexpr int NJ = BITS == 4 ? 8 : 4;
+        const int v = rest / (2 * NJ), j = rest / 2 % NJ, col = 2 * q + (rest & 1);
+        const int dim = BITS == 4 ? 2 * (32 * v + 4 * col + (j >> 1)) + (j & 1) : 32 * v + 4 * col + j;
+        s_x[hl][dim] = L != 0.0f ? (x[e] + Z) * inv : 0.0f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < EPL; e++) x[e] = s_x[hl][lane * EPL + e];
+    warp_wht_butterfly<EPL>(x, lane, D);
+    T *dst = static_cast<T *>(a.out) + (((int64_t)(row0 + row) * a.heads + h) * a.group + g) * D + lane * EPL;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) st_from_f32(dst + e, x[e] * sg[e]);
+}
+
+constexpr size_t kPrefixBytes = ((kMaxRows + 1) * sizeof(int) + 255) / 256 * 256;
+
+// Query heads of a unit: as many as one product carries.
+int head_block(int dtype) { return dtype == SA_DTYPE_FLOAT ? 4 : 8; }
+
+int64_t rows_per_launch(int64_t units_per_row) {
+    const int64_t n = kMaxUnits / units_per_row;
+    return n < 1 ? 1 : (n < kMaxRows ? n : kMaxRows);
+}
+
+template <typename T, int BITS, int D, int ND>
+int launch_shape(const PagesAttendArgs &a, void *workspace, cudaStream_t stream) {
+    using G = PGeo<BITS, D, ND>;
+    auto kern = pages_attend_kernel<T, BITS, D, ND>;
+    static int configured[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+        if (e != cudaSuccess) return check_cuda(e, "gqa_paged_attend smem attribute");
+        if (dev >= 0 && dev < 64) __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
+    }
+    const int hblocks = (a.group + G::HB - 1) / G::HB;
+    const int64_t upr = (int64_t)a.heads * hblocks, rows = (int64_t)a.batch * a.seq_len, per = rows_per_launch(upr);
+    const int64_t row_chunks = upr * a.rows.max_pages * G::CPP;
+    int *prefix = static_cast<int *>(workspace);
+    float *records = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPrefixBytes);
+    for (int64_t row0 = 0; row0 < rows;) {
+        int64_t n = rows - row0 < per ? rows - row0 : per;
+        if (n * row_chunks >= ((int64_t)1 << 31)) n = (((int64_t)1 << 31) - 1) / row_chunks;  // chunk indices are ints
+        if (n == 0)
+            return set_error(SA_ERR_UNSUPPORTED, "gqa_paged_attend: rows of %d pages are too long", a.rows.max_pages);
+        cudaLaunchAttribute pdl[1];
+        pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        pdl[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.stream = stream;
+        cfg.attrs = pdl;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3((unsigned)a.sm_count);
+        cfg.blockDim = dim3(kNWP * 32);
+        cfg.dynamicSmemBytes = G::SMEM;
+        int rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, a, (int)row0, (int)n, hblocks, prefix, records),
+                            "gqa_paged_attend launch");
+        count_launch();
+        if (rc != SA_OK) return rc;
+        cfg.gridDim = dim3((unsigned)(n * upr));
+        cfg.blockDim = dim3(32 * G::HB);
+        cfg.dynamicSmemBytes = 0;
+        rc = check_cuda(cudaLaunchKernelEx(&cfg, pages_merge_kernel<T, BITS, D, ND>, a, (int)row0, (int)n, hblocks,
+                                           a.sm_count * kNWP, (const int *)prefix, (const float *)records),
+                        "gqa_paged_attend merge launch");
+        count_launch();
+        if (rc != SA_OK) return rc;
+        row0 += n;
+    }
+    return SA_OK;
+}
+
+template <typename T, int ND>
+int launch_t(const PagesAttendArgs &a, void *workspace, cudaStream_t stream) {
+    if (a.bits == 4)
+        return a.head_dim == 128 ? launch_shape<T, 4, 128, ND>(a, workspace, stream)
+                                 : launch_shape<T, 4, 64, ND>(a, workspace, stream);
+    return a.head_dim == 128 ? launch_shape<T, 8, 128, ND>(a, workspace, stream)
+                             : launch_shape<T, 8, 64, ND>(a, workspace, stream);
+}
+
+}  // namespace
+
+size_t pages_attend_workspace(const kv_pages_impl *k, int batch, int seq_len, int dtype) {
+    const int hb = head_block(dtype);
+    const int64_t upr = (int64_t)k->cfg.kv_head_count * ((k->group + hb - 1) / hb);
+    const int64_t rows = (int64_t)batch * seq_len, per = rows_per_launch(upr), n = rows < per ? rows : per;
+    const int64_t records = (int64_t)k->sm_count * kNWP + n * upr;  // one per warp, and one more per unit
+    return kPrefixBytes + (size_t)records * hb * (k->cfg.head_dim + 4) * sizeof(float);
+}
+
+int launch_pages_attend(const PagesAttendArgs &a, void *workspace, cudaStream_t stream) {
+    switch (a.dtype) {
+        case SA_DTYPE_FLOAT: return launch_t<float, 3>(a, workspace, stream);
+        case SA_DTYPE_FLOAT16: return launch_t<__half, 2>(a, workspace, stream);
+        default: return launch_t<__nv_bfloat16, 2>(a, workspace, stream);
+    }
+}
+
+}  // namespace sa

@@ -241,5 +241,10 @@ int launch_matmul_nbits_packed(const void *a, const void *packed, const void *bi
 void count_launch(int n = 1);
 float host_sqrt_approx(float x);
 float host_sqrt_f32(float x);
+// Seed of a head's signs (CompressedKVCache::new, kv_compression.rs:776-779), and the signs themselves.
+inline uint64_t head_seed(uint64_t seed, int layer, int num_kv_heads, int head) {
+    return seed * 0x9E3779B97F4A7C15ULL + ((uint64_t)layer * (uint64_t)num_kv_heads + (uint64_t)head);
+}
+void make_signs(uint64_t seed, int dim, float *out);
 
 }  // namespace sa

@@ -60,7 +60,7 @@ float host_sqrt_f32(float x) {
 
 // Xorshift64 (kv_compression.rs:44-68) and the PolarQuantizer sign draw
 // (:207-210), seeded per (layer, head) as CompressedKVCache::new (:776-779).
-static void make_signs(uint64_t seed, int dim, float *out) {
+void make_signs(uint64_t seed, int dim, float *out) {
     uint64_t st = seed == 0 ? 0x5EEDDEADBEEFCAFEULL : seed;
     for (int i = 0; i < dim; i++) {
         uint64_t x = st;
@@ -217,9 +217,7 @@ int sa_kv_cache_create(const sa_kv_cache_config *cfg, sa_kv_cache **out) {
         std::vector<float> hs(L * H * D);
         for (size_t l = 0; l < L; l++)
             for (size_t h = 0; h < H; h++) {
-                const uint64_t hseed = c.seed * 0x9E3779B97F4A7C15ULL +
-                                       (uint64_t)(l * (uint64_t)c.num_kv_heads + (uint64_t)(c.kv_head_begin + h));
-                make_signs(hseed, (int)D, &hs[(l * H + h) * D]);
+                make_signs(head_seed(c.seed, (int)l, c.num_kv_heads, c.kv_head_begin + (int)h), (int)D, &hs[(l * H + h) * D]);
             }
         e = cudaMemcpy(k->signs, hs.data(), hs.size() * sizeof(float), cudaMemcpyHostToDevice);
     }

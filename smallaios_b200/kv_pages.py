@@ -1,0 +1,201 @@
+"""A pool of pages of the compressed KV cache, for sequences of different lengths.
+
+Where ``GpuKvCache`` holds a batch of sequences with one position, ``GpuKvPages`` holds pages of 64 tokens, and
+every call names the pages (``page_table``) and lengths (``seq_lens``) of its rows by device tensors.  Pages hold
+the same codes, scales and zero points.  Who owns which page is the caller's business: the pool allocates none.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .kv_cache import DEFAULT_SEED, _view
+
+
+@dataclass
+class PagesView:
+    """One layer's pages as torch tensors (zero-copy, strided: a page's arrays lie side by side)."""
+
+    k_codes: torch.Tensor  # uint8 (P, H, 64, CB)
+    v_codes: torch.Tensor  # uint8 (P, H, 4, CB/4, 4, 4, 4): 16-token blocks, see v_codes_tokens
+    k_meta: torch.Tensor   # f32 (P, H, 64, 2) {scale, zero_point}
+    v_meta: torch.Tensor   # f32 (P, H, 64, 2)
+    signs: torch.Tensor    # f32 (H, D) +-1
+    wht_scale: float
+    bits: int
+    code_bytes: int
+
+    def v_codes_tokens(self) -> torch.Tensor:
+        """V codes in per-token pack_bits order (P, H, 64, CB), as LayerView.v_codes_tokens."""
+        p, h, nblk, c4, g, jj, tt = self.v_codes.shape
+        return self.v_codes.permute(0, 1, 2, 4, 6, 3, 5).reshape(p, h, nblk * g * tt, c4 * jj)
+
+
+def page_rows(op: str, page_table, seq_lens, counts, batch: int):
+    """Checks of a call's rows; (table pointer, its row stride, pages per row, lengths pointer, counts pointer)."""
+    from .ops import ShapeMismatch, UnsupportedOp, _cuda
+
+    if not isinstance(page_table, torch.Tensor) or not page_table.is_cuda:
+        raise TypeError("page_table must be a CUDA tensor")
+    if page_table.dtype != torch.int32:
+        raise UnsupportedOp(f"{op}: page_table must be int32")
+    if page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise ShapeMismatch(f"{op}: page_table must be ({batch}, pages), got {tuple(page_table.shape)}")
+    pages = page_table.shape[1]
+    stride = page_table.stride(0) if batch > 1 else pages
+    if (pages > 1 and page_table.stride(1) != 1) or stride < pages:
+        raise ValueError("page_table must be contiguous, or a slice of columns of a contiguous tensor")
+    _cuda(seq_lens, "seq_lens")
+    _cuda(counts, "counts")
+    for name, t in (("seq_lens", seq_lens), ("counts", counts)):
+        if t is None and name == "counts":
+            continue
+        if t.dtype != torch.int32:
+            raise UnsupportedOp(f"{op}: {name} must be int32")
+        if t.numel() != batch:
+            raise ShapeMismatch(f"{op}: {name} must have {batch} entries, got {t.numel()}")
+    return page_table.data_ptr(), stride, pages, seq_lens.data_ptr(), None if counts is None else counts.data_ptr()
+
+
+def token_strides(op: str, t, width: int, what: str):
+    """(batch stride, token stride) of (B, S, width) vectors, which may be a slice of columns of a wider projection."""
+    from .ops import ShapeMismatch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{what} must be a CUDA tensor")
+    if t.dim() != 3:
+        raise ShapeMismatch(f"{op}: {what} must be rank-3")
+    if t.shape[2] != width:
+        raise ShapeMismatch(f"{op}: hidden size {t.shape[2]} of {what} does not match the pool's heads/head_dim ({width})")
+    b, s, _ = t.shape
+    if t.is_contiguous():
+        return s * width, width
+    token = t.stride(1) if s > 1 else width
+    batch = t.stride(0) if b > 1 else s * token
+    if t.stride(2) != 1 or token < width or batch < width:
+        raise ValueError(f"{what} must have contiguous rows")
+    return batch, token
+
+
+class GpuKvPages:
+    """Pages of every layer's K/V, quantized as ``GpuKvCache`` quantizes them, on one GPU.
+
+    ``num_pages`` pages of 64 tokens per layer; page p of a row's table is page p in all layers.
+    ``kv_head_begin/kv_head_count`` select a shard of the KV heads.  bits 4 or 8, head_dim 64 or 128.
+    """
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, *,
+                 num_heads: int | None = None, bits: int = 4, seed: int = DEFAULT_SEED, kv_head_begin: int = 0,
+                 kv_head_count: int | None = None, device=None):
+        self._handle = ctypes.c_void_p()
+        self.device = torch.device(device if device is not None else "cuda")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        cfg = _lib.KvPagesConfig()
+        cfg.num_layers = num_layers
+        cfg.num_pages = num_pages
+        cfg.num_heads = num_heads if num_heads is not None else num_kv_heads
+        cfg.num_kv_heads = num_kv_heads
+        cfg.kv_head_begin = kv_head_begin
+        cfg.kv_head_count = kv_head_count if kv_head_count is not None else num_kv_heads - kv_head_begin
+        cfg.head_dim = head_dim
+        cfg.bits = bits
+        cfg.seed = seed & (2**64 - 1)
+        with torch.cuda.device(self.device):
+            check(lib.sa_kv_pages_create(ctypes.byref(cfg), ctypes.byref(self._handle)))
+        self.config = cfg
+        self.kv_width = cfg.kv_head_count * head_dim
+        self.query_width = cfg.num_heads // cfg.num_kv_heads * self.kv_width
+        self._workspace_bytes: dict = {}
+
+    @property
+    def handle(self) -> int:
+        if not self._handle:
+            raise RuntimeError("GpuKvPages used after close()")
+        return self._handle.value
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor,
+               seq_lens: torch.Tensor, *, counts: torch.Tensor | None = None, cos_cache=None, sin_cache=None,
+               do_rotary: bool = False, rotary_interleaved: bool = False, stream=None) -> None:
+        """Quantize-on-append of (B, S, H*D) K/V: token s of row b goes to position seq_lens[b] + s
+        (sa_kv_pages_append).
+
+        ``page_table`` int32 (B, pages), ``seq_lens`` int32 (B), on the device: the row's pages, and its tokens
+        before these; a length below 0 leaves a row out.  ``counts`` int32 (B): only the first counts[b] of the S
+        tokens exist.  K is rotated to its position with ``do_rotary``.  ``seq_lens`` is not changed.  Tokens that
+        have no page, or no row in the tables, are left out and reported by ``device_status``.
+        """
+        from .ops import ShapeMismatch, UnsupportedOp, _dtype_code, _raise_op, _rope_tables, _stream_handle
+
+        strides = token_strides("kv_pages_append", key, self.kv_width, "key")
+        if not isinstance(value, torch.Tensor) or value.shape != key.shape:
+            raise ShapeMismatch("kv_pages_append: key and value must be (B, S, H*D) with equal shapes")
+        if value.dtype != key.dtype:
+            raise UnsupportedOp("kv_pages_append: key and value dtypes differ")
+        if token_strides("kv_pages_append", value, self.kv_width, "value") != strides:
+            raise ValueError("key and value must have the same strides")
+        b, s, _ = key.shape
+        table = page_rows("kv_pages_append", page_table, seq_lens, counts, b)
+        rows = _rope_tables(cos_cache, sin_cache)
+        self._check_tables("kv_pages_append", do_rotary, cos_cache, sin_cache)
+        rc = lib.sa_kv_pages_append(self.handle, layer, key.data_ptr(), value.data_ptr(), *strides, _dtype_code(key), b, s,
+                                    *table, None if cos_cache is None else cos_cache.data_ptr(),
+                                    None if sin_cache is None else sin_cache.data_ptr(), rows, int(bool(do_rotary)),
+                                    int(bool(rotary_interleaved)), _stream_handle(stream, self.device))
+        _raise_op(rc, "kv_pages_append")
+
+    def _check_tables(self, op: str, do_rotary, cos_cache, sin_cache) -> None:
+        """cos/sin tables have one column per pair, and as many rows each."""
+        from .ops import ShapeMismatch
+
+        if do_rotary and cos_cache is not None and sin_cache is not None and (
+                cos_cache.shape != sin_cache.shape or cos_cache.shape[1] != self.config.head_dim // 2):
+            raise ShapeMismatch(f"{op}: cos and sin caches must be (rows, {self.config.head_dim // 2})")
+
+    def workspace_bytes(self, batch: int, seq_len: int, dtype_code: int) -> int:
+        """sa_gqa_paged_workspace_bytes."""
+        key = (batch, seq_len, dtype_code)
+        n = self._workspace_bytes.get(key)
+        if n is None:
+            n = self._workspace_bytes[key] = lib.sa_gqa_paged_workspace_bytes(self.handle, batch, seq_len, dtype_code)
+        return n
+
+    def view(self, layer: int) -> PagesView:
+        """The layer's arrays.  The tensors keep the pool alive; ``close()`` ends them all the same."""
+        v = _lib.KvPagesView()
+        check(lib.sa_kv_pages_layer_view(self.handle, layer, ctypes.byref(v)))
+        p, h, cb, d = v.num_pages, v.kv_heads, v.code_bytes, v.head_dim
+        raw = _view(v.records, (p, h, v.record_bytes), "|u1", self)
+
+        def piece(offset, end):
+            return raw[:, :, offset:end]
+
+        return PagesView(k_codes=piece(0, v.k_meta_offset).unflatten(-1, (64, cb)),
+                         v_codes=piece(v.v_codes_offset, v.record_bytes).unflatten(-1, (4, cb // 4, 4, 4, 4)),
+                         k_meta=piece(v.k_meta_offset, v.v_meta_offset).view(torch.float32).unflatten(-1, (64, 2)),
+                         v_meta=piece(v.v_meta_offset, v.v_codes_offset).view(torch.float32).unflatten(-1, (64, 2)),
+                         signs=_view(v.signs, (h, d), "<f4", self), wht_scale=v.wht_scale, bits=v.bits, code_bytes=cb)
+
+    def device_status(self, clear: bool = False) -> int:
+        """Bits of what kernels on this pool met (sa_kv_pages_device_status): 1 a bounded wait gave up, 2 a page
+        outside the pool or the table, 4 a position outside the cos/sin tables, 8 beams that do not match.
+        Synchronises."""
+        st = ctypes.c_int32()
+        check(lib.sa_kv_pages_device_status(self.handle, ctypes.byref(st), int(bool(clear))))
+        return st.value
+
+    def close(self) -> None:
+        if self._handle:
+            with torch.cuda.device(self.device):
+                lib.sa_kv_pages_destroy(self._handle.value)
+            self._handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

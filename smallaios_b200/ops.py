@@ -24,6 +24,7 @@ import torch
 from . import _lib
 from ._lib import lib
 from .kv_cache import GpuKvCache
+from .kv_pages import GpuKvPages, page_rows, token_strides
 
 
 # ---- OpError mirror (onnx-rt/src/operators.rs) ------------------------------
@@ -351,6 +352,43 @@ def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_
                                   float(scale or 0.0), None if workspace is None else workspace.data_ptr(),
                                   0 if workspace is None else workspace.numel(), _stream_handle(stream, query.device))
     _raise_op(rc, "gqa_sparse_attend")
+    return out
+
+
+# ---- paged serving ----------------------------------------------------------------
+def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_table: torch.Tensor,
+                     seq_lens: torch.Tensor, *, num_heads: int, counts: torch.Tensor | None = None,
+                     scale: float | None = None, do_rotary: bool = False, rotary_interleaved: bool = False,
+                     cos_cache=None, sin_cache=None, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of new tokens over pages (sa_gqa_paged_attend): the decode step of rows of any lengths.
+
+    ``query`` (B, S, Hq*D); token s of row b sits at position seq_lens[b] + s, where its own key and value have been
+    appended (``GpuKvPages.append``), and attends to all of the row's tokens up to itself.  ``page_table``,
+    ``seq_lens`` and ``counts`` as for append; the query is rotated with ``do_rotary``.  Rows without tokens and
+    tokens that do not exist give zeros.  A row's pages are read once per new token: S is one, or a few.
+    ``workspace``: uint8, at least ``pages.workspace_bytes`` bytes; allocated when not given.
+    """
+    strides = token_strides("gqa_paged_attend", query, pages.query_width, "query")
+    b, s, _ = query.shape
+    code = _dtype_code(query)
+    table = page_rows("gqa_paged_attend", page_table, seq_lens, counts, b)
+    rows = _rope_tables(cos_cache, sin_cache)
+    pages._check_tables("gqa_paged_attend", do_rotary, cos_cache, sin_cache)
+    if out is None:
+        out = _empty(query.shape, query.dtype, query.device, stream)
+    else:
+        _cuda(out, "out")
+        if out.shape != query.shape or out.dtype != query.dtype:
+            raise ShapeMismatch("gqa_paged_attend: out must have query's shape and dtype")
+    workspace = _workspace(workspace, pages.workspace_bytes(b, s, code), query.device, stream)
+    rc = lib.sa_gqa_paged_attend(pages.handle, layer, query.data_ptr(), *strides, out.data_ptr(), code, b, s,
+                                 int(num_heads), int(scale is not None), float(scale or 0.0), *table,
+                                 None if cos_cache is None else cos_cache.data_ptr(),
+                                 None if sin_cache is None else sin_cache.data_ptr(), rows, int(bool(do_rotary)),
+                                 int(bool(rotary_interleaved)), None if workspace is None else workspace.data_ptr(),
+                                 0 if workspace is None else workspace.numel(), _stream_handle(stream, query.device))
+    _raise_op(rc, "gqa_paged_attend")
     return out
 
 
