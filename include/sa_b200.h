@@ -648,6 +648,43 @@ int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, in
                         const float *cos_cache, const float *sin_cache, int32_t cache_rows, int32_t do_rotary,
                         int32_t rotary_interleaved, void *workspace, int64_t workspace_bytes, sa_stream_t stream);
 
+/* Beam search, selection: the `keep` best continuations of each group's
+ * num_beams beams over the whole vocabulary.  Continuation (k, v) of a group:
+ *   score[k] + (logits[k][v] - log sum_u exp logits[k][u])
+ * and of a finished beam (finished[k] != 0) the single one (k, end_token) with
+ * score[k].  Order: larger scores first, of equal ones the lower k * vocab + v;
+ * NaN and -inf are never chosen (a beam whose logits hold NaN or +inf, or only
+ * -inf, offers nothing).  Scores are compared in 64 bits; the logarithm is off by
+ * some 1e-8 (its sum is taken in 32 bits, then 64).
+ *   logits    (batch * num_beams, vocab) of dtype, rows row_stride apart
+ *   scores    f32 (batch, num_beams); finished: NULL or uint8 (batch, num_beams)
+ *   parents, tokens int32, out_scores f32: (batch, keep); -1, -1, -inf behind the
+ *             last continuation.  num_beams <= SA_MAX_BEAMS, keep <= SA_MAX_BEAM_KEEP,
+ *             num_beams * vocab < 2^31; end_token outside [0, vocab) offers none.
+ * `workspace` as for sa_gqa_paged_attend. */
+int64_t sa_beam_select_workspace_bytes(int32_t batch, int32_t num_beams, int64_t vocab);
+int sa_beam_select(const void *logits, int64_t row_stride, int32_t dtype, const float *scores,
+                   const uint8_t *finished, int32_t batch, int32_t num_beams, int64_t vocab, int32_t end_token,
+                   int32_t keep, int32_t *parents, int32_t *tokens, float *out_scores, void *workspace,
+                   int64_t workspace_bytes, sa_stream_t stream);
+
+/* Beam search, states: beam i of group b (row b * num_beams + i of the table)
+ * goes on as beam parents[b][i] was.  The num_beams beams of a group have one
+ * length n = seq_lens[b * num_beams + i].  Their n / 64 full pages may be shared;
+ * the page in use and the pages behind it must be each beam's own.
+ *   - new_table[i][j] = page_table[parent][j] for the full pages j < n / 64;
+ *   - page in use (n % 64 > 0): of the beams that continue one parent, the one in
+ *     the parent's own slot takes its page over, else the first; each further one
+ *     takes the page of a beam that nobody continues (in ascending order) and the
+ *     parent's n % 64 tokens are copied there in every layer;
+ *   - the pages behind stay where they are.
+ * parents: int32 (batch, num_beams); -1 = the beam stays as it is.  new_table (its
+ * own memory, rows new_stride apart) must not overlap page_table.  Full pages that
+ * no row names any more are free for the caller to use. */
+int sa_kv_pages_reorder(sa_kv_pages *pages, const int32_t *page_table, int64_t table_stride, int32_t *new_table,
+                        int64_t new_stride, int32_t max_pages, const int32_t *seq_lens, const int32_t *parents,
+                        int32_t batch, int32_t num_beams, sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

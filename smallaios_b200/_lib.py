@@ -41,6 +41,7 @@ EXPORTED = [
     "sa_gqa_select_blocks", "sa_gqa_sparse_workspace_bytes", "sa_gqa_sparse_attend",
     "sa_kv_pages_create", "sa_kv_pages_destroy", "sa_kv_pages_get_config", "sa_kv_pages_layer_view",
     "sa_kv_pages_device_status", "sa_kv_pages_append", "sa_gqa_paged_workspace_bytes", "sa_gqa_paged_attend",
+    "sa_beam_select_workspace_bytes", "sa_beam_select", "sa_kv_pages_reorder",
 ]
 SA_MAX_DRAFT_NODES = 64
 SA_BLOCK_TOKENS = 64
@@ -220,6 +221,12 @@ def _declare(l: ctypes.CDLL) -> None:
     l.sa_gqa_paged_attend.restype = ctypes.c_int
     l.sa_gqa_paged_attend.argtypes = [_P, _I32, _P, _I64, _I64, _P, _I32, _I32, _I32, _I64, _I32, _F, _P, _I64, _I32, _P,
                                       _P, _P, _P, _I32, _I32, _I32, _P, _I64, _P]
+    l.sa_beam_select_workspace_bytes.restype = _I64
+    l.sa_beam_select_workspace_bytes.argtypes = [_I32, _I32, _I64]
+    l.sa_beam_select.restype = ctypes.c_int
+    l.sa_beam_select.argtypes = [_P, _I64, _I32, _P, _P, _I32, _I32, _I64, _I32, _I32, _P, _P, _P, _P, _I64, _P]
+    l.sa_kv_pages_reorder.restype = ctypes.c_int
+    l.sa_kv_pages_reorder.argtypes = [_P, _P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P]
     l.sa_qkv_project_append.restype = ctypes.c_int
     l.sa_qkv_project_append.argtypes = [_P, _I32, _P, _P, _P, _I32, _I32, _I64, _P, _P, _I32, _I32, _I32, _P, _P,
                                         _P, _P]

@@ -1,6 +1,6 @@
-// C entry points of paged serving: the page pool, appending to pages and
-// attention over pages (argument checks; the kernels are in
-// kv_pages_append.cu and gqa_pages.cu).
+// C entry points of paged serving: the page pool, appending to pages,
+// attention over pages, and beam search (argument checks; the kernels are in
+// kv_pages_append.cu, gqa_pages.cu, beam_select.cu and kv_pages_reorder.cu).
 #include <stdlib.h>
 #include <string.h>
 
@@ -262,6 +262,95 @@ int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, in
     a.rows = page_rows(k, page_table, table_stride, max_pages, seq_lens, counts);
     a.rope = RopeArgs{cos_cache, sin_cache, cache_rows, do_rotary != 0, rotary_interleaved != 0};
     return launch_pages_attend(a, workspace, static_cast<cudaStream_t>(stream));
+}
+
+int64_t sa_beam_select_workspace_bytes(int32_t batch, int32_t num_beams, int64_t vocab) {
+    if (batch <= 0 || num_beams <= 0 || num_beams > SA_MAX_BEAMS || vocab <= 0 || vocab * num_beams > INT32_MAX) return 0;
+    return beam_select_workspace((int64_t)batch * num_beams, vocab);
+}
+
+int sa_beam_select(const void *logits, int64_t row_stride, int32_t dtype, const float *scores, const uint8_t *finished,
+                   int32_t batch, int32_t num_beams, int64_t vocab, int32_t end_token, int32_t keep, int32_t *parents,
+                   int32_t *tokens, float *out_scores, void *workspace, int64_t workspace_bytes, sa_stream_t stream) {
+    if (!dtype_ok(dtype)) return set_error(SA_ERR_UNSUPPORTED, "beam_select: dtype %d not supported", dtype);
+    if (batch < 0) return set_error(SA_ERR_SHAPE_MISMATCH, "beam_select: negative batch");
+    if (num_beams < 1 || num_beams > SA_MAX_BEAMS)
+        return set_error(SA_ERR_INVALID_ATTRIBUTE, "beam_select: %d beams (1..%d)", num_beams, SA_MAX_BEAMS);
+    if (keep < 1 || keep > SA_MAX_BEAM_KEEP)
+        return set_error(SA_ERR_INVALID_ATTRIBUTE, "beam_select: keep %d (1..%d)", keep, SA_MAX_BEAM_KEEP);
+    if (vocab < 1 || row_stride < vocab)
+        return set_error(SA_ERR_SHAPE_MISMATCH, "beam_select: rows of %lld tokens, %lld apart", (long long)vocab,
+                         (long long)row_stride);
+    if (vocab > INT32_MAX / num_beams || batch > INT32_MAX / num_beams)
+        return set_error(SA_ERR_UNSUPPORTED, "beam_select: %d x %d beams over %lld tokens", batch, num_beams,
+                         (long long)vocab);
+    if (batch == 0) return SA_OK;
+    if (!logits || !scores || !parents || !tokens || !out_scores)
+        return set_error(SA_ERR_INVALID_ARGUMENT, "beam_select: NULL argument");
+    if (reinterpret_cast<uintptr_t>(logits) % (dtype == SA_DTYPE_FLOAT ? 4 : 2))
+        return set_error(SA_ERR_INVALID_ARGUMENT, "beam_select: logits must be aligned to their elements");
+    const int64_t need = sa_beam_select_workspace_bytes(batch, num_beams, vocab);
+    if (!workspace || workspace_bytes < need)
+        return set_error(SA_ERR_INVALID_ARGUMENT, "beam_select: workspace of %lld bytes, needs %lld",
+                         workspace ? (long long)workspace_bytes : 0ll, (long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return set_error(SA_ERR_INVALID_ARGUMENT, "beam_select: workspace must be 256-byte aligned");
+    BeamArgs a{};
+    a.logits = logits;
+    a.row_stride = row_stride;
+    a.dtype = dtype;
+    a.batch = batch;
+    a.beams = num_beams;
+    a.keep = keep;
+    a.end_token = end_token;
+    a.vocab = (int)vocab;
+    a.scores = scores;
+    a.finished = finished;
+    a.parents = parents;
+    a.tokens = tokens;
+    a.out_scores = out_scores;
+    return launch_beam_select(a, workspace, static_cast<cudaStream_t>(stream));
+}
+
+int sa_kv_pages_reorder(sa_kv_pages *pages, const int32_t *page_table, int64_t table_stride, int32_t *new_table,
+                        int64_t new_stride, int32_t max_pages, const int32_t *seq_lens, const int32_t *parents,
+                        int32_t batch, int32_t num_beams, sa_stream_t stream) {
+    if (!pages) return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_reorder: NULL pages");
+    const kv_pages_impl *k = impl(pages);
+    if (batch < 0) return set_error(SA_ERR_SHAPE_MISMATCH, "kv_pages_reorder: negative batch");
+    if (num_beams < 1 || num_beams > SA_MAX_BEAMS)
+        return set_error(SA_ERR_INVALID_ATTRIBUTE, "kv_pages_reorder: %d beams (1..%d)", num_beams, SA_MAX_BEAMS);
+    if (max_pages < 0 || max_pages > INT32_MAX / kPageTokens || table_stride < max_pages || new_stride < max_pages)
+        return set_error(SA_ERR_SHAPE_MISMATCH, "kv_pages_reorder: table rows of %d pages, %lld and %lld apart", max_pages,
+                         (long long)table_stride, (long long)new_stride);
+    if (batch > 65535 || k->cfg.num_layers > 65535)
+        return set_error(SA_ERR_UNSUPPORTED, "kv_pages_reorder: %d groups, %d layers", batch, k->cfg.num_layers);
+    if (batch == 0 || max_pages == 0) return SA_OK;
+    if (!page_table || !new_table || !seq_lens || !parents)
+        return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_reorder: NULL argument");
+    const int64_t rows = (int64_t)batch * num_beams;
+    const int32_t *end = page_table + (rows - 1) * table_stride + max_pages;
+    const int32_t *new_end = new_table + (rows - 1) * new_stride + max_pages;
+    if (page_table < new_end && new_table < end)
+        return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_reorder: the new table overlaps the old one");
+    ReorderArgs a{};
+    a.records = k->records;
+    a.layer_bytes = k->layer_bytes;
+    a.layers = k->cfg.num_layers;
+    a.heads = k->cfg.kv_head_count;
+    a.code_bytes = k->code_bytes;
+    a.table = page_table;
+    a.table_stride = table_stride;
+    a.out = new_table;
+    a.out_stride = new_stride;
+    a.max_pages = max_pages;
+    a.lens = seq_lens;
+    a.parents = parents;
+    a.batch = batch;
+    a.beams = num_beams;
+    a.num_pages = k->cfg.num_pages;
+    a.dev_status = k->dev_status;
+    return launch_pages_reorder(a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -75,6 +75,38 @@ struct PagesAttendArgs {
     RopeArgs rope;
 };
 
+// Beam selection (sa_beam_select).
+struct BeamArgs {
+    const void *logits;
+    int64_t row_stride;
+    int dtype, batch, beams, keep, end_token;
+    int vocab;
+    const float *scores;
+    const uint8_t *finished;  // nullptr: none
+    int32_t *parents, *tokens;
+    float *out_scores;
+    int sm_count;
+};
+
+// Beams over pages (sa_kv_pages_reorder).
+struct ReorderArgs {
+    uint8_t *records;  // [L][P][H][record]
+    size_t layer_bytes;
+    int layers, heads, code_bytes;
+    const int32_t *table;
+    int64_t table_stride;
+    int32_t *out;
+    int64_t out_stride;
+    int max_pages;
+    const int32_t *lens, *parents;
+    int batch, beams;
+    int num_pages;
+    int *dev_status;
+};
+
+int64_t beam_select_workspace(int64_t rows, int64_t vocab);
+int launch_beam_select(const BeamArgs &a, void *workspace, cudaStream_t stream);
+int launch_pages_reorder(const ReorderArgs &a, cudaStream_t stream);
 int launch_pages_append(const PagesAppendArgs &a, cudaStream_t stream);
 size_t pages_attend_workspace(const kv_pages_impl *k, int batch, int seq_len, int dtype);
 int launch_pages_attend(const PagesAttendArgs &a, void *workspace, cudaStream_t stream);

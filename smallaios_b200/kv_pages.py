@@ -156,6 +156,35 @@ class GpuKvPages:
                 cos_cache.shape != sin_cache.shape or cos_cache.shape[1] != self.config.head_dim // 2):
             raise ShapeMismatch(f"{op}: cos and sin caches must be (rows, {self.config.head_dim // 2})")
 
+    def reorder_beams(self, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, *,
+                      out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """The beams' new page table, and copies of the pages that several of them go on filling, in every layer
+        (sa_kv_pages_reorder).
+
+        ``parents`` int32 (B, K): beam i of group b (row b*K + i) goes on as beam parents[b, i] was; -1: it stays.
+        ``page_table`` int32 (B*K, pages), ``seq_lens`` int32 (B*K), equal within a group.  Full pages may be shared
+        by rows; a row's page in use and the pages behind it must be its own.  ``out`` must not overlap
+        ``page_table``.
+        """
+        from .ops import ShapeMismatch, UnsupportedOp, _cuda, _empty, _raise_op, _stream_handle
+
+        _cuda(parents, "parents")
+        if parents.dim() != 2:
+            raise ShapeMismatch("reorder_beams: parents must be (B, K)")
+        if parents.dtype != torch.int32:
+            raise UnsupportedOp("reorder_beams: parents must be int32")
+        b, k = parents.shape
+        table, stride, width, lens, _ = page_rows("reorder_beams", page_table, seq_lens, None, b * k)
+        if out is None:
+            out = _empty(page_table.shape, torch.int32, page_table.device, stream)
+        elif out.shape != page_table.shape:
+            raise ShapeMismatch("reorder_beams: out must have page_table's shape")
+        new, new_stride, _, _, _ = page_rows("reorder_beams", out, seq_lens, None, b * k)
+        rc = lib.sa_kv_pages_reorder(self.handle, table, stride, new, new_stride, width, lens, parents.data_ptr(), b, k,
+                                     _stream_handle(stream, self.device))
+        _raise_op(rc, "reorder_beams")
+        return out
+
     def workspace_bytes(self, batch: int, seq_len: int, dtype_code: int) -> int:
         """sa_gqa_paged_workspace_bytes."""
         key = (batch, seq_len, dtype_code)

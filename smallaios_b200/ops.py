@@ -392,6 +392,47 @@ def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_ta
     return out
 
 
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.Tensor | None = None,
+                end_token: int = -1, keep: int | None = None, workspace: torch.Tensor | None = None, stream=None):
+    """The best continuations of each group of beams (sa_beam_select): ``(parents, tokens, scores)``, each (B, keep).
+
+    ``logits`` (B*K, V), rows may be slices of wider ones; ``scores`` f32 (B, K), the beams' sums of log
+    probabilities.  Continuation (k, v) scores ``scores[b, k] + log_softmax(logits[b*K + k])[v]``; a beam marked in
+    ``finished`` (bool or uint8 (B, K)) has the single continuation ``end_token`` with its own score.  Best first,
+    of equal scores the lower k*V + v; -1, -1, -inf behind the last.  ``keep`` defaults to K.
+    """
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise TypeError("logits must be a CUDA tensor")
+    _cuda(scores, "scores")
+    _cuda(finished, "finished")
+    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
+        raise ShapeMismatch("beam_select: logits must be (B*K, V) of scores (B, K)")
+    if scores.dtype != torch.float32:
+        raise UnsupportedOp("beam_select: scores must be float32")
+    b, k = scores.shape
+    rows, vocab = logits.shape
+    stride = logits.stride(0) if rows > 1 else vocab
+    if (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+        raise ValueError("logits must have contiguous rows")
+    if finished is not None:
+        if finished.dtype not in (torch.bool, torch.uint8):
+            raise UnsupportedOp("beam_select: finished must be bool or uint8")
+        if finished.shape != scores.shape:
+            raise ShapeMismatch("beam_select: finished must have scores' shape")
+    keep = k if keep is None else int(keep)
+    code = _dtype_code(logits)
+    out = _empty((3, b, max(keep, 0)), torch.int32, logits.device, stream)
+    parents, tokens, best = out[0], out[1], out[2].view(torch.float32)
+    workspace = _workspace(workspace, lib.sa_beam_select_workspace_bytes(b, k, vocab), logits.device, stream)
+    rc = lib.sa_beam_select(logits.data_ptr(), stride, code, scores.data_ptr(),
+                            None if finished is None else finished.data_ptr(), b, k, vocab, int(end_token), keep,
+                            parents.data_ptr(), tokens.data_ptr(), best.data_ptr(),
+                            None if workspace is None else workspace.data_ptr(),
+                            0 if workspace is None else workspace.numel(), _stream_handle(stream, logits.device))
+    _raise_op(rc, "beam_select")
+    return parents, tokens, best
+
+
 def matmul_nbits(a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor | None = None,
                  bias: torch.Tensor | None = None, *, K: int, N: int, bits: int = 4, block_size: int = 32,
                  out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
