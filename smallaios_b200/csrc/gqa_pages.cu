@@ -28,8 +28,7 @@
 // (8 or 128), their zero points raised by as much, so that the large common part of
 // q'.c and of X need not cancel after both were rounded.
 //
-// Products are exact integers; the int8 MMAs, one ex2 and some fifteen other
-// instructions per (head pair, token) fit below the copy time of a chunk.
+// Products are exact integers.
 //
 // pages_merge_kernel: per unit, the sum of its warps' partial records, the
 // division, the inverse rotation and the store.
@@ -61,37 +60,91 @@ struct PGeo {
     static constexpr int VV = KB / 32;              // 16-byte V loads per 16-token block
     static constexpr int NF = D / 4;                // value sums per lane
     static constexpr int REC = HB * (D + 4);        // floats per partial record: values, then R, L, Z (and padding)
+    static constexpr int PREP = 32 * (NCH + 1);     // 16-byte words of a unit's query digits and score constants
     static constexpr int SMEM = kNWP * NST * STAGE + kNWP * NST * 8;
-    static constexpr float UMAX = ND == 2 ? 65535.0f : 16777215.0f;
     static constexpr float LOG2UMAX = ND == 2 ? 15.99997798605f : 23.99999991400867f;
     static constexpr int QMAX = ND == 2 ? 32639 : 8355711;  // 127 in the top digit
-    static constexpr float CENTRE = BITS == 4 ? 8.0f : 128.0f;
-    static constexpr float UNIT = BITS == 4 ? 0.0625f : 1.0f;  // 4-bit codes enter the products as 16 (c - 8)
+    static constexpr float CENTRE = BITS == 4 ? 8.0f : 128.0f;  // the codes' middle, which the products leave out
+    static constexpr float UNIT = BITS == 4 ? 0.0625f : 1.0f;  // high nibbles enter the products as 16 (c - 8)
     static_assert(SMEM + (kMaxRows + 1) * 4 + 256 <= 227 * 1024, "shared memory");
 };
 
-__device__ __forceinline__ void mma_s8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a.b + c, signed or unsigned digits times signed codes; c may be constant (the first product of a sum).
+__device__ __forceinline__ void mma_s8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1,
+                                         int c2, int c3) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 
-__device__ __forceinline__ void mma_u8s8_w(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1,
+                                         int c2, int c3) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 
-// Codes of a word as signed bytes less their middle: of 8 bits, or 16 times the low / high nibbles.
-__device__ __forceinline__ uint32_t centred8(uint32_t w) { return w ^ 0x80808080u; }
-__device__ __forceinline__ uint32_t centred_lo(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) ^ 0x80808080u; }
-__device__ __forceinline__ uint32_t centred_hi(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
+__device__ __forceinline__ void mma_u8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1,
+                                         int c2, int c3) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+}
 
-// Where a range is: chunk c of unit k of row r, whose units have n chunks.
+// Codes of a word as signed bytes: 8-bit ones less 128; 16 times the high nibbles less 8; the low nibbles as they are
+// (taking 8 off a low nibble in place costs a shift more: their sums start at -8 times the digits' sum instead).
+__device__ __forceinline__ uint32_t codes8(uint32_t w) { return w ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return w & 0x0F0F0F0Fu; }
+
+// Sums start at the bits of the float 1.5 * 2^23: while a sum's magnitude stays below 2^22 (the largest, 64 tokens or
+// 128 dimensions of 255 * 128, is 2.1e6) its bits are those of 1.5 * 2^23 plus the sum, and a float subtraction makes
+// the number of it where a conversion would take the integer pipe that the unpacking of codes already fills.
+constexpr int kMagicBits = 0x4B400000;
+constexpr float kMagic = 12582912.0f;
+
+// Pairs of floats.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float x, float y) {
+    f2 v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ f2 pair_bits(int x, int y) { return pair(__int_as_float(x), __int_as_float(y)); }
+__device__ __forceinline__ void split(f2 v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 x, f2 y) {
+    f2 v;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ f2 mul2(f2 x, f2 y) {
+    f2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ f2 fma2(f2 x, f2 y, f2 z) {
+    f2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+constexpr uint32_t kOnes = 0x01010101u;
+
+// A weight as a whole number up to `most`: of 16 bits the conversion saturates by itself.
+template <int ND>
+__device__ __forceinline__ uint32_t weight_digits(float u) {
+    if constexpr (ND == 2) {
+        uint16_t x;
+        asm("cvt.rni.u16.f32 %0, %1;\n" : "=h"(x) : "f"(u));
+        return x;
+    } else {
+        return __float2uint_rn(fminf(u, 16777215.0f));
+    }
+}
+
+// Where a range is: chunk c of unit (KV head h, block hb of its query heads) of row r, whose units have n chunks;
+// b: the row's sequence.
 struct Place {
-    int r, k, c, n;
+    int r, h, hb, c, n, b;
 };
 
 // Tokens that query row r (row0 + r of batch x seq_len) attends to.
@@ -112,13 +165,135 @@ __device__ __forceinline__ int visible(const PagesAttendArgs &a, int row, bool r
     return (int)pos + 1;
 }
 
-// Warps that share F chunks: at least two chunks each, so that a warp's copies overlap its work and half the
-// partial records are left to merge.
-__host__ __device__ __forceinline__ int sharing_warps(int F, int warps) { return min(warps, (F + 1) / 2); }
+// Warps that share F chunks.
+__host__ __device__ __forceinline__ int sharing_warps(int F, int warps) { return min(warps, F); }
+
+// One warp per unit: its query heads, rotated to their position and into the pages' frame, as digits arranged as the
+// A fragments of the scores' product; lane (r, q) holds a quarter of head r (of r & 3 where heads have three digits).
+// Units of rows without tokens are left out.
+template <typename T, int BITS, int D, int ND>
+__global__ void __launch_bounds__(64) pages_prep_kernel(PagesAttendArgs a, int row0, int units, int hblocks, uint4 *qprep) {
+    using G = PGeo<BITS, D, ND>;
+    constexpr int N = D / 4;
+    const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+    const int u = blockIdx.x * 2 + (threadIdx.x >> 5), upr = a.heads * hblocks;
+    // The attention kernel starts when all warps here have passed the wait: what the kernels before this one wrote
+    // (pages, table, lengths) is there for it, too, and only the digits are left to wait for.
+    griddep_wait();
+    griddep_launch_dependents();
+    if (u >= units) return;
+    const int row = u / upr, k = u - row * upr, h = k / hblocks, b = (row0 + row) / a.seq_len, s = row0 + row - b * a.seq_len;
+    if (visible(a, row0 + row, false) == 0) return;
+    const int g = (k - h * hblocks) * G::HB + (ND == 2 ? r : (r & 3));
+    const bool on = g < a.group;
+    float x[N];
+    if (on) {
+        const T *src = static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
+                       ((int64_t)h * a.group + g) * D + q * N;
+        load_run<T, N>(src, a.aligned, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = 0.0f;
+    }
+    float sg[N];
+    load_run<float, N>(a.signs + (int64_t)h * D + q * N, true, sg);
+    if (a.rope.on) {
+        const int64_t pos = (int64_t)a.rows.lens[b] + s;
+        if (a.rope.interleaved) {
+            float cs[N / 2], sn[N / 2];
+            load_run<float, N / 2>(a.rope.cos_cache + pos * (D / 2) + q * (N / 2), a.rope.aligned, cs);
+            load_run<float, N / 2>(a.rope.sin_cache + pos * (D / 2) + q * (N / 2), a.rope.aligned, sn);
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                x[2 * i] = __fsub_rn(__fmul_rn(cs[i], x0), __fmul_rn(sn[i], x1));
+                x[2 * i + 1] = __fadd_rn(__fmul_rn(sn[i], x0), __fmul_rn(cs[i], x1));
+            }
+        } else {
+            // the partner of dimension d is d +- D/2, the lane two away
+            float cs[N], sn[N];
+            load_run<float, N>(a.rope.cos_cache + pos * (D / 2) + (q & 1) * N, a.rope.aligned, cs);
+            load_run<float, N>(a.rope.sin_cache + pos * (D / 2) + (q & 1) * N, a.rope.aligned, sn);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float other = __shfl_xor_sync(0xffffffffu, x[i], 2);
+                const float own = __fmul_rn(cs[i], x[i]), cross = __fmul_rn(sn[i], other);
+                x[i] = (q & 2) ? __fadd_rn(cross, own) : __fsub_rn(own, cross);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] *= sg[i];
+#pragma unroll
+    for (int hs = 1; hs < N; hs <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if ((i & hs) == 0) {
+                const float p0 = x[i], p1 = x[i + hs];
+                x[i] = p0 + p1;
+                x[i + hs] = p0 - p1;
+            }
+#pragma unroll
+    for (int lm = 1; lm < 4; lm <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float other = __shfl_xor_sync(0xffffffffu, x[i], lm);
+            x[i] = (q & lm) ? other - x[i] : x[i] + other;
+        }
+    float sum = 0.0f, mabs = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        x[i] *= a.wht_scale;
+        sum += x[i];
+        mabs = fmaxf(mabs, fabsf(x[i]));
+    }
+#pragma unroll
+    for (int lm = 1; lm < 4; lm <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, lm);
+        mabs = fmaxf(mabs, __shfl_xor_sync(0xffffffffu, mabs, lm));
+    }
+    const float sigma = mabs > 0.0f ? mabs / (float)G::QMAX : 1.0f;
+    const float inv = 1.0f / sigma, sl2 = a.scale * kLog2eF;
+    uint32_t qa[G::NCH][4];
+#pragma unroll
+    for (int kk = 0; kk < G::NCH; kk++) {
+        qa[kk][0] = qa[kk][1] = qa[kk][2] = qa[kk][3] = 0u;
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // byte e of k-group hf: the dimension as the K words hold it.  8 bits: words 2k, 2k + 1;
+                // 4 bits: low nibbles of words 2k, 2k + 1 (first half of the steps), then high ones
+                constexpr int kHalf = G::NCH / 2;
+                const int i = BITS == 4 ? 16 * (kk % kHalf) + 8 * hf + 2 * e + kk / kHalf : 8 * kk + 4 * hf + e;
+                const int v = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
+                const int d2 = (int)(int8_t)(v & 0xff), rest = (v - d2) >> 8;
+                if constexpr (ND == 2) {
+                    qa[kk][2 * hf] |= ((uint32_t)rest & 0xffu) << (8 * e);
+                    qa[kk][2 * hf + 1] |= ((uint32_t)d2 & 0xffu) << (8 * e);
+                } else {
+                    const int d1 = (int)(int8_t)(rest & 0xff), d0 = (rest - d1) >> 8;
+                    qa[kk][2 * hf] |= ((uint32_t)(r < 4 ? d0 : d1) & 0xffu) << (8 * e);
+                    qa[kk][2 * hf + 1] |= (r < 4 ? (uint32_t)d2 & 0xffu : 0u) << (8 * e);
+                }
+            }
+    }
+    int ones[4] = {0, 0, 0, 0};  // 4 bits: the sums of the rows' digits over the even dimensions
+    if constexpr (BITS == 4) {
+        mma_s8s8(ones, qa[0], kOnes, kOnes, 0, 0, 0, 0);
+        if constexpr (G::NCH == 4) mma_s8s8(ones, qa[1], kOnes, kOnes, ones[0], ones[1], ones[2], ones[3]);
+    }
+    uint4 *dst = qprep + (int64_t)u * G::PREP + lane;
+#pragma unroll
+    for (int kk = 0; kk < G::NCH; kk++) dst[32 * kk] = make_uint4(qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3]);
+    dst[32 * G::NCH] = make_uint4(__float_as_uint(sigma * sl2 * G::UNIT), __float_as_uint(sum * sl2),
+                                  (uint32_t)(kMagicBits - 8 * ones[0]), (uint32_t)(kMagicBits - 8 * ones[2]));
+}
 
 template <typename T, int BITS, int D, int ND>
 __global__ void __launch_bounds__(kNWP * 32, 1)
-    pages_attend_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, int *prefix_out, float *records) {
+    pages_attend_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, const uint4 *qprep, int *prefix_out,
+                        float *records) {
     using G = PGeo<BITS, D, ND>;
     constexpr int KB = G::KB, CT = G::CT, N = D / 4;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -132,7 +307,6 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         for (int i = 0; i < G::NST; i++) mbar_init(bars + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     griddep_launch_dependents();
-    griddep_wait();  // pages, table, lengths and the query may come from the kernels before
 
     // prefix sums of the rows' chunks
     {
@@ -179,15 +353,19 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         }
         cur.r = lo;
         cur.n = s_prefix[lo + 1] - s_prefix[lo];
-        const int off = f0 - s_prefix[lo] * upr;
-        cur.k = off / cur.n;
-        cur.c = off - cur.k * cur.n;
+        const int off = f0 - s_prefix[lo] * upr, k = off / cur.n;
+        cur.c = off - k * cur.n;
+        cur.h = k / hblocks;
+        cur.hb = k - cur.h * hblocks;
+        cur.b = (row0 + lo) / a.seq_len;
     }
     auto advance = [&](Place &p) {
         if (++p.c < p.n) return;
         p.c = 0;
-        if (++p.k < upr) return;
-        p.k = 0;
+        if (++p.hb < hblocks) return;
+        p.hb = 0;
+        if (++p.h < a.heads) return;
+        p.h = 0;
         do {
             if (++p.r >= rows) {  // past the last chunk: never used again
                 p.r = rows - 1;
@@ -195,10 +373,9 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
             }
             p.n = s_prefix[p.r + 1] - s_prefix[p.r];
         } while (p.n == 0);
+        p.b = (row0 + p.r) / a.seq_len;
     };
-    auto page_of = [&](const Place &p) {
-        return a.rows.table[(int64_t)((row0 + p.r) / a.seq_len) * a.rows.table_stride + p.c / G::CPP];
-    };
+    auto page_of = [&](const Place &p) { return __ldcg(a.rows.table + (int64_t)p.b * a.rows.table_stride + p.c / G::CPP); };
 
     // copies run NST chunks ahead; the page of the next chunk to copy is fetched one step before
     Place ahead = cur;
@@ -216,7 +393,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                 }
             } else {
                 bad &= ~(1u << st);
-                const uint8_t *rec = a.records + ((int64_t)page * a.heads + ahead.k / hblocks) * page_record(KB);
+                const uint8_t *rec = a.records + ((int64_t)page * a.heads + ahead.h) * page_record(KB);
                 unsigned char *dst = ring + st * G::STAGE;
                 if (lane == 0) mbar_expect_tx(bar, G::STAGE);
                 if constexpr (G::CPP == 1) {
@@ -243,115 +420,221 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
     };
 #pragma unroll
     for (int i = 0; i < G::NST; i++) issue(i);
+    griddep_wait();  // the prep kernel's digits (it had waited for everything before it)
 
-    uint32_t qa[G::NCH][4];       // query digits, A fragments
-    float c1 = 0.0f, c2 = 0.0f;   // score constants of the lane's head
-    float facc[G::NF];            // value sums in the frame of R
+    uint32_t qa[G::NCH][4];       // query digits, A fragments; 4 bits: of even dimensions, then of odd ones
+    int qlo0 = 0, qlo1 = 0;       // 4 bits: where sums over even dimensions start, -8 times the digits' sum
+    float c1 = 0.0f, c2 = 0.0f, c3 = 0.0f;  // score constants of the lane's head
+    // what the digit in the accumulators' upper rows counts, beside 1 for the one in the lower rows
+    const float wtop = ND == 3 && r < 4 ? 65536.0f : 256.0f;
+    f2 facc[G::NF / 2];           // value sums in the frame of R, two columns each
     float R = -INFINITY, L = 0.0f, Z = 0.0f;
+    // One chunk's scores, weights and value sums; `part`: only its first n_tok tokens count.
+    auto chunk = [&](const unsigned char *sp, int n_tok, auto part) {
+        constexpr bool PART = decltype(part)::value;
+        const unsigned char *kmeta = sp + CT * KB, *vmeta = kmeta + CT * 8, *vcodes = vmeta + CT * 8;
+        // largest value scale: lanes share the tokens (scales are not negative; their bits order as they do)
+        uint32_t vbits = 0;
+#pragma unroll
+        for (int i = 0; i < CT / 32; i++)
+            if (!PART || 32 * i + lane < n_tok)
+                vbits = max(vbits, __float_as_uint(*reinterpret_cast<const float *>(vmeta + (32 * i + lane) * 8)) & 0x7fffffffu);
+        vbits = __reduce_max_sync(0xffffffffu, vbits);
+        // ---- scores: tile pair p holds tokens 16 p + 4 q + e of the lane's head ----
+        float sc[4 * G::NPR];
+        float smax = -INFINITY;
+        const f2 less = pair(-kMagic, -kMagic);
+#pragma unroll
+        for (int p = 0; p < G::NPR; p++) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const unsigned char *kp = sp + (16 * p + 4 * (r >> 1) + 2 * j + (r & 1)) * KB + q * (KB / 4);
+                uint32_t wv[G::SEGW];
+                if constexpr (G::SEGW == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+                    wv[0] = v.x;
+                    wv[1] = v.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < G::SEGW / 4; i++) {
+                        const uint4 v = reinterpret_cast<const uint4 *>(kp)[i];
+                        wv[4 * i] = v.x;
+                        wv[4 * i + 1] = v.y;
+                        wv[4 * i + 2] = v.z;
+                        wv[4 * i + 3] = v.w;
+                    }
+                }
+                int d[4];
+                f2 t0, t1;  // sums of the upper and of the lower digits, of two tokens
+                if constexpr (BITS == 4) {
+                    constexpr int kHalf = G::NCH / 2;
+                    int lo[4];
+                    mma_s8s8(lo, qa[0], codes_lo(wv[0]), codes_lo(wv[1]), qlo0, qlo0, qlo1, qlo1);
+                    if constexpr (kHalf == 2)
+                        mma_s8s8(lo, qa[1], codes_lo(wv[2]), codes_lo(wv[3]), lo[0], lo[1], lo[2], lo[3]);
+                    mma_s8s8(d, qa[kHalf], codes_hi(wv[0]), codes_hi(wv[1]), kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+                    if constexpr (kHalf == 2)
+                        mma_s8s8(d, qa[kHalf + 1], codes_hi(wv[2]), codes_hi(wv[3]), d[0], d[1], d[2], d[3]);
+                    const f2 sixteen = pair(16.0f, 16.0f);
+                    t0 = fma2(add2(pair_bits(lo[0], lo[1]), less), sixteen, add2(pair_bits(d[0], d[1]), less));
+                    t1 = fma2(add2(pair_bits(lo[2], lo[3]), less), sixteen, add2(pair_bits(d[2], d[3]), less));
+                } else {
+                    mma_s8s8(d, qa[0], codes8(wv[0]), codes8(wv[1]), kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+#pragma unroll
+                    for (int k = 1; k < G::NCH; k++)
+                        mma_s8s8(d, qa[k], codes8(wv[2 * k]), codes8(wv[2 * k + 1]), d[0], d[1], d[2], d[3]);
+                    t0 = add2(pair_bits(d[0], d[1]), less);
+                    t1 = add2(pair_bits(d[2], d[3]), less);
+                }
+                split(fma2(t0, pair(wtop, wtop), t1), sc[4 * p + 2 * j], sc[4 * p + 2 * j + 1]);
+                if constexpr (ND == 3) {  // the other digits' part is the lane's that is four heads away
+                    sc[4 * p + 2 * j] += __shfl_xor_sync(0xffffffffu, sc[4 * p + 2 * j], 16);
+                    sc[4 * p + 2 * j + 1] += __shfl_xor_sync(0xffffffffu, sc[4 * p + 2 * j + 1], 16);
+                }
+            }
+            const float4 km0 = *reinterpret_cast<const float4 *>(kmeta + (16 * p + 4 * q) * 8);
+            const float4 km1 = *reinterpret_cast<const float4 *>(kmeta + (16 * p + 4 * q) * 8 + 16);
+            const float ks[4] = {km0.x, km0.z, km1.x, km1.z}, kz[4] = {km0.y, km0.w, km1.y, km1.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // ks (q'.(c - C)) + (kz + C ks) sum(q')
+                float s = fmaf(ks[e], fmaf(c1, sc[4 * p + e], c3), kz[e] * c2);
+                if (PART && 16 * p + 4 * q + e >= n_tok) s = -INFINITY;
+                sc[4 * p + e] = s;
+                smax = fmaxf(smax, s);
+            }
+        }
+#pragma unroll
+        for (int lm = 1; lm < 4; lm <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, lm));
+        // the chunk's reference, the running one, and the factors that bring both sums to the latter
+        const float Rc = smax + __log2f(fmaxf(__uint_as_float(vbits), kVScaleMin));
+        const float Rn = fmaxf(R, Rc);
+        const float fo = R == -INFINITY ? 0.0f : ex2_approx(R - Rn), fn = Rc == -INFINITY ? 0.0f : ex2_approx(Rc - Rn);
+        R = Rn;
+        const float base = Rc == -INFINITY ? 0.0f : Rc - G::LOG2UMAX;
+        // ---- weights: u = 2^(s - Rc) vs as fixed-point digits, A fragments of 32 tokens each ----
+        uint32_t ua[CT / 32][4];
+        float lc = 0.0f, zc = 0.0f;
+#pragma unroll
+        for (int p = 0; p < G::NPR; p++) {
+            const float4 vm0 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8);
+            const float4 vm1 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8 + 16);
+            float vs[4] = {vm0.x, vm0.z, vm1.x, vm1.z}, vz[4] = {vm0.y, vm0.w, vm1.y, vm1.w};
+            uint32_t U[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (PART && 16 * p + 4 * q + e >= n_tok) vs[e] = vz[e] = 0.0f;  // whatever a page holds there
+                const float ee = ex2_approx(sc[4 * p + e] - base);
+                lc += ee;
+                zc = fmaf(ee, fmaf(G::CENTRE, vs[e], vz[e]), zc);
+                U[e] = weight_digits<ND>(ee * vs[e]);
+            }
+            if constexpr (ND == 2) {
+                const uint32_t p01 = __byte_perm(U[0], U[1], 0x5410), p23 = __byte_perm(U[2], U[3], 0x5410);
+                ua[p >> 1][2 * (p & 1)] = __byte_perm(p01, p23, 0x7531);
+                ua[p >> 1][2 * (p & 1) + 1] = __byte_perm(p01, p23, 0x6420);
+            } else {
+                const uint32_t top = r < 4 ? 0x0062u : 0x0051u;
+                ua[p >> 1][2 * (p & 1)] = __byte_perm(__byte_perm(U[0], U[1], top), __byte_perm(U[2], U[3], top), 0x5410);
+                ua[p >> 1][2 * (p & 1) + 1] =
+                    r < 4 ? __byte_perm(__byte_perm(U[0], U[1], 0x0040), __byte_perm(U[2], U[3], 0x0040), 0x5410) : 0u;
+            }
+        }
+        L = fmaf(L, fo, lc * fn);
+        Z = fmaf(Z, fo, zc * fn);
+        if (__any_sync(0xffffffffu, fo != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < G::NF / 2; i++) facc[i] = mul2(facc[i], pair(fo, fo));
+        }
+        // ---- values: 16-byte piece v of the V blocks at a time, its integer sums folded at once ----
+        // 4 bits: one sum over the bytes as they are, u (lo + 16 hi), and one over 16 (hi - 8); the first starts at
+        // -(8 + 128) sum(u), so that their difference is the sum of u (lo - 8)
+        int first[4] = {0, 0, 0, 0};
+        if constexpr (BITS == 4) {
+#pragma unroll
+            for (int t = 0; t < CT / 32; t++) mma_u8u8(first, ua[t], kOnes, kOnes, first[0], first[1], first[2], first[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) first[i] = first[i] * -136 + kMagicBits;
+        }
+        // weights of the upper and lower digit
+        const f2 w0 = pair(fn * wtop, fn * wtop), w1 = pair(fn, fn);
+        const f2 h0 = pair(fn * wtop * G::UNIT, fn * wtop * G::UNIT), h1 = pair(fn * G::UNIT, fn * G::UNIT);
+#pragma unroll
+        for (int v = 0; v < G::VV; v++) {
+            constexpr int NJ = BITS == 4 ? 8 : 4;  // n-tiles of the piece
+            int acc[NJ][4];
+#pragma unroll
+            for (int t = 0; t < CT / 32; t++) {
+                const unsigned char *vb = vcodes + 2 * t * (16 * KB) + (8 * v + r) * 64 + 16 * q;
+                const uint4 x0 = *reinterpret_cast<const uint4 *>(vb);
+                const uint4 x1 = *reinterpret_cast<const uint4 *>(vb + 16 * KB);
+                const uint32_t y0[4] = {x0.x, x0.y, x0.z, x0.w}, y1[4] = {x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (BITS == 4) {
+                        int (&raw)[4] = acc[2 * j], (&hi)[4] = acc[2 * j + 1];
+                        if (t == 0) {
+                            mma_u8u8(raw, ua[t], y0[j], y1[j], first[0], first[1], first[2], first[3]);
+                            mma_u8s8(hi, ua[t], codes_hi(y0[j]), codes_hi(y1[j]), kMagicBits, kMagicBits, kMagicBits,
+                                     kMagicBits);
+                        } else {
+                            mma_u8u8(raw, ua[t], y0[j], y1[j], raw[0], raw[1], raw[2], raw[3]);
+                            mma_u8s8(hi, ua[t], codes_hi(y0[j]), codes_hi(y1[j]), hi[0], hi[1], hi[2], hi[3]);
+                        }
+                    } else {
+                        int (&d)[4] = acc[j];
+                        if (t == 0)
+                            mma_u8s8(d, ua[t], codes8(y0[j]), codes8(y1[j]), kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+                        else mma_u8s8(d, ua[t], codes8(y0[j]), codes8(y1[j]), d[0], d[1], d[2], d[3]);
+                    }
+                }
+            }
+            const f2 minus = pair(-1.0f, -1.0f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (BITS == 4) {
+                    const int (&raw)[4] = acc[2 * j], (&hi)[4] = acc[2 * j + 1];
+                    const f2 ra = pair_bits(raw[0], raw[1]), rb = pair_bits(raw[2], raw[3]);
+                    const f2 ha = pair_bits(hi[0], hi[1]), hb = pair_bits(hi[2], hi[3]);
+                    f2 &lo_sum = facc[v * NJ + 2 * j], &hi_sum = facc[v * NJ + 2 * j + 1];
+                    lo_sum = fma2(fma2(hb, minus, rb), w1, fma2(fma2(ha, minus, ra), w0, lo_sum));
+                    hi_sum = fma2(add2(hb, less), h1, fma2(add2(ha, less), h0, hi_sum));
+                } else {
+                    f2 &sum = facc[v * NJ + j];
+                    sum = fma2(add2(pair_bits(acc[j][2], acc[j][3]), less), w1,
+                               fma2(add2(pair_bits(acc[j][0], acc[j][1]), less), w0, sum));
+                }
+            }
+        }
+    };
     int len = 0;
     bool fresh = true;
     int st = 0;
     uint32_t phase = 0;
     for (int f = f0; f < f1; f++) {
         if (fresh) {
-            // ---- a new unit: the lane's quarter of its head's query, rotated, as digits ----
+            // ---- a new unit: its digits and constants as the prep kernel left them ----
             fresh = false;
             R = -INFINITY;
             L = Z = 0.0f;
 #pragma unroll
-            for (int i = 0; i < G::NF; i++) facc[i] = 0.0f;
-            const int row = row0 + cur.r, b = row / a.seq_len, s = row - b * a.seq_len;
-            len = visible(a, row, false);
-            const int h = cur.k / hblocks, g = (cur.k - h * hblocks) * G::HB + (ND == 2 ? r : (r & 3));
-            const bool on = g < a.group;
-            float x[N];
-            if (on) {
-                const T *src = static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
-                               ((int64_t)h * a.group + g) * D + q * N;
-                load_run<T, N>(src, a.aligned, x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++) x[i] = 0.0f;
-            }
-            if (a.rope.on) {
-                const int64_t pos = (int64_t)a.rows.lens[b] + s;
-                if (a.rope.interleaved) {
-                    const float *cs = a.rope.cos_cache + pos * (D / 2) + q * (N / 2);
-                    const float *sn = a.rope.sin_cache + pos * (D / 2) + q * (N / 2);
-#pragma unroll
-                    for (int i = 0; i < N / 2; i++) {
-                        const float co = cs[i], si = sn[i], x0 = x[2 * i], x1 = x[2 * i + 1];
-                        x[2 * i] = __fsub_rn(__fmul_rn(co, x0), __fmul_rn(si, x1));
-                        x[2 * i + 1] = __fadd_rn(__fmul_rn(si, x0), __fmul_rn(co, x1));
-                    }
-                } else {
-                    // the partner of dimension d is d +- D/2, the lane two away
-                    const float *cs = a.rope.cos_cache + pos * (D / 2) + (q & 1) * N;
-                    const float *sn = a.rope.sin_cache + pos * (D / 2) + (q & 1) * N;
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const float co = cs[i], si = sn[i], other = __shfl_xor_sync(0xffffffffu, x[i], 2);
-                        const float own = __fmul_rn(co, x[i]), cross = __fmul_rn(si, other);
-                        x[i] = (q & 2) ? __fadd_rn(cross, own) : __fsub_rn(own, cross);
-                    }
-                }
-            }
-            const float *sg = a.signs + (int64_t)h * D + q * N;
-#pragma unroll
-            for (int i = 0; i < N; i++) x[i] *= sg[i];
-#pragma unroll
-            for (int hs = 1; hs < N; hs <<= 1)
-#pragma unroll
-                for (int i = 0; i < N; i++)
-                    if ((i & hs) == 0) {
-                        const float p0 = x[i], p1 = x[i + hs];
-                        x[i] = p0 + p1;
-                        x[i + hs] = p0 - p1;
-                    }
-#pragma unroll
-            for (int lm = 1; lm < 4; lm <<= 1)
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float other = __shfl_xor_sync(0xffffffffu, x[i], lm);
-                    x[i] = (q & lm) ? other - x[i] : x[i] + other;
-                }
-            float sum = 0.0f, mabs = 0.0f;
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                x[i] *= a.wht_scale;
-                sum += x[i];
-                mabs = fmaxf(mabs, fabsf(x[i]));
-            }
-#pragma unroll
-            for (int lm = 1; lm < 4; lm <<= 1) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, lm);
-                mabs = fmaxf(mabs, __shfl_xor_sync(0xffffffffu, mabs, lm));
-            }
-            const float sigma = mabs > 0.0f ? mabs / (float)G::QMAX : 1.0f;
-            const float inv = 1.0f / sigma, sl2 = a.scale * kLog2eF;
-            c1 = sigma * sl2 * G::UNIT;
-            c2 = sum * sl2;
+            for (int i = 0; i < G::NF / 2; i++) facc[i] = 0;
+            len = visible(a, row0 + cur.r, false);
+            const uint4 *src = qprep + ((int64_t)cur.r * upr + cur.h * hblocks + cur.hb) * G::PREP + lane;
 #pragma unroll
             for (int k = 0; k < G::NCH; k++) {
-                qa[k][0] = qa[k][1] = qa[k][2] = qa[k][3] = 0u;
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        // byte e of k-group hf: dimension as the K words hold it (even and odd nibbles, or bytes)
-                        const int i = 8 * k + (BITS == 4 ? 2 * e + hf : 4 * hf + e);
-                        const int v = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
-                        const int d2 = (int)(int8_t)(v & 0xff), rest = (v - d2) >> 8;
-                        if constexpr (ND == 2) {
-                            qa[k][2 * hf] |= ((uint32_t)rest & 0xffu) << (8 * e);
-                            qa[k][2 * hf + 1] |= ((uint32_t)d2 & 0xffu) << (8 * e);
-                        } else {
-                            const int d1 = (int)(int8_t)(rest & 0xff), d0 = (rest - d1) >> 8;
-                            qa[k][2 * hf] |= ((uint32_t)(r < 4 ? d0 : d1) & 0xffu) << (8 * e);
-                            qa[k][2 * hf + 1] |= (r < 4 ? (uint32_t)d2 & 0xffu : 0u) << (8 * e);
-                        }
-                    }
+                const uint4 v = src[32 * k];
+                qa[k][0] = v.x;
+                qa[k][1] = v.y;
+                qa[k][2] = v.z;
+                qa[k][3] = v.w;
             }
+            const uint4 v = src[32 * G::NCH];
+            c1 = __uint_as_float(v.x);
+            c2 = __uint_as_float(v.y);
+            c3 = G::CENTRE * c2;
+            qlo0 = (int)v.z;
+            qlo1 = (int)v.w;
         }
         if (!mbar_wait_bounded(bars + st, phase)) failed = true;
         if (__any_sync(0xffffffffu, failed)) {
@@ -360,153 +643,8 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         }
         pend &= ~(1u << st);
         const int n_tok = (bad >> st) & 1u ? 0 : min(CT, len - cur.c * CT);
-        if (n_tok > 0) {
-            const unsigned char *sp = ring + st * G::STAGE;
-            const unsigned char *vmeta = sp + CT * (KB + 8), *vcodes = sp + CT * (KB + 16);
-            // ---- scores: tile pair p holds tokens 16 p + 4 q + e of the lane's head ----
-            float sc[4 * G::NPR];
-            float smax = -INFINITY, vmax = 0.0f;
-#pragma unroll
-            for (int p = 0; p < G::NPR; p++) {
-                int acc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const unsigned char *kp = sp + (16 * p + 4 * (r >> 1) + 2 * j + (r & 1)) * KB + q * (KB / 4);
-                    uint32_t wv[G::SEGW];
-                    if constexpr (G::SEGW == 2) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(kp);
-                        wv[0] = v.x;
-                        wv[1] = v.y;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < G::SEGW / 4; i++) {
-                            const uint4 v = reinterpret_cast<const uint4 *>(kp)[i];
-                            wv[4 * i] = v.x;
-                            wv[4 * i + 1] = v.y;
-                            wv[4 * i + 2] = v.z;
-                            wv[4 * i + 3] = v.w;
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < G::NCH; k++) {
-                        if constexpr (BITS == 4) mma_s8s8(acc[j], qa[k], centred_lo(wv[k]), centred_hi(wv[k]));
-                        else mma_s8s8(acc[j], qa[k], centred8(wv[2 * k]), centred8(wv[2 * k + 1]));
-                    }
-                }
-                const float4 km0 = *reinterpret_cast<const float4 *>(sp + CT * KB + (16 * p + 4 * q) * 8);
-                const float4 km1 = *reinterpret_cast<const float4 *>(sp + CT * KB + (16 * p + 4 * q) * 8 + 16);
-                const float4 vm0 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8);
-                const float4 vm1 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8 + 16);
-                const float ks[4] = {km0.x, km0.z, km1.x, km1.z}, kz[4] = {km0.y, km0.w, km1.y, km1.w};
-                const float vs[4] = {vm0.x, vm0.z, vm1.x, vm1.z};
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int j = e >> 1, x = e & 1;
-                    float dot;
-                    if constexpr (ND == 2) {
-                        dot = (float)(acc[j][x] * 256 + acc[j][2 + x]);
-                    } else {
-                        const float part = r < 4 ? fmaf((float)acc[j][x], 65536.0f, (float)acc[j][2 + x])
-                                                 : (float)acc[j][x] * 256.0f;
-                        dot = part + __shfl_xor_sync(0xffffffffu, part, 16);
-                    }
-                    float s = fmaf(ks[e] * c1, dot, fmaf(G::CENTRE, ks[e], kz[e]) * c2);
-                    float v = vs[e];
-                    if (n_tok < CT && 16 * p + 4 * q + e >= n_tok) {
-                        s = -INFINITY;
-                        v = 0.0f;
-                    }
-                    sc[4 * p + e] = s;
-                    smax = fmaxf(smax, s);
-                    vmax = fmaxf(vmax, v);
-                }
-            }
-#pragma unroll
-            for (int lm = 1; lm < 4; lm <<= 1) {
-                smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, lm));
-                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, lm));
-            }
-            // the chunk's reference, the running one, and the factors that bring both sums to the latter
-            const float Rc = smax + __log2f(fmaxf(vmax, kVScaleMin));
-            const float Rn = fmaxf(R, Rc);
-            const float fo = R == -INFINITY ? 0.0f : exp2f(R - Rn), fn = Rc == -INFINITY ? 0.0f : exp2f(Rc - Rn);
-            R = Rn;
-            const float base = Rc == -INFINITY ? 0.0f : Rc - G::LOG2UMAX;
-            // ---- weights: u = 2^(s - Rc) vs as UMAX fixed-point digits, A fragments of 32 tokens each ----
-            uint32_t ua[CT / 32][4];
-            float lc = 0.0f, zc = 0.0f;
-#pragma unroll
-            for (int p = 0; p < G::NPR; p++) {
-                const float4 vm0 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8);
-                const float4 vm1 = *reinterpret_cast<const float4 *>(vmeta + (16 * p + 4 * q) * 8 + 16);
-                float vs[4] = {vm0.x, vm0.z, vm1.x, vm1.z}, vz[4] = {vm0.y, vm0.w, vm1.y, vm1.w};
-                uint32_t U[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (n_tok < CT && 16 * p + 4 * q + e >= n_tok) vs[e] = vz[e] = 0.0f;  // whatever a page holds there
-                    const float ee = ex2_approx(sc[4 * p + e] - base);
-                    lc += ee;
-                    zc = fmaf(ee, fmaf(G::CENTRE, vs[e], vz[e]), zc);
-                    U[e] = __float2uint_rn(fminf(ee * vs[e], G::UMAX));
-                }
-                if constexpr (ND == 2) {
-                    const uint32_t p01 = __byte_perm(U[0], U[1], 0x5410), p23 = __byte_perm(U[2], U[3], 0x5410);
-                    ua[p >> 1][2 * (p & 1)] = __byte_perm(p01, p23, 0x7531);
-                    ua[p >> 1][2 * (p & 1) + 1] = __byte_perm(p01, p23, 0x6420);
-                } else {
-                    const uint32_t top = r < 4 ? 0x0062u : 0x0051u;
-                    ua[p >> 1][2 * (p & 1)] =
-                        __byte_perm(__byte_perm(U[0], U[1], top), __byte_perm(U[2], U[3], top), 0x5410);
-                    ua[p >> 1][2 * (p & 1) + 1] =
-                        r < 4 ? __byte_perm(__byte_perm(U[0], U[1], 0x0040), __byte_perm(U[2], U[3], 0x0040), 0x5410)
-                              : 0u;
-                }
-            }
-            L = fmaf(L, fo, lc * fn);
-            Z = fmaf(Z, fo, zc * fn);
-            if (__any_sync(0xffffffffu, fo != 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < G::NF; i++) facc[i] *= fo;
-            }
-            // ---- values: 16-byte piece v of the V blocks at a time, its integer sums folded at once ----
-            const float fu = fn * G::UNIT;
-#pragma unroll
-            for (int v = 0; v < G::VV; v++) {
-                constexpr int NJ = BITS == 4 ? 8 : 4;  // n-tiles of the piece
-                int acc[NJ][4];
-#pragma unroll
-                for (int j = 0; j < NJ; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
-#pragma unroll
-                for (int t = 0; t < CT / 32; t++) {
-                    const unsigned char *vb = vcodes + 2 * t * (16 * KB) + (8 * v + r) * 64 + 16 * q;
-                    const uint4 x0 = *reinterpret_cast<const uint4 *>(vb);
-                    const uint4 x1 = *reinterpret_cast<const uint4 *>(vb + 16 * KB);
-                    const uint32_t y0[4] = {x0.x, x0.y, x0.z, x0.w}, y1[4] = {x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if constexpr (BITS == 4) {
-                            mma_u8s8_w(acc[2 * j], ua[t], centred_lo(y0[j]), centred_lo(y1[j]));
-                            mma_u8s8_w(acc[2 * j + 1], ua[t], centred_hi(y0[j]), centred_hi(y1[j]));
-                        } else {
-                            mma_u8s8_w(acc[j], ua[t], centred8(y0[j]), centred8(y1[j]));
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        float val;
-                        if constexpr (ND == 2)
-                            val = (float)(acc[j][x] * 256 + acc[j][2 + x]);
-                        else
-                            val = r < 4 ? fmaf((float)acc[j][x], 65536.0f, (float)acc[j][2 + x])
-                                        : (float)acc[j][x] * 256.0f;
-                        float &dst = facc[(v * NJ + j) * 2 + x];
-                        dst = fmaf(val, fu, dst);
-                    }
-            }
-        }
+        if (n_tok == CT) chunk(ring + st * G::STAGE, CT, std::false_type());
+        else if (n_tok > 0) chunk(ring + st * G::STAGE, n_tok, std::true_type());
         __syncwarp();
         issue(st);
         if (++st == G::NST) {
@@ -522,16 +660,18 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                 L += __shfl_xor_sync(0xffffffffu, L, lm);
                 Z += __shfl_xor_sync(0xffffffffu, Z, lm);
             }
+            float x[G::NF];
+#pragma unroll
+            for (int i = 0; i < G::NF / 2; i++) split(facc[i], x[2 * i], x[2 * i + 1]);
             if constexpr (ND == 3) {  // the two lanes of a head hold sums of different digits
 #pragma unroll
-                for (int i = 0; i < G::NF; i++) facc[i] += __shfl_xor_sync(0xffffffffu, facc[i], 16);
+                for (int i = 0; i < G::NF; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], 16);
             }
             if (r < G::HB) {
-                float *rec = records + ((int64_t)w + (int64_t)was.r * upr + was.k) * G::REC;
+                float *rec = records + ((int64_t)w + (int64_t)was.r * upr + was.h * hblocks + was.hb) * G::REC;
                 float4 *dst = reinterpret_cast<float4 *>(rec + r * D + q * N);
 #pragma unroll
-                for (int i = 0; i < N / 4; i++)
-                    dst[i] = make_float4(facc[4 * i], facc[4 * i + 1], facc[4 * i + 2], facc[4 * i + 3]);
+                for (int i = 0; i < N / 4; i++) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                 if (q == 0) *reinterpret_cast<float4 *>(rec + G::HB * D + 4 * r) = make_float4(R, L, Z, 0.0f);
             }
             fresh = true;
@@ -642,8 +782,10 @@ int launch_shape(const PagesAttendArgs &a, void *workspace, cudaStream_t stream)
     const int hblocks = (a.group + G::HB - 1) / G::HB;
     const int64_t upr = (int64_t)a.heads * hblocks, rows = (int64_t)a.batch * a.seq_len, per = rows_per_launch(upr);
     const int64_t row_chunks = upr * a.rows.max_pages * G::CPP;
+    const int64_t most = rows < per ? rows : per;
     int *prefix = static_cast<int *>(workspace);
-    float *records = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPrefixBytes);
+    uint4 *qprep = reinterpret_cast<uint4 *>(static_cast<char *>(workspace) + kPrefixBytes);
+    float *records = reinterpret_cast<float *>(qprep + most * upr * G::PREP);
     for (int64_t row0 = 0; row0 < rows;) {
         int64_t n = rows - row0 < per ? rows - row0 : per;
         if (n * row_chunks >= ((int64_t)1 << 31)) n = (((int64_t)1 << 31) - 1) / row_chunks;  // chunk indices are ints
@@ -656,10 +798,17 @@ int launch_shape(const PagesAttendArgs &a, void *workspace, cudaStream_t stream)
         cfg.stream = stream;
         cfg.attrs = pdl;
         cfg.numAttrs = 1;
+        cfg.gridDim = dim3((unsigned)((n * upr + 1) / 2));
+        cfg.blockDim = dim3(64);
+        int rc = check_cuda(cudaLaunchKernelEx(&cfg, pages_prep_kernel<T, BITS, D, ND>, a, (int)row0, (int)(n * upr), hblocks,
+                                               qprep),
+                            "gqa_paged_attend prep launch");
+        count_launch();
+        if (rc != SA_OK) return rc;
         cfg.gridDim = dim3((unsigned)a.sm_count);
         cfg.blockDim = dim3(kNWP * 32);
         cfg.dynamicSmemBytes = G::SMEM;
-        int rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, a, (int)row0, (int)n, hblocks, prefix, records),
+        rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, a, (int)row0, (int)n, hblocks, (const uint4 *)qprep, prefix, records),
                             "gqa_paged_attend launch");
         count_launch();
         if (rc != SA_OK) return rc;
@@ -692,7 +841,8 @@ size_t pages_attend_workspace(const kv_pages_impl *k, int batch, int seq_len, in
     const int64_t upr = (int64_t)k->cfg.kv_head_count * ((k->group + hb - 1) / hb);
     const int64_t rows = (int64_t)batch * seq_len, per = rows_per_launch(upr), n = rows < per ? rows : per;
     const int64_t records = (int64_t)k->sm_count * kNWP + n * upr;  // one per warp, and one more per unit
-    return kPrefixBytes + (size_t)records * hb * (k->cfg.head_dim + 4) * sizeof(float);
+    const size_t prep = (size_t)(n * upr) * 32 * (k->cfg.head_dim / 32 + 1) * 16;  // digits and constants of a unit
+    return kPrefixBytes + prep + (size_t)records * hb * (k->cfg.head_dim + 4) * sizeof(float);
 }
 
 int launch_pages_attend(const PagesAttendArgs &a, void *workspace, cudaStream_t stream) {

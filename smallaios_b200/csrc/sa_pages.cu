@@ -53,6 +53,11 @@ PageRows page_rows(const kv_pages_impl *k, const int32_t *page_table, int64_t ta
     return PageRows{page_table, table_stride, max_pages, seq_lens, counts, k->cfg.num_pages, k->dev_status};
 }
 
+RopeArgs rope_args(const float *cos_cache, const float *sin_cache, int32_t rows, int32_t on, int32_t interleaved) {
+    const int aligned = ((reinterpret_cast<uintptr_t>(cos_cache) | reinterpret_cast<uintptr_t>(sin_cache)) & 15) == 0;
+    return RopeArgs{cos_cache, sin_cache, rows, on != 0, interleaved != 0, aligned};
+}
+
 bool vectors_aligned(const void *p, int64_t batch_stride, int64_t token_stride, int32_t dtype, int batch, int seq_len) {
     const int64_t width = dtype == SA_DTYPE_FLOAT ? 4 : 2;
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (batch <= 1 || batch_stride * width % 16 == 0) &&
@@ -208,7 +213,7 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
     a.signs = k->signs + (size_t)layer * width;
     a.wht_scale = k->wht_scale;
     a.rows = page_rows(k, page_table, table_stride, max_pages, seq_lens, counts);
-    a.rope = RopeArgs{cos_cache, sin_cache, cache_rows, do_rotary != 0, rotary_interleaved != 0};
+    a.rope = rope_args(cos_cache, sin_cache, cache_rows, do_rotary, rotary_interleaved);
     return launch_pages_append(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -260,7 +265,7 @@ int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, in
     a.scale = has_scale ? scale : 1.0f / host_sqrt_f32((float)k->cfg.head_dim);
     a.sm_count = k->sm_count;
     a.rows = page_rows(k, page_table, table_stride, max_pages, seq_lens, counts);
-    a.rope = RopeArgs{cos_cache, sin_cache, cache_rows, do_rotary != 0, rotary_interleaved != 0};
+    a.rope = rope_args(cos_cache, sin_cache, cache_rows, do_rotary, rotary_interleaved);
     return launch_pages_attend(a, workspace, static_cast<cudaStream_t>(stream));
 }
 

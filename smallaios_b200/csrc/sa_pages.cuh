@@ -47,6 +47,7 @@ struct PageRows {
 struct RopeArgs {
     const float *cos_cache, *sin_cache;
     int rows, on, interleaved;
+    int aligned;  // both tables begin on 16 bytes
 };
 
 struct PagesAppendArgs {
@@ -113,11 +114,11 @@ int launch_pages_attend(const PagesAttendArgs &a, void *workspace, cudaStream_t 
 
 // New tokens of row b, and the position of its first one; 0 tokens for a row that takes no part.
 __device__ __forceinline__ int row_tokens(const PageRows &r, int b, int seq_len, int64_t &pos0) {
-    const int len = r.lens[b];
+    const int len = __ldcg(r.lens + b);
     pos0 = len;
     if (len < 0) return 0;
     if (!r.counts) return seq_len;
-    const int n = r.counts[b];
+    const int n = __ldcg(r.counts + b);
     return n < 0 ? 0 : (n < seq_len ? n : seq_len);
 }
 

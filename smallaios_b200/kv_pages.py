@@ -11,7 +11,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._lib import check, lib
 from .kv_cache import DEFAULT_SEED, _view
 
@@ -33,52 +33,6 @@ class PagesView:
         """V codes in per-token pack_bits order (P, H, 64, CB), as LayerView.v_codes_tokens."""
         p, h, nblk, c4, g, jj, tt = self.v_codes.shape
         return self.v_codes.permute(0, 1, 2, 4, 6, 3, 5).reshape(p, h, nblk * g * tt, c4 * jj)
-
-
-def page_rows(op: str, page_table, seq_lens, counts, batch: int):
-    """Checks of a call's rows; (table pointer, its row stride, pages per row, lengths pointer, counts pointer)."""
-    from .ops import ShapeMismatch, UnsupportedOp, _cuda
-
-    if not isinstance(page_table, torch.Tensor) or not page_table.is_cuda:
-        raise TypeError("page_table must be a CUDA tensor")
-    if page_table.dtype != torch.int32:
-        raise UnsupportedOp(f"{op}: page_table must be int32")
-    if page_table.dim() != 2 or page_table.shape[0] != batch:
-        raise ShapeMismatch(f"{op}: page_table must be ({batch}, pages), got {tuple(page_table.shape)}")
-    pages = page_table.shape[1]
-    stride = page_table.stride(0) if batch > 1 else pages
-    if (pages > 1 and page_table.stride(1) != 1) or stride < pages:
-        raise ValueError("page_table must be contiguous, or a slice of columns of a contiguous tensor")
-    _cuda(seq_lens, "seq_lens")
-    _cuda(counts, "counts")
-    for name, t in (("seq_lens", seq_lens), ("counts", counts)):
-        if t is None and name == "counts":
-            continue
-        if t.dtype != torch.int32:
-            raise UnsupportedOp(f"{op}: {name} must be int32")
-        if t.numel() != batch:
-            raise ShapeMismatch(f"{op}: {name} must have {batch} entries, got {t.numel()}")
-    return page_table.data_ptr(), stride, pages, seq_lens.data_ptr(), None if counts is None else counts.data_ptr()
-
-
-def token_strides(op: str, t, width: int, what: str):
-    """(batch stride, token stride) of (B, S, width) vectors, which may be a slice of columns of a wider projection."""
-    from .ops import ShapeMismatch
-
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{what} must be a CUDA tensor")
-    if t.dim() != 3:
-        raise ShapeMismatch(f"{op}: {what} must be rank-3")
-    if t.shape[2] != width:
-        raise ShapeMismatch(f"{op}: hidden size {t.shape[2]} of {what} does not match the pool's heads/head_dim ({width})")
-    b, s, _ = t.shape
-    if t.is_contiguous():
-        return s * width, width
-    token = t.stride(1) if s > 1 else width
-    batch = t.stride(0) if b > 1 else s * token
-    if t.stride(2) != 1 or token < width or batch < width:
-        raise ValueError(f"{what} must have contiguous rows")
-    return batch, token
 
 
 class GpuKvPages:
@@ -109,6 +63,7 @@ class GpuKvPages:
             check(lib.sa_kv_pages_create(ctypes.byref(cfg), ctypes.byref(self._handle)))
         self.config = cfg
         self.kv_width = cfg.kv_head_count * head_dim
+        self.half_dim = head_dim // 2
         self.query_width = cfg.num_heads // cfg.num_kv_heads * self.kv_width
         self._workspace_bytes: dict = {}
 
@@ -129,32 +84,19 @@ class GpuKvPages:
         tokens exist.  K is rotated to its position with ``do_rotary``.  ``seq_lens`` is not changed.  Tokens that
         have no page, or no row in the tables, are left out and reported by ``device_status``.
         """
-        from .ops import ShapeMismatch, UnsupportedOp, _dtype_code, _raise_op, _rope_tables, _stream_handle
-
-        strides = token_strides("kv_pages_append", key, self.kv_width, "key")
+        b, s, *strides = ops._token_rows("kv_pages_append", key, self.kv_width, "key")
         if not isinstance(value, torch.Tensor) or value.shape != key.shape:
-            raise ShapeMismatch("kv_pages_append: key and value must be (B, S, H*D) with equal shapes")
+            raise ops.ShapeMismatch("kv_pages_append: key and value must be (B, S, H*D) with equal shapes")
         if value.dtype != key.dtype:
-            raise UnsupportedOp("kv_pages_append: key and value dtypes differ")
-        if token_strides("kv_pages_append", value, self.kv_width, "value") != strides:
+            raise ops.UnsupportedOp("kv_pages_append: key and value dtypes differ")
+        if ops._token_rows("kv_pages_append", value, self.kv_width, "value") != (b, s, *strides):
             raise ValueError("key and value must have the same strides")
-        b, s, _ = key.shape
-        table = page_rows("kv_pages_append", page_table, seq_lens, counts, b)
-        rows = _rope_tables(cos_cache, sin_cache)
-        self._check_tables("kv_pages_append", do_rotary, cos_cache, sin_cache)
-        rc = lib.sa_kv_pages_append(self.handle, layer, key.data_ptr(), value.data_ptr(), *strides, _dtype_code(key), b, s,
-                                    *table, None if cos_cache is None else cos_cache.data_ptr(),
-                                    None if sin_cache is None else sin_cache.data_ptr(), rows, int(bool(do_rotary)),
-                                    int(bool(rotary_interleaved)), _stream_handle(stream, self.device))
-        _raise_op(rc, "kv_pages_append")
-
-    def _check_tables(self, op: str, do_rotary, cos_cache, sin_cache) -> None:
-        """cos/sin tables have one column per pair, and as many rows each."""
-        from .ops import ShapeMismatch
-
-        if do_rotary and cos_cache is not None and sin_cache is not None and (
-                cos_cache.shape != sin_cache.shape or cos_cache.shape[1] != self.config.head_dim // 2):
-            raise ShapeMismatch(f"{op}: cos and sin caches must be (rows, {self.config.head_dim // 2})")
+        table = ops._page_rows("kv_pages_append", page_table, seq_lens, counts, b)
+        rope = ops._page_rope("kv_pages_append", cos_cache, sin_cache, self.half_dim)
+        rc = lib.sa_kv_pages_append(self.handle, layer, key.data_ptr(), value.data_ptr(), *strides, ops._dtype_code(key),
+                                    b, s, *table, *rope, int(bool(do_rotary)), int(bool(rotary_interleaved)),
+                                    ops._stream_handle(stream, self.device))
+        ops._raise_op(rc, "kv_pages_append")
 
     def reorder_beams(self, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, *,
                       out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
@@ -166,23 +108,24 @@ class GpuKvPages:
         by rows; a row's page in use and the pages behind it must be its own.  ``out`` must not overlap
         ``page_table``.
         """
-        from .ops import ShapeMismatch, UnsupportedOp, _cuda, _empty, _raise_op, _stream_handle
-
-        _cuda(parents, "parents")
-        if parents.dim() != 2:
-            raise ShapeMismatch("reorder_beams: parents must be (B, K)")
+        ops._cuda(parents, "parents")
+        shape = parents.shape
+        if len(shape) != 2:
+            raise ops.ShapeMismatch("reorder_beams: parents must be (B, K)")
         if parents.dtype != torch.int32:
-            raise UnsupportedOp("reorder_beams: parents must be int32")
-        b, k = parents.shape
-        table, stride, width, lens, _ = page_rows("reorder_beams", page_table, seq_lens, None, b * k)
+            raise ops.UnsupportedOp("reorder_beams: parents must be int32")
+        b, k = shape
+        table, stride, width, lens, _ = ops._page_rows("reorder_beams", page_table, seq_lens, None, b * k)
         if out is None:
-            out = _empty(page_table.shape, torch.int32, page_table.device, stream)
-        elif out.shape != page_table.shape:
-            raise ShapeMismatch("reorder_beams: out must have page_table's shape")
-        new, new_stride, _, _, _ = page_rows("reorder_beams", out, seq_lens, None, b * k)
+            out = ops._empty(page_table.shape, torch.int32, page_table.device, stream)
+            new, new_stride = out.data_ptr(), width
+        else:
+            if not isinstance(out, torch.Tensor) or out.shape != page_table.shape:
+                raise ops.ShapeMismatch("reorder_beams: out must have page_table's shape")
+            new, new_stride, _ = ops._page_table("reorder_beams", out, b * k, "out")
         rc = lib.sa_kv_pages_reorder(self.handle, table, stride, new, new_stride, width, lens, parents.data_ptr(), b, k,
-                                     _stream_handle(stream, self.device))
-        _raise_op(rc, "reorder_beams")
+                                     ops._stream_handle(stream, self.device))
+        ops._raise_op(rc, "reorder_beams")
         return out
 
     def workspace_bytes(self, batch: int, seq_len: int, dtype_code: int) -> int:

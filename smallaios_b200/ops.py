@@ -17,14 +17,18 @@ Errors map the library's status codes onto the reference's OpError variants.
 from __future__ import annotations
 
 import contextlib
+import functools
 from dataclasses import dataclass, field
+from typing import TYPE_CHECKING
 
 import torch
 
 from . import _lib
 from ._lib import lib
 from .kv_cache import GpuKvCache
-from .kv_pages import GpuKvPages, page_rows, token_strides
+
+if TYPE_CHECKING:
+    from .kv_pages import GpuKvPages
 
 
 # ---- OpError mirror (onnx-rt/src/operators.rs) ------------------------------
@@ -356,6 +360,83 @@ def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_
 
 
 # ---- paged serving ----------------------------------------------------------------
+# The checks of a call take as long as its launch: each property of a tensor is read once, and what a contiguous
+# tensor's strides are is not asked.
+def _page_table(op: str, t, batch: int, what: str):
+    """(pointer, row stride, pages per row) of an int32 table of ``batch`` rows, which may be a slice of columns."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{what} must be a CUDA tensor")
+    if t.dtype != torch.int32:
+        raise UnsupportedOp(f"{op}: {what} must be int32")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != batch:
+        raise ShapeMismatch(f"{op}: {what} must be ({batch}, pages), got {tuple(shape)}")
+    pages = shape[1]
+    if t.is_contiguous():
+        return t.data_ptr(), pages, pages
+    row, column = t.stride()
+    if (pages > 1 and column != 1) or (batch > 1 and row < pages):
+        raise ValueError(f"{what} must be contiguous, or a slice of columns of a contiguous tensor")
+    return t.data_ptr(), row if batch > 1 else pages, pages
+
+
+def _page_rows(op: str, page_table, seq_lens, counts, batch: int):
+    """A call's rows: (table pointer, its row stride, pages per row, lengths pointer, counts pointer or None)."""
+    table = _page_table(op, page_table, batch, "page_table")
+    pointers = []
+    for name, t in (("seq_lens", seq_lens), ("counts", counts)):
+        if t is None and name == "counts":
+            pointers.append(None)
+            continue
+        _cuda(t, name)
+        if t is None:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        if t.dtype != torch.int32:
+            raise UnsupportedOp(f"{op}: {name} must be int32")
+        if t.numel() != batch:
+            raise ShapeMismatch(f"{op}: {name} must have {batch} entries, got {t.numel()}")
+        pointers.append(t.data_ptr())
+    return *table, *pointers
+
+
+def _token_rows(op: str, t, width: int, what: str):
+    """(B, S, batch stride, token stride) of (B, S, width) vectors, maybe a slice of columns of a wider projection."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{what} must be a CUDA tensor")
+    shape = t.shape
+    if len(shape) != 3:
+        raise ShapeMismatch(f"{op}: {what} must be rank-3")
+    b, s, w = shape
+    if w != width:
+        raise ShapeMismatch(f"{op}: hidden size {w} of {what} does not match the pool's heads/head_dim ({width})")
+    if t.is_contiguous():
+        return b, s, s * width, width
+    batch, token, column = t.stride()
+    if s <= 1:
+        token = width
+    if b <= 1:
+        batch = s * token
+    if column != 1 or token < width or batch < width:
+        raise ValueError(f"{what} must have contiguous rows")
+    return b, s, batch, token
+
+
+def _page_rope(op: str, cos_cache, sin_cache, half: int):
+    """(cos pointer, sin pointer, rows) of the rotary tables, (None, None, 0) without."""
+    if cos_cache is None and sin_cache is None:
+        return None, None, 0
+    _cuda(cos_cache, "cos_cache")
+    _cuda(sin_cache, "sin_cache")
+    if cos_cache is None or sin_cache is None:
+        raise ShapeMismatch(f"{op}: cos and sin caches come together")
+    if cos_cache.dtype != torch.float32 or sin_cache.dtype != torch.float32:
+        raise UnsupportedOp(f"{op}: cos and sin caches must be float32")
+    shape = cos_cache.shape
+    if len(shape) != 2 or shape[1] != half or sin_cache.shape != shape:
+        raise ShapeMismatch(f"{op}: cos and sin caches must be (rows, {half})")
+    return cos_cache.data_ptr(), sin_cache.data_ptr(), shape[0]
+
+
 def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_table: torch.Tensor,
                      seq_lens: torch.Tensor, *, num_heads: int, counts: torch.Tensor | None = None,
                      scale: float | None = None, do_rotary: bool = False, rotary_interleaved: bool = False,
@@ -369,27 +450,31 @@ def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_ta
     tokens that do not exist give zeros.  A row's pages are read once per new token: S is one, or a few.
     ``workspace``: uint8, at least ``pages.workspace_bytes`` bytes; allocated when not given.
     """
-    strides = token_strides("gqa_paged_attend", query, pages.query_width, "query")
-    b, s, _ = query.shape
+    b, s, *strides = _token_rows("gqa_paged_attend", query, pages.query_width, "query")
     code = _dtype_code(query)
-    table = page_rows("gqa_paged_attend", page_table, seq_lens, counts, b)
-    rows = _rope_tables(cos_cache, sin_cache)
-    pages._check_tables("gqa_paged_attend", do_rotary, cos_cache, sin_cache)
+    table = _page_rows("gqa_paged_attend", page_table, seq_lens, counts, b)
+    rope = _page_rope("gqa_paged_attend", cos_cache, sin_cache, pages.half_dim)
     if out is None:
-        out = _empty(query.shape, query.dtype, query.device, stream)
+        out = torch.empty_like(query) if stream is None and query.is_contiguous() else \
+            _empty(query.shape, query.dtype, query.device, stream)
     else:
         _cuda(out, "out")
         if out.shape != query.shape or out.dtype != query.dtype:
             raise ShapeMismatch("gqa_paged_attend: out must have query's shape and dtype")
-    workspace = _workspace(workspace, pages.workspace_bytes(b, s, code), query.device, stream)
+    need = pages.workspace_bytes(b, s, code)
+    workspace = _workspace(workspace, need, query.device, stream)
     rc = lib.sa_gqa_paged_attend(pages.handle, layer, query.data_ptr(), *strides, out.data_ptr(), code, b, s,
-                                 int(num_heads), int(scale is not None), float(scale or 0.0), *table,
-                                 None if cos_cache is None else cos_cache.data_ptr(),
-                                 None if sin_cache is None else sin_cache.data_ptr(), rows, int(bool(do_rotary)),
-                                 int(bool(rotary_interleaved)), None if workspace is None else workspace.data_ptr(),
+                                 int(num_heads), int(scale is not None), float(scale or 0.0), *table, *rope,
+                                 int(bool(do_rotary)), int(bool(rotary_interleaved)),
+                                 None if workspace is None else workspace.data_ptr(),
                                  0 if workspace is None else workspace.numel(), _stream_handle(stream, query.device))
     _raise_op(rc, "gqa_paged_attend")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _beam_workspace_bytes(batch: int, beams: int, vocab: int) -> int:
+    return lib.sa_beam_select_workspace_bytes(batch, beams, vocab)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.Tensor | None = None,
@@ -404,31 +489,38 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise TypeError("logits must be a CUDA tensor")
     _cuda(scores, "scores")
-    _cuda(finished, "finished")
-    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
+    if scores is None:
+        raise TypeError("scores must be a CUDA tensor")
+    shape, rows = scores.shape, logits.shape
+    if len(shape) != 2 or len(rows) != 2 or rows[0] != shape[0] * shape[1]:
         raise ShapeMismatch("beam_select: logits must be (B*K, V) of scores (B, K)")
     if scores.dtype != torch.float32:
         raise UnsupportedOp("beam_select: scores must be float32")
-    b, k = scores.shape
-    rows, vocab = logits.shape
-    stride = logits.stride(0) if rows > 1 else vocab
-    if (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
-        raise ValueError("logits must have contiguous rows")
+    b, k = shape
+    n, stride = rows
+    vocab = stride
+    if not logits.is_contiguous():
+        row, column = logits.stride()
+        if (vocab > 1 and column != 1) or (n > 1 and row < vocab):
+            raise ValueError("logits must have contiguous rows")
+        stride = row if n > 1 else vocab
     if finished is not None:
-        if finished.dtype not in (torch.bool, torch.uint8):
+        _cuda(finished, "finished")
+        if finished.dtype != torch.bool and finished.dtype != torch.uint8:
             raise UnsupportedOp("beam_select: finished must be bool or uint8")
-        if finished.shape != scores.shape:
+        if finished.shape != shape:
             raise ShapeMismatch("beam_select: finished must have scores' shape")
     keep = k if keep is None else int(keep)
-    code = _dtype_code(logits)
-    out = _empty((3, b, max(keep, 0)), torch.int32, logits.device, stream)
-    parents, tokens, best = out[0], out[1], out[2].view(torch.float32)
-    workspace = _workspace(workspace, lib.sa_beam_select_workspace_bytes(b, k, vocab), logits.device, stream)
+    code, device = _dtype_code(logits), logits.device
+    with contextlib.nullcontext() if stream is None else _owned_by(stream, device):
+        best = torch.empty_like(scores) if keep == k else scores.new_empty((b, max(keep, 0)))
+        parents, tokens = torch.empty_like(best, dtype=torch.int32), torch.empty_like(best, dtype=torch.int32)
+    workspace = _workspace(workspace, _beam_workspace_bytes(b, k, vocab), device, stream)
     rc = lib.sa_beam_select(logits.data_ptr(), stride, code, scores.data_ptr(),
                             None if finished is None else finished.data_ptr(), b, k, vocab, int(end_token), keep,
                             parents.data_ptr(), tokens.data_ptr(), best.data_ptr(),
                             None if workspace is None else workspace.data_ptr(),
-                            0 if workspace is None else workspace.numel(), _stream_handle(stream, logits.device))
+                            0 if workspace is None else workspace.numel(), _stream_handle(stream, device))
     _raise_op(rc, "beam_select")
     return parents, tokens, best
 
