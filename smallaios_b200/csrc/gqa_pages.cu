@@ -91,17 +91,9 @@ __device__ __forceinline__ void mma_u8u8(int (&d)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 
-// Codes of a word as signed bytes: 8-bit ones less 128; 16 times the high nibbles less 8; the low nibbles as they are
-// (taking 8 off a low nibble in place costs a shift more: their sums start at -8 times the digits' sum instead).
+// Codes of a word as signed bytes: 8-bit ones less 128; 16 times the high nibbles less 8 (low nibbles: of w * 16).
 __device__ __forceinline__ uint32_t codes8(uint32_t w) { return w ^ 0x80808080u; }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return w & 0x0F0F0F0Fu; }
-
-// Sums start at the bits of the float 1.5 * 2^23: while a sum's magnitude stays below 2^22 (the largest, 64 tokens or
-// 128 dimensions of 255 * 128, is 2.1e6) its bits are those of 1.5 * 2^23 plus the sum, and a float subtraction makes
-// the number of it where a conversion would take the integer pipe that the unpacking of codes already fills.
-constexpr int kMagicBits = 0x4B400000;
-constexpr float kMagic = 12582912.0f;
+__device__ __forceinline__ uint32_t codes4(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
 
 // Pairs of floats.
 using f2 = unsigned long long;
@@ -110,13 +102,7 @@ __device__ __forceinline__ f2 pair(float x, float y) {
     asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y));
     return v;
 }
-__device__ __forceinline__ f2 pair_bits(int x, int y) { return pair(__int_as_float(x), __int_as_float(y)); }
 __device__ __forceinline__ void split(f2 v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f2 add2(f2 x, f2 y) {
-    f2 v;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
-    return v;
-}
 __device__ __forceinline__ f2 mul2(f2 x, f2 y) {
     f2 v;
     asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
@@ -168,126 +154,84 @@ __device__ __forceinline__ int visible(const PagesAttendArgs &a, int row, bool r
 // Warps that share F chunks.
 __host__ __device__ __forceinline__ int sharing_warps(int F, int warps) { return min(warps, F); }
 
-// One warp per unit: its query heads, rotated to their position and into the pages' frame, as digits arranged as the
-// A fragments of the scores' product; lane (r, q) holds a quarter of head r (of r & 3 where heads have three digits).
-// Units of rows without tokens are left out.
+// A CTA per unit, a warp per query head: the query rotated to its position and into the pages' frame, as digits
+// arranged as the A fragments of the scores' product (the byte of a dimension's digit lies where frag_byte says), with
+// the score constants and the row's tokens behind them.
+template <int BITS, int D>
+__device__ __forceinline__ int frag_byte(int dim, int row, int upper) {
+    constexpr int N = D / 4, NCH = D / 32;
+    const int q = dim / N, i = dim % N;  // lane (row, q) holds dimensions [q N, q N + N)
+    // 8 bits: bytes of K words 2k, 2k + 1; 4 bits: low nibbles of words 2k, 2k + 1 (first half of the steps), then high ones
+    const int k = BITS == 4 ? (i & 1) * (NCH / 2) + (i >> 4) : i >> 3, hf = BITS == 4 ? (i >> 3) & 1 : (i >> 2) & 1;
+    const int e = BITS == 4 ? (i >> 1) & 3 : i & 3;
+    return ((32 * k + 4 * row + q) * 4 + 2 * hf + !upper) * 4 + e;
+}
+
 template <typename T, int BITS, int D, int ND>
-__global__ void __launch_bounds__(64) pages_prep_kernel(PagesAttendArgs a, int row0, int units, int hblocks, uint4 *qprep) {
+__global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
+    pages_prep_kernel(PagesAttendArgs a, int row0, int hblocks, uint4 *qprep) {
     using G = PGeo<BITS, D, ND>;
-    constexpr int N = D / 4;
-    const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
-    const int u = blockIdx.x * 2 + (threadIdx.x >> 5), upr = a.heads * hblocks;
-    // The attention kernel starts when all warps here have passed the wait: what the kernels before this one wrote
+    constexpr int EPL = D / 32;
+    __shared__ uint4 s_frag[G::PREP];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int u = blockIdx.x, upr = a.heads * hblocks;
+    const int row = u / upr, k = u - row * upr, h = k / hblocks, b = (row0 + row) / a.seq_len, s = row0 + row - b * a.seq_len;
+    const int g = (k - h * hblocks) * G::HB + w;
+    // The attention kernel starts when all CTAs here have passed the wait: what the kernels before this one wrote
     // (pages, table, lengths) is there for it, too, and only the digits are left to wait for.
     griddep_wait();
     griddep_launch_dependents();
-    if (u >= units) return;
-    const int row = u / upr, k = u - row * upr, h = k / hblocks, b = (row0 + row) / a.seq_len, s = row0 + row - b * a.seq_len;
-    if (visible(a, row0 + row, false) == 0) return;
-    const int g = (k - h * hblocks) * G::HB + (ND == 2 ? r : (r & 3));
+    float x[EPL], sg[EPL];
     const bool on = g < a.group;
-    float x[N];
+    load_elems<float, EPL>(a.signs + (int64_t)h * D + lane * EPL, sg);
     if (on) {
-        const T *src = static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
-                       ((int64_t)h * a.group + g) * D + q * N;
-        load_run<T, N>(src, a.aligned, x);
+        load_elems<T, EPL>(static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
+                               ((int64_t)h * a.group + g) * D + lane * EPL, x);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = 0.0f;
+        for (int i = 0; i < EPL; i++) x[i] = 0.0f;
     }
-    float sg[N];
-    load_run<float, N>(a.signs + (int64_t)h * D + q * N, true, sg);
-    if (a.rope.on) {
-        const int64_t pos = (int64_t)a.rows.lens[b] + s;
-        if (a.rope.interleaved) {
-            float cs[N / 2], sn[N / 2];
-            load_run<float, N / 2>(a.rope.cos_cache + pos * (D / 2) + q * (N / 2), a.rope.aligned, cs);
-            load_run<float, N / 2>(a.rope.sin_cache + pos * (D / 2) + q * (N / 2), a.rope.aligned, sn);
+    const int len = visible(a, row0 + row, false);
+    if (len == 0) return;  // the whole CTA
+    if (a.rope.on)
+        rope_lane<EPL>(x, lane, D, __ldcg(a.rows.lens + b) + s, a.rope.cos_cache, a.rope.sin_cache, a.rope.interleaved);
 #pragma unroll
-            for (int i = 0; i < N / 2; i++) {
-                const float x0 = x[2 * i], x1 = x[2 * i + 1];
-                x[2 * i] = __fsub_rn(__fmul_rn(cs[i], x0), __fmul_rn(sn[i], x1));
-                x[2 * i + 1] = __fadd_rn(__fmul_rn(sn[i], x0), __fmul_rn(cs[i], x1));
-            }
-        } else {
-            // the partner of dimension d is d +- D/2, the lane two away
-            float cs[N], sn[N];
-            load_run<float, N>(a.rope.cos_cache + pos * (D / 2) + (q & 1) * N, a.rope.aligned, cs);
-            load_run<float, N>(a.rope.sin_cache + pos * (D / 2) + (q & 1) * N, a.rope.aligned, sn);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float other = __shfl_xor_sync(0xffffffffu, x[i], 2);
-                const float own = __fmul_rn(cs[i], x[i]), cross = __fmul_rn(sn[i], other);
-                x[i] = (q & 2) ? __fadd_rn(cross, own) : __fsub_rn(own, cross);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] *= sg[i];
-#pragma unroll
-    for (int hs = 1; hs < N; hs <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if ((i & hs) == 0) {
-                const float p0 = x[i], p1 = x[i + hs];
-                x[i] = p0 + p1;
-                x[i + hs] = p0 - p1;
-            }
-#pragma unroll
-    for (int lm = 1; lm < 4; lm <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float other = __shfl_xor_sync(0xffffffffu, x[i], lm);
-            x[i] = (q & lm) ? other - x[i] : x[i] + other;
-        }
+    for (int i = 0; i < EPL; i++) x[i] *= sg[i];
+    warp_wht_butterfly<EPL>(x, lane, D);
     float sum = 0.0f, mabs = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
+    for (int i = 0; i < EPL; i++) {
         x[i] *= a.wht_scale;
         sum += x[i];
         mabs = fmaxf(mabs, fabsf(x[i]));
     }
-#pragma unroll
-    for (int lm = 1; lm < 4; lm <<= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, lm);
-        mabs = fmaxf(mabs, __shfl_xor_sync(0xffffffffu, mabs, lm));
-    }
+    sum = warp_sum(sum);
+    mabs = warp_max(mabs);
     const float sigma = mabs > 0.0f ? mabs / (float)G::QMAX : 1.0f;
     const float inv = 1.0f / sigma, sl2 = a.scale * kLog2eF;
-    uint32_t qa[G::NCH][4];
+    uint8_t *frag = reinterpret_cast<uint8_t *>(s_frag);
 #pragma unroll
-    for (int kk = 0; kk < G::NCH; kk++) {
-        qa[kk][0] = qa[kk][1] = qa[kk][2] = qa[kk][3] = 0u;
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                // byte e of k-group hf: the dimension as the K words hold it.  8 bits: words 2k, 2k + 1;
-                // 4 bits: low nibbles of words 2k, 2k + 1 (first half of the steps), then high ones
-                constexpr int kHalf = G::NCH / 2;
-                const int i = BITS == 4 ? 16 * (kk % kHalf) + 8 * hf + 2 * e + kk / kHalf : 8 * kk + 4 * hf + e;
-                const int v = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
-                const int d2 = (int)(int8_t)(v & 0xff), rest = (v - d2) >> 8;
-                if constexpr (ND == 2) {
-                    qa[kk][2 * hf] |= ((uint32_t)rest & 0xffu) << (8 * e);
-                    qa[kk][2 * hf + 1] |= ((uint32_t)d2 & 0xffu) << (8 * e);
-                } else {
-                    const int d1 = (int)(int8_t)(rest & 0xff), d0 = (rest - d1) >> 8;
-                    qa[kk][2 * hf] |= ((uint32_t)(r < 4 ? d0 : d1) & 0xffu) << (8 * e);
-                    qa[kk][2 * hf + 1] |= (r < 4 ? (uint32_t)d2 & 0xffu : 0u) << (8 * e);
-                }
-            }
+    for (int i = 0; i < EPL; i++) {
+        const int dim = lane * EPL + i;
+        const int v = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
+        const int d2 = (int)(int8_t)(v & 0xff), rest = (v - d2) >> 8;
+        if constexpr (ND == 2) {
+            frag[frag_byte<BITS, D>(dim, w, 1)] = (uint8_t)rest;
+            frag[frag_byte<BITS, D>(dim, w, 0)] = (uint8_t)d2;
+        } else {
+            const int d1 = (int)(int8_t)(rest & 0xff);
+            frag[frag_byte<BITS, D>(dim, w, 1)] = (uint8_t)((rest - d1) >> 8);
+            frag[frag_byte<BITS, D>(dim, w, 0)] = (uint8_t)d2;
+            frag[frag_byte<BITS, D>(dim, w + 4, 1)] = (uint8_t)d1;
+            frag[frag_byte<BITS, D>(dim, w + 4, 0)] = 0;
+        }
     }
-    int ones[4] = {0, 0, 0, 0};  // 4 bits: the sums of the rows' digits over the even dimensions
-    if constexpr (BITS == 4) {
-        mma_s8s8(ones, qa[0], kOnes, kOnes, 0, 0, 0, 0);
-        if constexpr (G::NCH == 4) mma_s8s8(ones, qa[1], kOnes, kOnes, ones[0], ones[1], ones[2], ones[3]);
+    if (lane < 32 / G::HB) {  // constants of the lanes that hold this head
+        const int to = 32 * G::NCH + (ND == 2 ? 4 * w + lane : 16 * (lane >> 2) + 4 * w + (lane & 3));
+        s_frag[to] = make_uint4(__float_as_uint(sigma * sl2 * G::UNIT), __float_as_uint(sum * sl2), (uint32_t)len, 0);
     }
-    uint4 *dst = qprep + (int64_t)u * G::PREP + lane;
-#pragma unroll
-    for (int kk = 0; kk < G::NCH; kk++) dst[32 * kk] = make_uint4(qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3]);
-    dst[32 * G::NCH] = make_uint4(__float_as_uint(sigma * sl2 * G::UNIT), __float_as_uint(sum * sl2),
-                                  (uint32_t)(kMagicBits - 8 * ones[0]), (uint32_t)(kMagicBits - 8 * ones[2]));
+    __syncthreads();
+    for (int i = threadIdx.x; i < G::PREP; i += 32 * G::HB) qprep[(int64_t)u * G::PREP + i] = s_frag[i];
 }
 
 template <typename T, int BITS, int D, int ND>
@@ -423,7 +367,6 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
     griddep_wait();  // the prep kernel's digits (it had waited for everything before it)
 
     uint32_t qa[G::NCH][4];       // query digits, A fragments; 4 bits: of even dimensions, then of odd ones
-    int qlo0 = 0, qlo1 = 0;       // 4 bits: where sums over even dimensions start, -8 times the digits' sum
     float c1 = 0.0f, c2 = 0.0f, c3 = 0.0f;  // score constants of the lane's head
     // what the digit in the accumulators' upper rows counts, beside 1 for the one in the lower rows
     const float wtop = ND == 3 && r < 4 ? 65536.0f : 256.0f;
@@ -443,7 +386,6 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         // ---- scores: tile pair p holds tokens 16 p + 4 q + e of the lane's head ----
         float sc[4 * G::NPR];
         float smax = -INFINITY;
-        const f2 less = pair(-kMagic, -kMagic);
 #pragma unroll
         for (int p = 0; p < G::NPR; p++) {
 #pragma unroll
@@ -465,31 +407,29 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                     }
                 }
                 int d[4];
-                f2 t0, t1;  // sums of the upper and of the lower digits, of two tokens
                 if constexpr (BITS == 4) {
                     constexpr int kHalf = G::NCH / 2;
-                    int lo[4];
-                    mma_s8s8(lo, qa[0], codes_lo(wv[0]), codes_lo(wv[1]), qlo0, qlo0, qlo1, qlo1);
+                    mma_s8s8(d, qa[0], codes4(wv[0] * 16u), codes4(wv[1] * 16u), 0, 0, 0, 0);
                     if constexpr (kHalf == 2)
-                        mma_s8s8(lo, qa[1], codes_lo(wv[2]), codes_lo(wv[3]), lo[0], lo[1], lo[2], lo[3]);
-                    mma_s8s8(d, qa[kHalf], codes_hi(wv[0]), codes_hi(wv[1]), kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+                        mma_s8s8(d, qa[1], codes4(wv[2] * 16u), codes4(wv[3] * 16u), d[0], d[1], d[2], d[3]);
+                    mma_s8s8(d, qa[kHalf], codes4(wv[0]), codes4(wv[1]), d[0], d[1], d[2], d[3]);
                     if constexpr (kHalf == 2)
-                        mma_s8s8(d, qa[kHalf + 1], codes_hi(wv[2]), codes_hi(wv[3]), d[0], d[1], d[2], d[3]);
-                    const f2 sixteen = pair(16.0f, 16.0f);
-                    t0 = fma2(add2(pair_bits(lo[0], lo[1]), less), sixteen, add2(pair_bits(d[0], d[1]), less));
-                    t1 = fma2(add2(pair_bits(lo[2], lo[3]), less), sixteen, add2(pair_bits(d[2], d[3]), less));
+                        mma_s8s8(d, qa[kHalf + 1], codes4(wv[2]), codes4(wv[3]), d[0], d[1], d[2], d[3]);
                 } else {
-                    mma_s8s8(d, qa[0], codes8(wv[0]), codes8(wv[1]), kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+                    mma_s8s8(d, qa[0], codes8(wv[0]), codes8(wv[1]), 0, 0, 0, 0);
 #pragma unroll
                     for (int k = 1; k < G::NCH; k++)
                         mma_s8s8(d, qa[k], codes8(wv[2 * k]), codes8(wv[2 * k + 1]), d[0], d[1], d[2], d[3]);
-                    t0 = add2(pair_bits(d[0], d[1]), less);
-                    t1 = add2(pair_bits(d[2], d[3]), less);
                 }
-                split(fma2(t0, pair(wtop, wtop), t1), sc[4 * p + 2 * j], sc[4 * p + 2 * j + 1]);
-                if constexpr (ND == 3) {  // the other digits' part is the lane's that is four heads away
-                    sc[4 * p + 2 * j] += __shfl_xor_sync(0xffffffffu, sc[4 * p + 2 * j], 16);
-                    sc[4 * p + 2 * j + 1] += __shfl_xor_sync(0xffffffffu, sc[4 * p + 2 * j + 1], 16);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    float &dot = sc[4 * p + 2 * j + x];
+                    if constexpr (ND == 2) {
+                        dot = (float)(d[x] * 256 + d[2 + x]);
+                    } else {  // the other digits' part is the lane's that is four heads away
+                        dot = fmaf((float)d[x], wtop, (float)d[2 + x]);
+                        dot += __shfl_xor_sync(0xffffffffu, dot, 16);
+                    }
                 }
             }
             const float4 km0 = *reinterpret_cast<const float4 *>(kmeta + (16 * p + 4 * q) * 8);
@@ -549,16 +489,22 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         // ---- values: 16-byte piece v of the V blocks at a time, its integer sums folded at once ----
         // 4 bits: one sum over the bytes as they are, u (lo + 16 hi), and one over 16 (hi - 8); the first starts at
         // -(8 + 128) sum(u), so that their difference is the sum of u (lo - 8)
-        int first[4] = {0, 0, 0, 0};
+        [[maybe_unused]] int first[4] = {0, 0, 0, 0};
         if constexpr (BITS == 4) {
 #pragma unroll
             for (int t = 0; t < CT / 32; t++) mma_u8u8(first, ua[t], kOnes, kOnes, first[0], first[1], first[2], first[3]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) first[i] = first[i] * -136 + kMagicBits;
+            for (int i = 0; i < 4; i++) first[i] *= -136;
         }
-        // weights of the upper and lower digit
-        const f2 w0 = pair(fn * wtop, fn * wtop), w1 = pair(fn, fn);
-        const f2 h0 = pair(fn * wtop * G::UNIT, fn * wtop * G::UNIT), h1 = pair(fn * G::UNIT, fn * G::UNIT);
+        // adds n-tile sums, weighed w, to the value sums
+        auto fold = [&](f2 &sum, const int (&d)[4], float w) {
+            if constexpr (ND == 2) {
+                sum = fma2(pair((float)(d[0] * 256 + d[2]), (float)(d[1] * 256 + d[3])), pair(w, w), sum);
+            } else {
+                sum = fma2(pair((float)d[0], (float)d[1]), pair(w * wtop, w * wtop), sum);
+                sum = fma2(pair((float)d[2], (float)d[3]), pair(w, w), sum);
+            }
+        };
 #pragma unroll
         for (int v = 0; v < G::VV; v++) {
             constexpr int NJ = BITS == 4 ? 8 : 4;  // n-tiles of the piece
@@ -575,34 +521,28 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                         int (&raw)[4] = acc[2 * j], (&hi)[4] = acc[2 * j + 1];
                         if (t == 0) {
                             mma_u8u8(raw, ua[t], y0[j], y1[j], first[0], first[1], first[2], first[3]);
-                            mma_u8s8(hi, ua[t], codes_hi(y0[j]), codes_hi(y1[j]), kMagicBits, kMagicBits, kMagicBits,
-                                     kMagicBits);
+                            mma_u8s8(hi, ua[t], codes4(y0[j]), codes4(y1[j]), 0, 0, 0, 0);
                         } else {
                             mma_u8u8(raw, ua[t], y0[j], y1[j], raw[0], raw[1], raw[2], raw[3]);
-                            mma_u8s8(hi, ua[t], codes_hi(y0[j]), codes_hi(y1[j]), hi[0], hi[1], hi[2], hi[3]);
+                            mma_u8s8(hi, ua[t], codes4(y0[j]), codes4(y1[j]), hi[0], hi[1], hi[2], hi[3]);
                         }
                     } else {
                         int (&d)[4] = acc[j];
-                        if (t == 0)
-                            mma_u8s8(d, ua[t], codes8(y0[j]), codes8(y1[j]), kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+                        if (t == 0) mma_u8s8(d, ua[t], codes8(y0[j]), codes8(y1[j]), 0, 0, 0, 0);
                         else mma_u8s8(d, ua[t], codes8(y0[j]), codes8(y1[j]), d[0], d[1], d[2], d[3]);
                     }
                 }
             }
-            const f2 minus = pair(-1.0f, -1.0f);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if constexpr (BITS == 4) {
-                    const int (&raw)[4] = acc[2 * j], (&hi)[4] = acc[2 * j + 1];
-                    const f2 ra = pair_bits(raw[0], raw[1]), rb = pair_bits(raw[2], raw[3]);
-                    const f2 ha = pair_bits(hi[0], hi[1]), hb = pair_bits(hi[2], hi[3]);
-                    f2 &lo_sum = facc[v * NJ + 2 * j], &hi_sum = facc[v * NJ + 2 * j + 1];
-                    lo_sum = fma2(fma2(hb, minus, rb), w1, fma2(fma2(ha, minus, ra), w0, lo_sum));
-                    hi_sum = fma2(add2(hb, less), h1, fma2(add2(ha, less), h0, hi_sum));
+                    int (&raw)[4] = acc[2 * j], (&hi)[4] = acc[2 * j + 1];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) raw[i] -= hi[i];
+                    fold(facc[v * NJ + 2 * j], raw, fn);
+                    fold(facc[v * NJ + 2 * j + 1], hi, fn * G::UNIT);
                 } else {
-                    f2 &sum = facc[v * NJ + j];
-                    sum = fma2(add2(pair_bits(acc[j][2], acc[j][3]), less), w1,
-                               fma2(add2(pair_bits(acc[j][0], acc[j][1]), less), w0, sum));
+                    fold(facc[v * NJ + j], acc[j], fn);
                 }
             }
         }
@@ -619,7 +559,6 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
             L = Z = 0.0f;
 #pragma unroll
             for (int i = 0; i < G::NF / 2; i++) facc[i] = 0;
-            len = visible(a, row0 + cur.r, false);
             const uint4 *src = qprep + ((int64_t)cur.r * upr + cur.h * hblocks + cur.hb) * G::PREP + lane;
 #pragma unroll
             for (int k = 0; k < G::NCH; k++) {
@@ -633,8 +572,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
             c1 = __uint_as_float(v.x);
             c2 = __uint_as_float(v.y);
             c3 = G::CENTRE * c2;
-            qlo0 = (int)v.z;
-            qlo1 = (int)v.w;
+            len = (int)v.z;
         }
         if (!mbar_wait_bounded(bars + st, phase)) failed = true;
         if (__any_sync(0xffffffffu, failed)) {
@@ -727,7 +665,7 @@ __global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
                 if (m.x == -INFINITY) L += m.y;  // NaN sums spoil the row
             }
             const int cnt = min(32, nrec - i0);
-#pragma unroll 8
+#pragma unroll 16
             for (int j = 0; j < cnt; j++) {
                 const float wj = __shfl_sync(0xffffffffu, wt, j);
                 const float *src = base + (int64_t)(i0 + j) * G::REC + hl * D + lane * EPL;
@@ -798,10 +736,9 @@ int launch_shape(const PagesAttendArgs &a, void *workspace, cudaStream_t stream)
         cfg.stream = stream;
         cfg.attrs = pdl;
         cfg.numAttrs = 1;
-        cfg.gridDim = dim3((unsigned)((n * upr + 1) / 2));
-        cfg.blockDim = dim3(64);
-        int rc = check_cuda(cudaLaunchKernelEx(&cfg, pages_prep_kernel<T, BITS, D, ND>, a, (int)row0, (int)(n * upr), hblocks,
-                                               qprep),
+        cfg.gridDim = dim3((unsigned)(n * upr));
+        cfg.blockDim = dim3(32 * G::HB);
+        int rc = check_cuda(cudaLaunchKernelEx(&cfg, pages_prep_kernel<T, BITS, D, ND>, a, (int)row0, hblocks, qprep),
                             "gqa_paged_attend prep launch");
         count_launch();
         if (rc != SA_OK) return rc;
