@@ -43,8 +43,11 @@ namespace {
 using namespace dec;
 
 constexpr int kNWP = 12;         // warps per CTA, one CTA per SM
-constexpr int kMaxRows = 1024;   // rows of a launch: its prefix sums fit in 4 KB
+constexpr int kMaxRows = 512;    // rows of a launch: their lengths and prefix sums fit in 4 KB
 constexpr int64_t kMaxUnits = 16384;  // units of a launch: bounds the workspace
+// What a unit costs beside its chunks, in chunks: its queries' preparation and the change to it take a CTA about as
+// long as four chunks' copies (0.2 us each).  48 sequences of 0 to 16000 tokens: KUNIT0 us without it, KUNIT1 with.
+constexpr int kUnitCost = 4;
 
 template <int BITS, int D, int ND>
 struct PGeo {
@@ -66,7 +69,7 @@ struct PGeo {
     static constexpr int QMAX = ND == 2 ? 32639 : 8355711;  // 127 in the top digit
     static constexpr float CENTRE = BITS == 4 ? 8.0f : 128.0f;  // the codes' middle, which the products leave out
     static constexpr float UNIT = BITS == 4 ? 0.0625f : 1.0f;  // high nibbles enter the products as 16 (c - 8)
-    static_assert(SMEM + (kMaxRows + 1) * 4 + 256 <= 227 * 1024, "shared memory");
+    static_assert(SMEM + (2 * kMaxRows + 1) * 4 + kNWP * D * (ND == 2 ? 2 : 4) + 256 <= 227 * 1024, "shared memory");
 };
 
 // d = a.b + c, signed or unsigned digits times signed codes; c may be constant (the first product of a sum).
@@ -127,10 +130,25 @@ __device__ __forceinline__ uint32_t weight_digits(float u) {
     }
 }
 
-// Where a range is: chunk c of unit (KV head h, block hb of its query heads) of row r, whose units have n chunks;
-// b: the row's sequence.
+// bulk_g2s whose lines leave L2 first: pages are read once, and everything else that the call needs (queries, tables,
+// partial records, the merge's code) stays.
+__device__ __forceinline__ uint64_t read_once_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void bulk_g2s_once(void *dst, const void *src, uint32_t bytes, uint64_t *bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;\n" ::"r"(
+            smem_u32(dst)),
+        "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
+}
+
+// Where a range is: at chunk c of unit (KV head h, block hb of its query heads) of row r, whose units have n chunks;
+// b: the row's sequence, f: the chunk's position among all.
 struct Place {
-    int r, h, hb, c, n, b;
+    int r, h, hb, c, n, b, f;
 };
 
 // Tokens that query row r (row0 + r of batch x seq_len) attends to.
@@ -151,50 +169,24 @@ __device__ __forceinline__ int visible(const PagesAttendArgs &a, int row, bool r
     return (int)pos + 1;
 }
 
-// Warps that share F chunks.
+// Warps that share F positions.
 __host__ __device__ __forceinline__ int sharing_warps(int F, int warps) { return min(warps, F); }
 
-// A CTA per unit, a warp per query head: the query rotated to its position and into the pages' frame, as digits
-// arranged as the A fragments of the scores' product (the byte of a dimension's digit lies where frag_byte says), with
-// the score constants and the row's tokens behind them.
-template <int BITS, int D>
-__device__ __forceinline__ int frag_byte(int dim, int row, int upper) {
-    constexpr int N = D / 4, NCH = D / 32;
-    const int q = dim / N, i = dim % N;  // lane (row, q) holds dimensions [q N, q N + N)
-    // 8 bits: bytes of K words 2k, 2k + 1; 4 bits: low nibbles of words 2k, 2k + 1 (first half of the steps), then high ones
-    const int k = BITS == 4 ? (i & 1) * (NCH / 2) + (i >> 4) : i >> 3, hf = BITS == 4 ? (i >> 3) & 1 : (i >> 2) & 1;
-    const int e = BITS == 4 ? (i >> 1) & 3 : i & 3;
-    return ((32 * k + 4 * row + q) * 4 + 2 * hf + !upper) * 4 + e;
-}
-
+// One query head of a unit by one warp: rotated to its position and into the pages' frame, as digits arranged as the A
+// fragments of the scores' product, with the score constants and the row's tokens behind them.  Head w of the unit
+// fills fragment row w (three digits: rows w and w + 4); head 0 also clears the rows of the heads that the unit lacks.
+// `v`: room for D digits.  Kept short: it runs once per head, and fetching long straight code costs more than running it.
 template <typename T, int BITS, int D, int ND>
-__global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
-    pages_prep_kernel(PagesAttendArgs a, int row0, int hblocks, uint4 *qprep) {
+__device__ __forceinline__ void prepare_head(const PagesAttendArgs &a, int grow, int len, int h, int hb, int w, int lane,
+                                             std::conditional_t<ND == 2, int16_t, int> *v, uint4 *unit) {
     using G = PGeo<BITS, D, ND>;
-    constexpr int EPL = D / 32;
-    __shared__ uint4 s_frag[G::PREP];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int u = blockIdx.x, upr = a.heads * hblocks;
-    const int row = u / upr, k = u - row * upr, h = k / hblocks, b = (row0 + row) / a.seq_len, s = row0 + row - b * a.seq_len;
-    const int g = (k - h * hblocks) * G::HB + w;
-    // The attention kernel starts when all CTAs here have passed the wait: what the kernels before this one wrote
-    // (pages, table, lengths) is there for it, too, and only the digits are left to wait for.
-    griddep_wait();
-    griddep_launch_dependents();
+    constexpr int EPL = D / 32, N = D / 4, kHalf = G::NCH / 2;
+    const int b = grow / a.seq_len, s = grow - b * a.seq_len, g = hb * G::HB + w;
     float x[EPL], sg[EPL];
-    const bool on = g < a.group;
     load_elems<float, EPL>(a.signs + (int64_t)h * D + lane * EPL, sg);
-    if (on) {
-        load_elems<T, EPL>(static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
-                               ((int64_t)h * a.group + g) * D + lane * EPL, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < EPL; i++) x[i] = 0.0f;
-    }
-    const int len = visible(a, row0 + row, false);
-    if (len == 0) return;  // the whole CTA
-    if (a.rope.on)
-        rope_lane<EPL>(x, lane, D, __ldcg(a.rows.lens + b) + s, a.rope.cos_cache, a.rope.sin_cache, a.rope.interleaved);
+    load_elems<T, EPL>(static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
+                           ((int64_t)h * a.group + g) * D + lane * EPL, x);
+    if (a.rope.on) rope_lane<EPL>(x, lane, D, len - 1, a.rope.cos_cache, a.rope.sin_cache, a.rope.interleaved);
 #pragma unroll
     for (int i = 0; i < EPL; i++) x[i] *= sg[i];
     warp_wht_butterfly<EPL>(x, lane, D);
@@ -208,41 +200,53 @@ __global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
     sum = warp_sum(sum);
     mabs = warp_max(mabs);
     const float sigma = mabs > 0.0f ? mabs / (float)G::QMAX : 1.0f;
-    const float inv = 1.0f / sigma, sl2 = a.scale * kLog2eF;
-    uint8_t *frag = reinterpret_cast<uint8_t *>(s_frag);
+    const float inv = 1.0f / sigma, sl2 = a.scale * kLog2eF, c1 = sigma * sl2 * G::UNIT, c2 = sum * sl2;
 #pragma unroll
-    for (int i = 0; i < EPL; i++) {
-        const int dim = lane * EPL + i;
-        const int v = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
-        const int d2 = (int)(int8_t)(v & 0xff), rest = (v - d2) >> 8;
-        if constexpr (ND == 2) {
-            frag[frag_byte<BITS, D>(dim, w, 1)] = (uint8_t)rest;
-            frag[frag_byte<BITS, D>(dim, w, 0)] = (uint8_t)d2;
-        } else {
-            const int d1 = (int)(int8_t)(rest & 0xff);
-            frag[frag_byte<BITS, D>(dim, w, 1)] = (uint8_t)((rest - d1) >> 8);
-            frag[frag_byte<BITS, D>(dim, w, 0)] = (uint8_t)d2;
-            frag[frag_byte<BITS, D>(dim, w + 4, 1)] = (uint8_t)d1;
-            frag[frag_byte<BITS, D>(dim, w + 4, 0)] = 0;
-        }
+    for (int i = 0; i < EPL; i++) v[lane * EPL + i] = min(max(__float2int_rn(x[i] * inv), -G::QMAX), G::QMAX);
+    __syncwarp();
+    // lane (side, k, q): the word of k-step k for quarter q, of row w or (side 1, three digits) w + 4
+    const int q = lane & 3, k = (lane >> 2) & 3, side = lane >> 4;
+    if (k < G::NCH && side <= ND - 2) {
+        uint32_t word[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // byte e of k-group hf: the dimension as the K words hold it.  8 bits: bytes of words 2k, 2k + 1;
+                // 4 bits: low nibbles of words 2k, 2k + 1 (first half of the steps), then high ones
+                const int i = BITS == 4 ? 16 * (k % kHalf) + 8 * hf + 2 * e + k / kHalf : 8 * k + 4 * hf + e;
+                const int x = v[q * N + i], d2 = (int)(int8_t)(x & 0xff), rest = (x - d2) >> 8;
+                int up = rest, low = d2;
+                if constexpr (ND == 3) {
+                    const int d1 = (int)(int8_t)(rest & 0xff);
+                    up = side ? d1 : (rest - d1) >> 8;
+                    low = side ? 0 : d2;
+                }
+                word[2 * hf] |= ((uint32_t)up & 0xffu) << (8 * e);
+                word[2 * hf + 1] |= ((uint32_t)low & 0xffu) << (8 * e);
+            }
+        unit[32 * k + 4 * (w + 4 * side) + q] = make_uint4(word[0], word[1], word[2], word[3]);
     }
-    if (lane < 32 / G::HB) {  // constants of the lanes that hold this head
-        const int to = 32 * G::NCH + (ND == 2 ? 4 * w + lane : 16 * (lane >> 2) + 4 * w + (lane & 3));
-        s_frag[to] = make_uint4(__float_as_uint(sigma * sl2 * G::UNIT), __float_as_uint(sum * sl2), (uint32_t)len, 0);
+    if (lane < 4 * (ND - 1))
+        unit[32 * G::NCH + 4 * (w + 4 * (lane >> 2)) + q] = make_uint4(__float_as_uint(c1), __float_as_uint(c2), (uint32_t)len, 0);
+    if (w == 0) {
+        const int mine = (lane >> 2) & (G::HB - 1);  // the head of this lane's row
+        if (hb * G::HB + mine >= a.group)
+            for (int i = 0; i <= G::NCH; i++) unit[32 * i + lane] = make_uint4(0, 0, i == G::NCH ? (uint32_t)len : 0, 0);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < G::PREP; i += 32 * G::HB) qprep[(int64_t)u * G::PREP + i] = s_frag[i];
+    __syncwarp();
 }
 
 template <typename T, int BITS, int D, int ND>
 __global__ void __launch_bounds__(kNWP * 32, 1)
-    pages_attend_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, const uint4 *qprep, int *prefix_out,
-                        float *records) {
+    pages_attend_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, uint4 *qprep, int *prefix_out, float *records) {
     using G = PGeo<BITS, D, ND>;
     constexpr int KB = G::KB, CT = G::CT, N = D / 4;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int s_prefix[kMaxRows + 1];
+    __shared__ int s_prefix[kMaxRows + 1];  // of the rows' units: chunks and kUnitCost, nothing for rows without tokens
+    __shared__ int s_len[kMaxRows];
     __shared__ int s_warp[kNWP];
+    __shared__ std::conditional_t<ND == 2, int16_t, int> s_digits[kNWP][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = lane >> 2, q = lane & 3;
     unsigned char *ring = smem + warp * G::NST * G::STAGE;
@@ -251,14 +255,17 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         for (int i = 0; i < G::NST; i++) mbar_init(bars + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     griddep_launch_dependents();
+    griddep_wait();  // pages, table, lengths and the query may come from the kernels before
 
-    // prefix sums of the rows' chunks
+    // lengths of the rows, and prefix sums of what their units cost
     {
         int carry = 0;
         if (tid == 0) s_prefix[0] = 0;
         for (int base = 0; base < rows; base += kNWP * 32) {
             const int i = base + tid;
-            int v = i < rows ? (visible(a, row0 + i, blockIdx.x == 0) + CT - 1) / CT : 0;
+            const int len = i < rows ? visible(a, row0 + i, blockIdx.x == 0) : 0;
+            if (i < rows) s_len[i] = len;
+            int v = len > 0 ? (len + CT - 1) / CT + kUnitCost : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, v, o);
@@ -279,33 +286,41 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
     const int upr = a.heads * hblocks;  // units per row
     if (blockIdx.x == 0)
         for (int i = tid; i <= rows; i += kNWP * 32) prefix_out[i] = s_prefix[i];
-    const int F = s_prefix[rows] * upr;  // fits: the launch bounds it
+    const int F = s_prefix[rows] * upr;  // positions; fits: the launch bounds it
     const int W = sharing_warps(F, (int)gridDim.x * kNWP);
-    const int w = warp * (int)gridDim.x + blockIdx.x;  // neighbours in the flat order run on different SMs
-    if (w >= W) return;  // warps are independent from here on
-    const int f0 = (int)((int64_t)w * F / W), f1 = (int)((int64_t)(w + 1) * F / W);
+    const int C = min((int)gridDim.x, W), cta = blockIdx.x;
+    if (cta >= C) return;
+    // this CTA's warps of the W, and this warp
+    const int w0 = (int)((int64_t)cta * W / C), w1 = (int)((int64_t)(cta + 1) * W / C), w = w0 + warp;
+    const int f0 = (int)((int64_t)min(w, w1) * F / W), f1 = w < w1 ? (int)((int64_t)(w + 1) * F / W) : f0;
 
-    Place cur;
-    {
-        // the last row that begins at or before f0 and has chunks
+    // where position f lies; a unit's first kUnitCost positions stand for its first chunk
+    auto place = [&](int f) {
+        // the last row that begins at or before f and has tokens
         int lo = 0, hi = rows;
-        const int target = f0 / upr;
+        const int target = f / upr;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (s_prefix[mid] <= target) lo = mid;
             else hi = mid;
         }
-        cur.r = lo;
-        cur.n = s_prefix[lo + 1] - s_prefix[lo];
-        const int off = f0 - s_prefix[lo] * upr, k = off / cur.n;
-        cur.c = off - k * cur.n;
-        cur.h = k / hblocks;
-        cur.hb = k - cur.h * hblocks;
-        cur.b = (row0 + lo) / a.seq_len;
-    }
+        Place p;
+        p.r = lo;
+        const int cost = s_prefix[lo + 1] - s_prefix[lo], off = f - s_prefix[lo] * upr, k = off / cost;
+        p.n = cost - kUnitCost;
+        p.c = max(off - k * cost - kUnitCost, 0);
+        p.f = s_prefix[lo] * upr + k * cost + kUnitCost + p.c;
+        p.h = k / hblocks;
+        p.hb = k - p.h * hblocks;
+        p.b = (row0 + lo) / a.seq_len;
+        return p;
+    };
+    Place cur = place(min(f0, F - 1));
     auto advance = [&](Place &p) {
+        p.f++;
         if (++p.c < p.n) return;
         p.c = 0;
+        p.f += kUnitCost;
         if (++p.hb < hblocks) return;
         p.hb = 0;
         if (++p.h < a.heads) return;
@@ -315,19 +330,20 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                 p.r = rows - 1;
                 return;
             }
-            p.n = s_prefix[p.r + 1] - s_prefix[p.r];
-        } while (p.n == 0);
+            p.n = s_prefix[p.r + 1] - s_prefix[p.r] - kUnitCost;
+        } while (p.n < 0);
         p.b = (row0 + p.r) / a.seq_len;
     };
     auto page_of = [&](const Place &p) { return __ldcg(a.rows.table + (int64_t)p.b * a.rows.table_stride + p.c / G::CPP); };
 
     // copies run NST chunks ahead; the page of the next chunk to copy is fetched one step before
+    const uint64_t policy = read_once_policy();
     Place ahead = cur;
-    int fa = f0, page = page_of(ahead);
+    int page = page_of(ahead);
     unsigned pend = 0, bad = 0;
     bool failed = false;
     auto issue = [&](int st) {
-        if (fa < f1) {
+        if (ahead.f < f1) {
             uint64_t *bar = bars + st;
             if (page < 0 || page >= a.rows.num_pages) {
                 bad |= 1u << st;
@@ -343,7 +359,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                 if constexpr (G::CPP == 1) {
                     if (lane == 0) {
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // after the warp's reads of the stage
-                        bulk_g2s(dst, rec, G::STAGE, bar);
+                        bulk_g2s_once(dst, rec, G::STAGE, bar, policy);
                     }
                 } else if (lane < 4) {
                     const int part = ahead.c % G::CPP;
@@ -352,19 +368,31 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                     const int from = lane == 0 ? 0 : lane == 1 ? page_k_meta(KB) : lane == 2 ? page_v_meta(KB) : page_v_codes(KB);
                     const int to = lane == 0 ? 0 : CT * KB + (lane - 1) * CT * 8;
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    bulk_g2s(dst + to, rec + from + part * nb, nb, bar);
+                    bulk_g2s_once(dst + to, rec + from + part * nb, nb, bar, policy);
                 }
             }
             pend |= 1u << st;
-            if (++fa < f1) {
-                advance(ahead);
-                page = page_of(ahead);
-            }
+            advance(ahead);
+            if (ahead.f < f1) page = page_of(ahead);
         }
     };
 #pragma unroll
     for (int i = 0; i < G::NST; i++) issue(i);
-    griddep_wait();  // the prep kernel's digits (it had waited for everything before it)
+
+    // the queries of the CTA's units, a warp per head, while the first copies are under way
+    uint4 *cta_prep = qprep + (int64_t)cta * G::PREP;  // unit u at u + cta: no two CTAs write the same words
+    {
+        const Place lo = place((int)((int64_t)w0 * F / W)), hi = place((int)((int64_t)w1 * F / W) - 1);
+        const int u0 = lo.r * upr + lo.h * hblocks + lo.hb, u1 = hi.r * upr + hi.h * hblocks + hi.hb;
+        const int per = min(a.group, G::HB);  // heads of a unit, but in a last block that has fewer
+        for (int t = warp; t < (u1 - u0 + 1) * per; t += kNWP) {
+            const int u = u0 + t / per, hw = t % per, row = u / upr, k = u - row * upr, h = k / hblocks, hb = k - h * hblocks;
+            if (s_len[row] > 0 && hb * G::HB + hw < a.group)
+                prepare_head<T, BITS, D, ND>(a, row0 + row, s_len[row], h, hb, hw, lane, s_digits[warp],
+                                             cta_prep + (int64_t)u * G::PREP);
+        }
+    }
+    __syncthreads();
 
     uint32_t qa[G::NCH][4];       // query digits, A fragments; 4 bits: of even dimensions, then of odd ones
     float c1 = 0.0f, c2 = 0.0f, c3 = 0.0f;  // score constants of the lane's head
@@ -551,15 +579,15 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
     bool fresh = true;
     int st = 0;
     uint32_t phase = 0;
-    for (int f = f0; f < f1; f++) {
+    while (cur.f < f1) {
         if (fresh) {
-            // ---- a new unit: its digits and constants as the prep kernel left them ----
+            // ---- a new unit: its digits and constants ----
             fresh = false;
             R = -INFINITY;
             L = Z = 0.0f;
 #pragma unroll
             for (int i = 0; i < G::NF / 2; i++) facc[i] = 0;
-            const uint4 *src = qprep + ((int64_t)cur.r * upr + cur.h * hblocks + cur.hb) * G::PREP + lane;
+            const uint4 *src = cta_prep + ((int64_t)cur.r * upr + cur.h * hblocks + cur.hb) * G::PREP + lane;
 #pragma unroll
             for (int k = 0; k < G::NCH; k++) {
                 const uint4 v = src[32 * k];
@@ -591,7 +619,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         }
         const Place was = cur;
         advance(cur);
-        if (f + 1 == f1 || cur.c == 0) {
+        if (cur.f >= f1 || cur.c == 0) {
             // ---- the unit's partial record ----
 #pragma unroll
             for (int lm = 1; lm < 4; lm <<= 1) {
@@ -631,7 +659,7 @@ __global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
     pages_merge_kernel(PagesAttendArgs a, int row0, int rows, int hblocks, int warps, const int *prefix,
                        const float *records) {
     using G = PGeo<BITS, D, ND>;
-    constexpr int EPL = D / 32;
+    constexpr int EPL = D / 32, kBatch = 8;
     __shared__ float s_x[G::HB][D];
     const int lane = threadIdx.x & 31, hl = threadIdx.x >> 5;
     const int upr = a.heads * hblocks;
@@ -642,16 +670,29 @@ __global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
     for (int e = 0; e < EPL; e++) sg[e] = a.wht_scale * a.signs[(int64_t)h * D + lane * EPL + e];
     griddep_wait();
     if (g >= a.group) return;
-    const int p0 = prefix[row], n = prefix[row + 1] - p0;
+    const int p0 = prefix[row], cost = prefix[row + 1] - p0;
     float x[EPL], L = 0.0f, Z = 0.0f;
 #pragma unroll
     for (int e = 0; e < EPL; e++) x[e] = 0.0f;
-    if (n > 0) {
+    if (cost > 0) {
         const int F = prefix[rows] * upr, W = sharing_warps(F, warps);
-        const int f0 = p0 * upr + k * n;
-        const int w_lo = warp_of_chunk(f0, F, W), w_hi = warp_of_chunk(f0 + n - 1, F, W);
+        const int f0 = p0 * upr + k * cost;  // the unit's chunks are at [f0 + kUnitCost, f0 + cost)
+        const int w_lo = warp_of_chunk(f0 + kUnitCost, F, W), w_hi = warp_of_chunk(f0 + cost - 1, F, W);
         const float *base = records + ((int64_t)u + w_lo) * G::REC;
         const int nrec = w_hi - w_lo + 1;
+        // batches of records are loaded together, the first one along with what weighs them
+        using Vec = std::conditional_t<EPL == 4, float4, float2>;
+        union {
+            Vec v;
+            float f[EPL];
+        } val[kBatch];
+        auto load = [&](int j0) {
+#pragma unroll
+            for (int j = 0; j < kBatch; j++)
+                if (j0 + j < nrec)
+                    val[j].v = *reinterpret_cast<const Vec *>(base + (int64_t)(j0 + j) * G::REC + hl * D + lane * EPL);
+        };
+        load(0);
         float M = -INFINITY;
         for (int i = lane; i < nrec; i += 32) M = fmaxf(M, base[(int64_t)i * G::REC + G::HB * D + 4 * hl]);
         M = warp_max(M);
@@ -664,13 +705,15 @@ __global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
                 Z = fmaf(wt, m.z, Z);
                 if (m.x == -INFINITY) L += m.y;  // NaN sums spoil the row
             }
-            const int cnt = min(32, nrec - i0);
-#pragma unroll 16
-            for (int j = 0; j < cnt; j++) {
-                const float wj = __shfl_sync(0xffffffffu, wt, j);
-                const float *src = base + (int64_t)(i0 + j) * G::REC + hl * D + lane * EPL;
+            for (int j0 = i0; j0 < min(nrec, i0 + 32); j0 += kBatch) {
+                if (j0 > 0) load(j0);
 #pragma unroll
-                for (int e = 0; e < EPL; e++) x[e] = fmaf(wj, src[e], x[e]);
+                for (int j = 0; j < kBatch; j++) {
+                    const float wj = __shfl_sync(0xffffffffu, wt, (j0 + j) & 31);
+                    if (j0 + j < nrec)
+#pragma unroll
+                        for (int e = 0; e < EPL; e++) x[e] = fmaf(wj, val[j].f[e], x[e]);
+                }
             }
         }
     }
@@ -719,11 +762,11 @@ int launch_shape(const PagesAttendArgs &a, void *workspace, cudaStream_t stream)
     }
     const int hblocks = (a.group + G::HB - 1) / G::HB;
     const int64_t upr = (int64_t)a.heads * hblocks, rows = (int64_t)a.batch * a.seq_len, per = rows_per_launch(upr);
-    const int64_t row_chunks = upr * a.rows.max_pages * G::CPP;
+    const int64_t row_chunks = upr * ((int64_t)a.rows.max_pages * G::CPP + kUnitCost);
     const int64_t most = rows < per ? rows : per;
     int *prefix = static_cast<int *>(workspace);
     uint4 *qprep = reinterpret_cast<uint4 *>(static_cast<char *>(workspace) + kPrefixBytes);
-    float *records = reinterpret_cast<float *>(qprep + most * upr * G::PREP);
+    float *records = reinterpret_cast<float *>(qprep + (most * upr + a.sm_count) * G::PREP);
     for (int64_t row0 = 0; row0 < rows;) {
         int64_t n = rows - row0 < per ? rows - row0 : per;
         if (n * row_chunks >= ((int64_t)1 << 31)) n = (((int64_t)1 << 31) - 1) / row_chunks;  // chunk indices are ints
@@ -736,16 +779,10 @@ int launch_shape(const PagesAttendArgs &a, void *workspace, cudaStream_t stream)
         cfg.stream = stream;
         cfg.attrs = pdl;
         cfg.numAttrs = 1;
-        cfg.gridDim = dim3((unsigned)(n * upr));
-        cfg.blockDim = dim3(32 * G::HB);
-        int rc = check_cuda(cudaLaunchKernelEx(&cfg, pages_prep_kernel<T, BITS, D, ND>, a, (int)row0, hblocks, qprep),
-                            "gqa_paged_attend prep launch");
-        count_launch();
-        if (rc != SA_OK) return rc;
         cfg.gridDim = dim3((unsigned)a.sm_count);
         cfg.blockDim = dim3(kNWP * 32);
         cfg.dynamicSmemBytes = G::SMEM;
-        rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, a, (int)row0, (int)n, hblocks, (const uint4 *)qprep, prefix, records),
+        int rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, a, (int)row0, (int)n, hblocks, qprep, prefix, records),
                             "gqa_paged_attend launch");
         count_launch();
         if (rc != SA_OK) return rc;
@@ -778,7 +815,7 @@ size_t pages_attend_workspace(const kv_pages_impl *k, int batch, int seq_len, in
     const int64_t upr = (int64_t)k->cfg.kv_head_count * ((k->group + hb - 1) / hb);
     const int64_t rows = (int64_t)batch * seq_len, per = rows_per_launch(upr), n = rows < per ? rows : per;
     const int64_t records = (int64_t)k->sm_count * kNWP + n * upr;  // one per warp, and one more per unit
-    const size_t prep = (size_t)(n * upr) * 32 * (k->cfg.head_dim / 32 + 1) * 16;  // digits and constants of a unit
+    const size_t prep = (size_t)(n * upr + k->sm_count) * 32 * (k->cfg.head_dim / 32 + 1) * 16;  // digits and constants of a unit
     return kPrefixBytes + prep + (size_t)records * hb * (k->cfg.head_dim + 4) * sizeof(float);
 }
 
