@@ -16,6 +16,8 @@
 // not depend on where a row begins, so that beams that are equal tie exactly.
 #include <math.h>
 
+#include <type_traits>
+
 #include "sa_decode_common.cuh"
 #include "sa_pages.cuh"
 
@@ -26,7 +28,6 @@ namespace {
 constexpr int kGroup = 256;      // tokens of a group
 constexpr int kScanThreads = 256;
 constexpr int kPickThreads = 512;
-constexpr int kAhead = 4;        // groups a warp loads at once
 constexpr int kScanWarps = 148 * 48;  // warps that the scan is split into where rows allow it
 constexpr float kL = 1.4426950408889634f;  // log2(e)
 
@@ -38,26 +39,82 @@ struct Part {
 
 int64_t groups_of(int64_t vocab) { return (vocab + kGroup - 1) / kGroup; }
 int parts_per_row(int64_t rows, int64_t groups) {
-    const int64_t want = (kScanWarps + rows - 1) / rows, most = (groups + kAhead - 1) / kAhead;
+    const int64_t want = (kScanWarps + rows - 1) / rows, most = (groups + 3) / 4;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-// Eight tokens of group g; -inf outside the row.  PIECES (all rows begin on 16 bytes): neighbours, one 16-byte load
-// (two of f32); else every 32nd, so that the warp's loads are neighbours wherever the row begins.
+// Eight tokens of a group that a lane holds, as they were loaded; -inf outside the row.  PIECES (all rows begin on 16
+// bytes): neighbours, one 16-byte load (two of f32); else every 32nd, so that the warp's loads are neighbours wherever
+// the row begins.  160 rows of 50257 f16: ODD0 us so, against ODD1 with eight neighbours loaded one by one.
 template <typename T, bool PIECES>
-__device__ __forceinline__ void load_tokens(const T *row, int vocab, int g, int lane, float (&x)[8]) {
-    const int64_t e0 = (int64_t)g * kGroup + (PIECES ? lane * 8 : lane);
-    constexpr int kStep = PIECES ? 1 : 32;
-    if (PIECES && e0 + 8 <= vocab) {
-        load_run<T, 8>(row + e0, true, x);
-    } else {
+struct Tokens {
+    float x[8];
+    __device__ __forceinline__ void load(const T *row, int vocab, int g, int lane) {
+        const int64_t e0 = (int64_t)g * kGroup + (PIECES ? lane * 8 : lane);
+        constexpr int kStep = PIECES ? 1 : 32;
+        if (PIECES && e0 + 8 <= vocab) {
+            load_run<T, 8>(row + e0, true, x);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = e0 + kStep * i < vocab ? ld_f32(row + e0 + kStep * i) : -INFINITY;
+            for (int i = 0; i < 8; i++) x[i] = e0 + kStep * i < vocab ? ld_f32(row + e0 + kStep * i) : -INFINITY;
+        }
     }
+    __device__ __forceinline__ float get(int i) const { return x[i]; }
+    __device__ __forceinline__ float top() const {
+        return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    }
+};
+
+// 16-bit pieces stay packed until they are used: four registers, and the largest of two at once.
+template <typename T>
+struct PackedTokens {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const T *row, int vocab, int g, int lane) {
+        const int64_t e0 = (int64_t)g * kGroup + lane * 8;
+        if (e0 + 8 <= vocab) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(row + e0);
+            w[0] = v.x;
+            w[1] = v.y;
+            w[2] = v.z;
+            w[3] = v.w;
+        } else {
+            constexpr uint32_t kNone = std::is_same<T, __half>::value ? 0xFC00u : 0xFF80u;  // -inf
+            const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                w[i] = (e0 + 2 * i < vocab ? p[e0 + 2 * i] : kNone) | (e0 + 2 * i + 1 < vocab ? p[e0 + 2 * i + 1] : kNone) << 16;
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (std::is_same<T, __half>::value)
+            return __half2float(__ushort_as_half((unsigned short)(w[i >> 1] >> (16 * (i & 1)))));
+        return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    }
+    __device__ __forceinline__ float top() const {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        T2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const T2 *>(&w[i]);
+        const T2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+        return fmaxf(DT<T>::to_f32(m.x), DT<T>::to_f32(m.y));
+    }
+};
+template <>
+struct Tokens<__half, true> : PackedTokens<__half> {};
+template <>
+struct Tokens<__nv_bfloat16, true> : PackedTokens<__nv_bfloat16> {};
+
+// The largest value of a warp; NaN counts for nothing, as in fmaxf.
+__device__ __forceinline__ float warp_top(float x) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(m) : "f"(x));
+    return m;
 }
 
 template <typename T, bool PIECES>
 __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(BeamArgs a, int groups, int parts, float *maxima, Part *sums) {
+    // groups that a warp takes at a time, while the next ones are on their way
+    constexpr int kAhead = PIECES && sizeof(T) == 2 ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * (kScanThreads / 32) + (threadIdx.x >> 5);
     dec::griddep_launch_dependents();
@@ -69,29 +126,26 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(BeamArgs a, int
     const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
     const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
     float top = -INFINITY, sum = 0.0f;
+    Tokens<T, PIECES> next[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) next[j].load(row, g0 + j < g1 ? a.vocab : 0, g0 + j, lane);
     for (int g = g0; g < g1; g += kAhead) {
-        float x[kAhead][8], m[kAhead];
+        Tokens<T, PIECES> now[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-            if (g + j < g1) {
-                load_tokens<T, PIECES>(row, a.vocab, g + j, lane, x[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[j][i] = -INFINITY;
-            }
+            now[j] = next[j];
+            next[j].load(row, g + kAhead + j < g1 ? a.vocab : 0, g + kAhead + j, lane);
         }
-        float most = top;
+        float most = top, mine = 0.0f;
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-            m[j] = x[j][0];
-#pragma unroll
-            for (int i = 1; i < 8; i++) m[j] = fmaxf(m[j], x[j][i]);
-            m[j] = warp_max(m[j]);
-            most = fmaxf(most, m[j]);
-            if (lane == 0 && g + j < g1) maxima[r * groups + g + j] = m[j];
+            const float m = warp_top(now[j].top());
+            most = fmaxf(most, m);
+            if (lane == j) mine = m;
         }
+        if (lane < kAhead && g + lane < g1) maxima[r * groups + g + lane] = mine;
         if (most > top) {
-            sum = top == -INFINITY ? sum : sum * exp2f((top - most) * kL);
+            if (top > -INFINITY) sum *= exp2f((top - most) * kL);
             top = most;
         }
         const float ref = top == -INFINITY ? 0.0f : top;
@@ -99,7 +153,7 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(BeamArgs a, int
         for (int j = 0; j < kAhead; j++) {
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) e[i] = dec::ex2_approx((x[j][i] - ref) * kL);
+            for (int i = 0; i < 8; i++) e[i] = dec::ex2_approx((now[j].get(i) - ref) * kL);
             sum += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
         }
     }
@@ -109,148 +163,207 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(BeamArgs a, int
     if (lane == 0) sums[r * parts + part] = Part{total, top, 0.0f};
 }
 
-// Scores as unsigned numbers of the same order; 0 for what is never chosen.
-__device__ __forceinline__ unsigned long long order_of(double s) {
-    if (!(s > -INFINITY)) return 0;
-    s += 0.0;  // -0 counts as 0
-    const long long b = __double_as_longlong(s);
-    return (unsigned long long)(b >= 0 ? b : ~b) ^ (b >= 0 ? 0x8000000000000000ull : 0ull);
-}
-
-struct Best {
-    unsigned long long key;
+struct Choice {
+    double score;
     unsigned place;
 };
 
-// Whether x comes before y: the larger key, then the lower place.
-__device__ __forceinline__ bool before(const Best &x, const Best &y) {
-    return x.key > y.key || (x.key == y.key && x.place < y.place);
+// Whether x comes before y: the larger score, of equal ones the lower place.
+__device__ __forceinline__ bool before(const Choice &x, const Choice &y) {
+    return x.score > y.score || (x.score == y.score && x.place < y.place);
 }
 
-__device__ __forceinline__ Best warp_best(Best b) {
-    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(b.key >> 32));
-    const bool at_hi = (unsigned)(b.key >> 32) == hi;
-    const unsigned lo = __reduce_max_sync(0xffffffffu, at_hi ? (unsigned)b.key : 0u);
-    const unsigned place = __reduce_min_sync(0xffffffffu, at_hi && (unsigned)b.key == lo ? b.place : 0xffffffffu);
-    return Best{((unsigned long long)hi << 32) | lo, place};
-}
+constexpr int kListed = 1024;  // choices that are ranked against each other
+constexpr int kEights = kPickThreads / 8;
 
-// The best of a CTA, of each thread's own best; `box` alternates between calls.
-__device__ __forceinline__ Best block_best(Best b, Best (*box)[kPickThreads / 32], int turn) {
-    const int lane = threadIdx.x & 31;
-    b = warp_best(b);
-    if (lane == 0) box[turn & 1][threadIdx.x >> 5] = b;
-    __syncthreads();
-    return warp_best(lane < kPickThreads / 32 ? box[turn & 1][lane] : Best{0, 0xffffffffu});
-}
-
+// The choice is made twice in the same way, among groups and then among the tokens of the best ones (and the finished
+// beams): the keep-th largest of the 64 best scores of eight threads each bounds the keep-th best from below (mode 0),
+// the few choices that reach it are listed (mode 1) and ranked against each other.  Where they are too many, scores
+// that are equal by the hundreds, the best is taken out one at a time (mode 2).  One piece of code serves all of that:
+// this kernel runs for a few microseconds, of which fetching its code is a good part (unrolled copies for every step
+// took 15 us after the scan of 64 x 8 beams, PICKT now).
 template <typename T>
 __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a, int groups, int parts, const float *maxima,
                                                                  const Part *sums) {
-    __shared__ double s_lse[SA_MAX_BEAMS];
-    __shared__ float s_score[SA_MAX_BEAMS];
-    __shared__ bool s_done[SA_MAX_BEAMS];
-    __shared__ unsigned s_group[SA_MAX_BEAM_KEEP];
-    __shared__ Best s_box[2][kPickThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.x, K = a.beams;
+    __shared__ double s_lse[SA_MAX_BEAMS], s_score[SA_MAX_BEAMS];  // of beams that go on; a score of -inf for the others
+    __shared__ int s_beam[SA_MAX_BEAM_KEEP], s_first[SA_MAX_BEAM_KEEP];  // of the best groups: beam, first token
+    __shared__ double s_top[kEights], s_least;
+    __shared__ Choice s_list[kListed], s_out[SA_MAX_BEAM_KEEP], s_box[2][kPickThreads / 32];
+    __shared__ int s_listed;
+    constexpr Choice kNone{-INFINITY, 0xffffffffu};
+    const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.x, K = a.beams, keep = a.keep;
     const int64_t r0 = (int64_t)b * K;
+    const T *logits = static_cast<const T *>(a.logits) + r0 * a.row_stride;
     dec::griddep_launch_dependents();
     dec::griddep_wait();
     for (int k = tid >> 5; k < K; k += kPickThreads / 32) {
+        // (a finished beam's parts were not written, and are not used)
+        const Part *p = sums + (r0 + k) * parts;
         const bool done = a.finished && a.finished[r0 + k];
-        double lse = 0.0;
-        if (!done) {
-            const Part *p = sums + (r0 + k) * parts;
-            float top = -INFINITY;
-            for (int i = lane; i < parts; i += 32) top = fmaxf(top, p[i].top);
-            top = warp_max(top);
-            double total = 0.0;
-            for (int i = lane; i < parts; i += 32)
-                if (p[i].top > -INFINITY) total += p[i].sum * exp((double)p[i].top - (double)top);
-                else total += p[i].sum;  // 0, or NaN
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            lse = (double)top + log(total);
-        }
+        float top = -INFINITY;
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, p[i].top);
+        top = warp_max(top);
+        double total = 0.0;
+        for (int i = lane; i < parts; i += 32)  // a part without a largest logit: 0, or NaN
+            total += p[i].top > -INFINITY ? p[i].sum * exp((double)p[i].top - (double)top) : p[i].sum;
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         if (lane == 0) {
-            s_lse[k] = lse;
-            s_score[k] = a.scores[r0 + k];
-            s_done[k] = done;
+            s_lse[k] = (double)top + log(total);
+            s_score[k] = done ? -INFINITY : (double)a.scores[r0 + k];
         }
     }
     __syncthreads();
 
-    // the best groups over all beams
-    int turn = 0, found = 0;
-    {
-        auto group_of = [&](int i) {
-            const int k = i / groups, g = i - k * groups;
-            double s;
-            if (s_done[k]) s = g == 0 && a.end_token >= 0 && a.end_token < a.vocab ? (double)s_score[k] : -INFINITY;
-            else s = (double)s_score[k] + ((double)maxima[(r0 + k) * groups + g] - s_lse[k]);
-            return Best{order_of(s), (unsigned)i};
-        };
-        Best last{~0ull, 0}, mine{0, 0xffffffffu};
-        bool first = true;
-        for (; found < a.keep; found++) {
-            if (first) {  // this thread's best that has not been taken
-                mine = Best{0, 0xffffffffu};
-                for (int i = tid; i < K * groups; i += kPickThreads) {
-                    const Best c = group_of(i);
-                    if (before(c, mine) && before(last, c)) mine = c;
+    int found = 0;
+#pragma unroll 1
+    for (int phase = 0; phase < 2; phase++) {
+        // keep groups hold a token each that scores what the last of them does
+        int mode = phase == 1 && found == keep ? 1 : 0, n = 0;
+        double least = mode == 1 ? s_out[keep - 1].score : -INFINITY;
+        // a thread's choices in eights; a single eight is worked out once
+        const int beams8 = (K + 7) / 8;
+        const int eights = phase == 0 ? (groups + kPickThreads - 1) / kPickThreads * beams8 : (found + 15) / 16;
+        double score[8];
+        unsigned place[8];
+        bool known = false;
+        if (tid == 0) s_listed = 0;
+        __syncthreads();
+        Choice last = kNone, mine = kNone;  // mode 2: the last one taken from this thread, its best of the others
+        bool taken = false, search = true;
+#pragma unroll 1
+        for (;;) {
+            double top = -INFINITY;
+            auto take = [&](double sc, unsigned pl) {
+                if (!(sc > -INFINITY)) return;  // NaN too
+                if (mode == 0) {
+                    if (sc > top) top = sc;
+                } else if (mode == 1) {
+                    if (sc >= least) {
+                        const int at = atomicAdd(&s_listed, 1);
+                        if (at < kListed) s_list[at] = Choice{sc, pl};
+                    }
+                } else if (search) {
+                    const Choice c{sc, pl};
+                    if (before(c, mine) && (!taken || before(last, c))) mine = c;
+                }
+            };
+#pragma unroll 1
+            for (int e = 0; e < eights; e++) {
+                if (known) {
+                } else if (phase == 0) {  // the threads share the groups of each beam
+                    const int g = e / beams8 * kPickThreads + tid, k0 = e % beams8 * 8;
+                    float m[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) m[i] = g < groups && k0 + i < K ? maxima[(r0 + k0 + i) * groups + g] : -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int k = min(k0 + i, K - 1);
+                        score[i] = s_score[k] + ((double)m[i] - s_lse[k]);
+                        place[i] = (unsigned)((k0 + i) * groups + g);
+                    }
+                } else {  // the threads share the tokens of each group
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int j = 16 * e + 2 * i + tid / kGroup, v = j < found ? s_first[j] + tid % kGroup : a.vocab;
+                        x[i] = v < a.vocab ? ld_f32(logits + s_beam[j] * a.row_stride + v) : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int j = min(16 * e + 2 * i + tid / kGroup, found - 1), k = s_beam[j];
+                        score[i] = s_score[k] + ((double)x[i] - s_lse[k]);
+                        place[i] = (unsigned)k * (unsigned)a.vocab + s_first[j] + tid % kGroup;
+                    }
+                }
+                known = eights == 1;
+#pragma unroll
+                for (int i = 0; i < 8; i++) take(score[i], place[i]);
+            }
+            if (phase == 1 && tid < K && a.finished && a.finished[r0 + tid] && a.end_token >= 0 && a.end_token < a.vocab)
+                take((double)a.scores[r0 + tid], (unsigned)tid * (unsigned)a.vocab + a.end_token);
+            if (mode == 0) {
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) {
+                    const double other = __shfl_xor_sync(0xffffffffu, top, o);
+                    if (other > top) top = other;
+                }
+                if ((tid & 7) == 0) s_top[tid >> 3] = top;
+                __syncthreads();
+                // eight threads rank one of the 64 among all
+                const double own = s_top[tid >> 3];
+                int ahead = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int j = 8 * i + (tid & 7);
+                    ahead += s_top[j] > own || (s_top[j] == own && j < tid >> 3);
+                }
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+                if ((tid & 7) == 0 && ahead == keep - 1) s_least = own;
+                __syncthreads();
+                least = s_least;
+                mode = 1;
+            } else if (mode == 1) {
+                __syncthreads();
+                n = s_listed;
+                if (n <= kListed) {
+#pragma unroll 1
+                    for (int i = tid; i < n; i += kPickThreads) {
+                        const Choice own = s_list[i];
+                        int ahead = 0;
+#pragma unroll 4
+                        for (int j = 0; j < n; j++) ahead += before(s_list[j], own);
+                        if (ahead < keep) s_out[ahead] = own;
+                    }
+                    n = min(n, keep);
+                    break;
+                }
+                n = 0;
+                mode = 2;
+            } else {
+                search = false;
+                Choice best = mine;
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {  // of a warp, then of the warps
+#pragma unroll 1
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const Choice other{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.place, o)};
+                        if (before(other, best)) best = other;
+                    }
+                    if (half == 1) break;
+                    if (lane == 0) s_box[n & 1][tid >> 5] = best;
+                    __syncthreads();
+                    best = lane < kPickThreads / 32 ? s_box[n & 1][lane] : kNone;
+                }
+                if (best.place == kNone.place || n == keep) break;
+                if (tid == 0) s_out[n] = best;
+                n++;
+                if (best.place == mine.place) {
+                    last = best;
+                    taken = search = true;
+                    mine = kNone;
                 }
             }
-            const Best best = block_best(mine, s_box, turn++);
-            if (best.key == 0) break;
-            if (tid == 0) s_group[found] = best.place;
-            first = best.place == mine.place;
-            if (first) last = best;
         }
-    }
-    __syncthreads();
-
-    // the best tokens of those groups
-    {
-        auto token_of = [&](int i) {
-            const unsigned gi = s_group[i / kGroup];
-            const int k = (int)(gi / (unsigned)groups), g = (int)(gi - (unsigned)k * groups), x = i % kGroup;
-            if (s_done[k])
-                return x == 0 ? Best{order_of((double)s_score[k]), (unsigned)(k * a.vocab + a.end_token)}
-                              : Best{0, 0xffffffffu};
-            const T *row = static_cast<const T *>(a.logits) + (r0 + k) * a.row_stride;
-            const int64_t v = (int64_t)g * kGroup + x;
-            if (v >= a.vocab) return Best{0, 0xffffffffu};
-            return Best{order_of((double)s_score[k] + ((double)ld_f32(row + v) - s_lse[k])), (unsigned)(k * a.vocab + (int)v)};
-        };
-        Best last{~0ull, 0}, mine{0, 0xffffffffu};
-        bool first = true;
-        int n = 0;
-        for (; n < a.keep; n++) {
-            if (first) {
-                mine = Best{0, 0xffffffffu};
-                for (int i = tid; i < found * kGroup; i += kPickThreads) {
-                    const Best c = token_of(i);
-                    if (before(c, mine) && before(last, c)) mine = c;
-                }
+        __syncthreads();
+        if (phase == 0) {
+            found = n;
+            if (tid < n) {
+                const int k = (int)(s_out[tid].place / (unsigned)groups);
+                s_beam[tid] = k;
+                s_first[tid] = (int)(s_out[tid].place - (unsigned)(k * groups)) * kGroup;
             }
-            const Best best = block_best(mine, s_box, turn++);
-            if (best.key == 0) break;
-            if (tid == 0) {
-                const int k = (int)(best.place / (unsigned)a.vocab);
-                const unsigned long long bits =
-                    best.key & 0x8000000000000000ull ? best.key ^ 0x8000000000000000ull : ~best.key;
-                a.parents[(int64_t)b * a.keep + n] = k;
-                a.tokens[(int64_t)b * a.keep + n] = (int)(best.place - (unsigned)k * (unsigned)a.vocab);
-                a.out_scores[(int64_t)b * a.keep + n] = (float)__longlong_as_double((long long)bits);
-            }
-            first = best.place == mine.place;
-            if (first) last = best;
+        } else if (tid < keep) {
+            const bool some = tid < n;
+            const Choice c = some ? s_out[tid] : Choice{-INFINITY, 0};
+            const int k = (int)(c.place / (unsigned)a.vocab);
+            const int64_t at = (int64_t)b * keep + tid;
+            a.parents[at] = some ? k : -1;
+            a.tokens[at] = some ? (int)(c.place - (unsigned)k * (unsigned)a.vocab) : -1;
+            a.out_scores[at] = (float)c.score;
         }
-        for (int i = n + tid; i < a.keep; i += kPickThreads) {
-            a.parents[(int64_t)b * a.keep + i] = -1;
-            a.tokens[(int64_t)b * a.keep + i] = -1;
-            a.out_scores[(int64_t)b * a.keep + i] = -INFINITY;
-        }
+        __syncthreads();
     }
 }
 
