@@ -98,24 +98,6 @@ __device__ __forceinline__ void mma_u8u8(int (&d)[4], const uint32_t (&a)[4], ui
 __device__ __forceinline__ uint32_t codes8(uint32_t w) { return w ^ 0x80808080u; }
 __device__ __forceinline__ uint32_t codes4(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
 
-// Pairs of floats.
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pair(float x, float y) {
-    f2 v;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ void split(f2 v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f2 mul2(f2 x, f2 y) {
-    f2 v;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
-    return v;
-}
-__device__ __forceinline__ f2 fma2(f2 x, f2 y, f2 z) {
-    f2 v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(x), "l"(y), "l"(z));
-    return v;
-}
 constexpr uint32_t kOnes = 0x01010101u;
 
 // A weight as a whole number up to `most`: of 16 bits the conversion saturates by itself.

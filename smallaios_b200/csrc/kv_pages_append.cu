@@ -9,6 +9,9 @@
 // vector (kv_append.cu) that saves most of the shuffles, reductions and the
 // per-vector bookkeeping.
 //
+// Sums and differences are taken in pairs (f2).  A product that a sum follows is not: a product of a pair may be
+// contracted with the sum to one rounding, __fmul_rn never is.  (Products with signs are exact either way.)
+//
 // Codes: (y - z)/s rounded half away from zero, the quotient itself rounded to
 // f32 first.  t = (y - z) * RN(1/s) is within 3 * 2^-24 * 255 of that quotient,
 // so round(t) is the same unless t lies within kTie of a half; a vector with
@@ -28,7 +31,7 @@ constexpr int kWarps = 4;
 // STEP: one new token per row, the warp's vectors are eight consecutive (row, head); else the eight positions of one
 // (row, head) that share p >> 3.
 template <typename T, int BITS, int D, bool STEP>
-__global__ void __launch_bounds__(32 * kWarps) pages_append_kernel(PagesAppendArgs a, uint32_t octs, uint32_t items) {
+__global__ void __launch_bounds__(32 * kWarps, 8) pages_append_kernel(PagesAppendArgs a, uint32_t octs, uint32_t items) {
     constexpr int N = D / 4;            // elements per lane
     constexpr int CH = N / 8;           // runs of eight
     constexpr int CB = D * BITS / 8;
@@ -44,74 +47,82 @@ __global__ void __launch_bounds__(32 * kWarps) pages_append_kernel(PagesAppendAr
     int64_t pos;
     bool live;
     int tokens = 0;
+    f2 x[N / 2];
+    auto load_vector = [&]() {
+        const T *src = static_cast<const T *>(which ? a.value : a.key) + b * a.batch_stride + s * a.token_stride +
+                       (int64_t)h * D + 8 * q;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            float v[8];
+            load_run<T, 8>(src + 32 * c, a.aligned, v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[4 * c + i] = pair(v[2 * i], v[2 * i + 1]);
+        }
+    };
     if constexpr (STEP) {
         const uint32_t u = (item >> 1) * 8 + vi;
         live = u < (uint32_t)a.batch * (uint32_t)a.heads;
         b = live ? (int)(u / (uint32_t)a.heads) : 0;
         h = live ? (int)(u - (uint32_t)b * (uint32_t)a.heads) : 0;
         s = 0;
+        load_vector();  // (of row 0 behind the last one) while the row's length and page are looked up
         live = live && row_tokens(a.rows, b, 1, pos) > 0;
         if (!live) pos = 0;
     } else {
-        const uint32_t u = item >> 1, bh = u / octs, oct = u - bh * octs;
-        b = (int)(bh / (uint32_t)a.heads);
-        h = (int)(bh - (uint32_t)b * (uint32_t)a.heads);
+        // the heads of eight tokens are neighbours in the input and in the page: they go together
+        const uint32_t u = item >> 1, bo = u / (uint32_t)a.heads, oct = bo % octs;
+        h = (int)(u - bo * (uint32_t)a.heads);
+        b = (int)(bo / octs);
         int64_t pos0;
         tokens = row_tokens(a.rows, b, a.seq_len, pos0);
         pos = (pos0 & ~(int64_t)7) + (int64_t)oct * 8 + vi;
         live = pos >= pos0 && pos < pos0 + tokens;
         s = (int)(pos - pos0);
     }
-    // the vector's place
-    uint8_t *rec = nullptr;
-    if (live) {
-        const int64_t j = pos / kPageTokens;
-        int page = -1;
-        if (j < a.rows.max_pages) page = a.rows.table[b * a.rows.table_stride + j];
-        if (page < 0 || page >= a.rows.num_pages) {
-            if (q == 0) atomicOr(a.rows.dev_status, kPagesBadPage);
-            live = false;
-        } else if (a.rope.on && pos >= a.rope.rows) {
-            if (q == 0) atomicOr(a.rows.dev_status, kPagesBadPosition);
-            live = false;
-        } else {
-            rec = a.records + ((int64_t)page * a.heads + h) * page_record(CB);
-        }
+    if (live && a.rope.on && pos >= a.rope.rows) {
+        if (q == 0) atomicOr(a.rows.dev_status, kPagesBadPosition);
+        live = false;
     }
     if (!__any_sync(0xffffffffu, live)) return;
-
-    float x[N];
-    if (live) {
-        const T *src = static_cast<const T *>(which ? a.value : a.key) + b * a.batch_stride + s * a.token_stride +
-                       (int64_t)h * D + 8 * q;
+    // the vector's page is on its way along with the vector; it is wanted for the stores only
+    int page = -1;
+    if (live && pos / kPageTokens < a.rows.max_pages) page = a.rows.table[b * a.rows.table_stride + pos / kPageTokens];
+    if (!STEP && live) load_vector();
+    if (!live) {
 #pragma unroll
-        for (int c = 0; c < CH; c++) load_run<T, 8>(src + 32 * c, a.aligned, x + 8 * c);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = 0.0f;
+        for (int i = 0; i < N / 2; i++) x[i] = 0;
     }
     if (which == 0 && a.rope.on) {  // warp-uniform
         const float *cs = a.rope.cos_cache + (live ? pos : 0) * (D / 2), *sn = a.rope.sin_cache + (live ? pos : 0) * (D / 2);
         if (a.rope.interleaved) {
 #pragma unroll
             for (int c = 0; c < CH; c++) {
-                const int p0 = 16 * c + 4 * q;  // pairs of this run
+                float co[4], si[4];  // the pairs of this run
+                load_run<float, 4>(cs + 16 * c + 4 * q, a.rope.aligned, co);
+                load_run<float, 4>(sn + 16 * c + 4 * q, a.rope.aligned, si);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float co = cs[p0 + i], si = sn[p0 + i], x0 = x[8 * c + 2 * i], x1 = x[8 * c + 2 * i + 1];
-                    x[8 * c + 2 * i] = __fsub_rn(__fmul_rn(co, x0), __fmul_rn(si, x1));
-                    x[8 * c + 2 * i + 1] = __fadd_rn(__fmul_rn(si, x0), __fmul_rn(co, x1));
+                    float x0, x1;
+                    split(x[4 * c + i], x0, x1);
+                    x[4 * c + i] = pair(__fsub_rn(__fmul_rn(co[i], x0), __fmul_rn(si[i], x1)),
+                                        __fadd_rn(__fmul_rn(si[i], x0), __fmul_rn(co[i], x1)));
                 }
             }
         } else {
 #pragma unroll
             for (int c = 0; c < CH / 2; c++) {
+                float co[8], si[8];
+                load_run<float, 8>(cs + 32 * c + 8 * q, a.rope.aligned, co);
+                load_run<float, 8>(sn + 32 * c + 8 * q, a.rope.aligned, si);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int p = 32 * c + 8 * q + i;
-                    const float co = cs[p], si = sn[p], x0 = x[8 * c + i], x1 = x[8 * (c + CH / 2) + i];
-                    x[8 * c + i] = __fsub_rn(__fmul_rn(co, x0), __fmul_rn(si, x1));
-                    x[8 * (c + CH / 2) + i] = __fadd_rn(__fmul_rn(si, x0), __fmul_rn(co, x1));
+                for (int i = 0; i < 4; i++) {
+                    f2 &lo = x[4 * c + i], &hi = x[4 * (c + CH / 2) + i];
+                    float x0[2], x1[2];
+                    split(lo, x0[0], x0[1]);
+                    split(hi, x1[0], x1[1]);
+                    const float c0 = co[2 * i], c1 = co[2 * i + 1], s0 = si[2 * i], s1 = si[2 * i + 1];
+                    lo = sub2(pair(__fmul_rn(c0, x0[0]), __fmul_rn(c1, x0[1])), pair(__fmul_rn(s0, x1[0]), __fmul_rn(s1, x1[1])));
+                    hi = add2(pair(__fmul_rn(s0, x0[0]), __fmul_rn(s1, x0[1])), pair(__fmul_rn(c0, x1[0]), __fmul_rn(c1, x1[1])));
                 }
             }
         }
@@ -119,45 +130,55 @@ __global__ void __launch_bounds__(32 * kWarps) pages_append_kernel(PagesAppendAr
     {
         const float *sg = a.signs + (int64_t)h * D + 8 * q;
 #pragma unroll
-        for (int c = 0; c < CH; c++)
+        for (int c = 0; c < CH; c++) {
+            float sgn[8];
+            load_run<float, 8>(sg + 32 * c, true, sgn);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[8 * c + i] = __fmul_rn(x[8 * c + i], sg[32 * c + i]);
+            for (int i = 0; i < 4; i++) x[4 * c + i] = mul2(x[4 * c + i], pair(sgn[2 * i], sgn[2 * i + 1]));
+        }
     }
-    // butterfly stages h = 1, 2, 4 (in a run), 8, 16 (across lanes), 32, 64 (between runs)
+    // butterfly stages h = 1 (in a pair), 2, 4 (in a run), 8, 16 (across lanes), 32, 64 (between runs)
 #pragma unroll
-    for (int hs = 1; hs < 8; hs <<= 1)
+    for (int i = 0; i < N / 2; i++) {
+        float p0, p1;
+        split(x[i], p0, p1);
+        x[i] = pair(__fadd_rn(p0, p1), __fsub_rn(p0, p1));
+    }
+    auto butterfly = [&](int hs) {  // of pairs
 #pragma unroll
-        for (int i = 0; i < N; i++)
+        for (int i = 0; i < N / 2; i++)
             if ((i & hs) == 0) {
-                const float p0 = x[i], p1 = x[i + hs];
-                x[i] = __fadd_rn(p0, p1);
-                x[i + hs] = __fsub_rn(p0, p1);
+                const f2 p0 = x[i], p1 = x[i + hs];
+                x[i] = add2(p0, p1);
+                x[i + hs] = sub2(p0, p1);
             }
+    };
+    butterfly(1);
+    butterfly(2);
 #pragma unroll
     for (int lm = 1; lm < 4; lm <<= 1) {
-        // upper lane: other - x, lower lane: x + other = other - (-x), exactly
-        const uint32_t flip = (lane & lm) ? 0u : 0x80000000u;
+        // upper lane: other - x, lower lane: x + other
+        const float side = (lane & lm) ? -1.0f : 1.0f;
+        const f2 sides = pair(side, side);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float other = __shfl_xor_sync(0xffffffffu, x[i], lm);
-            x[i] = __fsub_rn(other, __uint_as_float(__float_as_uint(x[i]) ^ flip));
+        for (int i = 0; i < N / 2; i++) {
+            float p0, p1;
+            split(x[i], p0, p1);
+            x[i] = fma2(x[i], sides, pair(__shfl_xor_sync(0xffffffffu, p0, lm), __shfl_xor_sync(0xffffffffu, p1, lm)));
         }
     }
 #pragma unroll
-    for (int hs = 8; hs < N; hs <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if ((i & hs) == 0) {
-                const float p0 = x[i], p1 = x[i + hs];
-                x[i] = __fadd_rn(p0, p1);
-                x[i + hs] = __fsub_rn(p0, p1);
-            }
+    for (int hs = 4; hs < N / 2; hs <<= 1) butterfly(hs);
     float mn = INFINITY, mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        x[i] = __fmul_rn(x[i], a.wht_scale);
-        mn = fminf(mn, x[i]);
-        mx = fmaxf(mx, x[i]);
+    for (int i = 0; i < N / 2; i++) {
+        float p0, p1;
+        split(x[i], p0, p1);
+        p0 = __fmul_rn(p0, a.wht_scale);
+        p1 = __fmul_rn(p1, a.wht_scale);
+        x[i] = pair(p0, p1);
+        mn = fminf(mn, fminf(p0, p1));
+        mx = fmaxf(mx, fmaxf(p0, p1));
     }
 #pragma unroll
     for (int lm = 1; lm < 4; lm <<= 1) {
@@ -168,8 +189,11 @@ __global__ void __launch_bounds__(32 * kWarps) pages_append_kernel(PagesAppendAr
         // a minimum of zero has the sign of its first occurrence
         int first = 0x7fffffff;
 #pragma unroll
-        for (int i = N - 1; i >= 0; i--)
-            if (x[i] == 0.0f) first = 2 * ((i >> 3) * 32 + 8 * q + (i & 7)) + (__float_as_int(x[i]) < 0);
+        for (int i = N - 1; i >= 0; i--) {
+            float p[2];
+            split(x[i / 2], p[0], p[1]);
+            if (p[i & 1] == 0.0f) first = 2 * ((i >> 3) * 32 + 8 * q + (i & 7)) + (__float_as_int(p[i & 1]) < 0);
+        }
 #pragma unroll
         for (int lm = 1; lm < 4; lm <<= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, lm));
         if (mn == 0.0f) mn = (first & 1) ? -0.0f : 0.0f;
@@ -183,18 +207,22 @@ __global__ void __launch_bounds__(32 * kWarps) pages_append_kernel(PagesAppendAr
     uint32_t word[CH * WPC];
     {
         const float rcp = safe ? __frcp_rn(sc) : 1.0f;
+        const f2 rcps = pair(rcp, rcp), magic = pair(kMagic, kMagic), least = pair(-mn, -mn);
         float far = 0.0f;
+        constexpr int kPer = 32 / BITS;  // codes per word
+        // a code sits in the low bits of its sum with kMagic, whose own bits a constant takes off again
+        constexpr uint32_t kOff = BITS == 4 ? 0x4B400000u * 0x11111111u : 0x4B400000u * 0x01010101u;
 #pragma unroll
         for (int w = 0; w < CH * WPC; w++) {
-            constexpr int kPer = 32 / BITS;  // codes per word
-            uint32_t acc = 0;
+            uint32_t acc = 0u - kOff;
 #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const float num = __fsub_rn(x[w * kPer + i], mn);
-                const float k = __fmaf_rn(num, rcp, kMagic);
-                far = fmaxf(far, fabsf(__fmaf_rn(num, rcp, -__fsub_rn(k, kMagic))));
-                // the code sits in the low bits of k; the exponent's bits cancel in the constant below
-                acc += (__float_as_uint(k) - 0x4B400000u) << (BITS * i);
+            for (int i = 0; i < kPer; i += 2) {
+                const f2 num = add2(x[(w * kPer + i) / 2], least), k = fma2(num, rcps, magic);
+                float d0, d1, k0, k1;
+                split(fma2(num, rcps, sub2(magic, k)), d0, d1);
+                split(k, k0, k1);
+                far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
+                acc += (__float_as_uint(k0) << (BITS * i)) + (__float_as_uint(k1) << (BITS * (i + 1)));
             }
             word[w] = acc;
         }
@@ -202,18 +230,25 @@ __global__ void __launch_bounds__(32 * kWarps) pages_append_kernel(PagesAppendAr
         if (__any_sync(0xffffffffu, redo) && redo) {
 #pragma unroll
             for (int w = 0; w < CH * WPC; w++) {
-                constexpr int kPer = 32 / BITS;
                 uint32_t acc = 0;
 #pragma unroll
                 for (int i = 0; i < kPer; i++) {
-                    const float num = __fsub_rn(x[w * kPer + i], mn);
-                    uint32_t c = sc > 0.0f ? __float2uint_rz(rust_round_f32(__fdiv_rn(num, sc))) : 0u;
+                    float p[2];
+                    split(x[(w * kPer + i) / 2], p[0], p[1]);
+                    const float num = __fsub_rn(p[i & 1], mn);
+                    const uint32_t c = sc > 0.0f ? __float2uint_rz(rust_round_f32(__fdiv_rn(num, sc))) : 0u;
                     acc |= min(c, kLevels) << (BITS * i);
                 }
                 word[w] = acc;
             }
         }
     }
+
+    if (live && (page < 0 || page >= a.rows.num_pages)) {
+        if (q == 0) atomicOr(a.rows.dev_status, kPagesBadPage);
+        live = false;
+    }
+    uint8_t *rec = a.records + ((int64_t)(live ? page : 0) * a.heads + h) * page_record(CB);
 
     // stores: word w of run c holds code bytes 4*j0 .. of the vector, j0 = (c*4 + q)*WPC + w
     const int t = (int)(pos & (kPageTokens - 1));

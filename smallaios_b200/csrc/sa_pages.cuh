@@ -122,6 +122,32 @@ __device__ __forceinline__ int row_tokens(const PageRows &r, int b, int seq_len,
     return n < 0 ? 0 : (n < seq_len ? n : seq_len);
 }
 
+// Pairs of floats: two operations to an instruction.  (A product and a sum of its result may be contracted.)
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float x, float y) {
+    f2 v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void split(f2 v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 x, f2 y) {
+    f2 v;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ f2 mul2(f2 x, f2 y) {
+    f2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ f2 fma2(f2 x, f2 y, f2 z) {
+    f2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+// x - y (a product with -1 is exact).
+__device__ __forceinline__ f2 sub2(f2 x, f2 y) { return fma2(y, pair(-1.0f, -1.0f), x); }
+
 // N consecutive elements as f32, 16 bytes at a time when `aligned`.
 template <typename T, int N>
 __device__ __forceinline__ void load_run(const T *p, bool aligned, float *x) {
