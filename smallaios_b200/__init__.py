@@ -13,7 +13,7 @@ from .ops import (CapacityError, InternalError, InvalidAttribute, KvCacheDispatc
                   gqa_select_blocks, gqa_sparse_attend, gqa_tree_attend, group_query_attention, kv_block_means,
                   matmul_nbits, matmul_nbits_packed, qkv_project_append, rms_norm,
                   rotary_device_status, rotary_embedding, silu_mul, supports_op)
-from .layer import LayerWeights, decoder_layer_step, prefill_layer_step, tree_layer_step
+from .layer import LayerWeights, decoder_layer_step, paged_layer_step, prefill_layer_step, tree_layer_step
 
 __all__ = [
     "DEFAULT_SEED", "GpuKvCache", "LayerView", "CapacityError", "InternalError", "InvalidAttribute",
@@ -22,5 +22,5 @@ __all__ = [
     "qkv_project_append", "rms_norm", "silu_mul", "supports_op", "LayerWeights", "decoder_layer_step", "prefill_layer_step",
     "qjl_correction", "rotary_embedding", "rotary_device_status", "gqa_tree_attend", "kv_block_means",
     "gqa_select_blocks", "gqa_sparse_attend", "tree_layer_step", "GpuKvPages", "PagesView", "gqa_paged_attend",
-    "beam_select",
+    "beam_select", "paged_layer_step",
 ]

@@ -17,6 +17,19 @@ bool dtype_ok(int32_t dt) { return dt == SA_DTYPE_FLOAT || dt == SA_DTYPE_FLOAT1
 kv_pages_impl *impl(sa_kv_pages *p) { return reinterpret_cast<kv_pages_impl *>(p); }
 const kv_pages_impl *impl(const sa_kv_pages *p) { return reinterpret_cast<const kv_pages_impl *>(p); }
 
+// Makes the pool's device current while a call launches on it.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        if (before == device) before = -1;
+        else cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
 // Checks shared by the calls over rows of new tokens.
 int check_rows(const char *op, const kv_pages_impl *k, int32_t layer, int32_t dtype, int32_t batch, int32_t seq_len,
                int64_t batch_stride, int64_t token_stride, int64_t width, const int32_t *page_table,
@@ -42,9 +55,8 @@ int check_rows(const char *op, const kv_pages_impl *k, int32_t layer, int32_t dt
 // As check_rope of the contiguous cache; the positions themselves are on the device.
 int check_tables(const char *op, int32_t do_rotary, const float *cos_cache, const float *sin_cache, int32_t rows) {
     if (!do_rotary) return SA_OK;
-    if (!cos_cache || !sin_cache)
-        return set_error(SA_ERR_SHAPE_MISMATCH, "%s: do_rotary=1 requires cos_cache and sin_cache", op);
-    if (rows <= 0) return set_error(SA_ERR_SHAPE_MISMATCH, "%s: cos/sin tables of %d rows", op, rows);
+    if (!cos_cache || !sin_cache || rows <= 0)
+        return set_error(SA_ERR_SHAPE_MISMATCH, "%s: do_rotary=1 requires cos_cache and sin_cache (tables of %d rows)", op, rows);
     return SA_OK;
 }
 
@@ -130,11 +142,11 @@ int sa_kv_pages_create(const sa_kv_pages_config *config, sa_kv_pages **out) {
 int sa_kv_pages_destroy(sa_kv_pages *pages) {
     if (!pages) return SA_OK;
     kv_pages_impl *k = impl(pages);
-    int dev = -1;
-    cudaGetDevice(&dev);
-    if (dev != k->device) cudaSetDevice(k->device);
-    cudaError_t e = cudaFree(k->base);
-    if (dev >= 0 && dev != k->device) cudaSetDevice(dev);
+    cudaError_t e;
+    {
+        OnDevice on(k->device);
+        e = cudaFree(k->base);
+    }
     delete k;
     return check_cuda(e, "kv_pages_destroy cudaFree");
 }
@@ -168,18 +180,14 @@ int sa_kv_pages_layer_view(const sa_kv_pages *pages, int32_t layer, sa_kv_pages_
 int sa_kv_pages_device_status(sa_kv_pages *pages, int32_t *status, int32_t clear) {
     if (!pages || !status) return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_device_status: NULL argument");
     kv_pages_impl *k = impl(pages);
-    int dev = -1;
-    cudaGetDevice(&dev);
-    if (dev != k->device) cudaSetDevice(k->device);
+    OnDevice on(k->device);
     int v = 0;
     int rc = check_cuda(cudaDeviceSynchronize(), "kv_pages_device_status");
     if (rc == SA_OK)
         rc = check_cuda(cudaMemcpy(&v, k->dev_status, sizeof(int), cudaMemcpyDeviceToHost), "kv_pages_device_status read");
-    if (rc == SA_OK) {
-        *status = v;
-        if (clear && v) rc = check_cuda(cudaMemset(k->dev_status, 0, sizeof(int)), "kv_pages_device_status clear");
-    }
-    if (dev >= 0 && dev != k->device) cudaSetDevice(dev);
+    if (rc != SA_OK) return rc;
+    *status = v;
+    if (clear && v) rc = check_cuda(cudaMemset(k->dev_status, 0, sizeof(int)), "kv_pages_device_status clear");
     return rc;
 }
 
@@ -214,6 +222,7 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
     a.wht_scale = k->wht_scale;
     a.rows = page_rows(k, page_table, table_stride, max_pages, seq_lens, counts);
     a.rope = rope_args(cos_cache, sin_cache, cache_rows, do_rotary, rotary_interleaved);
+    OnDevice on(k->device);
     return launch_pages_append(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -266,6 +275,7 @@ int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, in
     a.sm_count = k->sm_count;
     a.rows = page_rows(k, page_table, table_stride, max_pages, seq_lens, counts);
     a.rope = rope_args(cos_cache, sin_cache, cache_rows, do_rotary, rotary_interleaved);
+    OnDevice on(k->device);
     return launch_pages_attend(a, workspace, static_cast<cudaStream_t>(stream));
 }
 
@@ -355,6 +365,7 @@ int sa_kv_pages_reorder(sa_kv_pages *pages, const int32_t *page_table, int64_t t
     a.beams = num_beams;
     a.num_pages = k->cfg.num_pages;
     a.dev_status = k->dev_status;
+    OnDevice on(k->device);
     return launch_pages_reorder(a, static_cast<cudaStream_t>(stream));
 }
 

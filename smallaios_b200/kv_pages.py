@@ -84,15 +84,16 @@ class GpuKvPages:
         tokens exist.  K is rotated to its position with ``do_rotary``.  ``seq_lens`` is not changed.  Tokens that
         have no page, or no row in the tables, are left out and reported by ``device_status``.
         """
-        b, s, *strides = ops._token_rows("kv_pages_append", key, self.kv_width, "key")
+        index = self.device.index
+        b, s, *strides = ops._token_rows("kv_pages_append", key, self.kv_width, index, "key")
         if not isinstance(value, torch.Tensor) or value.shape != key.shape:
             raise ops.ShapeMismatch("kv_pages_append: key and value must be (B, S, H*D) with equal shapes")
         if value.dtype != key.dtype:
             raise ops.UnsupportedOp("kv_pages_append: key and value dtypes differ")
-        if ops._token_rows("kv_pages_append", value, self.kv_width, "value") != (b, s, *strides):
+        if ops._token_rows("kv_pages_append", value, self.kv_width, index, "value") != (b, s, *strides):
             raise ValueError("key and value must have the same strides")
-        table = ops._page_rows("kv_pages_append", page_table, seq_lens, counts, b)
-        rope = ops._page_rope("kv_pages_append", cos_cache, sin_cache, self.half_dim)
+        table = ops._page_rows("kv_pages_append", page_table, seq_lens, counts, b, index)
+        rope = ops._page_rope("kv_pages_append", cos_cache, sin_cache, self.half_dim, index)
         rc = lib.sa_kv_pages_append(self.handle, layer, key.data_ptr(), value.data_ptr(), *strides, ops._dtype_code(key),
                                     b, s, *table, *rope, int(bool(do_rotary)), int(bool(rotary_interleaved)),
                                     ops._stream_handle(stream, self.device))
@@ -108,21 +109,24 @@ class GpuKvPages:
         by rows; a row's page in use and the pages behind it must be its own.  ``out`` must not overlap
         ``page_table``.
         """
-        ops._cuda(parents, "parents")
+        index = self.device.index
+        ops._on(parents, index, "parents")
+        if not parents.is_contiguous():
+            raise ValueError("parents must be contiguous")
         shape = parents.shape
         if len(shape) != 2:
             raise ops.ShapeMismatch("reorder_beams: parents must be (B, K)")
         if parents.dtype != torch.int32:
             raise ops.UnsupportedOp("reorder_beams: parents must be int32")
         b, k = shape
-        table, stride, width, lens, _ = ops._page_rows("reorder_beams", page_table, seq_lens, None, b * k)
+        table, stride, width, lens, _ = ops._page_rows("reorder_beams", page_table, seq_lens, None, b * k, index)
         if out is None:
             out = ops._empty(page_table.shape, torch.int32, page_table.device, stream)
             new, new_stride = out.data_ptr(), width
         else:
             if not isinstance(out, torch.Tensor) or out.shape != page_table.shape:
                 raise ops.ShapeMismatch("reorder_beams: out must have page_table's shape")
-            new, new_stride, _ = ops._page_table("reorder_beams", out, b * k, "out")
+            new, new_stride, _ = ops._page_table("reorder_beams", out, b * k, index, "out")
         rc = lib.sa_kv_pages_reorder(self.handle, table, stride, new, new_stride, width, lens, parents.data_ptr(), b, k,
                                      ops._stream_handle(stream, self.device))
         ops._raise_op(rc, "reorder_beams")

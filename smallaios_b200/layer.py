@@ -24,8 +24,8 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import SA_BLOCK_TOKENS
-from .ops import (gqa_attend, gqa_select_blocks, gqa_sparse_attend, gqa_tree_attend, kv_block_means, matmul_nbits,
-                  qkv_project_append, rms_norm, rotary_embedding, silu_mul)
+from .ops import (gqa_attend, gqa_paged_attend, gqa_select_blocks, gqa_sparse_attend, gqa_tree_attend, kv_block_means,
+                  matmul_nbits, qkv_project_append, rms_norm, rotary_embedding, silu_mul)
 
 
 @dataclass
@@ -117,6 +117,29 @@ def tree_layer_step(x: torch.Tensor, resid: torch.Tensor | None, w: LayerWeights
     cache.append(layer, k, v)
     a = gqa_tree_attend(q, cache, layer, parents, num_heads=cfg.num_heads)
     return _after_attention(a.view(batch * nodes, qd), pre1, w)
+
+
+def paged_layer_step(x: torch.Tensor, resid: torch.Tensor | None, w: LayerWeights, pages, layer: int, *,
+                     page_table: torch.Tensor, seq_lens: torch.Tensor, cos_cache: torch.Tensor,
+                     sin_cache: torch.Tensor, rotary_interleaved: bool = False):
+    """One decode step of one layer over pages: ``x`` (B, hidden) plus ``resid`` -> ``(d, pre2)``, as decoder_layer_step.
+
+    Row b's new token goes to position seq_lens[b] of its pages (``page_table`` int32 (B, pages)); rows with a length
+    below 0 take no part (their attention output is zero).  The keys and values are slices of one projection.  After
+    the last layer the caller raises ``seq_lens``; a beam search then selects and reorders:
+
+        parents, tokens, scores = beam_select(logits, scores, finished=..., end_token=...)
+        table = pages.reorder_beams(table, seq_lens, parents)
+    """
+    b, hidden = x.shape
+    cfg = pages.config
+    qd, kd = pages.query_width, pages.kv_width
+    h1, pre1 = rms_norm(x, w.input_norm, skip=resid, epsilon=w.epsilon)
+    qkv = matmul_nbits(h1, w.wqkv_codes, w.wqkv_scales, K=hidden, N=qd + 2 * kd).view(b, 1, qd + 2 * kd)
+    rope = dict(do_rotary=True, rotary_interleaved=rotary_interleaved, cos_cache=cos_cache, sin_cache=sin_cache)
+    pages.append(layer, qkv[..., qd:qd + kd], qkv[..., qd + kd:], page_table, seq_lens, **rope)
+    a = gqa_paged_attend(qkv[..., :qd], pages, layer, page_table, seq_lens, num_heads=cfg.num_heads, **rope)
+    return _after_attention(a.view(b, qd), pre1, w)
 
 
 def prefill_layer_step(x: torch.Tensor, resid: torch.Tensor | None, w: LayerWeights, cache, layer: int, *,

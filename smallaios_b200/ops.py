@@ -362,10 +362,17 @@ def gqa_sparse_attend(query: torch.Tensor, cache: GpuKvCache, layer: int, block_
 # ---- paged serving ----------------------------------------------------------------
 # The checks of a call take as long as its launch: each property of a tensor is read once, and what a contiguous
 # tensor's strides are is not asked.
-def _page_table(op: str, t, batch: int, what: str):
-    """(pointer, row stride, pages per row) of an int32 table of ``batch`` rows, which may be a slice of columns."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _on(t, index: int, what: str) -> None:
+    """``t`` is a tensor on GPU ``index``."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        if isinstance(t, torch.Tensor) and t.is_cuda:
+            raise ValueError(f"{what} is on GPU {t.get_device()}, not {index}")
         raise TypeError(f"{what} must be a CUDA tensor")
+
+
+def _page_table(op: str, t, batch: int, index: int, what: str):
+    """(pointer, row stride, pages per row) of an int32 table of ``batch`` rows, which may be a slice of columns."""
+    _on(t, index, what)
     if t.dtype != torch.int32:
         raise UnsupportedOp(f"{op}: {what} must be int32")
     shape = t.shape
@@ -380,29 +387,28 @@ def _page_table(op: str, t, batch: int, what: str):
     return t.data_ptr(), row if batch > 1 else pages, pages
 
 
-def _page_rows(op: str, page_table, seq_lens, counts, batch: int):
+def _page_rows(op: str, page_table, seq_lens, counts, batch: int, index: int):
     """A call's rows: (table pointer, its row stride, pages per row, lengths pointer, counts pointer or None)."""
-    table = _page_table(op, page_table, batch, "page_table")
+    table = _page_table(op, page_table, batch, index, "page_table")
     pointers = []
     for name, t in (("seq_lens", seq_lens), ("counts", counts)):
         if t is None and name == "counts":
             pointers.append(None)
             continue
-        _cuda(t, name)
-        if t is None:
-            raise TypeError(f"{name} must be a CUDA tensor")
+        _on(t, index, name)
         if t.dtype != torch.int32:
             raise UnsupportedOp(f"{op}: {name} must be int32")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
         if t.numel() != batch:
             raise ShapeMismatch(f"{op}: {name} must have {batch} entries, got {t.numel()}")
         pointers.append(t.data_ptr())
     return *table, *pointers
 
 
-def _token_rows(op: str, t, width: int, what: str):
+def _token_rows(op: str, t, width: int, index: int, what: str):
     """(B, S, batch stride, token stride) of (B, S, width) vectors, maybe a slice of columns of a wider projection."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{what} must be a CUDA tensor")
+    _on(t, index, what)
     shape = t.shape
     if len(shape) != 3:
         raise ShapeMismatch(f"{op}: {what} must be rank-3")
@@ -421,14 +427,16 @@ def _token_rows(op: str, t, width: int, what: str):
     return b, s, batch, token
 
 
-def _page_rope(op: str, cos_cache, sin_cache, half: int):
+def _page_rope(op: str, cos_cache, sin_cache, half: int, index: int):
     """(cos pointer, sin pointer, rows) of the rotary tables, (None, None, 0) without."""
     if cos_cache is None and sin_cache is None:
         return None, None, 0
-    _cuda(cos_cache, "cos_cache")
-    _cuda(sin_cache, "sin_cache")
     if cos_cache is None or sin_cache is None:
         raise ShapeMismatch(f"{op}: cos and sin caches come together")
+    _on(cos_cache, index, "cos_cache")
+    _on(sin_cache, index, "sin_cache")
+    if not cos_cache.is_contiguous() or not sin_cache.is_contiguous():
+        raise ValueError("cos_cache and sin_cache must be contiguous")
     if cos_cache.dtype != torch.float32 or sin_cache.dtype != torch.float32:
         raise UnsupportedOp(f"{op}: cos and sin caches must be float32")
     shape = cos_cache.shape
@@ -450,17 +458,20 @@ def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_ta
     tokens that do not exist give zeros.  A row's pages are read once per new token: S is one, or a few.
     ``workspace``: uint8, at least ``pages.workspace_bytes`` bytes; allocated when not given.
     """
-    b, s, *strides = _token_rows("gqa_paged_attend", query, pages.query_width, "query")
+    index = pages.device.index
+    b, s, *strides = _token_rows("gqa_paged_attend", query, pages.query_width, index, "query")
     code = _dtype_code(query)
-    table = _page_rows("gqa_paged_attend", page_table, seq_lens, counts, b)
-    rope = _page_rope("gqa_paged_attend", cos_cache, sin_cache, pages.half_dim)
+    table = _page_rows("gqa_paged_attend", page_table, seq_lens, counts, b, index)
+    rope = _page_rope("gqa_paged_attend", cos_cache, sin_cache, pages.half_dim, index)
     if out is None:
         out = torch.empty_like(query) if stream is None and query.is_contiguous() else \
             _empty(query.shape, query.dtype, query.device, stream)
     else:
-        _cuda(out, "out")
+        _on(out, index, "out")
         if out.shape != query.shape or out.dtype != query.dtype:
             raise ShapeMismatch("gqa_paged_attend: out must have query's shape and dtype")
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
     need = pages.workspace_bytes(b, s, code)
     workspace = _workspace(workspace, need, query.device, stream)
     rc = lib.sa_gqa_paged_attend(pages.handle, layer, query.data_ptr(), *strides, out.data_ptr(), code, b, s,
@@ -486,11 +497,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     ``finished`` (bool or uint8 (B, K)) has the single continuation ``end_token`` with its own score.  Best first,
     of equal scores the lower k*V + v; -1, -1, -inf behind the last.  ``keep`` defaults to K.
     """
+    _cuda(scores, "scores")
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise TypeError("logits must be a CUDA tensor")
-    _cuda(scores, "scores")
     if scores is None:
         raise TypeError("scores must be a CUDA tensor")
+    index = logits.get_device()
+    _on(scores, index, "scores")
     shape, rows = scores.shape, logits.shape
     if len(shape) != 2 or len(rows) != 2 or rows[0] != shape[0] * shape[1]:
         raise ShapeMismatch("beam_select: logits must be (B*K, V) of scores (B, K)")
@@ -505,7 +518,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
             raise ValueError("logits must have contiguous rows")
         stride = row if n > 1 else vocab
     if finished is not None:
-        _cuda(finished, "finished")
+        _on(finished, index, "finished")
+        if not finished.is_contiguous():
+            raise ValueError("finished must be contiguous")
         if finished.dtype != torch.bool and finished.dtype != torch.uint8:
             raise UnsupportedOp("beam_select: finished must be bool or uint8")
         if finished.shape != shape:
@@ -516,11 +531,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
         best = torch.empty_like(scores) if keep == k else scores.new_empty((b, max(keep, 0)))
         parents, tokens = torch.empty_like(best, dtype=torch.int32), torch.empty_like(best, dtype=torch.int32)
     workspace = _workspace(workspace, _beam_workspace_bytes(b, k, vocab), device, stream)
-    rc = lib.sa_beam_select(logits.data_ptr(), stride, code, scores.data_ptr(),
-                            None if finished is None else finished.data_ptr(), b, k, vocab, int(end_token), keep,
-                            parents.data_ptr(), tokens.data_ptr(), best.data_ptr(),
-                            None if workspace is None else workspace.data_ptr(),
-                            0 if workspace is None else workspace.numel(), _stream_handle(stream, device))
+    # (launches go to the current device's context, which need not be the tensors')
+    with contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index):
+        rc = lib.sa_beam_select(logits.data_ptr(), stride, code, scores.data_ptr(),
+                                None if finished is None else finished.data_ptr(), b, k, vocab, int(end_token), keep,
+                                parents.data_ptr(), tokens.data_ptr(), best.data_ptr(),
+                                None if workspace is None else workspace.data_ptr(),
+                                0 if workspace is None else workspace.numel(), _stream_handle(stream, device))
     _raise_op(rc, "beam_select")
     return parents, tokens, best
 

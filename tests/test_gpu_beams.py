@@ -199,3 +199,182 @@ def test_reorder_matches_the_plain_form(cuda_device, layers, b, k, h, d, bits, l
         for i in range(layers):
             for got, x in zip(_tokens(pool.view(i)), arrays[i]):
                 assert np.array_equal(got, x)
+
+
+@pytest.mark.parametrize("bad", [9, -2, 2**31 - 1])
+def test_beams_that_do_not_match_stay_and_are_reported(cuda_device, bad):
+    import smallaios_b200 as sa
+
+    pool = sa.GpuKvPages(1, 1, 64, 40, bits=8, device=cuda_device)
+    table = torch.arange(24, dtype=torch.int32, device=cuda_device).view(8, 3)
+    before = pool.view(0).k_codes.copy_(torch.randint(0, 256, pool.view(0).k_codes.shape, device=cuda_device,
+                                                      dtype=torch.uint8)).clone()
+    lens = torch.full((8,), 70, dtype=torch.int32, device=cuda_device)
+    parents = torch.tensor([[0, 0, 2, 3], [1, 1, 1, 1]], dtype=torch.int32, device=cuda_device)
+    uneven = lens.clone()
+    uneven[5] = 71
+    got = pool.reorder_beams(table, uneven, parents)  # the second group's beams differ in length
+    assert pool.device_status(clear=True) == 8 and torch.equal(got[4:], table[4:]) and got[1].tolist() == [0, 4, 5]
+    pool.view(0).k_codes.copy_(before)
+    stray = parents.clone()
+    stray[0, 3] = bad                                  # a parent outside the group: that beam stays
+    assert torch.equal(pool.reorder_beams(table, lens, stray), pool.reorder_beams(table, lens, parents))
+    assert pool.device_status(clear=True) == 8
+    broken = table.clone()
+    broken[1, 1] = 40                                  # the page to copy to is outside the pool
+    pool.view(0).k_codes.copy_(before)
+    pool.reorder_beams(broken, lens, parents[:1].repeat(2, 1))
+    assert pool.device_status(clear=True) == 2
+    long = torch.full((8,), 193, dtype=torch.int32, device=cuda_device)  # more tokens than three pages hold
+    assert torch.equal(pool.reorder_beams(table, long, parents), table) and pool.device_status(clear=True) == 2
+
+
+def test_refused_arguments(cuda_device):
+    import smallaios_b200 as sa
+
+    x = torch.zeros(8, 100, device=cuda_device)
+    scores = torch.zeros(2, 4, device=cuda_device)
+    done = torch.zeros(2, 4, dtype=torch.bool, device=cuda_device)
+    for error, match, args, kw in (
+            (sa.ShapeMismatch, "logits", (x[:7], scores), {}), (sa.ShapeMismatch, "logits", (x[0], scores), {}),
+            (sa.ShapeMismatch, "logits", (x, scores[0]), {}), (sa.UnsupportedOp, "float32", (x, scores.half()), {}),
+            (sa.UnsupportedOp, "dtype", (x.double(), scores), {}), (sa.UnsupportedOp, "finished", (x, scores), dict(finished=done.int())),
+            (sa.ShapeMismatch, "finished", (x, scores), dict(finished=done[:1])), (ValueError, "rows", (x[:, ::2], scores), {}),
+            (ValueError, "rows", (x[:1].expand(8, 100), scores), {}), (sa.InvalidAttribute, "keep", (x, scores), dict(keep=0)),
+            (sa.InvalidAttribute, "keep", (x, scores), dict(keep=65)), (sa.ShapeMismatch, "rows of 0", (x[:, :0], scores), {}),
+            (sa.InvalidAttribute, "33 beams", (torch.zeros(33, 9, device=cuda_device), torch.zeros(1, 33, device=cuda_device)), {}),
+            (sa.InvalidAttribute, "workspace", (x, scores), dict(workspace=torch.empty(16, dtype=torch.uint8, device=cuda_device))),
+            (TypeError, "logits", (x.cpu(), scores), {}), (TypeError, "scores", (x, scores.cpu()), {})):
+        with pytest.raises(error, match=match):
+            sa.beam_select(*args, **kw)
+    assert [t.shape for t in sa.beam_select(x[:0], scores[:0])] == [(0, 4)] * 3
+
+    pool = sa.GpuKvPages(1, 1, 64, 8, device=cuda_device)
+    table = torch.zeros(8, 2, dtype=torch.int32, device=cuda_device)
+    lens, parents = torch.zeros(8, dtype=torch.int32, device=cuda_device), torch.zeros(2, 4, dtype=torch.int32, device=cuda_device)
+    for error, match, args, kw in (
+            (sa.UnsupportedOp, "parents", (table, lens, parents.long()), {}), (sa.ShapeMismatch, "parents", (table, lens, parents[0]), {}),
+            (sa.ShapeMismatch, "page_table", (table[:7], lens, parents), {}), (sa.ShapeMismatch, "entries", (table, lens[:7], parents), {}),
+            (sa.ShapeMismatch, "out", (table, lens, parents), dict(out=table[:7])), (sa.UnsupportedOp, "out", (table, lens, parents), dict(out=table.long())),
+            (sa.InvalidAttribute, "overlaps", (table, lens, parents), dict(out=table)),
+            (sa.InvalidAttribute, "beams", (torch.zeros(33, 2, dtype=torch.int32, device=cuda_device),
+                                            torch.zeros(33, dtype=torch.int32, device=cuda_device),
+                                            torch.zeros(1, 33, dtype=torch.int32, device=cuda_device)), {}),
+            (TypeError, "page_table", (table.cpu(), lens, parents), {})):
+        with pytest.raises(error, match=match):
+            pool.reorder_beams(*args, **kw)
+    assert pool.reorder_beams(table[:0], lens[:0], parents[:0]).shape == (0, 2)
+    wide = torch.full((8, 5), 7, dtype=torch.int32, device=cuda_device)
+    pool.reorder_beams(table, lens, parents, out=wide[:, 1:3])
+    assert wide.tolist() == [[7, 0, 0, 7, 7]] * 8
+
+
+def test_selection_on_another_stream_and_in_a_graph(cuda_device):
+    import smallaios_b200 as sa
+
+    r = np.random.default_rng(9)
+    x = torch.from_numpy((r.standard_normal((3, 32, 5000)) * 3).astype(np.float32)).to(cuda_device).bfloat16()
+    scores = -torch.rand(8, 4, device=cuda_device)
+    want = [sa.beam_select(t, scores, keep=6) for t in x]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for handle in (s, s.cuda_stream):
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(2_000_000)
+        got = sa.beam_select(x[0], scores, keep=6, stream=handle)
+        for _ in range(4):
+            torch.full((1 << 20,), 255, dtype=torch.uint8, device=cuda_device)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    static = x[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sa.beam_select(static, scores, keep=6)
+    for t, w in zip(x, want):
+        static.copy_(t)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
+# ---- all of it -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lift", [2.0, 9.0])  # of the end token's logits: few beams end, or most
+def test_a_beam_search_over_pages(cuda_device, lift):
+    """Appending, attention, selection and reordering as a serving loop runs them, against histories kept apart: every
+    beam's keys and values encoded by the oracle, attention and selection in 64 bits."""
+    import smallaios_b200 as sa
+    from tests.helpers import oracle_append, rope_tables
+
+    r = np.random.default_rng(10)
+    b, k, h, g, d, bits, vocab, steps, end = 2, 4, 1, 2, 64, 8, 300, 75, 7
+    prompt = [50, 61]
+    tk, tv = (r.standard_normal((vocab, h * d)).astype(np.float32) for _ in range(2))
+    tq = (r.standard_normal((vocab, h * g * d)) * 1.5).astype(np.float32)
+    wout = (r.standard_normal((h * g * d, vocab)) * 1.2).astype(np.float32)
+    rows = max(prompt) + steps + 1
+    cos, sin = rope_tables(rows, d)
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).to(cuda_device)  # noqa: E731
+    gk, gv, gq, gw, gcos, gsin = (dev(x) for x in (tk, tv, tq, wout, cos, sin))
+    rope = dict(do_rotary=True, cos_cache=gcos, sin_cache=gsin)
+
+    width = (rows + 63) // 64
+    pool = sa.GpuKvPages(1, h, d, b * k * width, num_heads=h * g, bits=bits, device=cuda_device)
+    signs = pool.view(0).signs.cpu().numpy()
+    table = dev(r.permutation(b * k * width).astype(np.int32).reshape(b * k, width))
+    words = [r.integers(0, vocab, n) for n in prompt]
+    longest = max(prompt)
+    ids = np.zeros((b * k, longest), np.int64)
+    for i in range(b * k):
+        ids[i, :prompt[i // k]] = words[i // k]
+    counts = dev(np.repeat(prompt, k).astype(np.int32))
+    lens = torch.zeros_like(counts)
+    pool.append(0, gk[dev(ids)], gv[dev(ids)], table, lens, counts=counts, **rope)
+    lens += counts
+
+    # what a token at a position holds, as the oracle encodes it
+    held = {}
+
+    def vectors(token, pos):
+        if (token, pos) not in held:
+            kc, km, vc, vm = oracle_append(tk[token].reshape(1, 1, h, d), tv[token].reshape(1, 1, h, d), signs, bits, pos, cos, sin,
+                                           do_rotary=True)
+            held[token, pos] = [ref.decode(ref.unpack(c, bits, d), m, signs.astype(np.float64))[0, :, 0] for c, m in ((kc, km), (vc, vm))]
+        return held[token, pos]
+
+    hist = [[list(words[i]) for _ in range(k)] for i in range(b)]
+    scores = np.full((b, k), -np.inf, np.float32)
+    scores[:, 0] = 0.0
+    tokens = np.array([[w[-1]] * k for w in words])  # the first new token repeats the prompt's last one
+    finished = np.zeros((b, k), bool)
+    ended = 0
+    for step in range(steps):
+        tok = dev(tokens.reshape(-1))
+        pool.append(0, gk[tok][:, None], gv[tok][:, None], table, lens, **rope)
+        attn = sa.gqa_paged_attend(gq[tok][:, None].contiguous(), pool, 0, table, lens, num_heads=h * g, **rope)
+        logits = attn[:, 0] @ gw
+        logits[:, end] += lift
+        got = [x.cpu().numpy() for x in sa.beam_select(logits, dev(scores), finished=dev(finished), end_token=end)]
+        lens += 1
+        table = pool.reorder_beams(table, lens, dev(got[0]))
+
+        want_logits = np.zeros((b, k, vocab))
+        for i in range(b):
+            for j in range(k):
+                hist[i][j].append(int(tokens[i, j]))
+                n = len(hist[i][j])
+                kv = [vectors(t, p) for p, t in enumerate(hist[i][j])]
+                q = pr.rotate(tq[tokens[i, j]].reshape(h, g, d), n - 1, cos, sin, False)
+                w = np.einsum("hgd,thd->hgt", q, np.stack([x[0] for x in kv])) / np.sqrt(d)
+                w = np.exp(w - w.max(-1, keepdims=True))
+                o = np.einsum("hgt,thd->hgd", w / w.sum(-1, keepdims=True), np.stack([x[1] for x in kv]))
+                want_logits[i, j] = o.reshape(-1) @ wout
+                want_logits[i, j, end] += lift
+        want = _select(want_logits, scores, finished, end, k)
+        # attention is off by 1e-5 at most, a logit by that times the norm of a column of wout
+        live = want[2] > -np.inf
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]), step
+        assert np.abs(got[2][live] - want[2][live]).max() < 1e-3
+        parents = np.where(got[0] < 0, np.arange(k), got[0])
+        hist = [[list(hist[i][p]) for p in parents[i]] for i in range(b)]
+        scores, tokens, finished = got[2], np.maximum(got[1], 0), got[1] == end
+        ended += int(finished.sum())
+    assert pool.device_status() == 0 and (lift < 5 or ended > 0)
