@@ -12,6 +12,11 @@
 // `keep` groups over all beams by score + (maximum - log sum), then the best `keep`
 // tokens of those groups, which are read again.
 //
+// 64 x 8 rows of 128256 bf16 (131 MB, a seventh of the rows finished and skipped): scan 26 us, 5 TB/s, between HBM and
+// the exponentials (one a token, 15 us); pick 11 us, a chain of dependent steps over 16 KB.  Of the maxima and lists of
+// one CTA a group of beams needs no more than that, and fewer groups take as long: one of 4 beams over 32000 tokens
+// 11 us in all.
+//
 // Equal rows give equal sums: which lane takes which token, and in which order, does
 // not depend on where a row begins, so that beams that are equal tie exactly.
 #include <math.h>
@@ -47,7 +52,7 @@ int parts_per_row(int64_t rows, int64_t groups) {
 
 // Eight tokens of a group that a lane holds, as they were loaded; -inf outside the row.  PIECES (all rows begin on 16
 // bytes): neighbours, one 16-byte load (two of f32); else every 32nd, so that the warp's loads are neighbours wherever
-// the row begins.  160 rows of 50257 f16: ODD0 us so, against ODD1 with eight neighbours loaded one by one.
+// the row begins.  32 x 5 rows of 50257 f16, scan and pick: 21.0 us so, 22.0 with eight neighbours loaded one by one.
 template <typename T, bool PIECES>
 struct Tokens {
     float x[8];
@@ -176,20 +181,20 @@ __device__ __forceinline__ bool before(const Choice &x, const Choice &y) {
 }
 
 constexpr int kListed = 1024;  // choices that are ranked against each other
-constexpr int kEights = kPickThreads / 8;
+constexpr int kTops = kPickThreads / 4;
 
 // The choice is made twice in the same way, among groups and then among the tokens of the best ones (and the finished
-// beams): the keep-th largest of the 64 best scores of eight threads each bounds the keep-th best from below (mode 0),
+// beams): the keep-th largest of the 128 best scores of four threads each bounds the keep-th best from below (mode 0),
 // the few choices that reach it are listed (mode 1) and ranked against each other.  Where they are too many, scores
 // that are equal by the hundreds, the best is taken out one at a time (mode 2).  One piece of code serves all of that:
 // this kernel runs for a few microseconds, of which fetching its code is a good part (unrolled copies for every step
-// took 15 us after the scan of 64 x 8 beams, PICKT now).
+// took 15 us after the scan of 64 x 8 beams, this takes 11).
 template <typename T>
 __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a, int groups, int parts, const float *maxima,
                                                                  const Part *sums) {
     __shared__ double s_lse[SA_MAX_BEAMS], s_score[SA_MAX_BEAMS];  // of beams that go on; a score of -inf for the others
     __shared__ int s_beam[SA_MAX_BEAM_KEEP], s_first[SA_MAX_BEAM_KEEP];  // of the best groups: beam, first token
-    __shared__ double s_top[kEights], s_least;
+    __shared__ double s_top[kTops], s_least;
     __shared__ Choice s_list[kListed], s_out[SA_MAX_BEAM_KEEP], s_box[2][kPickThreads / 32];
     __shared__ int s_listed;
     constexpr Choice kNone{-INFINITY, 0xffffffffu};
@@ -224,8 +229,11 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a, int
         int mode = phase == 1 && found == keep ? 1 : 0, n = 0;
         double least = mode == 1 ? s_out[keep - 1].score : -INFINITY;
         // a thread's choices in eights; a single eight is worked out once
-        const int beams8 = (K + 7) / 8;
-        const int eights = phase == 0 ? (groups + kPickThreads - 1) / kPickThreads * beams8 : (found + 15) / 16;
+        // groups: 2^wide threads share a beam's (few groups: several beams side by side)
+        int wide = 9;
+        while (wide > 0 && 1 << (wide - 1) >= groups) wide--;
+        const int side = kPickThreads >> wide, beams8 = (K + 8 * side - 1) / (8 * side);
+        const int eights = phase == 0 ? ((groups - 1) >> wide) * beams8 + beams8 : (found + 15) / 16;
         double score[8];
         unsigned place[8];
         bool known = false;
@@ -253,16 +261,19 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a, int
 #pragma unroll 1
             for (int e = 0; e < eights; e++) {
                 if (known) {
-                } else if (phase == 0) {  // the threads share the groups of each beam
-                    const int g = e / beams8 * kPickThreads + tid, k0 = e % beams8 * 8;
+                } else if (phase == 0) {
+                    const int g = (e / beams8 << wide) + (tid & ((1 << wide) - 1)), k0 = e % beams8 * 8 * side + (tid >> wide);
                     float m[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) m[i] = g < groups && k0 + i < K ? maxima[(r0 + k0 + i) * groups + g] : -INFINITY;
+                    for (int i = 0; i < 8; i++) {
+                        const int k = k0 + i * side;
+                        m[i] = g < groups && k < K ? maxima[(r0 + k) * groups + g] : -INFINITY;
+                    }
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int k = min(k0 + i, K - 1);
+                        const int k = min(k0 + i * side, K - 1);
                         score[i] = s_score[k] + ((double)m[i] - s_lse[k]);
-                        place[i] = (unsigned)((k0 + i) * groups + g);
+                        place[i] = (unsigned)(k * groups + g);
                     }
                 } else {  // the threads share the tokens of each group
                     float x[8];
@@ -286,23 +297,23 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a, int
                 take((double)a.scores[r0 + tid], (unsigned)tid * (unsigned)a.vocab + a.end_token);
             if (mode == 0) {
 #pragma unroll
-                for (int o = 1; o < 8; o <<= 1) {
+                for (int o = 1; o < 4; o <<= 1) {
                     const double other = __shfl_xor_sync(0xffffffffu, top, o);
                     if (other > top) top = other;
                 }
-                if ((tid & 7) == 0) s_top[tid >> 3] = top;
+                if ((tid & 3) == 0) s_top[tid >> 2] = top;
                 __syncthreads();
-                // eight threads rank one of the 64 among all
-                const double own = s_top[tid >> 3];
+                // four threads rank one of the 128 among all
+                const double own = s_top[tid >> 2];
                 int ahead = 0;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int j = 8 * i + (tid & 7);
-                    ahead += s_top[j] > own || (s_top[j] == own && j < tid >> 3);
+#pragma unroll 8
+                for (int i = 0; i < kTops / 4; i++) {
+                    const int j = 4 * i + (tid & 3);
+                    ahead += s_top[j] > own || (s_top[j] == own && j < tid >> 2);
                 }
 #pragma unroll
-                for (int o = 1; o < 8; o <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-                if ((tid & 7) == 0 && ahead == keep - 1) s_least = own;
+                for (int o = 1; o < 4; o <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+                if ((tid & 3) == 0 && ahead == keep - 1) s_least = own;
                 __syncthreads();
                 least = s_least;
                 mode = 1;

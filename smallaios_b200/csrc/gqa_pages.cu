@@ -3,17 +3,18 @@
 //
 // pages_attend_kernel: every SM runs one CTA of twelve independent warps.  The
 // chunks (64 tokens, or 32 where a token has 128 code bytes) of all units (row,
-// KV head, block of query heads) lie end to end and each warp owns an equal
-// range, so rows of very different lengths keep all SMs busy; a warp streams its
-// chunks through a ring of shared-memory stages, one bulk copy per chunk (a
+// KV head, block of query heads) lie end to end and each warp owns an equal range,
+// so rows of very different lengths keep all SMs busy; a CTA's warps have
+// neighbouring ranges and prepare the queries of their few units together.  A warp
+// streams its chunks through two shared-memory stages, one bulk copy per chunk (a
 // record's K codes, metadata and V codes are contiguous).
 //
 // The arithmetic of a chunk stays in registers.  With A = the query digits (row r
 // of the MMA: head r's high byte, row r + 8 its low byte) and B = K codes (columns:
-// tokens), lane (r, q) of the accumulator holds head r's scores of tokens; with the
-// tokens assigned to columns as tok() says, these are exactly the tokens whose
-// weights the lane has to supply as the A operand of the value product, whose
-// B operand is a word of the V layout.  So scores become weights without passing
+// tokens), lane (r, q) of the accumulator holds head r's scores of tokens, and with
+// the tokens assigned to columns as below these are exactly the tokens whose
+// weights the lane has to supply as the A operand of the value product, whose B
+// operand is a word of the V layout.  So scores become weights without passing
 // through shared memory, and one MMA carries eight query heads: 16 rows = 8 heads x
 // 2 digits.  f32 callers get three digits and four heads (12 rows).
 //
@@ -26,12 +27,19 @@
 // are added: a weight far below the context's largest keeps 16 bits relative to its
 // neighbours, not to that largest one.  Codes enter both products less their middle
 // (8 or 128), their zero points raised by as much, so that the large common part of
-// q'.c and of X need not cancel after both were rounded.
-//
-// Products are exact integers.
+// q'.c and of X need not cancel after both were rounded.  Products are exact
+// integers.
 //
 // pages_merge_kernel: per unit, the sum of its warps' partial records, the
 // division, the inverse rotation and the store.
+//
+// Bound by HBM once it streams (6.1 TB/s, 0.93 of the measured copy): 64 sequences of
+// 8192 int4 tokens, 8 KV heads of 4, 112 us for 605 MB; 32 of 32768, 8 heads of 8, 200 us
+// for 1209 MB.  What is left: some 9 us before the first product (lengths, table, queries;
+// the first 33 MB arrive meanwhile), warps of a range end 6 us apart, the merge takes 4.
+// Tried: sixteen warps of half chunks (128 registers spill; D = 64 and 8 bits, which do
+// not, got 4 to 10% slower); the merge by the last CTA of a unit (123 us: code that runs
+// once costs its fetch); the queries in a launch of their own (114 us, and a launch more).
 #include "sa_async.cuh"
 #include "sa_decode_common.cuh"
 #include "sa_pages.cuh"
@@ -45,9 +53,9 @@ using namespace dec;
 constexpr int kNWP = 12;         // warps per CTA, one CTA per SM
 constexpr int kMaxRows = 512;    // rows of a launch: their lengths and prefix sums fit in 4 KB
 constexpr int64_t kMaxUnits = 16384;  // units of a launch: bounds the workspace
-// What a unit costs beside its chunks, in chunks: its queries' preparation and the change to it take a CTA about as
-// long as four chunks' copies (0.2 us each).  48 sequences of 0 to 16000 tokens: KUNIT0 us without it, KUNIT1 with.
-constexpr int kUnitCost = 4;
+// What a unit counts for beside its chunks, in chunks: its queries' preparation and the change to it.  48 sequences of 0
+// to 16000 tokens: 77 us at 0, 74 at 2, 75 at 8; 64 sequences of 8192, which need no such balance: 110, 112, 116.
+constexpr int kUnitCost = 2;
 
 template <int BITS, int D, int ND>
 struct PGeo {
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                 return;
             }
             p.n = s_prefix[p.r + 1] - s_prefix[p.r] - kUnitCost;
-        } while (p.n < 0);
+        } while (p.n <= 0);
         p.b = (row0 + p.r) / a.seq_len;
     };
     auto page_of = [&](const Place &p) { return __ldcg(a.rows.table + (int64_t)p.b * a.rows.table_stride + p.c / G::CPP); };

@@ -12,6 +12,10 @@
 // Sums and differences are taken in pairs (f2).  A product that a sum follows is not: a product of a pair may be
 // contracted with the sum to one rounding, __fmul_rn never is.  (Products with signs are exact either way.)
 //
+// Bound by instruction issue and shuffles (2.4 of 4 instructions per cycle): eight ragged prompts of up to 2048 bf16
+// tokens, 8 heads of 128, int4, in 28 us (44.5 MB, 1.6 TB/s); a decode step of 64 rows in 5.6 us, which is latency.
+// More warps, fewer registers or the sums in pairs did not change the former.
+//
 // Codes: (y - z)/s rounded half away from zero, the quotient itself rounded to
 // f32 first.  t = (y - z) * RN(1/s) is within 3 * 2^-24 * 255 of that quotient,
 // so round(t) is the same unless t lies within kTie of a half; a vector with

@@ -204,6 +204,8 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
     if (rc == SA_OK) rc = check_tables("kv_pages_append", do_rotary, cos_cache, sin_cache, cache_rows);
     if (rc != SA_OK || batch == 0 || seq_len == 0) return rc;
     if (!key || !value) return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_append: NULL key/value");
+    if ((int64_t)batch * k->cfg.kv_head_count > INT32_MAX)
+        return set_error(SA_ERR_UNSUPPORTED, "kv_pages_append: %d rows of %d heads", batch, k->cfg.kv_head_count);
     PagesAppendArgs a{};
     a.key = key;
     a.value = value;

@@ -281,6 +281,27 @@ def test_appends_and_queries_from_slices_at_any_element(cuda_device):
             assert all(torch.equal(x, y) for x, y in zip(*outs))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("s", [1, 9])
+def test_rotary_tables_that_start_at_any_element(cuda_device, s, interleaved):
+    import smallaios_b200 as sa
+
+    h, g, d, b = 2, 3, 128, 2
+    tables = [_to(x, cuda_device) for x in rope_tables(100, d)]
+    shifted = [torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape) for x in tables]
+    assert all(x.data_ptr() % 16 for x in shifted)
+    k, v, q = (torch.randn(b, s, w * d, device=cuda_device) for w in (h, h, h * g))
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=cuda_device)
+    lens = torch.tensor([3, 60], dtype=torch.int32, device=cuda_device)
+    outs = []
+    for cos, sin in (tables, shifted):
+        pool = _pool(1, h, g, d, 4, 4, cuda_device)
+        kw = dict(do_rotary=True, rotary_interleaved=interleaved, cos_cache=cos, sin_cache=sin)
+        pool.append(0, k, v, table, lens, **kw)
+        outs.append([sa.gqa_paged_attend(q, pool, 0, table, lens, num_heads=h * g, **kw), pool.view(0).k_codes, pool.view(0).k_meta])
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
 def test_attend_in_place_and_into_a_given_workspace(cuda_device):
     import smallaios_b200 as sa
 
