@@ -12,10 +12,10 @@
 // `keep` groups over all beams by score + (maximum - log sum), then the best `keep`
 // tokens of those groups, which are read again.
 //
-// 64 x 8 rows of 128256 bf16 (131 MB, a seventh of the rows finished and skipped): scan 26 us, 5 TB/s, between HBM and
-// the exponentials (one a token, 15 us); pick 11 us, a chain of dependent steps over 16 KB.  Of the maxima and lists of
-// one CTA a group of beams needs no more than that, and fewer groups take as long: one of 4 beams over 32000 tokens
-// 11 us in all.
+// 64 x 8 rows of 128256 bf16 (131 MB, a seventh of the rows finished and skipped), 35 us: scan 24 us, 4.7 TB/s, two
+// thirds of the cycles issue (some eight instructions a token) and the exponentials alone take 15 us; pick 11 us, a
+// chain of dependent steps over 16 KB a group, which one group of 4 beams over 32000 tokens needs as well (11 us in
+// all).
 //
 // Equal rows give equal sums: which lane takes which token, and in which order, does
 // not depend on where a row begins, so that beams that are equal tie exactly.
@@ -34,7 +34,7 @@ constexpr int kGroup = 256;      // tokens of a group
 constexpr int kScanThreads = 256;
 constexpr int kPickThreads = 512;
 // Warps that the scan is split into where rows allow it: two waves of the 32 that fit on an SM.  64 x 8 rows of 128256
-// bf16, scan and pick: one wave 46 us, two 37, three 41, four 46.
+// bf16, scan and pick: one wave 46 us, two 37, three 41, four 46 (all before whole groups had loads of their own).
 constexpr int kScanWarps = 148 * 64;
 constexpr float kL = 1.4426950408889634f;  // log2(e)
 
@@ -56,6 +56,15 @@ int parts_per_row(int64_t rows, int64_t groups) {
 template <typename T, bool PIECES>
 struct Tokens {
     float x[8];
+    __device__ __forceinline__ void load_whole(const T *row, int g, int lane) {  // of a group that is all in the row
+        const T *p = row + (int64_t)g * kGroup + (PIECES ? lane * 8 : lane);
+        if constexpr (PIECES) {
+            load_run<T, 8>(p, true, x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = ld_f32(p + 32 * i);
+        }
+    }
     __device__ __forceinline__ void load(const T *row, int vocab, int g, int lane) {
         const int64_t e0 = (int64_t)g * kGroup + (PIECES ? lane * 8 : lane);
         constexpr int kStep = PIECES ? 1 : 32;
@@ -76,14 +85,17 @@ struct Tokens {
 template <typename T>
 struct PackedTokens {
     uint32_t w[4];
+    __device__ __forceinline__ void load_whole(const T *row, int g, int lane) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(row + (int64_t)g * kGroup + lane * 8);
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+    }
     __device__ __forceinline__ void load(const T *row, int vocab, int g, int lane) {
         const int64_t e0 = (int64_t)g * kGroup + lane * 8;
         if (e0 + 8 <= vocab) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row + e0);
-            w[0] = v.x;
-            w[1] = v.y;
-            w[2] = v.z;
-            w[3] = v.w;
+            load_whole(row, g, lane);
         } else {
             constexpr uint32_t kNone = std::is_same<T, __half>::value ? 0xFC00u : 0xFF80u;  // -inf
             const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
@@ -133,16 +145,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
     const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
     const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
     float top = -INFINITY, sum = 0.0f;
-    Tokens<T, PIECES> next[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; j++) next[j].load(row, g0 + j < g1 ? a.vocab : 0, g0 + j, lane);
-    for (int g = g0; g < g1; g += kAhead) {
-        Tokens<T, PIECES> now[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; j++) {
-            now[j] = next[j];
-            next[j].load(row, g + kAhead + j < g1 ? a.vocab : 0, g + kAhead + j, lane);
-        }
+    auto consume = [&](const Tokens<T, PIECES> (&now)[kAhead], int g) {
         float most = top, mine = 0.0f;
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
@@ -156,13 +159,43 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
             top = most;
         }
         const float ref = top == -INFINITY ? 0.0f : top;
+        const f2 less = pair(-ref, -ref), log2e = pair(kL, kL);
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-            float e[8];
+            f2 e[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) e[i] = dec::ex2_approx((now[j].get(i) - ref) * kL);
-            sum += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+            for (int i = 0; i < 4; i++) {
+                float x0, x1;
+                split(mul2(add2(pair(now[j].get(2 * i), now[j].get(2 * i + 1)), less), log2e), x0, x1);
+                e[i] = pair(dec::ex2_approx(x0), dec::ex2_approx(x1));
+            }
+            float s0, s1;
+            split(add2(add2(e[0], e[1]), add2(e[2], e[3])), s0, s1);
+            sum += s0 + s1;
         }
+    };
+    // whole groups, the next ones on their way; then the others
+    Tokens<T, PIECES> now[kAhead], next[kAhead];
+    const int whole = min(g1, a.vocab / kGroup);
+    int g = g0;
+    bool more = g + kAhead <= whole;
+    if (more)
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) next[j].load_whole(row, g + j, lane);
+    while (more) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) now[j] = next[j];
+        more = g + 2 * kAhead <= whole;
+        if (more)
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) next[j].load_whole(row, g + kAhead + j, lane);
+        consume(now, g);
+        g += kAhead;
+    }
+    for (; g < g1; g += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) now[j].load(row, g + j < g1 ? a.vocab : 0, g + j, lane);
+        consume(now, g);
     }
     double total = sum;
 #pragma unroll
