@@ -14,13 +14,14 @@
 //
 // Bound by instruction issue and shuffles (2.4 of 4 instructions per cycle): eight ragged prompts of up to 2048 bf16
 // tokens, 8 heads of 128, int4, in 28 us (44.5 MB, 1.6 TB/s); a decode step of 64 rows in 5.6 us, which is latency.
-// More warps, fewer registers or the sums in pairs did not change the former.
+// More warps, fewer registers or the sums in pairs did not change the former, and it is no single pipe (L1 50%, ALU and
+// FMA 37% busy): a warp for many vectors, with the next ones on their way and none idle for rows that end early, took 31.
 //
 // Codes: (y - z)/s rounded half away from zero, the quotient itself rounded to
-// f32 first.  t = (y - z) * RN(1/s) is within 3 * 2^-24 * 255 of that quotient,
-// so round(t) is the same unless t lies within kTie of a half; a vector with
-// such a t (or a scale outside the range where 1/s is safe) is done again by the
-// exact quotient.
+// f32 first.  t = (y - z) * RN(1/s) is within 3 * 2^-24 times the largest code of
+// that quotient (less than 2^-18 and 2^-14), so round(t) is the same unless t lies
+// as near to a half (kTie); a vector with such a t (or a scale outside the range
+// where 1/s is safe) is done again by the exact quotient.
 #include "sa_async.cuh"
 #include "sa_append.cuh"
 #include "sa_decode_common.cuh"
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(32 * kWarps, 8) pages_append_kernel(PagesAppen
     }
     const float range = __fsub_rn(mx, mn);
     const float sc = range > 0.0f ? __fdiv_rn(range, (float)kLevels) : 1.0f;
-    constexpr float kTie = BITS == 4 ? 0.5f - 0x1p-17f : 0.5f - 0x1p-13f;
+    constexpr float kTie = BITS == 4 ? 0.5f - 0x1p-18f : 0.5f - 0x1p-14f;
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum with it is rounded to whole numbers
     // (a vector of NaN leaves the minimum above the maximum, one with infinities an infinite one of them)
     const bool safe = sc >= 0x1p-90f && sc <= 0x1p100f && mn <= mx && fabsf(mn) < INFINITY && mx < INFINITY;
