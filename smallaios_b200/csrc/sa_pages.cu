@@ -94,6 +94,10 @@ int sa_kv_pages_create(const sa_kv_pages_config *config, sa_kv_pages **out) {
     if (c.kv_head_count <= 0 || c.kv_head_begin < 0 || c.kv_head_count > c.num_kv_heads - c.kv_head_begin)
         return set_error(SA_ERR_INVALID_ATTRIBUTE, "kv head range [%d, +%d) outside [0, %d)", c.kv_head_begin,
                          c.kv_head_count, c.num_kv_heads);
+    // more than any B200 holds, and the products below fit in 64 bits
+    if ((double)c.num_layers * c.num_pages * c.kv_head_count * page_record(c.head_dim * c.bits / 8) > 0x1p38)
+        return set_error(SA_ERR_OUT_OF_MEMORY, "kv_pages_create: %d layers of %d pages for %d heads need more than 256 GiB",
+                         c.num_layers, c.num_pages, c.kv_head_count);
     kv_pages_impl *k = new (std::nothrow) kv_pages_impl();
     if (!k) return set_error(SA_ERR_OUT_OF_MEMORY, "kv_pages_create: no host memory");
     memset(k, 0, sizeof(*k));

@@ -526,15 +526,20 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
         if finished.shape != shape:
             raise ShapeMismatch("beam_select: finished must have scores' shape")
     keep = k if keep is None else int(keep)
+    if not 1 <= keep <= _lib.SA_MAX_BEAM_KEEP:
+        raise InvalidAttribute(f"beam_select: keep {keep} (1..{_lib.SA_MAX_BEAM_KEEP})")
+    end_token = int(end_token)
+    if not 0 <= end_token < vocab:
+        end_token = -1
     code, device = _dtype_code(logits), logits.device
     with contextlib.nullcontext() if stream is None else _owned_by(stream, device):
-        best = torch.empty_like(scores) if keep == k else scores.new_empty((b, max(keep, 0)))
+        best = torch.empty_like(scores) if keep == k else scores.new_empty((b, keep))
         parents, tokens = torch.empty_like(best, dtype=torch.int32), torch.empty_like(best, dtype=torch.int32)
     workspace = _workspace(workspace, _beam_workspace_bytes(b, k, vocab), device, stream)
     # (launches go to the current device's context, which need not be the tensors')
     with contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index):
         rc = lib.sa_beam_select(logits.data_ptr(), stride, code, scores.data_ptr(),
-                                None if finished is None else finished.data_ptr(), b, k, vocab, int(end_token), keep,
+                                None if finished is None else finished.data_ptr(), b, k, vocab, end_token, keep,
                                 parents.data_ptr(), tokens.data_ptr(), best.data_ptr(),
                                 None if workspace is None else workspace.data_ptr(),
                                 0 if workspace is None else workspace.numel(), _stream_handle(stream, device))

@@ -229,6 +229,19 @@ def test_beams_that_do_not_match_stay_and_are_reported(cuda_device, bad):
     assert torch.equal(pool.reorder_beams(table, long, parents), table) and pool.device_status(clear=True) == 2
 
 
+def test_numbers_beyond_32_bits_are_not_cut(cuda_device):
+    """An end token outside the vocabulary offers nothing, also one whose low 32 bits name a token."""
+    import smallaios_b200 as sa
+
+    x, scores = torch.zeros(4, 100, device=cuda_device), torch.zeros(1, 4, device=cuda_device)
+    done = torch.ones(1, 4, dtype=torch.bool, device=cuda_device)
+    for end in (-1, 100, 2**32 + 5, -2**32 + 5):
+        parents, tokens, out = sa.beam_select(x, scores, finished=done, end_token=end)
+        assert (parents == -1).all() and (tokens == -1).all() and (out == -float("inf")).all()
+    with pytest.raises(sa.InvalidAttribute, match="keep"):
+        sa.beam_select(x, scores, keep=2**32 + 4)
+
+
 def test_refused_arguments(cuda_device):
     import smallaios_b200 as sa
 

@@ -35,6 +35,19 @@ def test_pool_config_validation_without_gpu(kw, status, msg):
     assert not h.value
 
 
+@pytest.mark.parametrize("kw", [
+    dict(num_pages=2**31 - 1, num_layers=2**31 - 1), dict(num_pages=2**30, num_layers=2**10),
+    dict(num_heads=2**30, num_kv_heads=2**30, kv_head_count=2**30, num_pages=2**20, num_layers=2**20),
+])
+def test_a_pool_beyond_any_memory_is_refused_before_it_is_counted_in_bytes(kw):
+    from smallaios_b200._lib import lib
+
+    h = ctypes.c_void_p()
+    assert lib.sa_kv_pages_create(ctypes.byref(_cfg(**kw)), ctypes.byref(h)) == 5
+    assert b"256 GiB" in lib.sa_last_error_string()
+    assert not h.value
+
+
 def test_null_handles_are_rejected():
     from smallaios_b200._lib import lib
 
