@@ -636,8 +636,9 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
  * seq_len, q_heads_local * head_dim), contiguous, zero for tokens that do not
  * exist and rows without tokens.  A row's pages are read once per new token:
  * this is the decode step, for one new token or a few.
- * Precision: queries and weights are held to 16 bits for f16 and bf16 callers
- * (weights relative to the largest of each 32 or 64 tokens), to 24 for f32.
+ * Precision: queries and weights are held to 16 bits for f16 and bf16 callers,
+ * to 24 for f32 (a weight times its value scale relative to the largest such
+ * product of each 32 or 64 tokens, or to up to four times that).
  * `workspace` (device, 256-byte aligned, at least what
  * sa_gqa_paged_workspace_bytes says) is the call's alone until it has run. */
 int64_t sa_gqa_paged_workspace_bytes(const sa_kv_pages *pages, int32_t batch, int32_t seq_len, int32_t dtype);

@@ -19,16 +19,19 @@
 // 2 digits.  f32 callers get three digits and four heads (12 rows).
 //
 //   s_t = ks_t (q'.c_t) + kz_t sum(q')           (log2 units, scale folded in)
-//   R = max s + log2 max vs,  u_t = 2^(s_t - R) vs_t in (0, 1], 16 or 24 bits of it
+//   R >= max (s_t + log2 vs_t), u_t = 2^(s_t - R) vs_t in (0, 1], 16 or 24 bits of it
 //   L = sum 2^(s_t - R), Z = sum 2^(s_t - R) vz_t, X = sum u_t c_t
 //   out = S.H.((X + Z) / L) / sqrt(D)
 //
 // R is each chunk's own, and its sums are moved to the running reference when they
 // are added: a weight far below the context's largest keeps 16 bits relative to its
-// neighbours, not to that largest one.  Codes enter both products less their middle
+// neighbours, not to that largest one.  R is that maximum, or, where the value scales
+// of a chunk lie within a factor of 4, max s + log2 max vs, which exceeds it by 2 at
+// most and needs one logarithm.  Codes enter both products less their middle
 // (8 or 128), their zero points raised by as much, so that the large common part of
 // q'.c and of X need not cancel after both were rounded.  Products are exact
-// integers.
+// integers.  A vector whose codes are all 0 is its zero point alone: the scale of 1
+// that the format gives it would count codes of -128 there (drop_constant_scales).
 //
 // pages_merge_kernel: per unit, the sum of its warps' partial records, the
 // division, the inverse rotation and the store.
@@ -79,6 +82,11 @@ struct PGeo {
     static constexpr float UNIT = BITS == 4 ? 0.0625f : 1.0f;  // high nibbles enter the products as 16 (c - 8)
     static_assert(SMEM + (2 * kMaxRows + 1) * 4 + kNWP * D * (ND == 2 ? 2 : 4) + 256 <= 227 * 1024, "shared memory");
 };
+
+// Value scales this near to each other, as the difference of their bits: a factor of 4 (R above).  The maximum over the
+// tokens in every chunk, with the logarithms shared by a warp's lanes, took 64 sequences of 8192 tokens 116.6 us, and
+// those of D = 64 86.3; so, 115.2 and 81.9; without either, and with the errors that it keeps out, 112.7 and 78.4.
+constexpr uint32_t kEvenScales = 2u << 23;
 
 // d = a.b + c, signed or unsigned digits times signed codes; c may be constant (the first product of a sum).
 __device__ __forceinline__ void mma_s8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1,
@@ -133,6 +141,32 @@ __device__ __forceinline__ void bulk_g2s_once(void *dst, const void *src, uint32
             smem_u32(dst)),
         "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
+}
+
+// Sets a scale of 1 to 0, in a copied chunk, where the vector's codes are all 0: so the format holds vectors of equal
+// components.  At scale 1 such a value's centred codes, -8 or -128 throughout, are the largest step of the chunk, and such
+// a key's are off by 128 times the sum of the query digits' errors: zero values in every seventh token cost the others
+// log2(1 / scale) bits, 8 to 16 of them.
+template <int KB, int CT>
+__device__ __forceinline__ void drop_constant_scales(unsigned char *sp, int n_tok, int lane) {
+#pragma unroll 1
+    for (int t = lane; t < n_tok; t += 32) {
+        float *ks = reinterpret_cast<float *>(sp + CT * KB + 8 * t), *vs = ks + 2 * CT;
+        const bool key = *ks == 1.0f, value = *vs == 1.0f;
+        if (!key && !value) continue;
+        const unsigned char *k = sp + t * KB, *v = sp + CT * (KB + 16) + (t >> 4) * (16 * KB) + 16 * ((t >> 2) & 3);
+        uint32_t kany = 0, vany = 0;
+#pragma unroll 1
+        for (int i = 0; i < KB / 4; i++) {
+            kany |= reinterpret_cast<const uint32_t *>(k)[i];
+            const uint4 x = *reinterpret_cast<const uint4 *>(v + 64 * i);
+            vany |= x.x | x.y | x.z | x.w;
+        }
+        if (key && kany == 0) *ks = 0.0f;
+        if (value && (vany & (0xffu << (8 * (t & 3)))) == 0) *vs = 0.0f;
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before the next copy into this stage
+    }
+    __syncwarp();
 }
 
 // Where a range is: at chunk c of unit (KV head h, block hb of its query heads) of row r, whose units have n chunks;
@@ -391,16 +425,24 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
     f2 facc[G::NF / 2];           // value sums in the frame of R, two columns each
     float R = -INFINITY, L = 0.0f, Z = 0.0f;
     // One chunk's scores, weights and value sums; `part`: only its first n_tok tokens count.
-    auto chunk = [&](const unsigned char *sp, int n_tok, auto part) {
+    auto chunk = [&](unsigned char *sp, int n_tok, auto part) {
         constexpr bool PART = decltype(part)::value;
         const unsigned char *kmeta = sp + CT * KB, *vmeta = kmeta + CT * 8, *vcodes = vmeta + CT * 8;
         // largest value scale: lanes share the tokens (scales are not negative; their bits order as they do)
-        uint32_t vbits = 0;
+        uint32_t vbits[CT / 32], most = 0;
+        bool other = false;  // a scale of 1, or value scales that are not even
 #pragma unroll
-        for (int i = 0; i < CT / 32; i++)
-            if (!PART || 32 * i + lane < n_tok)
-                vbits = max(vbits, __float_as_uint(*reinterpret_cast<const float *>(vmeta + (32 * i + lane) * 8)) & 0x7fffffffu);
-        vbits = __reduce_max_sync(0xffffffffu, vbits);
+        for (int i = 0; i < CT / 32; i++) {
+            vbits[i] = 0x7fffffffu;
+            if (!PART || 32 * i + lane < n_tok) {
+                vbits[i] = __float_as_uint(*reinterpret_cast<const float *>(vmeta + (32 * i + lane) * 8)) & 0x7fffffffu;
+                other |= vbits[i] == __float_as_uint(1.0f);
+                most = max(most, vbits[i]);
+            }
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+        for (int i = 0; i < CT / 32; i++) other |= vbits[i] + kEvenScales < most;
         // ---- scores: tile pair p holds tokens 16 p + 4 q + e of the lane's head ----
         float sc[4 * G::NPR];
         float smax = -INFINITY;
@@ -460,12 +502,30 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
                 if (PART && 16 * p + 4 * q + e >= n_tok) s = -INFINITY;
                 sc[4 * p + e] = s;
                 smax = fmaxf(smax, s);
+                other |= ks[e] == 1.0f;
             }
         }
+        // the chunk's reference: the largest weight times value scale, or a little more where the scales are alike
+        float Rc;
+        if (!__any_sync(0xffffffffu, other)) {
+            Rc = smax + __log2f(fmaxf(__uint_as_float(most), kVScaleMin));
+        } else {
+            drop_constant_scales<KB, CT>(sp, n_tok, lane);
+            Rc = -INFINITY;
 #pragma unroll
-        for (int lm = 1; lm < 4; lm <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, lm));
-        // the chunk's reference, the running one, and the factors that bring both sums to the latter
-        const float Rc = smax + __log2f(fmaxf(__uint_as_float(vbits), kVScaleMin));
+            for (int p = 0; p < G::NPR; p++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float2 km = *reinterpret_cast<const float2 *>(kmeta + (16 * p + 4 * q + e) * 8);
+                    const float vs = *reinterpret_cast<const float *>(vmeta + (16 * p + 4 * q + e) * 8);
+                    float &s = sc[4 * p + e];
+                    if (km.x == 0.0f && s > -INFINITY) s = km.y * c2;
+                    Rc = fmaxf(Rc, s + __log2f(fmaxf(fabsf(vs), kVScaleMin)));
+                }
+        }
+#pragma unroll
+        for (int lm = 1; lm < 4; lm <<= 1) Rc = fmaxf(Rc, __shfl_xor_sync(0xffffffffu, Rc, lm));
+        // the running reference, and the factors that bring both sums to it
         const float Rn = fmaxf(R, Rc);
         const float fo = R == -INFINITY ? 0.0f : ex2_approx(R - Rn), fn = Rc == -INFINITY ? 0.0f : ex2_approx(Rc - Rn);
         R = Rn;
