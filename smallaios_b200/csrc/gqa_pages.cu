@@ -175,7 +175,8 @@ struct Place {
     int r, h, hb, c, n, b, f;
 };
 
-// Tokens that query row r (row0 + r of batch x seq_len) attends to.
+// Tokens that query row r (row0 + r of batch x seq_len) attends to; their negative where its own position lies behind them,
+// as its table is too short.
 __device__ __forceinline__ int visible(const PagesAttendArgs &a, int row, bool report) {
     const int b = row / a.seq_len, s = row - b * a.seq_len;
     int64_t pos0;
@@ -188,7 +189,7 @@ __device__ __forceinline__ int visible(const PagesAttendArgs &a, int row, bool r
     const int64_t most = (int64_t)a.rows.max_pages * kPageTokens;
     if (pos >= most) {
         if (report) atomicOr(a.rows.dev_status, kPagesBadPage);
-        return (int)most;
+        return -(int)most;
     }
     return (int)pos + 1;
 }
@@ -201,7 +202,7 @@ __host__ __device__ __forceinline__ int sharing_warps(int F, int warps) { return
 // fills fragment row w (three digits: rows w and w + 4); head 0 also clears the rows of the heads that the unit lacks.
 // `v`: room for D digits.  Kept short: it runs once per head, and fetching long straight code costs more than running it.
 template <typename T, int BITS, int D, int ND>
-__device__ __forceinline__ void prepare_head(const PagesAttendArgs &a, int grow, int len, int h, int hb, int w, int lane,
+__device__ __forceinline__ void prepare_head(const PagesAttendArgs &a, int grow, int sees, int h, int hb, int w, int lane,
                                              std::conditional_t<ND == 2, int16_t, int> *v, uint4 *unit) {
     using G = PGeo<BITS, D, ND>;
     constexpr int EPL = D / 32, N = D / 4, kHalf = G::NCH / 2;
@@ -210,7 +211,9 @@ __device__ __forceinline__ void prepare_head(const PagesAttendArgs &a, int grow,
     load_elems<float, EPL>(a.signs + (int64_t)h * D + lane * EPL, sg);
     load_elems<T, EPL>(static_cast<const T *>(a.query) + b * a.batch_stride + s * a.token_stride +
                            ((int64_t)h * a.group + g) * D + lane * EPL, x);
-    if (a.rope.on) rope_lane<EPL>(x, lane, D, len - 1, a.rope.cos_cache, a.rope.sin_cache, a.rope.interleaved);
+    const int len = abs(sees);
+    // (a position in the rotary tables, that is below 2^31: visible)
+    if (a.rope.on) rope_lane<EPL>(x, lane, D, sees > 0 ? len - 1 : __ldcg(a.rows.lens + b) + s, a.rope.cos_cache, a.rope.sin_cache, a.rope.interleaved);
 #pragma unroll
     for (int i = 0; i < EPL; i++) x[i] *= sg[i];
     warp_wht_butterfly<EPL>(x, lane, D);
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
             const int i = base + tid;
             const int len = i < rows ? visible(a, row0 + i, blockIdx.x == 0) : 0;
             if (i < rows) s_len[i] = len;
-            int v = len > 0 ? (len + CT - 1) / CT + kUnitCost : 0;
+            int v = len != 0 ? (abs(len) + CT - 1) / CT + kUnitCost : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, v, o);
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(kNWP * 32, 1)
         const int per = min(a.group, G::HB);  // heads of a unit, but in a last block that has fewer
         for (int t = warp; t < (u1 - u0 + 1) * per; t += kNWP) {
             const int u = u0 + t / per, hw = t % per, row = u / upr, k = u - row * upr, h = k / hblocks, hb = k - h * hblocks;
-            if (s_len[row] > 0 && hb * G::HB + hw < a.group)
+            if (s_len[row] != 0 && hb * G::HB + hw < a.group)
                 prepare_head<T, BITS, D, ND>(a, row0 + row, s_len[row], h, hb, hw, lane, s_digits[warp],
                                              cta_prep + (int64_t)u * G::PREP);
         }
