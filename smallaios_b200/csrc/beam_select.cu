@@ -3,7 +3,7 @@
 //
 // beam_scan_kernel: a warp takes a run of a row in groups of 256 neighbouring
 // tokens and leaves, per group, the largest logit, and per run the sum of
-// exponentials and its reference.  Nothing else of the row is needed to choose:
+// exponentials and its reference (a lane's in f64, over sums of 16 or 32 terms in f32).  Nothing else of the row is needed to choose:
 // the best n tokens lie in the n groups with the largest maxima (each of n better
 // groups holds a better token; between equal maxima the lower group holds the lower
 // token).
@@ -37,6 +37,10 @@ constexpr int kPickThreads = 512;
 // bf16, scan and pick: one wave 46 us, two 37, three 41, four 46 (all before whole groups had loads of their own).
 constexpr int kScanWarps = 148 * 64;
 constexpr float kL = 1.4426950408889634f;  // log2(e)
+// How far the largest logit may lie above the reference of a run's sum before the reference is raised to it.  A raise is
+// off by 2^-22: one in every step, in rows that climb slowly, added up to 2e-6; with 4, what comes before two or three
+// raises no longer counts.
+constexpr float kLag = 4.0f;
 
 struct Part {
     double sum;  // of e^(x - top)
@@ -144,7 +148,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
     const int part = (int)(w - r * parts);
     const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
     const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
-    float top = -INFINITY, sum = 0.0f;
+    float top = -INFINITY;  // the reference of the sum: up to kLag below the largest logit
+    double sum = 0.0;
     auto consume = [&](const Tokens<T, PIECES> (&now)[kAhead], int g) {
         float most = top, mine = 0.0f;
 #pragma unroll
@@ -154,12 +159,13 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
             if (lane == j) mine = m;
         }
         if (lane < kAhead && g + lane < g1) maxima[r * groups + g + lane] = mine;
-        if (most > top) {
+        if (most > top + kLag) {
             if (top > -INFINITY) sum *= exp2f((top - most) * kL);
             top = most;
         }
         const float ref = top == -INFINITY ? 0.0f : top;
         const f2 less = pair(-ref, -ref), log2e = pair(kL, kL);
+        float few = 0.0f;  // (32 terms)
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             f2 e[4];
@@ -171,8 +177,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
             }
             float s0, s1;
             split(add2(add2(e[0], e[1]), add2(e[2], e[3])), s0, s1);
-            sum += s0 + s1;
+            few += s0 + s1;
         }
+        sum += (double)few;
     };
     // whole groups, the next ones on their way; then the others
     Tokens<T, PIECES> now[kAhead], next[kAhead];
@@ -197,10 +204,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
         for (int j = 0; j < kAhead; j++) now[j].load(row, g + j < g1 ? a.vocab : 0, g + j, lane);
         consume(now, g);
     }
-    double total = sum;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) sums[r * parts + part] = Part{total, top, 0.0f};
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[r * parts + part] = Part{sum, top, 0.0f};
 }
 
 struct Choice {
