@@ -76,6 +76,22 @@ bool vectors_aligned(const void *p, int64_t batch_stride, int64_t token_stride, 
            (seq_len <= 1 || token_stride * width % 16 == 0);
 }
 
+// Whether two tables of `rows` rows of `width` pages share an element.  Column slices of one table lie between each
+// other's rows and share none.
+bool tables_overlap(const int32_t *x, int64_t x_stride, const int32_t *y, int64_t y_stride, int64_t rows, int64_t width) {
+    const int64_t bytes = width * 4, step = y_stride * 4;
+    const int64_t first = (int64_t)(reinterpret_cast<uintptr_t>(y) - reinterpret_cast<uintptr_t>(x));  // of y, from x on
+    if (first >= (rows - 1) * x_stride * 4 + bytes || first + (rows - 1) * step + bytes <= 0) return false;
+    for (int64_t i = 0; i < rows; i++) {
+        // the last row of y that begins before row i of x ends
+        const int64_t before = i * x_stride * 4 + bytes - 1 - first;
+        if (before < 0) continue;
+        const int64_t j = before / step < rows - 1 ? before / step : rows - 1;
+        if (first + j * step + bytes > i * x_stride * 4) return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -349,10 +365,7 @@ int sa_kv_pages_reorder(sa_kv_pages *pages, const int32_t *page_table, int64_t t
     if (batch == 0 || max_pages == 0) return SA_OK;
     if (!page_table || !new_table || !seq_lens || !parents)
         return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_reorder: NULL argument");
-    const int64_t rows = (int64_t)batch * num_beams;
-    const int32_t *end = page_table + (rows - 1) * table_stride + max_pages;
-    const int32_t *new_end = new_table + (rows - 1) * new_stride + max_pages;
-    if (page_table < new_end && new_table < end)
+    if (tables_overlap(page_table, table_stride, new_table, new_stride, (int64_t)batch * num_beams, max_pages))
         return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_reorder: the new table overlaps the old one");
     ReorderArgs a{};
     a.records = k->records;
