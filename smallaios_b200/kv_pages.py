@@ -59,6 +59,10 @@ class GpuKvPages:
         cfg.head_dim = head_dim
         cfg.bits = bits
         cfg.seed = seed & (2**64 - 1)
+        for name, n in (("num_layers", num_layers), ("num_pages", num_pages), ("num_heads", num_heads or 0),
+                        ("num_kv_heads", num_kv_heads), ("kv_head_begin", kv_head_begin),
+                        ("kv_head_count", kv_head_count or 0), ("head_dim", head_dim), ("bits", bits)):
+            ops._fits("kv_pages_create", name, n)
         with torch.cuda.device(self.device):
             check(lib.sa_kv_pages_create(ctypes.byref(cfg), ctypes.byref(self._handle)))
         self.config = cfg
@@ -94,9 +98,9 @@ class GpuKvPages:
             raise ValueError("key and value must have the same strides")
         table = ops._page_rows("kv_pages_append", page_table, seq_lens, counts, b, index)
         rope = ops._page_rope("kv_pages_append", cos_cache, sin_cache, self.half_dim, index)
-        rc = lib.sa_kv_pages_append(self.handle, layer, key.data_ptr(), value.data_ptr(), *strides, ops._dtype_code(key),
-                                    b, s, *table, *rope, int(bool(do_rotary)), int(bool(rotary_interleaved)),
-                                    ops._stream_handle(stream, self.device))
+        rc = lib.sa_kv_pages_append(self.handle, ops._fits("kv_pages_append", "layer_idx", layer), key.data_ptr(),
+                                    value.data_ptr(), *strides, ops._dtype_code(key), b, s, *table, *rope,
+                                    int(bool(do_rotary)), int(bool(rotary_interleaved)), ops._stream_handle(stream, self.device))
         ops._raise_op(rc, "kv_pages_append")
 
     def reorder_beams(self, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, *,
@@ -119,6 +123,8 @@ class GpuKvPages:
         if parents.dtype != torch.int32:
             raise ops.UnsupportedOp("reorder_beams: parents must be int32")
         b, k = shape
+        if b >= 2**31 or not 1 <= k <= _lib.SA_MAX_BEAMS:
+            raise ops.InvalidAttribute(f"reorder_beams: {b} groups of {k} beams (1..{_lib.SA_MAX_BEAMS})")
         table, stride, width, lens, _ = ops._page_rows("reorder_beams", page_table, seq_lens, None, b * k, index)
         if out is None:
             out = ops._empty(page_table.shape, torch.int32, page_table.device, stream)
@@ -143,7 +149,7 @@ class GpuKvPages:
     def view(self, layer: int) -> PagesView:
         """The layer's arrays.  The tensors keep the pool alive; ``close()`` ends them all the same."""
         v = _lib.KvPagesView()
-        check(lib.sa_kv_pages_layer_view(self.handle, layer, ctypes.byref(v)))
+        check(lib.sa_kv_pages_layer_view(self.handle, ops._fits("kv_pages_layer_view", "layer_idx", layer), ctypes.byref(v)))
         p, h, cb, d = v.num_pages, v.kv_heads, v.code_bytes, v.head_dim
         raw = _view(v.records, (p, h, v.record_bytes), "|u1", self)
 

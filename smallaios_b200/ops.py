@@ -370,6 +370,13 @@ def _on(t, index: int, what: str) -> None:
         raise TypeError(f"{what} must be a CUDA tensor")
 
 
+def _fits(op: str, name: str, x) -> int:
+    """``x`` where an argument of the library has 32 bits (ctypes would cut it)."""
+    if not -2**31 <= x < 2**31:
+        raise InvalidAttribute(f"{op}: {name} {x}")
+    return x
+
+
 def _page_table(op: str, t, batch: int, index: int, what: str):
     """(pointer, row stride, pages per row) of an int32 table of ``batch`` rows, which may be a slice of columns."""
     _on(t, index, what)
@@ -379,6 +386,8 @@ def _page_table(op: str, t, batch: int, index: int, what: str):
     if len(shape) != 2 or shape[0] != batch:
         raise ShapeMismatch(f"{op}: {what} must be ({batch}, pages), got {tuple(shape)}")
     pages = shape[1]
+    if pages >= 2**31:
+        raise ShapeMismatch(f"{op}: {what} of {pages} pages")
     if t.is_contiguous():
         return t.data_ptr(), pages, pages
     row, column = t.stride()
@@ -474,9 +483,9 @@ def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_ta
             raise ValueError("out must be contiguous")
     need = pages.workspace_bytes(b, s, code)
     workspace = _workspace(workspace, need, query.device, stream)
-    rc = lib.sa_gqa_paged_attend(pages.handle, layer, query.data_ptr(), *strides, out.data_ptr(), code, b, s,
-                                 int(num_heads), int(scale is not None), float(scale or 0.0), *table, *rope,
-                                 int(bool(do_rotary)), int(bool(rotary_interleaved)),
+    rc = lib.sa_gqa_paged_attend(pages.handle, _fits("gqa_paged_attend", "layer_idx", layer), query.data_ptr(), *strides,
+                                 out.data_ptr(), code, b, s, int(num_heads), int(scale is not None), float(scale or 0.0),
+                                 *table, *rope, int(bool(do_rotary)), int(bool(rotary_interleaved)),
                                  None if workspace is None else workspace.data_ptr(),
                                  0 if workspace is None else workspace.numel(), _stream_handle(stream, query.device))
     _raise_op(rc, "gqa_paged_attend")
@@ -510,6 +519,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     if scores.dtype != torch.float32:
         raise UnsupportedOp("beam_select: scores must be float32")
     b, k = shape
+    if b >= 2**31 or not 1 <= k <= _lib.SA_MAX_BEAMS:
+        raise InvalidAttribute(f"beam_select: {b} groups of {k} beams (1..{_lib.SA_MAX_BEAMS})")
     n, stride = rows
     vocab = stride
     if not logits.is_contiguous():
