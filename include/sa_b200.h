@@ -565,7 +565,8 @@ int sa_gqa_sparse_attend(sa_kv_cache *cache, int32_t layer, const void *query, c
  * Calls allocate nothing and wait for nothing; calls that write pages, tables
  * or lengths and calls that read them are ordered by the caller (one stream, or
  * events).  Attention calls on one pool may overlap on the device if each has a
- * workspace of its own.  The calls read the handle only: any threads.
+ * workspace of its own.  The calls read the handle only: any threads (but see
+ * sa_kv_pages_set_precision).
  * ====================================================================== */
 #define SA_PAGE_TOKENS 64
 #define SA_MAX_BEAMS 32
@@ -639,8 +640,14 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
  * Precision: queries and weights are held to 16 bits for f16 and bf16 callers,
  * to 24 for f32 (a weight times its value scale relative to the largest such
  * product of each 32 or 64 tokens, or to up to four times that).
+ * sa_kv_pages_set_precision(pages, 1) gives f16 and bf16 callers 24 bits too, as
+ * the decode path over sa_kv_cache has (a row's pages are read once for every
+ * four query heads of a KV head then, else for every eight).  It changes what
+ * sa_gqa_paged_workspace_bytes says, holds for the calls after it, and is not
+ * for a thread while others call.  0 is the default.
  * `workspace` (device, 256-byte aligned, at least what
  * sa_gqa_paged_workspace_bytes says) is the call's alone until it has run. */
+int sa_kv_pages_set_precision(sa_kv_pages *pages, int32_t full);
 int64_t sa_gqa_paged_workspace_bytes(const sa_kv_pages *pages, int32_t batch, int32_t seq_len, int32_t dtype);
 int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, int64_t batch_stride,
                         int64_t token_stride, void *attn_out, int32_t dtype, int32_t batch, int32_t seq_len,

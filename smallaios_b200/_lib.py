@@ -40,7 +40,7 @@ EXPORTED = [
     "sa_gqa_tree_workspace_bytes", "sa_gqa_tree_attend", "sa_kv_cache_set_tree_precision", "sa_kv_cache_keep_drafts", "sa_kv_block_means",
     "sa_gqa_select_blocks", "sa_gqa_sparse_workspace_bytes", "sa_gqa_sparse_attend",
     "sa_kv_pages_create", "sa_kv_pages_destroy", "sa_kv_pages_get_config", "sa_kv_pages_layer_view",
-    "sa_kv_pages_device_status", "sa_kv_pages_append", "sa_gqa_paged_workspace_bytes", "sa_gqa_paged_attend",
+    "sa_kv_pages_device_status", "sa_kv_pages_append", "sa_kv_pages_set_precision", "sa_gqa_paged_workspace_bytes", "sa_gqa_paged_attend",
     "sa_beam_select_workspace_bytes", "sa_beam_select", "sa_kv_pages_reorder",
 ]
 SA_MAX_DRAFT_NODES = 64
@@ -216,6 +216,8 @@ def _declare(l: ctypes.CDLL) -> None:
     l.sa_kv_pages_append.restype = ctypes.c_int
     l.sa_kv_pages_append.argtypes = [_P, _I32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _P, _P, _P, _I32,
                                      _I32, _I32, _P]
+    l.sa_kv_pages_set_precision.restype = ctypes.c_int
+    l.sa_kv_pages_set_precision.argtypes = [_P, _I32]
     l.sa_gqa_paged_workspace_bytes.restype = _I64
     l.sa_gqa_paged_workspace_bytes.argtypes = [_P, _I32, _I32, _I32]
     l.sa_gqa_paged_attend.restype = ctypes.c_int

@@ -16,7 +16,8 @@
 // weights the lane has to supply as the A operand of the value product, whose B
 // operand is a word of the V layout.  So scores become weights without passing
 // through shared memory, and one MMA carries eight query heads: 16 rows = 8 heads x
-// 2 digits.  f32 callers get three digits and four heads (12 rows).
+// 2 digits.  Callers of f32, and others by choice, get three digits and four heads
+// (12 rows).
 //
 //   s_t = ks_t (q'.c_t) + kz_t sum(q')           (log2 units, scale folded in)
 //   R >= max (s_t + log2 vs_t), u_t = 2^(s_t - R) vs_t in (0, 1], 16 or 24 bits of it
@@ -793,8 +794,12 @@ __global__ void __launch_bounds__(32 * PGeo<BITS, D, ND>::HB)
 
 constexpr size_t kPrefixBytes = ((kMaxRows + 1) * sizeof(int) + 255) / 256 * 256;
 
-// Query heads of a unit: as many as one product carries.
-int head_block(int dtype) { return dtype == SA_DTYPE_FLOAT ? 4 : 8; }
+// Whether queries and weights have three digits.  A unit has as many query heads as one product carries, four of three
+// digits or eight of two.  64 sequences of 8192 tokens, 8 heads of 4, take bf16 callers 121 us with three and 114 with
+// two, and 32 of 32768, 8 heads of 8, which are two units with three, f16 callers 456 and 206; against 64 bits the output
+// is off by 1.6662e-3 and 1.6668e-3 of its norm, and by 2.074e-4 and 2.126e-4, nearly all of it its own rounding.
+bool three_digits(int dtype, int full) { return dtype == SA_DTYPE_FLOAT || full; }
+int head_block(int dtype, int full) { return three_digits(dtype, full) ? 4 : 8; }
 
 int64_t rows_per_launch(int64_t units_per_row) {
     const int64_t n = kMaxUnits / units_per_row;
@@ -864,7 +869,7 @@ int launch_t(const PagesAttendArgs &a, void *workspace, cudaStream_t stream) {
 }  // namespace
 
 size_t pages_attend_workspace(const kv_pages_impl *k, int batch, int seq_len, int dtype) {
-    const int hb = head_block(dtype);
+    const int hb = head_block(dtype, k->full);
     const int64_t upr = (int64_t)k->cfg.kv_head_count * ((k->group + hb - 1) / hb);
     const int64_t rows = (int64_t)batch * seq_len, per = rows_per_launch(upr), n = rows < per ? rows : per;
     const int64_t records = (int64_t)k->sm_count * kNWP + n * upr;  // one per warp, and one more per unit
@@ -873,10 +878,12 @@ size_t pages_attend_workspace(const kv_pages_impl *k, int batch, int seq_len, in
 }
 
 int launch_pages_attend(const PagesAttendArgs &a, void *workspace, cudaStream_t stream) {
+    const bool three = three_digits(a.dtype, a.full);
     switch (a.dtype) {
         case SA_DTYPE_FLOAT: return launch_t<float, 3>(a, workspace, stream);
-        case SA_DTYPE_FLOAT16: return launch_t<__half, 2>(a, workspace, stream);
-        default: return launch_t<__nv_bfloat16, 2>(a, workspace, stream);
+        case SA_DTYPE_FLOAT16: return three ? launch_t<__half, 3>(a, workspace, stream) : launch_t<__half, 2>(a, workspace, stream);
+        default:
+            return three ? launch_t<__nv_bfloat16, 3>(a, workspace, stream) : launch_t<__nv_bfloat16, 2>(a, workspace, stream);
     }
 }
 

@@ -248,6 +248,12 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
     return launch_pages_append(a, static_cast<cudaStream_t>(stream));
 }
 
+int sa_kv_pages_set_precision(sa_kv_pages *pages, int32_t full) {
+    if (!pages) return set_error(SA_ERR_INVALID_ARGUMENT, "kv_pages_set_precision: NULL pages");
+    impl(pages)->full = full != 0;
+    return SA_OK;
+}
+
 int64_t sa_gqa_paged_workspace_bytes(const sa_kv_pages *pages, int32_t batch, int32_t seq_len, int32_t dtype) {
     if (!pages || batch <= 0 || seq_len <= 0 || !dtype_ok(dtype) || (int64_t)batch * seq_len > INT32_MAX) return 0;
     return (int64_t)pages_attend_workspace(impl(pages), batch, seq_len, dtype);
@@ -290,6 +296,7 @@ int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, in
     a.group = k->group;
     a.head_dim = k->cfg.head_dim;
     a.bits = k->cfg.bits;
+    a.full = k->full;
     a.records = k->records + (size_t)layer * k->layer_bytes;
     a.signs = k->signs + (size_t)layer * k->cfg.kv_head_count * k->cfg.head_dim;
     a.wht_scale = k->wht_scale;

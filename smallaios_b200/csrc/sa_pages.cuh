@@ -26,6 +26,7 @@ struct kv_pages_impl {
     int code_bytes;
     int group;  // num_heads / num_kv_heads
     float wht_scale;
+    int full;   // 24 bits of queries and weights for f16 and bf16 callers too
     void *base;
     uint8_t *records;  // [L][P][H][record]
     float *signs;      // [L][H][D]
@@ -67,7 +68,7 @@ struct PagesAttendArgs {
     int64_t batch_stride, token_stride;
     int aligned;
     void *out;
-    int dtype, batch, seq_len, heads, group, head_dim, bits;
+    int dtype, batch, seq_len, heads, group, head_dim, bits, full;
     const uint8_t *records;
     const float *signs;
     float wht_scale, scale;

@@ -138,8 +138,14 @@ class GpuKvPages:
         ops._raise_op(rc, "reorder_beams")
         return out
 
+    def set_precision(self, full: bool) -> None:
+        """Bits of queries and weights in ``gqa_paged_attend`` for f16 and bf16 callers (sa_kv_pages_set_precision): 24
+        with ``full``, as f32 callers and the decode path over ``GpuKvCache`` have; else 16, the default."""
+        check(lib.sa_kv_pages_set_precision(self.handle, int(bool(full))))
+        self._workspace_bytes.clear()
+
     def workspace_bytes(self, batch: int, seq_len: int, dtype_code: int) -> int:
-        """sa_gqa_paged_workspace_bytes."""
+        """sa_gqa_paged_workspace_bytes, which a pool's configuration and precision fix."""
         key = (batch, seq_len, dtype_code)
         n = self._workspace_bytes.get(key)
         if n is None:

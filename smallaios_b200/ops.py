@@ -465,6 +465,7 @@ def gqa_paged_attend(query: torch.Tensor, pages: GpuKvPages, layer: int, page_ta
     appended (``GpuKvPages.append``), and attends to all of the row's tokens up to itself.  ``page_table``,
     ``seq_lens`` and ``counts`` as for append; the query is rotated with ``do_rotary``.  Rows without tokens and
     tokens that do not exist give zeros.  A row's pages are read once per new token: S is one, or a few.
+    ``pages.set_precision`` sets the bits of f16 and bf16 callers.
     ``workspace``: uint8, at least ``pages.workspace_bytes`` bytes; allocated when not given.
     """
     index = pages.device.index
