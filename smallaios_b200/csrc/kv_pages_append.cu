@@ -22,7 +22,6 @@
 // that quotient (less than 2^-18 and 2^-14), so round(t) is the same unless t lies
 // as near to a half (kTie); a vector with such a t (or a scale outside the range
 // where 1/s is safe) is done again by the exact quotient.
-#include "sa_async.cuh"
 #include "sa_append.cuh"
 #include "sa_decode_common.cuh"
 #include "sa_pages.cuh"

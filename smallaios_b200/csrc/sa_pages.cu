@@ -287,7 +287,6 @@ int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, in
     a.query = query;
     a.batch_stride = batch_stride;
     a.token_stride = token_stride;
-    a.aligned = vectors_aligned(query, batch_stride, token_stride, dtype, batch, seq_len);
     a.out = attn_out;
     a.dtype = dtype;
     a.batch = batch;

@@ -66,7 +66,6 @@ struct PagesAppendArgs {
 struct PagesAttendArgs {
     const void *query;
     int64_t batch_stride, token_stride;
-    int aligned;
     void *out;
     int dtype, batch, seq_len, heads, group, head_dim, bits, full;
     const uint8_t *records;
@@ -87,7 +86,6 @@ struct BeamArgs {
     const uint8_t *finished;  // nullptr: none
     int32_t *parents, *tokens;
     float *out_scores;
-    int sm_count;
 };
 
 // Beams over pages (sa_kv_pages_reorder).

@@ -507,13 +507,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     ``finished`` (bool or uint8 (B, K)) has the single continuation ``end_token`` with its own score.  Best first,
     of equal scores the lower k*V + v; -1, -1, -inf behind the last.  ``keep`` defaults to K.
     """
-    _cuda(scores, "scores")
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise TypeError("logits must be a CUDA tensor")
-    if scores is None:
-        raise TypeError("scores must be a CUDA tensor")
     index = logits.get_device()
     _on(scores, index, "scores")
+    if not scores.is_contiguous():
+        raise ValueError("scores must be contiguous")
     shape, rows = scores.shape, logits.shape
     if len(shape) != 2 or len(rows) != 2 or rows[0] != shape[0] * shape[1]:
         raise ShapeMismatch("beam_select: logits must be (B*K, V) of scores (B, K)")
