@@ -147,7 +147,8 @@ __device__ __forceinline__ void bulk_g2s_once(void *dst, const void *src, uint32
 // Sets a scale of 1 to 0, in a copied chunk, where the vector's codes are all 0: so the format holds vectors of equal
 // components.  At scale 1 such a value's centred codes, -8 or -128 throughout, are the largest step of the chunk, and such
 // a key's are off by 128 times the sum of the query digits' errors: zero values in every seventh token cost the others
-// log2(1 / scale) bits, 8 to 16 of them.
+// log2(1 / scale) bits, 8 to 16 of them.  Not for speed: 64 sequences of 8192 tokens whose every fourth value is constant
+// take 146 us (114 without any), and 129 where every sixteenth scale is a twentieth of the others'.
 template <int KB, int CT>
 __device__ __forceinline__ void drop_constant_scales(unsigned char *sp, int n_tok, int lane) {
 #pragma unroll 1
@@ -155,16 +156,25 @@ __device__ __forceinline__ void drop_constant_scales(unsigned char *sp, int n_to
         float *ks = reinterpret_cast<float *>(sp + CT * KB + 8 * t), *vs = ks + 2 * CT;
         const bool key = *ks == 1.0f, value = *vs == 1.0f;
         if (!key && !value) continue;
-        const unsigned char *k = sp + t * KB, *v = sp + CT * (KB + 16) + (t >> 4) * (16 * KB) + 16 * ((t >> 2) & 3);
-        uint32_t kany = 0, vany = 0;
-#pragma unroll 1
-        for (int i = 0; i < KB / 4; i++) {
-            kany |= reinterpret_cast<const uint32_t *>(k)[i];
-            const uint4 x = *reinterpret_cast<const uint4 *>(v + 64 * i);
-            vany |= x.x | x.y | x.z | x.w;
+        if (key) {
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int i = 0; i < KB / 16; i++) {
+                const uint4 x = reinterpret_cast<const uint4 *>(sp + t * KB)[i];
+                any |= x.x | x.y | x.z | x.w;
+            }
+            if (any == 0) *ks = 0.0f;
         }
-        if (key && kany == 0) *ks = 0.0f;
-        if (value && (vany & (0xffu << (8 * (t & 3)))) == 0) *vs = 0.0f;
+        if (value) {
+            const unsigned char *v = sp + CT * (KB + 16) + (t >> 4) * (16 * KB) + 16 * ((t >> 2) & 3);
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int i = 0; i < KB / 4; i++) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(v + 64 * i);
+                any |= x.x | x.y | x.z | x.w;
+            }
+            if ((any & (0xffu << (8 * (t & 3)))) == 0) *vs = 0.0f;
+        }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before the next copy into this stage
     }
     __syncwarp();
