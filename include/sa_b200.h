@@ -620,7 +620,7 @@ int sa_kv_pages_device_status(sa_kv_pages *pages, int32_t *status, int32_t clear
  * position seq_lens[b] + s of its pages (s < counts[b]), K rotated to that
  * position when do_rotary is set (tables as for sa_kv_append).  key / value:
  * row b, token s at + b * batch_stride + s * token_stride elements of `dtype`,
- * kv_heads * head_dim consecutive values.  Bit-exact with sa_kv_append.  Rows
+ * kv_heads * head_dim consecutive values; both have the same strides.  Bit-exact with sa_kv_append.  Rows
  * that share a page must not write the same token of it.  seq_lens is not
  * changed: a forward pass appends in every layer and then raises it once. */
 int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const void *value,
@@ -646,7 +646,9 @@ int sa_kv_pages_append(sa_kv_pages *pages, int32_t layer, const void *key, const
  * sa_gqa_paged_workspace_bytes says, holds for the calls after it, and is not
  * for a thread while others call.  0 is the default.
  * `workspace` (device, 256-byte aligned, at least what
- * sa_gqa_paged_workspace_bytes says) is the call's alone until it has run. */
+ * sa_gqa_paged_workspace_bytes says) is the call's alone until it has run.
+ * Tables of 2^31 chunks (32 or 64 tokens) and more over a row's KV heads and
+ * blocks of query heads are refused, whatever the lengths. */
 int sa_kv_pages_set_precision(sa_kv_pages *pages, int32_t full);
 int64_t sa_gqa_paged_workspace_bytes(const sa_kv_pages *pages, int32_t batch, int32_t seq_len, int32_t dtype);
 int sa_gqa_paged_attend(sa_kv_pages *pages, int32_t layer, const void *query, int64_t batch_stride,
@@ -690,8 +692,9 @@ int sa_beam_select(const void *logits, int64_t row_stride, int32_t dtype, const 
  *     parent's n % 64 tokens are copied there in every layer;
  *   - the pages behind stay where they are.
  * parents: int32 (batch, num_beams); -1 = the beam stays as it is.  new_table (its
- * own memory, rows new_stride apart) must not overlap page_table.  Full pages that
- * no row names any more are free for the caller to use. */
+ * own memory, rows new_stride apart) must share no element with page_table (column
+ * slices of one tensor do not).  Full pages that no row names any more are free
+ * for the caller to use. */
 int sa_kv_pages_reorder(sa_kv_pages *pages, const int32_t *page_table, int64_t table_stride, int32_t *new_table,
                         int64_t new_stride, int32_t max_pages, const int32_t *seq_lens, const int32_t *parents,
                         int32_t batch, int32_t num_beams, sa_stream_t stream);

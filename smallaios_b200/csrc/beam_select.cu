@@ -12,10 +12,10 @@
 // `keep` groups over all beams by score + (maximum - log sum), then the best `keep`
 // tokens of those groups, which are read again.
 //
-// 64 x 8 rows of 128256 bf16 (131 MB, a seventh of the rows finished and skipped), 35 us: scan 24 us, 4.7 TB/s, two
-// thirds of the cycles issue (some eight instructions a token) and the exponentials alone take 15 us; pick 11 us, a
-// chain of dependent steps over 16 KB a group, which one group of 4 beams over 32000 tokens needs as well (11 us in
-// all).
+// 64 x 8 rows of 128256 bf16 (131 MB, a seventh of the rows finished and skipped), 35.5 us: the scan some 25, 4.4 TB/s
+// of the 108 MB that it reads, eight instructions a token, 58% of the cycles issue; the choice 11, a chain of dependent
+// steps over 16 KB a group, which one group of 4 beams over 32000 tokens needs as well (10.7 us in all).  At 64 registers
+// the scan of aligned 16-bit rows spills 16 bytes a thread, the choice 16 to 28.
 //
 // Equal rows give equal sums: which lane takes which token, and in which order, does
 // not depend on where a row begins, so that beams that are equal tie exactly.
@@ -33,8 +33,10 @@ namespace {
 constexpr int kGroup = 256;      // tokens of a group
 constexpr int kScanThreads = 256;
 constexpr int kPickThreads = 512;
-// Warps that the scan is split into where rows allow it: two waves of the 32 that fit on an SM.  64 x 8 rows of 128256
-// bf16, scan and pick: one wave 46 us, two 37, three 41, four 46 (all before whole groups had loads of their own).
+// Warps that the scan is split into where rows allow it: two waves of the 32 that fit on an SM.  Scan and choice at one,
+// two, three and four waves, in us: 64 x 8 rows of 128256 bf16 38.2, 35.5, 38.3, 42.4; of 32000 20.7, 21.0, 24.4, 20.9;
+// 16 x 8 of 128256 f32 21.3, 22.8, 24.6, 23.0; 32 x 5 of 50257 f16 18.5 and 18.3 three times; 4 of 32000 10.7 in all;
+// 1250 x 4 of 32000 bf16 120, 120, 104, 102 (a row per warp, then two).
 constexpr int kScanWarps = 148 * 64;
 constexpr float kL = 1.4426950408889634f;  // log2(e)
 // How far the largest logit may lie above the reference of a run's sum before the reference is raised to it.  A raise is

@@ -37,13 +37,15 @@
 // pages_merge_kernel: per unit, the sum of its warps' partial records, the
 // division, the inverse rotation and the store.
 //
-// Bound by HBM once it streams (6.1 TB/s, 0.93 of the measured copy): 64 sequences of
-// 8192 int4 tokens, 8 KV heads of 4, 112 us for 605 MB; 32 of 32768, 8 heads of 8, 200 us
-// for 1209 MB.  What is left: some 9 us before the first product (lengths, table, queries;
-// the first 33 MB arrive meanwhile), warps of a range end 6 us apart, the merge takes 4.
+// 64 sequences of 8192 int4 tokens, 8 KV heads of 4, 115 us for 605 MB (5.2 TB/s, 0.80
+// of the measured copy); 32 of 32768, 8 heads of 8, 207 us for 1209 MB (0.89).  Some 9 us
+// pass before the first product (lengths, table, queries; the first 33 MB arrive
+// meanwhile), warps of a range end 6 us apart, the merge takes 4; what is left over is
+// near the copy's rate, with half of the issue slots in use.
 // Tried: sixteen warps of half chunks (128 registers spill; D = 64 and 8 bits, which do
-// not, got 4 to 10% slower); the merge by the last CTA of a unit (123 us: code that runs
-// once costs its fetch); the queries in a launch of their own (114 us, and a launch more).
+// not, got 4 to 10% slower; with twelve only three digits at int4, D = 128 spill, 12
+// bytes); the merge by the last CTA of a unit (6% slower: code that runs once costs its
+// fetch); the queries in a launch of their own (2% slower, and a launch more).
 #include "sa_async.cuh"
 #include "sa_decode_common.cuh"
 #include "sa_pages.cuh"
@@ -57,8 +59,9 @@ using namespace dec;
 constexpr int kNWP = 12;         // warps per CTA, one CTA per SM
 constexpr int kMaxRows = 512;    // rows of a launch: their lengths and prefix sums fit in 4 KB
 constexpr int64_t kMaxUnits = 16384;  // units of a launch: bounds the workspace
-// What a unit counts for beside its chunks, in chunks: its queries' preparation and the change to it.  48 sequences of 0
-// to 16000 tokens: 77 us at 0, 74 at 2, 75 at 8; 64 sequences of 8192, which need no such balance: 110, 112, 116.
+// What a unit counts for beside its chunks, in chunks: its queries' preparation and the change to it.  At 1, 2 and 8, in
+// us: 48 sequences of 0 to 16000 tokens 75.6, 75.6, 76.7 (and 3 more than at 2 without); 64 of 8192 115.3, 116.2, 119.2,
+// of D = 64 82.0, 81.4, 84.1; 64 of 4096 int8 ones 105, 105, 108; 64 of up to 200 15.7, 17.2, 20.1.
 constexpr int kUnitCost = 2;
 
 template <int BITS, int D, int ND>
@@ -129,8 +132,9 @@ __device__ __forceinline__ uint32_t weight_digits(float u) {
     }
 }
 
-// bulk_g2s whose lines leave L2 first: pages are read once, and everything else that the call needs (queries, tables,
-// partial records, the merge's code) stays.
+// bulk_g2s whose lines leave L2 first: a row's pages are read once by a block of its query heads, and everything else that
+// the call needs (queries, tables, partial records, the merge's code) stays.  64 sequences of 8192 tokens 116 us, 119
+// without.  Rows that share pages do not lose by it: 16 groups of 8 beams over 8000 common tokens 209 and 214 us.
 __device__ __forceinline__ uint64_t read_once_policy() {
     uint64_t p;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));

@@ -12,10 +12,11 @@
 // Sums and differences are taken in pairs (f2).  A product that a sum follows is not: a product of a pair may be
 // contracted with the sum to one rounding, __fmul_rn never is.  (Products with signs are exact either way.)
 //
-// Bound by instruction issue and shuffles (2.4 of 4 instructions per cycle): eight ragged prompts of up to 2048 bf16
-// tokens, 8 heads of 128, int4, in 28 us (44.5 MB, 1.6 TB/s); a decode step of 64 rows in 5.6 us, which is latency.
-// More warps, fewer registers or the sums in pairs did not change the former, and it is no single pipe (L1 50%, ALU and
-// FMA 37% busy): a warp for many vectors, with the next ones on their way and none idle for rows that end early, took 31.
+// Eight ragged prompts of up to 2048 bf16 tokens, 8 heads of 128, int4, take 27 us (44.5 MB, 1.6 TB/s) at 2.4 of 4
+// instructions per cycle, no single pipe full (L1 50%, ALU and FMA 37% busy); a decode step of 64 rows 5.6 us, which is
+// latency.  Eight CTAs per SM leave 64 registers, and D = 128 spills 48 bytes a thread there, 80 in a step; six, without
+// spills, take 27.8 and 5.3 us, seven 27.2 and 5.5.  A warp for many vectors, with the next ones on their way and none
+// idle for rows that end early, took 31.
 //
 // Codes: (y - z)/s rounded half away from zero, the quotient itself rounded to
 // f32 first.  t = (y - z) * RN(1/s) is within 3 * 2^-24 times the largest code of

@@ -80,8 +80,8 @@ class GpuKvPages:
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor,
                seq_lens: torch.Tensor, *, counts: torch.Tensor | None = None, cos_cache=None, sin_cache=None,
                do_rotary: bool = False, rotary_interleaved: bool = False, stream=None) -> None:
-        """Quantize-on-append of (B, S, H*D) K/V: token s of row b goes to position seq_lens[b] + s
-        (sa_kv_pages_append).
+        """Quantize-on-append of (B, S, H*D) K/V, both of the same strides: token s of row b goes to position
+        seq_lens[b] + s (sa_kv_pages_append).
 
         ``page_table`` int32 (B, pages), ``seq_lens`` int32 (B), on the device: the row's pages, and its tokens
         before these; a length below 0 leaves a row out.  ``counts`` int32 (B): only the first counts[b] of the S
@@ -110,8 +110,8 @@ class GpuKvPages:
 
         ``parents`` int32 (B, K): beam i of group b (row b*K + i) goes on as beam parents[b, i] was; -1: it stays.
         ``page_table`` int32 (B*K, pages), ``seq_lens`` int32 (B*K), equal within a group.  Full pages may be shared
-        by rows; a row's page in use and the pages behind it must be its own.  ``out`` must not overlap
-        ``page_table``.
+        by rows; a row's page in use and the pages behind it must be its own.  ``out`` must share no element
+        with ``page_table``.
         """
         index = self.device.index
         ops._on(parents, index, "parents")
