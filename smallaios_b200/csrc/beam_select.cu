@@ -3,10 +3,10 @@
 //
 // beam_scan_kernel: a warp takes a run of a row in groups of 256 neighbouring
 // tokens and leaves, per group, the largest logit, and per run the sum of
-// exponentials and its reference (a lane's in f64, over sums of 16 or 32 terms in f32).  Nothing else of the row is needed to choose:
-// the best n tokens lie in the n groups with the largest maxima (each of n better
-// groups holds a better token; between equal maxima the lower group holds the lower
-// token).
+// exponentials and its reference (a lane's in f64, over sums of 16 or 32 terms in
+// f32).  Nothing else of the row is needed to choose: the best n tokens lie in the n
+// groups with the largest maxima (each of n better groups holds a better token;
+// between equal maxima the lower group holds the lower token).
 //
 // beam_pick_kernel, a CTA per group of beams: the beams' logarithms, the best
 // `keep` groups over all beams by score + (maximum - log sum), then the best `keep`
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(BeamArgs a, 
         }
         const float ref = top == -INFINITY ? 0.0f : top;
         const f2 less = pair(-ref, -ref), log2e = pair(kL, kL);
-        float few = 0.0f;  // (32 terms)
+        float few = 0.0f;  // of 8 * kAhead terms
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             f2 e[4];
